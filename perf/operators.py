@@ -3,9 +3,10 @@ one pass), the attention that reads it (one token a sequence, a tree of drafted
 tokens, a chunk of a prompt), the commit of a tree's accepted path and the
 read-back, each in elementary torch operations and as calls through nlgpu.
 
-A pool holds a record of bs * (hd + 4) bytes for each (block, kv head): the
-codes, then one f32 scale a position.  K codes lie [bs][hd], V codes
-[bs / 16][hd][16].  A value is its code (int8 or e4m3) times its position's scale.
+A pool is [block][kv head][bs / 16] tiles of sixteen positions, each of
+16 * (hd + 4) bytes: the codes, then one f32 scale a position.  K codes lie
+[16][hd], V codes [hd][16].  A value is its code (int8 or e4m3) times its
+position's scale.
 """
 from __future__ import annotations
 
@@ -149,20 +150,19 @@ class Inputs:
     def pool(self):
         """A pool whose every position holds a row: codes of normal values, scales that differ by position."""
         c = self.c
-        n = c["bs"] * c["head_dim"]
-        p = torch.empty(self.npool, c["kvheads"], n + 4 * c["bs"], device=DEV, dtype=torch.uint8)
-        step = max(1, (1 << 26) // (n * c["kvheads"]))
-        for b in range(0, self.npool, step):
-            x = self.normal(min(step, self.npool - b), c["kvheads"], n)
+        n, tiles = 16 * c["head_dim"], self.npool * c["kvheads"] * c["bs"] // 16
+        p = torch.empty(tiles, n + 64, device=DEV, dtype=torch.uint8)
+        step = (1 << 26) // n
+        for b in range(0, tiles, step):
+            x = self.normal(min(step, tiles - b), n)
             if c["fmt"] == "int8":
                 codes = torch.clamp(torch.round(x * 40.0), -127, 127).to(torch.int8)
             else:
                 codes = torch.clamp(x * 140.0, -448, 448).to(torch.float8_e4m3fn)
-            p[b:b + step, :, :n] = codes.view(torch.uint8)
+            p[b:b + step, :n] = codes.view(torch.uint8)
         top = 40.0 if c["fmt"] == "int8" else 140.0
-        s = self.uniform(self.npool, c["kvheads"], c["bs"], lo=0.6, hi=1.6) / top
-        p[:, :, n:] = s.view(torch.uint8).view(self.npool, c["kvheads"], 4 * c["bs"])
-        return p
+        p[:, n:] = (self.uniform(tiles, 16, lo=0.6, hi=1.6) / top).view(torch.uint8)
+        return p.view(self.npool, c["kvheads"], c["bs"] // 16, n + 64)
 
     def rope(self, rows):
         m = np.arange(self.c["head_dim"] // 2, dtype=np.float64)
@@ -239,15 +239,13 @@ def _rows_at(s, seq, slot, which):
     c = s["c"]
     bs, hd = c["bs"], c["head_dim"]
     block = s["table"].long()[seq, slot // bs]
-    at = slot % bs
-    record = (block[:, None] * c["kvheads"] + torch.arange(c["kvheads"], device=DEV)) * (bs * (hd + 4))
+    record = block[:, None] * c["kvheads"] + torch.arange(c["kvheads"], device=DEV)
+    tile = (record * (bs // 16) + (slot % bs // 16)[:, None]) * (16 * (hd + 4))
+    at = (slot % 16)[:, None]
     d = torch.arange(hd, device=DEV)
-    if which == "k":
-        code = at[:, None] * hd + d
-    else:
-        code = (at[:, None] // 16 * hd + d) * 16 + at[:, None] % 16
-    scale = bs * hd + 4 * at[:, None] + torch.arange(4, device=DEV)
-    return record[:, :, None] + torch.cat([code, scale], dim=1)[:, None, :]
+    code = at * hd + d if which == "k" else d * 16 + at
+    scale = 16 * hd + 4 * at + torch.arange(4, device=DEV)
+    return tile[:, :, None] + torch.cat([code, scale], dim=1)[:, None, :]
 
 
 def _read(s, seq, slot, which):
@@ -295,16 +293,12 @@ def _append(s):
 
 def _whole(s, which):
     """The whole sequences' values in 32 bits, [batch, kvheads, positions, hd]."""
-    c = s["c"]
-    bs, hd, n = c["bs"], c["head_dim"], c["bs"] * c["head_dim"]
-    raw = s[which + "pool"][s["table"].long().clamp(min=0)]  # [batch, mbps, kvheads, record]
-    lead = raw.shape[:3]
-    scale = raw[..., n:].contiguous().view(torch.float32)[..., None]
-    codes = _values(c, raw[..., :n].contiguous())
-    if which == "v":
-        codes = codes.view(*lead, bs // 16, hd, 16).transpose(-1, -2).reshape(*lead, bs, hd)
-    x = codes.view(*lead, bs, hd) * scale
-    return x.permute(0, 2, 1, 3, 4).reshape(lead[0], lead[2], -1, hd)
+    c, hd = s["c"], s["c"]["head_dim"]
+    raw = s[which + "pool"][s["table"].long().clamp(min=0)]  # [batch, mbps, kvheads, bs / 16, tile]
+    scale = raw[..., 16 * hd:].contiguous().view(torch.float32)[..., None]
+    codes = _values(c, raw[..., :16 * hd].contiguous())
+    codes = codes.view(*raw.shape[:-1], 16, hd) if which == "k" else codes.view(*raw.shape[:-1], hd, 16).transpose(-1, -2)
+    return (codes * scale).transpose(1, 2).reshape(raw.shape[0], raw.shape[2], -1, hd)
 
 
 def _attend(s, q, seen):
@@ -364,7 +358,7 @@ def _commit(s):
 def _pools(s):
     """Both pools as the codes and the scales that they hold, without a copy."""
     c = s["c"]
-    n = c["bs"] * c["head_dim"]
+    n = 16 * c["head_dim"]
     t = torch.int8 if c["fmt"] == "int8" else torch.float8_e4m3fn
     return {w: (s[w][..., :n].view(t), s[w][..., n:].view(torch.float32)) for w in ("kpool", "vpool")}
 
@@ -475,16 +469,14 @@ def _held64(s, b, which, slots):
     """Values [kvheads, slots, hd] of sequence b's given slots."""
     c = s["c"]
     bs, hd = c["bs"], c["head_dim"]
-    rec = s[which + "pool"][s["table"][b].long()[slots // bs]]  # [slots, kvheads, record]
-    pick = (slots % bs)[:, None, None]
+    pool = s[which + "pool"].movedim(2, 1)  # [block, tile of the block, kvheads, bytes]
+    tile = pool[s["table"][b].long()[slots // bs], slots % bs // 16]
+    pick = (slots % 16)[:, None, None]
     t = torch.int8 if c["fmt"] == "int8" else torch.float8_e4m3fn
-    codes = rec[..., :bs * hd].contiguous().view(t)
-    if which == "k":
-        codes = codes.float().view(len(slots), c["kvheads"], bs, hd)
-    else:
-        codes = codes.float().view(len(slots), c["kvheads"], bs // 16, hd, 16).movedim(-1, -2).flatten(2, 3)
+    codes = tile[..., :16 * hd].contiguous().view(t).float()
+    codes = codes.view(-1, c["kvheads"], 16, hd) if which == "k" else codes.view(-1, c["kvheads"], hd, 16).mT
     codes = codes.take_along_dim(pick[..., None], dim=2)[:, :, 0].double()
-    scale = rec[..., bs * hd:].contiguous().view(torch.float32).take_along_dim(pick, dim=2)
+    scale = tile[..., 16 * hd:].contiguous().view(torch.float32).take_along_dim(pick, dim=2)
     return (codes * scale.double()).transpose(0, 1)
 
 
