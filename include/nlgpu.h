@@ -363,6 +363,109 @@ size_t nlg_attn_entries_f16_workspace(uint32_t batch, uint32_t heads, uint32_t k
 int nlg_block_copy_f16(uint16_t *kpool, uint16_t *vpool, const int32_t *pairs, uint32_t n, uint32_t npool,
                        uint32_t bs, uint32_t kvdim, void *stream);
 
+/* ------------------------------------------------------------------------
+ * The 8-bit paged KV cache.  The reference has paged f32 caches
+ * (cache-append-paged-v, decode-attn-paged-v, kernels.el:1211-1246) and, by
+ * name, rmsnorm-heads and rope-half (kernels.el:823-882); a cache in 8 bits,
+ * drafted tokens and these in one pass have no counterpart there.
+ *
+ * Two pools, one for K and one for V, of npool blocks of bs positions (bs a
+ * multiple of 16), shared by all sequences through a block table
+ * [batch x mbps] as in nlg_decode_attn_paged_f16.  A pool is
+ * [block][kvheads][bs/16] tiles of sixteen positions, each of 16*(head_dim+4)
+ * bytes: the codes, then sixteen f32 scales.  K codes lie [16][head_dim], V
+ * codes [head_dim][16].  Position p of a sequence is row p % 16 of tile
+ * (p % bs) / 16 of block table[b*mbps + p/bs].  A value is code * scale:
+ *   NLG_KV_I8    scale = a/127, code = x/scale to the nearest whole number
+ *                (ties to even), an int8
+ *   NLG_KV_E4M3  scale = a/448, code = x/scale to the nearest e4m3 (finite)
+ * with a the row's largest magnitude (f32) and one scale a position and kv
+ * head.  A row with a value that is not finite (in f32) is stored as codes 0 and scale
+ * NaN, and so reads as NaN; a zero row has scale 0.
+ * nlg_block_copy_f16 copies blocks of these pools when it is given kvdim =
+ * kvheads * (head_dim + 4) / 2.  nlg_kv_q8_pool_bytes: bytes of one pool (0:
+ * sizes that the cache does not take).  head_dim is 64 or 128, heads any
+ * multiple of kvheads; pools are 16-byte aligned.  Nothing here allocates, so every call may be
+ * captured into a graph.
+ * ---------------------------------------------------------------------- */
+#define NLG_KV_I8 0
+#define NLG_KV_E4M3 1
+size_t nlg_kv_q8_pool_bytes(uint32_t npool, uint32_t kvheads, uint32_t head_dim, uint32_t bs);
+
+/* The rows of a Q|K|V projection made ready for attention and cached, in one
+ * launch.  Row r of qkv [rows x (heads + 2*kvheads)*head_dim] belongs to
+ * sequence seq[r] (NULL: r; then rows <= batch).  Its q and k heads are
+ * normed, y = x / sqrt(mean(x*x) + eps) * gain (rmsnorm-heads; a NULL gain:
+ * not normed), and rotated by table row rpos[r] (NULL: slot[r]; a row outside
+ * [0, trows) rotates by zeros) of rope_cos/rope_sin [trows x head_dim/2]:
+ * pairs (2m, 2m+1), or with rope_half != 0 pairs (m, m + head_dim/2), C0 =
+ * a0*cos - a1*sin, C1 = a0*sin + a1*cos.  q [rows x heads*head_dim] receives
+ * the queries; k and v are quantised into position slot[r] of the sequence.
+ * Rows whose sequence, slot or block is out of range (a negative slot:
+ * padding) cache nothing.  The rows of one call name distinct positions; q
+ * does not overlap qkv.  All is computed in 64 bits, so a row's codes depend
+ * on its inputs alone.  For drafted tokens rpos is the node's depth behind
+ * the context, and slot the node's place. */
+int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const float *kgain, float eps,
+                                     const float *rope_cos, const float *rope_sin, uint32_t trows, int rope_half,
+                                     const int32_t *seq, const int32_t *slot, const int32_t *rpos,
+                                     const int32_t *table, uint32_t npool, float *q, uint8_t *kpool, uint8_t *vpool,
+                                     int fmt, uint32_t rows, uint32_t batch, uint32_t heads, uint32_t kvheads,
+                                     uint32_t head_dim, uint32_t bs, uint32_t mbps, void *stream);
+
+/* Single-query attention of every sequence over its positions 0..lens[b]
+ * (nlg_decode_attn_paged_f16's, with K and V from the 8-bit pools): out and q
+ * [batch x heads*head_dim], 16-byte aligned.  lens[b] < 0: nothing is attended and the row is
+ * zero; positions past the block table are not attended; table entries
+ * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
+ * and carry 22 bits of q and of the probabilities.  V rows
+ * whose scales lie more than 2^18 below the largest in a chunk lose bits.
+ * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0 bytes: none is read), as
+ * below; calls that share one run in stream order. */
+int nlg_decode_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt,
+                             const int32_t *lens, const int32_t *table, uint32_t npool, float *out, uint32_t batch,
+                             uint32_t heads, uint32_t kvheads, uint32_t head_dim, uint32_t bs, uint32_t mbps,
+                             void *workspace, size_t workspace_bytes, void *stream);
+size_t nlg_decode_attn_paged_q8_workspace(uint32_t batch, uint32_t heads, uint32_t kvheads, uint32_t head_dim,
+                                          uint32_t bs, uint32_t mbps);
+
+/* Attention of several queries a sequence: a tree of drafted tokens, or a
+ * chunk of a prompt.  q and out are [batch][tmax][heads*head_dim].  Node i <
+ * nodes[b] (NULL: tmax) of sequence b is cached at position base[b] + i; it
+ * attends all positions below base[b] and of the nodes those that bit j of
+ * mask[b*tmax + i] names (tmax <= 64; a node attends itself only if its own
+ * bit is set), or with mask NULL nodes 0..i (any tmax).  A row that attends
+ * nothing is zero.  Rows of nodes past nodes[b], and of sequences with
+ * base[b] < 0, keep what they held.  Every node below nodes[b] has been
+ * appended.  Otherwise as nlg_decode_attn_paged_q8. */
+int nlg_tree_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt, const int32_t *base,
+                           const int32_t *nodes, const uint64_t *mask, const int32_t *table, uint32_t npool,
+                           float *out, uint32_t batch, uint32_t tmax, uint32_t heads, uint32_t kvheads,
+                           uint32_t head_dim, uint32_t bs, uint32_t mbps, void *workspace, size_t workspace_bytes,
+                           void *stream);
+size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax, uint32_t heads, uint32_t kvheads,
+                                        uint32_t head_dim, uint32_t bs, uint32_t mbps);
+
+/* A tree's accepted path moved behind the context: for i < accepted[b] (at
+ * most tmax <= 64) the cached row of node path[b*tmax + i], position base[b] +
+ * path[..], goes to position base[b] + i, as if all of a sequence's rows were read before
+ * any is written.  Entries outside [0, tmax), and rows whose source or
+ * destination has no block, move nothing; sequences with base[b] < 0 are
+ * left alone.  Blocks written here belong to one sequence. */
+int nlg_tree_commit_paged_q8(uint8_t *kpool, uint8_t *vpool, const int32_t *base, const int32_t *path,
+                             const int32_t *accepted, const int32_t *table, uint32_t npool, uint32_t batch,
+                             uint32_t tmax, uint32_t kvheads, uint32_t head_dim, uint32_t bs, uint32_t mbps,
+                             void *stream);
+
+/* Cached rows read back: k and v [rows][kvheads][head_dim] fp16 (16-byte
+ * aligned) receive position slot[r] of sequence seq[r] (NULL: r; then rows <=
+ * batch), code * scale in f32 rounded to nearest even; rows out of range or
+ * without a block read as zeros. */
+int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt, const int32_t *seq,
+                            const int32_t *slot, const int32_t *table, uint32_t npool, uint16_t *k, uint16_t *v,
+                            uint32_t rows, uint32_t batch, uint32_t kvheads, uint32_t head_dim, uint32_t bs,
+                            uint32_t mbps, void *stream);
+
 /* The first of nlg_decode_attn_f16's two launches alone: per chunk of
  * positions and head, the chunk's maximum score m (in base 2: q.k/sqrt(hd)
  * times log2 e), its sum of 2^(s - m) and the matching weighted sum of V,

@@ -15,6 +15,8 @@ hipStream_t nlg_stream(void *s);
 // Ensure the device is initialised (nlg_init(-1) on first use).
 int nlg_ensure_init(void);
 int nlg_num_cu(void);
+// The device that nlg_init selected.
+int nlg_device(void);
 
 #define NLG_HIP(call)                                                              \
   do {                                                                             \

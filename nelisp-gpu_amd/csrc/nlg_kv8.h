@@ -1,0 +1,126 @@
+// nlg_kv8.h -- the 8-bit paged KV cache: its layout and how the attention
+// over it is split, in one place (plain C++, so both are checked on the CPU).
+//
+// A pool (one for K, one for V) is [block][kv head][bs / 16] tiles of sixteen
+// positions; a tile is 16 * hd codes, then sixteen f32 scales.  K codes lie
+// [16][hd]: a lane's sixteen bytes are matrix-operand depth.  V codes lie
+// [hd][16]: in the product with the probabilities the positions are the depth,
+// so a lane's sixteen bytes are that again, and neither needs a transposition
+// when it is read.
+#pragma once
+
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#include <hip/hip_runtime.h>
+#define NLG_KV8_HD __host__ __device__ __forceinline__
+#else
+#define NLG_KV8_HD inline
+#endif
+
+#define KV8_TILE 16  // positions of a tile
+#define KV8_STEP 64  // positions that a wave attends at once
+#define KV8_WAVES 4  // waves of an attention workgroup
+
+NLG_KV8_HD constexpr uint32_t kv8_tile_bytes(uint32_t hd) { return KV8_TILE * (hd + 4); }
+// Byte of position `at` (0..15), dimension d in a tile; of its scale.
+NLG_KV8_HD constexpr uint32_t kv8_k_byte(uint32_t hd, uint32_t at, uint32_t d) { return at * hd + d; }
+NLG_KV8_HD constexpr uint32_t kv8_v_byte(uint32_t at, uint32_t d) { return d * KV8_TILE + at; }
+NLG_KV8_HD constexpr uint32_t kv8_scale_byte(uint32_t hd, uint32_t at) { return KV8_TILE * hd + 4 * at; }
+
+// Bytes of one pool, 0 for sizes that the cache does not take.
+inline uint64_t kv8_pool_bytes(uint32_t npool, uint32_t bs, uint32_t kvheads, uint32_t hd) {
+  if (!npool || !bs || bs % KV8_TILE || !kvheads || (hd != 64 && hd != 128)) return 0;
+  const uint64_t tiles = (uint64_t)npool * kvheads * (bs / KV8_TILE);
+  // a tile's number is held in 32 bits, the largest standing for "none"
+  if ((uint64_t)npool * kvheads > 0xffffffffull || tiles >= 0xffffffffull) return 0;
+  return tiles * kv8_tile_bytes(hd);
+}
+
+// What finds a position's tile.
+struct Kv8Pages {
+  const int32_t *table;                // [batch][mbps]
+  uint32_t npool, mbps, bpt, kvheads;  // bpt: tiles of a block
+};
+#define KV8_NONE 0xffffffffu
+// The tile of sequence b's tile number t (position / 16) and kv head h, or
+// KV8_NONE outside the table or the pool.
+NLG_KV8_HD uint32_t kv8_tile(const Kv8Pages &g, uint32_t b, uint32_t h, uint32_t t) {
+  const uint32_t blk = t / g.bpt;
+  if (blk >= g.mbps) return KV8_NONE;
+  const int32_t ph = g.table[(uint64_t)b * g.mbps + blk];
+  if (ph < 0 || (uint32_t)ph >= g.npool) return KV8_NONE;
+  return ((uint32_t)ph * g.kvheads + h) * g.bpt + t % g.bpt;
+}
+
+// The positions of a sequence: those below `base` all rows attend, those from
+// base to end hold nodes (none without a tree); on: it takes part at all.
+struct Kv8Extent {
+  uint32_t base, end, nodes;
+  bool on;
+};
+// at: the last position, or with a tree the slot of node 0; cap: the block table's positions.
+NLG_KV8_HD Kv8Extent kv8_extent(bool tree, int32_t at, int32_t nodes, uint32_t tmax, uint32_t cap) {
+  Kv8Extent e;
+  if (!tree) {
+    e.end = at < 0 ? 0u : (uint32_t)at >= cap ? cap : (uint32_t)at + 1;
+    e.base = e.end;
+    e.nodes = 1;
+    e.on = true;
+  } else {
+    e.nodes = nodes < 0 ? 0u : (uint32_t)nodes > tmax ? tmax : (uint32_t)nodes;
+    e.base = at < 0 ? 0u : (uint32_t)at;
+    e.end = e.base + e.nodes < cap ? e.base + e.nodes : cap;
+    e.on = at >= 0 && e.nodes;
+  }
+  return e;
+}
+// Where the rows of nodes up to `last` stop attending, without a mask.
+NLG_KV8_HD uint32_t kv8_stop(const Kv8Extent &e, uint32_t last) {
+  return last < e.nodes && e.base + last + 1 < e.end ? e.base + last + 1 : e.end;
+}
+// Positions c0.. of a chunk, up to:
+NLG_KV8_HD uint32_t kv8_chunk_end(uint32_t c0, uint32_t stop, uint32_t chunk) {
+  return c0 >= stop ? c0 : stop - c0 < chunk ? stop : c0 + chunk;
+}
+// How many of the sixteen positions from p0 on exist.
+NLG_KV8_HD int kv8_left(const Kv8Extent &e, uint32_t p0) { return p0 >= e.end ? 0 : e.end - p0 < 16 ? (int)(e.end - p0) : 16; }
+// Which of the sixteen positions from p0 on a row of `node` attends; word: the
+// node's mask (its bits past the nodes cleared), without one those up to itself.
+NLG_KV8_HD uint32_t kv8_bits(const Kv8Extent &e, bool masked, uint32_t node, uint64_t word, uint32_t p0) {
+  const uint32_t all = (1u << kv8_left(e, p0)) - 1;
+  if (p0 + 16 <= e.base) return all;
+  if (!masked) {
+    const int64_t lim = (int64_t)e.base + node + 1 - p0;
+    return all & (lim <= 0 ? 0u : lim >= 16 ? 0xffffu : (1u << (int)lim) - 1);
+  }
+  if (p0 < e.base) {
+    const uint32_t off = e.base - p0;  // 1..15
+    return all & ((uint32_t)(word << off) | ((1u << off) - 1));
+  }
+  return p0 - e.base < 64 ? all & (uint32_t)(word >> (p0 - e.base)) : 0u;
+}
+NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 ? mask & ((1ull << nodes) - 1) : mask; }
+
+// How an attention call is laid over workgroups: rows (queries x query heads
+// of a kv head) in groups of `rowsper`, positions in `nchunk` chunks of `chunk`.
+struct Kv8Split {
+  uint32_t rowsper, groups, chunk, nchunk;
+  uint64_t blocks;  // workgroups
+};
+inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint64_t positions) {
+  Kv8Split s;
+  s.rowsper = rows > 16 ? 32 : 16;
+  s.groups = (uint32_t)(((uint64_t)rows + s.rowsper - 1) / s.rowsper);
+  const uint64_t units = (uint64_t)batch * kvheads * s.groups, per = KV8_STEP * KV8_WAVES;
+  const uint64_t most = (positions + per - 1) / per;
+  uint64_t want = (2048 + units - 1) / units;
+  if (want > most) want = most;
+  if (!want) want = 1;
+  const uint64_t steps = (most + want - 1) / want;
+  s.chunk = (uint32_t)(steps * per);
+  s.nchunk = (uint32_t)((most + steps - 1) / steps);
+  if (!s.nchunk) s.nchunk = 1;
+  s.blocks = units * s.nchunk;
+  return s;
+}

@@ -85,6 +85,7 @@ void *nlg_noalloc_scratch(void) {
   return g_noalloc_scratch[g_device];
 }
 int nlg_num_cu(void) { return g_num_cu; }
+int nlg_device(void) { return g_device; }
 
 hipStream_t nlg_stream(void *s) { return s ? (hipStream_t)s : g_stream; }
 

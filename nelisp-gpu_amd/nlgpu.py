@@ -125,6 +125,17 @@ def lib() -> C.CDLL:
                                        vp]),
         "nlg_attn_entries_f16_workspace": (sz, [u32, u32, u32, u32, u32]),
         "nlg_block_copy_f16": (i32, [vp, vp, vp, u32, u32, u32, u32, vp]),
+        "nlg_kv_q8_pool_bytes": (sz, [u32, u32, u32, u32]),
+        "nlg_qk_norm_rope_append_paged_q8": (i32, [vp, vp, vp, C.c_float, vp, vp, u32, i32, vp, vp, vp, vp, u32, vp,
+                                                   vp, vp, i32, u32, u32, u32, u32, u32, u32, u32, vp]),
+        "nlg_decode_attn_paged_q8": (i32, [vp, vp, vp, i32, vp, vp, u32, vp, u32, u32, u32, u32, u32, u32, vp, sz,
+                                           vp]),
+        "nlg_decode_attn_paged_q8_workspace": (sz, [u32, u32, u32, u32, u32, u32]),
+        "nlg_tree_attn_paged_q8": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, u32, vp, u32, u32, u32, u32, u32, u32, u32,
+                                         vp, sz, vp]),
+        "nlg_tree_attn_paged_q8_workspace": (sz, [u32, u32, u32, u32, u32, u32, u32]),
+        "nlg_tree_commit_paged_q8": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, vp]),
+        "nlg_cache_read_paged_q8": (i32, [vp, vp, i32, vp, vp, vp, u32, vp, vp, u32, u32, u32, u32, u32, u32, vp]),
         "nlg_repack_packed_to_2bit": (i32, [vp, u32, u32, u32, u32, vp, vp, vp]),
         "nlg_ternary_tiled_register": (i32, [vp, u32, u32, vp]),
         "nlg_ternary_tiled_unregister": (i32, [vp]),
@@ -436,6 +447,67 @@ def attn_entries_f16(q, kc, vc, ent, qrank, co, si, out, batch, heads, kvheads, 
 
 def block_copy_f16(kpool, vpool, pairs, n, npool, bs, kvdim, stream=None) -> None:
     _check(lib().nlg_block_copy_f16(kpool.ptr, vpool.ptr, pairs.ptr, n, npool, bs, kvdim, stream), "block_copy_f16")
+
+
+# The 8-bit paged KV cache's formats (NLG_KV_* in nlgpu.h).
+KV_I8, KV_E4M3 = 0, 1
+
+
+def kv_q8_pool_bytes(npool, kvheads, head_dim, bs) -> int:
+    """Bytes of one 8-bit pool (K or V) of npool blocks of bs positions."""
+    return int(lib().nlg_kv_q8_pool_bytes(npool, kvheads, head_dim, bs))
+
+
+def qk_norm_rope_append_paged_q8(qkv, qgain, kgain, eps, co, si, trows, slot, table, npool, q, kpool, vpool, rows,
+                                 batch, heads, kvheads, head_dim, bs, mbps, seq=None, rpos=None, half=False,
+                                 fmt=KV_I8, stream=None) -> None:
+    """Rows of Q|K|V: head norms and rotation of q and k, q out, k and v quantised into the 8-bit pools."""
+    _check(lib().nlg_qk_norm_rope_append_paged_q8(
+        qkv.ptr, _ptr(qgain), _ptr(kgain), eps, co.ptr, si.ptr, trows, int(half), _ptr(seq), slot.ptr, _ptr(rpos),
+        table.ptr, npool, q.ptr, kpool.ptr, vpool.ptr, fmt, rows, batch, heads, kvheads, head_dim, bs, mbps, stream),
+        "qk_norm_rope_append_paged_q8")
+
+
+def decode_attn_paged_q8_workspace(batch, heads, kvheads, head_dim, bs, mbps) -> int:
+    return int(lib().nlg_decode_attn_paged_q8_workspace(batch, heads, kvheads, head_dim, bs, mbps))
+
+
+def decode_attn_paged_q8(q, kpool, vpool, lens, table, npool, out, batch, heads, kvheads, head_dim, bs, mbps,
+                         workspace, fmt=KV_I8, stream=None) -> None:
+    """Single-query attention over 8-bit paged pools, sequence b over positions 0..lens[b]."""
+    _check(lib().nlg_decode_attn_paged_q8(q.ptr, kpool.ptr, vpool.ptr, fmt, lens.ptr, table.ptr, npool, out.ptr, batch,
+                                          heads, kvheads, head_dim, bs, mbps, _ptr(workspace),
+                                          workspace.nbytes if workspace is not None else 0, stream),
+           "decode_attn_paged_q8")
+
+
+def tree_attn_paged_q8_workspace(batch, tmax, heads, kvheads, head_dim, bs, mbps) -> int:
+    return int(lib().nlg_tree_attn_paged_q8_workspace(batch, tmax, heads, kvheads, head_dim, bs, mbps))
+
+
+def tree_attn_paged_q8(q, kpool, vpool, base, table, npool, out, batch, tmax, heads, kvheads, head_dim, bs, mbps,
+                       workspace, nodes=None, mask=None, fmt=KV_I8, stream=None) -> None:
+    """Attention of a tree of drafted tokens (mask [batch][tmax] uint64) or, without mask, of a causal chunk, over
+    8-bit paged pools; q and out [batch][tmax][heads*head_dim]."""
+    _check(lib().nlg_tree_attn_paged_q8(q.ptr, kpool.ptr, vpool.ptr, fmt, base.ptr, _ptr(nodes), _ptr(mask), table.ptr,
+                                        npool, out.ptr, batch, tmax, heads, kvheads, head_dim, bs, mbps,
+                                        _ptr(workspace), workspace.nbytes if workspace is not None else 0, stream),
+           "tree_attn_paged_q8")
+
+
+def tree_commit_paged_q8(kpool, vpool, base, path, accepted, table, npool, batch, tmax, kvheads, head_dim, bs, mbps,
+                         stream=None) -> None:
+    """The rows of a tree's accepted path moved to positions base, base + 1, ..."""
+    _check(lib().nlg_tree_commit_paged_q8(kpool.ptr, vpool.ptr, base.ptr, path.ptr, accepted.ptr, table.ptr, npool,
+                                          batch, tmax, kvheads, head_dim, bs, mbps, stream), "tree_commit_paged_q8")
+
+
+def cache_read_paged_q8(kpool, vpool, slot, table, npool, k, v, rows, batch, kvheads, head_dim, bs, mbps, seq=None,
+                        fmt=KV_I8, stream=None) -> None:
+    """Cached rows (sequence seq[r], position slot[r]) back as fp16 [rows][kvheads][head_dim]."""
+    _check(lib().nlg_cache_read_paged_q8(kpool.ptr, vpool.ptr, fmt, _ptr(seq), slot.ptr, table.ptr, npool, k.ptr,
+                                         v.ptr, rows, batch, kvheads, head_dim, bs, mbps, stream),
+           "cache_read_paged_q8")
 
 
 def cache_append_ring_f16(src, pos, cache, batch, kvheads, head_dim, nsink, win, stream=None) -> None:

@@ -1,0 +1,252 @@
+"""The 8-bit paged KV cache on the CPU: the addressing and the masks that its
+kernels use (nelisp-gpu_amd/csrc/nlg_kv8.h, compiled here) against their
+definition, for every row and position of small cases; the split of large
+ones; and every refusal, which needs no device."""
+import ctypes
+import os
+import subprocess
+import tempfile
+
+import numpy as np
+import pytest
+
+import kv8_ref as ref
+import nlgpu
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+PROGRAM = r'''
+#include <stdio.h>
+#include <stdlib.h>
+#include <vector>
+#include "nlg_kv8.h"
+static uint64_t seed = 1;
+static uint32_t rnd(uint32_t n) { seed = seed * 6364136223846793005ull + 1442695040888963407ull; return (uint32_t)(seed >> 33) % n; }
+#define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
+// the layout: each byte of a tile once
+static int layout(uint32_t hd) {
+  for (int v = 0; v < 2; v++) {
+    std::vector<int> seen(kv8_tile_bytes(hd));
+    for (uint32_t at = 0; at < 16; at++) {
+      for (uint32_t d = 0; d < hd; d++) seen[v ? kv8_v_byte(at, d) : kv8_k_byte(hd, at, d)]++;
+      for (int i = 0; i < 4; i++) seen[kv8_scale_byte(hd, at) + i]++;
+    }
+    for (int n : seen) CHECK(n == 1);
+  }
+  return 0;
+}
+// one call: what the workgroups and waves attend, by row and position
+static int call(bool tree, bool masked, int32_t at, int32_t nodes, uint32_t tmax, uint32_t grp, uint32_t bs, uint32_t mbps,
+                uint32_t batch, uint32_t kvheads) {
+  const uint32_t cap = bs * mbps, rows = tmax * grp;
+  const Kv8Split s = kv8_split(batch, rows, kvheads, cap);
+  CHECK(s.chunk % (KV8_STEP * KV8_WAVES) == 0 && s.nchunk >= 1 && (uint64_t)s.chunk * s.nchunk >= cap);
+  CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows);
+  CHECK(s.blocks == (uint64_t)batch * kvheads * s.groups * s.nchunk);
+  const Kv8Extent e = kv8_extent(tree, at, nodes, tmax, cap);
+  CHECK(e.end <= cap);
+  std::vector<uint64_t> mask(tmax);
+  for (auto &m : mask) m = (uint64_t)rnd(1u << 31) << 33 ^ (uint64_t)rnd(1u << 31) << 10 ^ rnd(1024);
+  const int64_t nn = !tree ? 1 : nodes < 0 ? 0 : nodes > (int64_t)tmax ? tmax : nodes;
+  CHECK(e.on == (!tree || (at >= 0 && nn > 0)));
+  if (!e.on) return 0;
+  for (uint32_t g = 0; g < s.groups; g++)
+    for (uint32_t r = g * s.rowsper; r < (g + 1) * s.rowsper && r < rows; r++) {
+      const uint32_t node = r / grp;
+      if (node >= nn) continue;
+      std::vector<int> seen(cap + 64);
+      const uint32_t stop = tree && !masked ? kv8_stop(e, (g * s.rowsper + s.rowsper - 1) / grp) : e.end;
+      for (uint32_t c = 0; c < s.nchunk; c++) {
+        const uint32_t c0 = c * s.chunk;
+        if (c0 >= e.end && c) continue;
+        const uint32_t c1 = kv8_chunk_end(c0, stop, s.chunk);
+        for (uint32_t p = c0; p < c1; p += KV8_STEP)
+          for (uint32_t t = 0; t < 4; t++) {
+            const uint32_t q0 = p + t * 16;
+            const bool whole = p + KV8_STEP <= (e.base < stop ? e.base : stop);
+            const uint32_t bits = whole ? 0xffffu
+                                  : tree ? kv8_bits(e, masked, node, masked ? kv8_word(mask[node], e.nodes) : 0, q0)
+                                         : (1u << kv8_left(e, q0)) - 1;
+            CHECK(bits < 65536);
+            for (uint32_t j = 0; j < 16; j++) seen[q0 + j < cap + 63 ? q0 + j : cap + 63] += bits >> j & 1;
+          }
+      }
+      for (uint32_t p = 0; p < cap + 64; p++) {
+        int want;
+        if (p >= cap) want = 0;
+        else if (!tree) want = (int64_t)p <= at;
+        else if ((int64_t)p < at) want = 1;
+        else if ((int64_t)p >= at + nn) want = 0;
+        else if (masked) want = mask[node] >> (p - at) & 1;
+        else want = p - at <= node;
+        CHECK(seen[p] == want);
+      }
+    }
+  return 0;
+}
+int main(void) {
+  if (layout(64) || layout(128)) return 1;
+  // pages: entries outside the pool, positions behind the table
+  const int32_t table[6] = {3, -1, 0, 7, 2147483647, 1};
+  const Kv8Pages g = {table, 7, 3, 2, 5};
+  CHECK(kv8_tile(g, 0, 4, 1) == (3 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 4) == 0);
+  CHECK(kv8_tile(g, 0, 0, 2) == KV8_NONE && kv8_tile(g, 0, 0, 6) == KV8_NONE && kv8_tile(g, 1, 0, 0) == KV8_NONE);
+  CHECK(kv8_tile(g, 1, 0, 3) == KV8_NONE && kv8_tile(g, 1, 4, 5) == (1 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 0xffffffffu) == KV8_NONE);
+  for (int i = 0; i < 400; i++) {
+    const uint32_t bs = 16 * (1 + rnd(4)), mbps = 1 + rnd(20), cap = bs * mbps;
+    const uint32_t grp = 1 + rnd(9), kvh = 1 + rnd(3), batch = 1 + rnd(40);
+    if (call(false, false, (int32_t)rnd(cap + 20) - 2, 1, 1, grp, bs, mbps, batch, kvh)) return 1;
+    const uint32_t tm = 1 + rnd(64), tc = 1 + rnd(90);
+    if (call(true, true, (int32_t)rnd(cap + 4) - 2, (int32_t)rnd(tm + 4) - 1, tm, grp, bs, mbps, batch, kvh)) return 1;
+    if (call(true, false, (int32_t)rnd(cap + 4) - 2, (int32_t)rnd(tc + 4) - 1, tc, grp, bs, mbps, batch, kvh)) return 1;
+  }
+  // extremes
+  if (call(false, false, 2147483647, 1, 1, 1, 16, 1, 1, 1) || call(true, false, 2147483647, 5, 5, 1, 16, 2, 1, 1)) return 1;
+  const Kv8Extent e = kv8_extent(true, 2147483647, 2147483647, 2147483647u, 2147483632u);
+  CHECK(e.end == 2147483632u && e.base == 2147483647u && kv8_left(e, 2147483616u) == 16);
+  for (uint64_t pos : {16ull, 4096ull, 2147483632ull})
+    for (uint32_t batch : {1u, 65535u})
+      for (uint32_t rows : {1u, 16u, 17u, 2147483647u}) {
+        const Kv8Split s = kv8_split(batch, rows, 8, pos);
+        CHECK((uint64_t)s.chunk * s.nchunk >= pos && (uint64_t)s.chunk * (s.nchunk - 1) < pos);
+        CHECK((uint64_t)s.groups * s.rowsper >= rows);
+      }
+  printf("ok\n");
+  return 0;
+}
+'''
+
+
+def test_addressing_and_masks():
+    with tempfile.TemporaryDirectory() as d:
+        src, exe = os.path.join(d, "t.cpp"), os.path.join(d, "t")
+        with open(src, "w") as f:
+            f.write(PROGRAM)
+        subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=undefined,address",
+                        "-fno-sanitize-recover=all", "-I", os.path.join(ROOT, "nelisp-gpu_amd", "csrc"), src, "-o",
+                        exe], check=True)
+        r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+        assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+def test_reference_formats():
+    """The reference's own quantisation: within half a step of the value, the largest value kept, ties to even."""
+    rng = np.random.default_rng(1)
+    x = rng.standard_normal((64, 128)) * np.exp(rng.uniform(-20, 20, (64, 1)))
+    for fmt in (ref.I8, ref.E4M3):
+        c, s = ref.quantise(x, fmt)
+        y = ref.values(c, fmt) * s[:, None].astype(np.float64)
+        u = np.abs(x / s[:, None].astype(np.float64))
+        step = np.ones_like(u) if fmt == ref.I8 else 2.0 ** np.maximum(np.floor(np.log2(u)) - 3, -9)
+        assert (np.abs(x - y) <= s[:, None].astype(np.float64) * step * 0.5 * (1 + 1e-6)).all()
+        assert np.allclose(np.abs(y).max(axis=1), np.abs(x).max(axis=1), rtol=1e-6)
+    c, s = ref.quantise(np.array([[127.0, 0.5, 1.5, -2.5, 0, -0.5]]), ref.I8)
+    assert s[0] == 1 and c.view(np.int8).tolist() == [[127, 0, 2, -2, 0, 0]]
+    for bad in (np.nan, np.inf, 1e39):
+        c, s = ref.quantise(np.array([[1.0, bad]]), ref.E4M3)
+        assert not c.any() and np.isnan(s[0])
+
+
+def test_pool_bytes():
+    f = nlgpu.kv_q8_pool_bytes
+    assert f(10, 5, 128, 16) == 10 * 5 * 16 * 132 and f(3, 2, 64, 48) == 3 * 2 * 48 * 68
+    assert f(0, 5, 128, 16) == f(4, 0, 128, 16) == f(4, 5, 96, 16) == f(4, 5, 128, 0) == f(4, 5, 128, 24) == 0
+    assert f(1 << 27, 8, 64, 32) == (1 << 27) * 8 * 32 * 68 and f(1 << 30, 4, 64, 16) == 0
+
+
+def test_workspace_bytes():
+    """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
+    w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
+    assert w(1, 20, 5, 128, 16, 16) == 0 and w(1, 20, 5, 128, 16, 17) == 5 * 2 * 4 * 130 * 4
+    assert w(1, 20, 5, 128, 16, 17) == t(1, 1, 20, 5, 128, 16, 17)
+    for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
+                (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
+                (1, 1, 20, 5, 128, 20, 64), (1, 1, 20, 5, 128, 16, 0), (1, 1, 20, 5, 128, 16, 1 << 27),
+                (1, 1 << 31, 20, 5, 128, 16, 64)):
+        assert t(*bad) == 0, bad
+
+
+class At:
+    """A buffer at an address that no call below gets to use."""
+
+    def __init__(self, ptr, nbytes=1 << 40):
+        self.ptr, self.nbytes = ptr, nbytes
+
+
+GOOD = At(1 << 20)
+ODD = At((1 << 20) + 4)
+
+
+def refused(call, kw, words):
+    """The call is refused with these words, before any device is asked for."""
+    with pytest.raises(nlgpu.NlgError) as e:
+        call(**kw)
+    for w in words.split("|"):
+        assert w in str(e.value), (kw, str(e.value))
+
+
+CACHE = dict(kpool=GOOD, vpool=GOOD, table=GOOD, npool=64, batch=2, kvheads=4, head_dim=128, bs=16, mbps=32)
+BAD_CACHE = [(dict(kpool=At(None)), "null"), (dict(vpool=At(None)), "null"), (dict(table=At(None)), "null"),
+             (dict(kpool=ODD), "aligned"), (dict(vpool=ODD), "aligned"), (dict(table=At((1 << 20) + 2)), "aligned"),
+             (dict(head_dim=96), "head_dim"), (dict(kvheads=0), "kvheads"), (dict(bs=0), "block size"),
+             (dict(bs=24), "block size"), (dict(mbps=0), "block"), (dict(mbps=1 << 27), "positions"),
+             (dict(npool=0), "pool"), (dict(npool=1 << 31, kvheads=4), "pool")]
+
+
+@pytest.mark.parametrize("bad,words", BAD_CACHE + [
+    (dict(fmt=2), "format"), (dict(fmt=-1), "format"), (dict(qkv=At(None)), "null"), (dict(co=At(None)), "null"),
+    (dict(si=At(None)), "null"), (dict(slot=At(None)), "null"), (dict(q=At(None)), "null"), (dict(heads=0), "heads"),
+    (dict(batch=0), "batch"), (dict(trows=0), "trows"), (dict(qkv=At((1 << 20) + 4)), "aligned"),
+    (dict(q=At((1 << 20) + 4)), "aligned"), (dict(rows=3, seq=None), "sequence"),
+    (dict(rows=1 << 30), "too many"), (dict(heads=0xffffffff), "too many")])
+def test_append_refuses(bad, words):
+    kw = dict(CACHE, qkv=GOOD, qgain=None, kgain=None, eps=1e-6, co=GOOD, si=GOOD, trows=10, slot=GOOD, q=GOOD, rows=2,
+              heads=8, seq=GOOD)
+    refused(nlgpu.qk_norm_rope_append_paged_q8, dict(kw, **bad), words)
+
+
+ATTN = dict(CACHE, q=GOOD, out=GOOD, heads=8, workspace=GOOD)
+BAD_ATTN = BAD_CACHE + [
+    (dict(fmt=2), "format"), (dict(q=At(None)), "null"), (dict(out=At(None)), "null"), (dict(heads=9), "heads"),
+    (dict(heads=0), "heads"), (dict(q=ODD), "aligned"), (dict(out=ODD), "aligned"), (dict(workspace=ODD), "aligned"),
+    (dict(workspace=None), "workspace"), (dict(workspace=At(1 << 20, 100)), "workspace"),
+    (dict(batch=1 << 28), "too many")]
+
+
+@pytest.mark.parametrize("bad,words", BAD_ATTN + [(dict(lens=At(None)), "null")])
+def test_decode_refuses(bad, words):
+    refused(nlgpu.decode_attn_paged_q8, dict(ATTN, lens=GOOD, **{}) | bad, words)
+
+
+@pytest.mark.parametrize("bad,words", BAD_ATTN + [
+    (dict(base=At(None)), "null"), (dict(mask=GOOD, tmax=65), "mask"), (dict(mask=ODD), "aligned"),
+    (dict(tmax=1 << 31), "queries"), (dict(tmax=1 << 26), "too many")])
+def test_tree_refuses(bad, words):
+    refused(nlgpu.tree_attn_paged_q8, dict(ATTN, base=GOOD, tmax=8) | bad, words)
+
+
+@pytest.mark.parametrize("bad,words", BAD_CACHE + [
+    (dict(base=At(None)), "null"), (dict(path=At(None)), "null"), (dict(accepted=At(None)), "null"),
+    (dict(tmax=65), "at most"), (dict(batch=65536), "batch")])
+def test_commit_refuses(bad, words):
+    refused(nlgpu.tree_commit_paged_q8, dict(CACHE, base=GOOD, path=GOOD, accepted=GOOD, tmax=8) | bad, words)
+
+
+@pytest.mark.parametrize("bad,words", BAD_CACHE + [
+    (dict(fmt=2), "format"), (dict(slot=At(None)), "null"), (dict(k=At(None)), "null"), (dict(v=At(None)), "null"),
+    (dict(k=ODD), "aligned"), (dict(v=ODD), "aligned"), (dict(batch=0), "batch"), (dict(rows=3, seq=None), "sequence"),
+    (dict(rows=0xffffffff), "too many")])
+def test_read_refuses(bad, words):
+    refused(nlgpu.cache_read_paged_q8, dict(CACHE, slot=GOOD, k=GOOD, v=GOOD, rows=2, seq=GOOD) | bad, words)
+
+
+def test_nothing_to_do_is_no_error():
+    """No rows or sequences: nothing is checked further, nothing runs."""
+    n = At(None)
+    kw = dict(kpool=n, vpool=n, table=n, npool=0, kvheads=0, head_dim=0, bs=0, mbps=0)
+    nlgpu.qk_norm_rope_append_paged_q8(qkv=n, qgain=None, kgain=None, eps=0.0, co=n, si=n, trows=0, slot=n, q=n, rows=0,
+                                       heads=0, batch=0, **kw)
+    nlgpu.decode_attn_paged_q8(q=n, lens=n, out=n, heads=0, workspace=None, batch=0, **kw)
+    nlgpu.tree_attn_paged_q8(q=n, base=n, out=n, heads=0, workspace=None, batch=4, tmax=0, **kw)
+    nlgpu.tree_commit_paged_q8(base=n, path=n, accepted=n, batch=0, tmax=4, **kw)
+    nlgpu.cache_read_paged_q8(slot=n, k=n, v=n, rows=0, batch=0, **kw)
