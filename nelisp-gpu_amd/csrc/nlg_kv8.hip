@@ -39,8 +39,8 @@ struct AppendArgs {
   uint8_t *kpool, *vpool;
   Kv8Pages pg;
   double eps;
-  uint64_t units;
-  uint32_t batch, heads, trows;
+  uint64_t rows;
+  uint32_t batch, heads, trows, qblocks;
 };
 
 template <int CTRL>
@@ -50,38 +50,21 @@ __device__ __forceinline__ double dpp_f64(double v) {
   const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-template <int OFF>
-__device__ __forceinline__ double pair_sum_f64(double v) {
-  const uint64_t u = __builtin_bit_cast(uint64_t, v);
-  const float2 lo = nlg_pair_f32<OFF>(__uint_as_float((uint32_t)u));
-  const float2 hi = nlg_pair_f32<OFF>(__uint_as_float((uint32_t)(u >> 32)));
-  const double a = __builtin_bit_cast(double, (uint64_t)__float_as_uint(hi.x) << 32 | __float_as_uint(lo.x));
-  const double b = __builtin_bit_cast(double, (uint64_t)__float_as_uint(hi.y) << 32 | __float_as_uint(lo.y));
-  return a + b;
-}
-// Over aligned groups of L lanes (32 or 64), in every lane.
+// Over aligned groups of L lanes (8 or 16), in every lane.
 template <int L>
 __device__ __forceinline__ double lanes_sum_f64(double v) {
   v = v + dpp_f64<0xB1>(v);   // quad_perm [1,0,3,2]
   v = v + dpp_f64<0x4E>(v);   // quad_perm [2,3,0,1]
   v = v + dpp_f64<0x141>(v);  // row_half_mirror
-  v = v + dpp_f64<0x140>(v);  // row_mirror
-  v = pair_sum_f64<16>(v);
-  if (L == 64) v = pair_sum_f64<32>(v);
+  if (L == 16) v = v + dpp_f64<0x140>(v);  // row_mirror
   return v;
 }
 template <int L>
-__device__ __forceinline__ float lanes_max_f32(float v) {
-  v = fmaxf(v, __int_as_float(nlg_dpp<0xB1>(__float_as_int(v))));
-  v = fmaxf(v, __int_as_float(nlg_dpp<0x4E>(__float_as_int(v))));
-  v = fmaxf(v, __int_as_float(nlg_dpp<0x141>(__float_as_int(v))));
-  v = fmaxf(v, __int_as_float(nlg_dpp<0x140>(__float_as_int(v))));
-  float2 r = nlg_pair_f32<16>(v);
-  v = fmaxf(r.x, r.y);
-  if (L == 64) {
-    r = nlg_pair_f32<32>(v);
-    v = fmaxf(r.x, r.y);
-  }
+__device__ __forceinline__ uint32_t lanes_max_u32(uint32_t v) {
+  v = max(v, nlg_qperm<0xB1>(v));
+  v = max(v, nlg_qperm<0x4E>(v));
+  v = max(v, nlg_qperm<0x141>(v));
+  if (L == 16) v = max(v, nlg_qperm<0x140>(v));
   return v;
 }
 
@@ -104,85 +87,149 @@ __device__ __forceinline__ uint32_t kv8_code2(double a, double b) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32((float)a, (float)b, 0, false) & 0xffffu;
 }
 
-// A lane holds one rotation pair of a head row: (2m, 2m + 1), or (m, m + hd/2)
-// with HALF.  All in 64 bits, at no cost (the rows' bytes bound it): a code then
-// depends on the inputs alone and not on the order of a sum, so a prefix cached
-// twice holds the same bytes.
+// A row's eight values of this lane as codes (two words) and the row's scale; L
+// lanes hold the row.
+template <int FMT, int L>
+__device__ __forceinline__ float kv8_quantise(const double *y, uint2 &code) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 8; i++) top = max(top, __float_as_uint((float)y[i]) & 0x7fffffffu);
+  top = lanes_max_u32<L>(top);  // magnitudes in their bits' order, infinities and NaN above all
+  const float scale = (float)((double)__uint_as_float(top) / (FMT == NLG_KV_I8 ? 127.0 : 448.0));
+  code = make_uint2(0, 0);
+  // a row with a value that is not finite: no codes, a scale that says so
+  if (top >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  if (scale > 0.0f) {
+    const double s = scale, rs = 1.0 / s;
+    double r[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = kv8_round<FMT>(y[i], s, rs);
+    code.x = kv8_code2<FMT>(r[0], r[1]) | kv8_code2<FMT>(r[2], r[3]) << 16;
+    code.y = kv8_code2<FMT>(r[4], r[5]) | kv8_code2<FMT>(r[6], r[7]) << 16;
+  }
+  return scale;
+}
+__device__ __forceinline__ void load8(const float *p, const float *q, double *y) {
+  const float4 a = *(const float4 *)p, b = *(const float4 *)q;
+  y[0] = a.x; y[1] = a.y; y[2] = a.z; y[3] = a.w;
+  y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
+}
+
+// All in 64 bits: a code then depends on the inputs alone and not on the order
+// of a sum, so a prefix cached twice holds the same bytes.  They cost little
+// only where lanes share a row's root and quotients: a head row is on HD / 8
+// lanes, eight values (four rotation pairs) each.  The first qblocks workgroups
+// take the q and k heads; the others V, a wave sixteen rows of one head, whose
+// codes pass through LDS: a position's bytes of a tile lie sixteen apart, and a
+// store then runs over 64 dimensions (8 lines) instead of one byte a line.
 template <int HD, int FMT, bool HALF>
 __global__ __launch_bounds__(256) void k_append_q8(AppendArgs a) {
-  constexpr int L = HD / 2;
-  const uint64_t unit = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const int m = threadIdx.x % L;
+  constexpr int L = HD / 8, RP = 64 / L;  // lanes a row, rows at once
+  constexpr int VS = 20;                  // bytes between a dimension's codes in LDS: two lanes a bank
+  __shared__ __align__(16) uint8_t s_v[4][HD * VS];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, m = lane % L;
   const uint32_t per = a.heads + 2 * a.pg.kvheads;
-  const bool live = unit < a.units;
-  const uint64_t u = live ? unit : a.units - 1;
-  const uint64_t row = u / per;
-  const uint32_t h = (uint32_t)(u % per);
-  const float *x = a.qkv + u * HD;
-  const int d0 = HALF ? m : 2 * m, d1 = HALF ? m + L : 2 * m + 1;
-  double y0, y1;
-  if (HALF) {
-    y0 = x[d0]; y1 = x[d1];
-  } else {
-    const float2 t = *(const float2 *)(x + d0);
-    y0 = t.x; y1 = t.y;
-  }
-  const int32_t slot = a.slot[row];
-  const bool isv = h >= a.heads + a.pg.kvheads;
-  const float *gain = h < a.heads ? a.qgain : a.kgain;
-  const double ss = lanes_sum_f64<L>(fma(y0, y0, y1 * y1));
-  if (!isv) {
-    if (gain) {
-      const double inv = 1.0 / sqrt(ss / HD + a.eps);
-      y0 = y0 * inv * gain[d0];
-      y1 = y1 * inv * gain[d1];
+  if (blockIdx.x >= a.qblocks) {
+    const uint64_t w = (uint64_t)(blockIdx.x - a.qblocks) * 4 + wv;
+    const uint32_t h = (uint32_t)(w % a.pg.kvheads);
+    const uint64_t r0 = w / a.pg.kvheads * 16;
+    if (r0 >= a.rows) return;
+    const int n = a.rows - r0 < 16 ? (int)(a.rows - r0) : 16;
+    float4 x[16 / RP][2];
+#pragma unroll
+    for (int p = 0; p < 16 / RP; p++) {
+      const int i = p * RP + lane / L;
+      const float *src = a.qkv + ((r0 + (i < n ? i : 0)) * per + a.heads + a.pg.kvheads + h) * HD + m * 8;
+      x[p][0] = *(const float4 *)src;
+      x[p][1] = *(const float4 *)(src + 4);
     }
-    const int32_t rp = a.rpos ? a.rpos[row] : slot;
-    const bool in = rp >= 0 && (uint32_t)rp < a.trows;
-    const size_t at = (size_t)(in ? rp : 0) * L + m;
-    const double c = in ? a.co[at] : 0.0f, s = in ? a.si[at] : 0.0f;
-    const double t = y0 * c - y1 * s;
-    y1 = y0 * s + y1 * c;
-    y0 = t;
-  }
-  const float f0 = (float)y0, f1 = (float)y1;
-  if (h < a.heads) {
-    if (!live) return;
-    float *q = a.q + (row * a.heads + h) * HD;
-    if (HALF) {
-      q[d0] = f0; q[d1] = f1;
-    } else {
-      *(float2 *)(q + d0) = make_float2(f0, f1);
+    // where row r0 + lane goes
+    uint32_t tile = KV8_NONE, at = 0;
+    if (lane < n) {
+      const int32_t slot = a.slot[r0 + lane];
+      const uint32_t b = a.seq ? (uint32_t)a.seq[r0 + lane] : (uint32_t)(r0 + lane);
+      if (slot >= 0 && b < a.batch) tile = kv8_tile(a.pg, b, h, (uint32_t)slot / KV8_TILE);
+      at = (uint32_t)slot % KV8_TILE;
+    }
+#pragma unroll
+    for (int p = 0; p < 16 / RP; p++) {
+      const int i = p * RP + lane / L;
+      if (p * RP >= n) break;
+      const double y[8] = {x[p][0].x, x[p][0].y, x[p][0].z, x[p][0].w, x[p][1].x, x[p][1].y, x[p][1].z, x[p][1].w};
+      uint2 code;
+      const float scale = kv8_quantise<FMT, L>(y, code);
+#pragma unroll
+      for (int d = 0; d < 8; d++)
+        s_v[wv][(m * 8 + d) * VS + i] = (uint8_t)((d < 4 ? code.x : code.y) >> (8 * (d & 3)));
+      const uint32_t to = __shfl(tile, i), ta = __shfl(at, i);
+      if (m == 0 && to != KV8_NONE)
+        *(float *)(a.vpool + (size_t)to * kv8_tile_bytes(HD) + kv8_scale_byte(HD, ta)) = scale;
+    }
+    __builtin_amdgcn_wave_barrier();  // (LDS of one wave: its operations keep their order)
+    for (int i = 0; i < n; i++) {
+      const uint32_t to = __builtin_amdgcn_readlane(tile, i), ta = __builtin_amdgcn_readlane(at, i);
+      if (to == KV8_NONE) continue;
+      uint8_t *t = a.vpool + (size_t)to * kv8_tile_bytes(HD);
+#pragma unroll
+      for (int d = 0; d < HD; d += 64) t[kv8_v_byte(ta, d + lane)] = s_v[wv][(d + lane) * VS + i];
     }
     return;
   }
-  const float top = lanes_max_f32<L>(fmaxf(fabsf(f0), fabsf(f1)));
-  // a row with a value that is not finite: no codes, a scale that says so
-  const bool odd0 = !(fabsf(f0) <= 3.4028234663852886e38f) || !(fabsf(f1) <= 3.4028234663852886e38f);
-  const uint64_t odds = __ballot(odd0);
-  const bool odd = L == 64 ? odds != 0 : (uint32_t)(odds >> (threadIdx.x & 32)) != 0;
-  float scale = (float)((double)top / (FMT == NLG_KV_I8 ? 127.0 : 448.0));
-  uint32_t code = 0;
-  if (!odd && scale > 0.0f) {
-    const double s = scale, rs = 1.0 / s;
-    code = kv8_code2<FMT>(kv8_round<FMT>(y0, s, rs), kv8_round<FMT>(y1, s, rs));
+  const uint32_t perq = a.heads + a.pg.kvheads;
+  const uint64_t unit = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
+  if (unit >= a.rows * perq) return;
+  const uint64_t row = unit / perq;
+  const uint32_t h = (uint32_t)(unit % perq);
+  // this lane's dimensions: 8 m .., or with HALF 4 m .. and HD / 2 + 4 m ..
+  const int d0 = HALF ? 4 * m : 8 * m, d1 = HALF ? HD / 2 + 4 * m : 8 * m + 4;
+  const float *x = a.qkv + (row * per + h) * HD;
+  double y[8];
+  load8(x + d0, x + d1, y);
+  const int32_t slot = a.slot[row];
+  const int32_t rp = a.rpos ? a.rpos[row] : slot;
+  const bool in = rp >= 0 && (uint32_t)rp < a.trows;
+  const size_t trow = (size_t)(in ? rp : 0) * (HD / 2) + 4 * m;
+  const float4 c4 = *(const float4 *)(a.co + trow), s4 = *(const float4 *)(a.si + trow);
+  // (looked up ahead of the arithmetic, which hides it)
+  uint32_t tile = KV8_NONE;
+  if (h >= a.heads) {
+    const uint32_t b = a.seq ? (uint32_t)a.seq[row] : (uint32_t)row;
+    if (slot >= 0 && b < a.batch) tile = kv8_tile(a.pg, b, h - a.heads, (uint32_t)slot / KV8_TILE);
   }
-  if (odd) scale = __uint_as_float(0x7fc00000u);
-  const uint32_t b = a.seq ? (uint32_t)a.seq[row] : (uint32_t)row;
-  if (!live || slot < 0 || b >= a.batch) return;
-  const uint32_t kh = h - a.heads - (isv ? a.pg.kvheads : 0);
-  const uint32_t tile = kv8_tile(a.pg, b, kh, (uint32_t)slot / KV8_TILE), at = (uint32_t)slot % KV8_TILE;
+  const float *gain = h < a.heads ? a.qgain : a.kgain;
+  if (gain) {
+    double ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) ss = fma(y[i], y[i], ss);
+    ss = lanes_sum_f64<L>(ss);
+    const double inv = 1.0 / sqrt(ss / HD + a.eps);
+    double g[8];
+    load8(gain + d0, gain + d1, g);
+#pragma unroll
+    for (int i = 0; i < 8; i++) y[i] = y[i] * inv * g[i];
+  }
+  const float cf[4] = {c4.x, c4.y, c4.z, c4.w}, sf[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const double c = in ? cf[i] : 0.0f, s = in ? sf[i] : 0.0f;
+    double &p = y[HALF ? i : 2 * i], &r = y[HALF ? i + 4 : 2 * i + 1];
+    const double t = p * c - r * s;
+    r = p * s + r * c;
+    p = t;
+  }
+  if (h < a.heads) {
+    float *q = a.q + (row * a.heads + h) * HD;
+    *(float4 *)(q + d0) = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
+    *(float4 *)(q + d1) = make_float4((float)y[4], (float)y[5], (float)y[6], (float)y[7]);
+    return;
+  }
+  uint2 code;
+  const float scale = kv8_quantise<FMT, L>(y, code);
   if (tile == KV8_NONE) return;
-  uint8_t *t = (isv ? a.vpool : a.kpool) + (size_t)tile * kv8_tile_bytes(HD);
-  if (isv) {
-    t[kv8_v_byte(at, d0)] = (uint8_t)code;
-    t[kv8_v_byte(at, d1)] = (uint8_t)(code >> 8);
-  } else if (HALF) {
-    t[kv8_k_byte(HD, at, d0)] = (uint8_t)code;
-    t[kv8_k_byte(HD, at, d1)] = (uint8_t)(code >> 8);
-  } else {
-    *(uint16_t *)(t + kv8_k_byte(HD, at, d0)) = (uint16_t)code;
-  }
+  const uint32_t at = (uint32_t)slot % KV8_TILE;
+  uint8_t *t = a.kpool + (size_t)tile * kv8_tile_bytes(HD);
+  *(uint32_t *)(t + kv8_k_byte(HD, at, d0)) = code.x;
+  *(uint32_t *)(t + kv8_k_byte(HD, at, d1)) = code.y;
   if (m == 0) *(float *)(t + kv8_scale_byte(HD, at)) = scale;
 }
 
@@ -333,7 +380,7 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w,
   // then use the type's whole range
   float vtop = fabsf(vs);
   vtop = vtop <= 3.4028234663852886e38f ? vtop : 0.0f;
-  vtop = lanes_max_f32<64>(vtop);
+  vtop = nlg_wave_max_f32(vtop);
   float vresc = 1.0f;
   if (vtop > w.vref) {  // the same in every lane
     const int e = __builtin_amdgcn_frexp_expf(vtop);
@@ -629,41 +676,114 @@ struct ReadArgs {
   const int32_t *seq, *slot;
   Kv8Pages pg;
   uint16_t *k, *v;  // [rows][kvheads][hd]
-  uint64_t units;
+  uint64_t rows;
   uint32_t batch;
 };
-template <int FMT>
-__device__ __forceinline__ float2 kv8_value2(uint32_t w) {
-  if (FMT == NLG_KV_I8) return make_float2((float)(int8_t)(w & 0xff), (float)(int8_t)(w >> 8 & 0xff));
-  const half2v t = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
-  return make_float2((float)t[0], (float)t[1]);
-}
-// A lane: two neighbouring dimensions of one row and kv head, K and V.
-template <int HD, int FMT>
-__global__ __launch_bounds__(256) void k_read_q8(ReadArgs a) {
-  constexpr int L = HD / 2;
-  const uint64_t u = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / L;
-  const uint32_t d = threadIdx.x % L * 2;
-  if (u >= a.units) return;
-  const uint64_t row = u / a.pg.kvheads;
-  const uint32_t h = (uint32_t)(u % a.pg.kvheads);
-  const int32_t slot = a.slot[row];
-  const uint32_t b = a.seq ? (uint32_t)a.seq[row] : (uint32_t)row;
-  const uint32_t tile = slot < 0 || b >= a.batch ? KV8_NONE : kv8_tile(a.pg, b, h, (uint32_t)slot / KV8_TILE);
-  float2 k = make_float2(0.0f, 0.0f), v = k;
-  if (tile != KV8_NONE) {
-    const uint32_t at = (uint32_t)slot % KV8_TILE;
-    const uint8_t *kt = a.kpool + (size_t)tile * kv8_tile_bytes(HD), *vt = a.vpool + (size_t)tile * kv8_tile_bytes(HD);
-    const float ks = *(const float *)(kt + kv8_scale_byte(HD, at)), vs = *(const float *)(vt + kv8_scale_byte(HD, at));
-    k = kv8_value2<FMT>(*(const uint16_t *)(kt + kv8_k_byte(HD, at, d)));
-    v = kv8_value2<FMT>(vt[kv8_v_byte(at, d)] | (uint32_t)vt[kv8_v_byte(at, d + 1)] << 8);
-    k.x *= ks; k.y *= ks; v.x *= vs; v.y *= vs;
-    // the products are f32 numbers: not folded with their rounding to fp16 into one
-    asm("" : "+v"(k.x), "+v"(k.y), "+v"(v.x), "+v"(v.y));
+// Codes 2 i and 2 i + 1 of a word times their scale, rounded to fp16.  The
+// products are f32 numbers: not folded with their rounding into one.
+template <int FMT, int I>
+__device__ __forceinline__ half2v kv8_value2(uint32_t w, float scale) {
+  float x, y;
+  if (FMT == NLG_KV_I8) {
+    x = (float)(int8_t)(w >> 16 * I);
+    y = (float)(int8_t)(w >> (16 * I + 8));
+  } else {
+    const half2v t = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, I != 0);
+    x = (float)t[0];
+    y = (float)t[1];
   }
-  const half2v kh = {(_Float16)k.x, (_Float16)k.y}, vh = {(_Float16)v.x, (_Float16)v.y};
-  *(half2v *)(a.k + u * HD + d) = kh;
-  *(half2v *)(a.v + u * HD + d) = vh;
+  x = x * scale;
+  y = y * scale;
+  asm("" : "+v"(x), "+v"(y));
+  const float2v f = {x, y};
+  return __builtin_convertvector(f, half2v);
+}
+// Sixteen positions of two dimensions (held in 64-bit values: a choice between
+// words of a struct would put it in memory).
+struct Columns {
+  uint64_t a0, a1, b0, b1;
+};
+// Byte `at` (the same for the wave) of sixteen.
+__device__ __forceinline__ uint32_t kv8_pick(uint64_t lo, uint64_t hi, uint32_t at) {
+  return (uint32_t)((at < 8 ? lo : hi) >> 8 * (at & 7)) & 0xffu;
+}
+// A wave reads N rows of one kv head: sixteen, or four where there are too few
+// rows to fill the card.  K: HD / 8 lanes a row.  V: a lane holds the sixteen
+// positions of two (HD 128) or one dimensions of a tile, and gives each of its
+// rows that lie there theirs; of rows that follow each other in a sequence the
+// first's and the last's tiles are all there are, and both are loaded ahead.
+template <int HD, int FMT, int N>
+__global__ __launch_bounds__(256) void k_read_q8(ReadArgs a) {
+  constexpr int L = HD / 8, RP = 64 / L < N ? 64 / L : N, DV = HD / 64;
+  const int lane = threadIdx.x & 63, m = lane % L;
+  const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t h = (uint32_t)(w % a.pg.kvheads);
+  const uint64_t r0 = w / a.pg.kvheads * N;
+  if (r0 >= a.rows) return;
+  const int n = a.rows - r0 < N ? (int)(a.rows - r0) : N;
+  uint32_t tile = KV8_NONE, at = 0;
+  if (lane < n) {
+    const int32_t slot = a.slot[r0 + lane];
+    const uint32_t b = a.seq ? (uint32_t)a.seq[r0 + lane] : (uint32_t)(r0 + lane);
+    if (slot >= 0 && b < a.batch) tile = kv8_tile(a.pg, b, h, (uint32_t)slot / KV8_TILE);
+    at = (uint32_t)slot % KV8_TILE;
+  }
+  auto columns = [&](uint32_t from) {
+    const uint8_t *t = a.vpool + (size_t)(from == KV8_NONE ? 0 : from) * kv8_tile_bytes(HD) + lane * DV * KV8_TILE;
+    const uint4 x = *(const uint4 *)t, y = DV == 2 ? *(const uint4 *)(t + KV8_TILE) : x;
+    return Columns{(uint64_t)x.y << 32 | x.x, (uint64_t)x.w << 32 | x.z, (uint64_t)y.y << 32 | y.x,
+                   (uint64_t)y.w << 32 | y.z};
+  };
+  const uint32_t last = __builtin_amdgcn_readlane(tile, n - 1);
+  uint32_t held = __builtin_amdgcn_readlane(tile, 0);
+  Columns c = columns(held);
+  const Columns cl = columns(last);
+  // row r0 + lane's scale of V
+  const float vscale =
+      tile == KV8_NONE ? 0.0f : *(const float *)(a.vpool + (size_t)tile * kv8_tile_bytes(HD) + kv8_scale_byte(HD, at));
+  uint2 k[N / RP];
+  float ks[N / RP];
+#pragma unroll
+  for (int p = 0; p < N / RP; p++) {
+    const int i = p * RP + lane / L;
+    const uint32_t from = __shfl(tile, i), fa = __shfl(at, i);
+    k[p] = make_uint2(0, 0);
+    ks[p] = 0.0f;
+    if (from != KV8_NONE) {
+      const uint8_t *t = a.kpool + (size_t)from * kv8_tile_bytes(HD);
+      k[p] = *(const uint2 *)(t + kv8_k_byte(HD, fa, m * 8));
+      ks[p] = *(const float *)(t + kv8_scale_byte(HD, fa));
+    }
+  }
+  for (int i = 0; i < n; i++) {
+    const uint32_t from = __builtin_amdgcn_readlane(tile, i), fa = __builtin_amdgcn_readlane(at, i);
+    if (from != held) {
+      held = from;
+      if (from == last) c = cl;
+      else c = columns(from);
+    }
+    const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(vscale), i));
+    const uint64_t o = ((r0 + i) * a.pg.kvheads + h) * HD + lane * DV;
+    uint32_t pair = kv8_pick(c.a0, c.a1, fa) | (DV == 2 ? kv8_pick(c.b0, c.b1, fa) << 8 : 0u);
+    if (from == KV8_NONE) pair = 0;
+    const half2v v = kv8_value2<FMT, 0>(pair, s);
+    if (DV == 2) *(half2v *)(a.v + o) = v;
+    else *(_Float16 *)(a.v + o) = v[0];
+  }
+#pragma unroll
+  for (int p = 0; p < N / RP; p++) {
+    const int i = p * RP + lane / L;
+    if (i >= n) continue;
+    union {
+      half2v h[4];
+      uint4 u;
+    } o;
+    o.h[0] = kv8_value2<FMT, 0>(k[p].x, ks[p]);
+    o.h[1] = kv8_value2<FMT, 1>(k[p].x, ks[p]);
+    o.h[2] = kv8_value2<FMT, 0>(k[p].y, ks[p]);
+    o.h[3] = kv8_value2<FMT, 1>(k[p].y, ks[p]);
+    *(uint4 *)(a.k + ((r0 + i) * a.pg.kvheads + h) * HD + m * 8) = o.u;
+  }
 }
 
 // ------------------------------------------------------------------ host side
@@ -707,16 +827,20 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   if (kv8_check(what, kpool, vpool, table, npool, fmt, batch, kvheads, head_dim, bs, mbps, a.pg)) return NLG_ERR;
   if (!qkv || !rope_cos || !rope_sin || !slot || !q) return nlg_fail("%s: null pointer", what);
   if (!heads || !batch || !trows) return nlg_fail("%s: heads, batch and trows must be nonzero", what);
-  if (((uintptr_t)qkv & 7) || ((uintptr_t)q & 7)) return nlg_fail("%s: qkv and q must be 8-byte aligned", what);
+  if (((uintptr_t)qkv & 15) || ((uintptr_t)q & 15) || ((uintptr_t)rope_cos & 15) || ((uintptr_t)rope_sin & 15) ||
+      ((uintptr_t)qgain & 15) || ((uintptr_t)kgain & 15))
+    return nlg_fail("%s: qkv, q, gains and rotation tables must be 16-byte aligned", what);
   if (!seq && rows > batch) return nlg_fail("%s: %u rows without a sequence each, batch %u", what, rows, batch);
-  const uint64_t per = (uint64_t)heads + 2ull * kvheads, units = rows * per;
-  if (per > 0xffffffffull || !nlg_fits((units * (head_dim / 2) + 255) / 256, 256))
+  const uint64_t per = (uint64_t)heads + 2ull * kvheads;
+  const uint64_t qb = ((uint64_t)rows * (heads + (uint64_t)kvheads) * (head_dim / 8) + 255) / 256;
+  const uint64_t vb = (((uint64_t)rows + 15) / 16 * kvheads + 3) / 4;
+  if (per > 0xffffffffull || !nlg_fits(qb + vb, 256))
     return nlg_fail("%s: too many rows and heads (%u x %llu) for one launch", what, rows, (unsigned long long)per);
   KV8_SCOPE(what);
   a.qkv = qkv; a.qgain = qgain; a.kgain = kgain; a.co = rope_cos; a.si = rope_sin;
   a.seq = seq; a.slot = slot; a.rpos = rpos; a.q = q; a.kpool = kpool; a.vpool = vpool;
-  a.eps = eps; a.units = units; a.batch = batch; a.heads = heads; a.trows = trows;
-  const dim3 grid((uint32_t)((units * (head_dim / 2) + 255) / 256)), blk(256);
+  a.eps = eps; a.rows = rows; a.batch = batch; a.heads = heads; a.trows = trows; a.qblocks = (uint32_t)qb;
+  const dim3 grid((uint32_t)(qb + vb)), blk(256);
   hipStream_t st = nlg_stream(stream);
 #define GO(HD, F)                                                                          \
   do {                                                                                     \
@@ -864,19 +988,24 @@ extern "C" int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpoo
   if (!batch) return nlg_fail("%s: batch must be nonzero", what);
   if (((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return nlg_fail("%s: k and v must be 16-byte aligned", what);
   if (!seq && rows > batch) return nlg_fail("%s: %u rows without a sequence each, batch %u", what, rows, batch);
-  const uint64_t units = (uint64_t)rows * kvheads;
-  if (!nlg_fits((units * (head_dim / 2) + 255) / 256, 256)) return nlg_fail("%s: too many rows for one launch", what);
+  const bool few = (uint64_t)rows * kvheads < 16384;  // (2,000 rows of 8 heads of 128: 7.9 us, 8.1 in sixteens; 480: 4.1, 6.7; 16,000: 48, 24)
+  const uint64_t per = few ? 1 : 16, blocks = (((uint64_t)rows + per - 1) / per * kvheads + 3) / 4;
+  if (!nlg_fits(blocks, 256)) return nlg_fail("%s: too many rows for one launch", what);
   KV8_SCOPE(what);
-  a.kpool = kpool; a.vpool = vpool; a.seq = seq; a.slot = slot; a.k = k; a.v = v; a.units = units; a.batch = batch;
-  const dim3 grid((uint32_t)((units * (head_dim / 2) + 255) / 256)), blk(256);
+  a.kpool = kpool; a.vpool = vpool; a.seq = seq; a.slot = slot; a.k = k; a.v = v; a.rows = rows; a.batch = batch;
+  const dim3 grid((uint32_t)blocks), blk(256);
   hipStream_t st = nlg_stream(stream);
+#define GO(HD, F)                                                                     \
+  do {                                                                                \
+    if (few) hipLaunchKernelGGL((k_read_q8<HD, F, 1>), grid, blk, 0, st, a);          \
+    else hipLaunchKernelGGL((k_read_q8<HD, F, 16>), grid, blk, 0, st, a);             \
+  } while (0)
   if (head_dim == 128) {
-    if (fmt == NLG_KV_I8) hipLaunchKernelGGL((k_read_q8<128, NLG_KV_I8>), grid, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_read_q8<128, NLG_KV_E4M3>), grid, blk, 0, st, a);
+    if (fmt == NLG_KV_I8) GO(128, NLG_KV_I8); else GO(128, NLG_KV_E4M3);
   } else {
-    if (fmt == NLG_KV_I8) hipLaunchKernelGGL((k_read_q8<64, NLG_KV_I8>), grid, blk, 0, st, a);
-    else hipLaunchKernelGGL((k_read_q8<64, NLG_KV_E4M3>), grid, blk, 0, st, a);
+    if (fmt == NLG_KV_I8) GO(64, NLG_KV_I8); else GO(64, NLG_KV_E4M3);
   }
+#undef GO
   NLG_LAUNCHED(what);
   return NLG_OK;
 }
