@@ -79,10 +79,6 @@ NLG_KV8_HD Kv8Extent kv8_extent(bool tree, int32_t at, int32_t nodes, uint32_t t
 NLG_KV8_HD uint32_t kv8_stop(const Kv8Extent &e, uint32_t last) {
   return last < e.nodes && e.base + last + 1 < e.end ? e.base + last + 1 : e.end;
 }
-// Positions c0.. of a chunk, up to:
-NLG_KV8_HD uint32_t kv8_chunk_end(uint32_t c0, uint32_t stop, uint32_t chunk) {
-  return c0 >= stop ? c0 : stop - c0 < chunk ? stop : c0 + chunk;
-}
 // How many of the sixteen positions from p0 on exist.
 NLG_KV8_HD int kv8_left(const Kv8Extent &e, uint32_t p0) { return p0 >= e.end ? 0 : e.end - p0 < 16 ? (int)(e.end - p0) : 16; }
 // Which of the sixteen positions from p0 on a row of `node` attends; word: the
@@ -102,25 +98,48 @@ NLG_KV8_HD uint32_t kv8_bits(const Kv8Extent &e, bool masked, uint32_t node, uin
 }
 NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 ? mask & ((1ull << nodes) - 1) : mask; }
 
-// How an attention call is laid over workgroups: rows (queries x query heads
-// of a kv head) in groups of `rowsper`, positions in `nchunk` chunks of `chunk`.
+// How an attention call is laid over workgroups.  Rows (queries x query heads
+// of a kv head) come in groups of `rowsper`; up to 32 of them a workgroup's
+// waves share (they split the positions), from 33 on each wave has its own
+// (`wide`: they share K and V).  Positions are split by the lengths that the
+// kernel finds on the device: of all sequences' steps (64 positions) a chunk
+// takes 1 / want, at least `least`, in multiples of `unit`; a sequence's chunks
+// are of one size.  want fills the card once (two workgroups a CU), so there
+// are at most `slots` = want + batch chunks for each kv head and group.
 struct Kv8Split {
-  uint32_t rowsper, groups, chunk, nchunk;
+  uint32_t rowsper, groups, want, least, unit;
+  uint64_t slots;
+  bool wide, one;   // one: no sequence can have two chunks
   uint64_t blocks;  // workgroups
 };
 inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint64_t positions) {
   Kv8Split s;
-  s.rowsper = rows > 16 ? 32 : 16;
+  s.wide = rows > 32;
+  s.rowsper = rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
   s.groups = (uint32_t)(((uint64_t)rows + s.rowsper - 1) / s.rowsper);
-  const uint64_t units = (uint64_t)batch * kvheads * s.groups, per = KV8_STEP * KV8_WAVES;
-  const uint64_t most = (positions + per - 1) / per;
-  uint64_t want = (2048 + units - 1) / units;
-  if (want > most) want = most;
-  if (!want) want = 1;
-  const uint64_t steps = (most + want - 1) / want;
-  s.chunk = (uint32_t)(steps * per);
-  s.nchunk = (uint32_t)((most + steps - 1) / steps);
-  if (!s.nchunk) s.nchunk = 1;
-  s.blocks = units * s.nchunk;
+  s.unit = s.wide ? 1 : KV8_WAVES;
+  s.least = 4;
+  const uint64_t units = (uint64_t)kvheads * s.groups, most = (positions + KV8_STEP - 1) / KV8_STEP;
+  const uint64_t want = 512 / units ? 512 / units : 1, all = batch * ((most + s.least - 1) / s.least);
+  s.want = (uint32_t)want;
+  s.slots = want + batch < all ? want + batch : all;
+  s.one = most <= s.least;
+  // (a multiple of eight of (slot, kv head)s: the groups of one lie on one XCD)
+  s.blocks = (s.slots * kvheads + 7) / 8 * 8 * s.groups;
   return s;
+}
+// Steps of a sequence; of a chunk, with `total` steps in all sequences; and a
+// sequence's chunks, each of kv8_share steps (the last what is left).
+NLG_KV8_HD uint32_t kv8_steps(const Kv8Extent &e) {
+  return !e.on ? 0u : e.end ? (e.end - 1) / KV8_STEP + 1 : 1u;
+}
+NLG_KV8_HD uint32_t kv8_per(uint64_t total, uint32_t want, uint32_t least, uint32_t unit) {
+  uint64_t per = (total + want - 1) / want;
+  if (per < least) per = least;
+  per = (per + unit - 1) / unit * unit;
+  return per > 0x7fffffffu ? 0x7fffffffu / unit * unit : (uint32_t)per;
+}
+NLG_KV8_HD uint32_t kv8_chunks(uint32_t steps, uint32_t per) { return (steps + per - 1) / per; }
+NLG_KV8_HD uint32_t kv8_share(uint32_t steps, uint32_t chunks, uint32_t unit) {
+  return ((steps + chunks - 1) / chunks + unit - 1) / unit * unit;
 }

@@ -242,9 +242,9 @@ struct Kv8Attn {
   const int32_t *nodes;   // tree: [batch] or null
   const uint64_t *mask;   // tree: [batch][tmax] or null
   Kv8Pages pg;
-  float *out, *pctx, *pmz;  // partials: [batch][kvheads][nchunk][rows][hd], [..][rows][2]
+  float *out, *pctx, *pmz;  // partials: [slots][kvheads][rows][hd], [slots][kvheads][rows][2]
   uint32_t batch, tmax, heads, grp, rows;  // rows = tmax * grp
-  uint32_t groups, chunk, nchunk;
+  uint32_t groups, want, least, unit, slots;  // Kv8Split
   float coef;  // log2(e) / sqrt(hd): scores in base 2
 };
 
@@ -319,6 +319,108 @@ __device__ __forceinline__ float rows_sum(float v) {
   return r.x + r.y;
 }
 
+// The positions of sequence b.
+template <bool TREE>
+__device__ __forceinline__ Kv8Extent kv8_of(const Kv8Attn &a, uint32_t b) {
+  return kv8_extent(TREE, a.base[b], TREE && a.nodes ? a.nodes[b] : (int32_t)a.tmax, a.tmax,
+                    a.pg.mbps * a.pg.bpt * KV8_TILE);
+}
+
+// A wave's view of the split: lanes hold 64 sequences at a time.
+template <bool TREE>
+struct Kv8Plan {
+  uint32_t per;
+  Kv8Extent mine;  // of sequence `lane`
+
+  __device__ __forceinline__ Kv8Extent at(const Kv8Attn &a, uint32_t b0, int lane) const {
+    if (b0 == 0) return mine;
+    return of(a, b0, lane);
+  }
+  static __device__ __forceinline__ Kv8Extent of(const Kv8Attn &a, uint32_t b0, int lane) {
+    Kv8Extent e = kv8_of<TREE>(a, b0 + lane < a.batch ? b0 + lane : a.batch - 1);
+    e.on = e.on && b0 + lane < a.batch;
+    return e;
+  }
+  __device__ __forceinline__ Kv8Plan(const Kv8Attn &a, int lane) {
+    mine = of(a, 0, lane);
+    uint64_t total = kv8_steps(mine);
+    for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += kv8_steps(of(a, b0, lane));
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor((unsigned long long)total, o);
+    per = kv8_per(total, a.want, a.least, a.unit);
+  }
+  // inclusive sums over the lanes
+  static __device__ __forceinline__ uint32_t sums(uint32_t v, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up(v, o);
+      if (lane >= o) v += u;
+    }
+    return v;
+  }
+  // The sequence and chunk of slot x; false: there are fewer.
+  __device__ __forceinline__ bool find(const Kv8Attn &a, uint32_t x, int lane, uint32_t &b, Kv8Extent &e, uint32_t &chunk,
+                                       uint32_t &chunks) const {
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+      const Kv8Extent l = at(a, b0, lane);
+      const uint32_t n = kv8_chunks(kv8_steps(l), per), to = sums(n, lane);
+      const uint64_t past = __ballot(before + to > x);
+      if (past) {
+        const int i = __builtin_ctzll(past);
+        b = b0 + i;
+        chunks = __builtin_amdgcn_readlane(n, i);
+        chunk = x - before - (__builtin_amdgcn_readlane(to, i) - chunks);
+        e.base = __builtin_amdgcn_readlane(l.base, i);
+        e.end = __builtin_amdgcn_readlane(l.end, i);
+        e.nodes = __builtin_amdgcn_readlane(l.nodes, i);
+        e.on = true;
+        return true;
+      }
+      before += __builtin_amdgcn_readlane(to, 63);
+    }
+    return false;
+  }
+  // Sequence b's first slot and its chunks.
+  __device__ __forceinline__ uint32_t first(const Kv8Attn &a, uint32_t b, int lane, uint32_t &chunks) const {
+    uint32_t before = 0;
+    for (uint32_t b0 = 0;; b0 += 64) {
+      const uint32_t n = kv8_chunks(kv8_steps(at(a, b0, lane)), per), to = sums(n, lane);
+      if (b < b0 + 64) {
+        chunks = __builtin_amdgcn_readlane(n, b - b0);
+        return before + __builtin_amdgcn_readlane(to, b - b0) - chunks;
+      }
+      before += __builtin_amdgcn_readlane(to, 63);
+    }
+  }
+};
+
+// What a workgroup does: which rows of which sequence and kv head over which positions.
+struct Kv8Work {
+  uint32_t b, h, row0, c0, c1, slot, chunks;
+  Kv8Extent e;
+  bool masked;
+};
+template <bool TREE>
+__device__ __forceinline__ bool kv8_work(const Kv8Attn &a, uint32_t rowsper, int lane, Kv8Work &w) {
+  const uint32_t u = blockIdx.x / (8 * a.groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % a.groups;
+  w.slot = u / a.pg.kvheads;
+  w.h = u % a.pg.kvheads;
+  if (w.slot >= a.slots) return false;
+  const Kv8Plan<TREE> plan(a, lane);
+  uint32_t chunk;
+  if (!plan.find(a, w.slot, lane, w.b, w.e, chunk, w.chunks)) return false;
+  w.row0 = grp * rowsper;
+  if (w.row0 >= (uint64_t)w.e.nodes * a.grp) return false;
+  w.masked = TREE && a.mask;
+  // a causal group of rows ends at its last node
+  const uint32_t stop = TREE && !w.masked ? kv8_stop(w.e, (w.row0 + rowsper - 1) / a.grp) : w.e.end;
+  const uint32_t share = kv8_share(kv8_steps(w.e), w.chunks, a.unit) * KV8_STEP;
+  w.c0 = chunk * share;
+  w.c1 = w.c0 >= stop ? w.c0 : stop - w.c0 < share ? stop : w.c0 + share;
+  return true;
+}
+
 // A wave's running state over NT tiles of sixteen query rows.  A lane holds the
 // query row n = lane & 15 of each tile, and of its scores the sixteen positions
 // of the step's tile g = lane >> 4.
@@ -329,69 +431,169 @@ struct WaveState {
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
   float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^15 / vref
   float vref;              // a power of two no V scale so far exceeds, or 0
+  uint32_t node[NT];
+  uint64_t word[NT];       // the node's mask
+
+  __device__ __forceinline__ void begin(const Kv8Attn &a, const Kv8Work &k, uint32_t row0, int lane) {
+    constexpr int C = HD / 64;
+    const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      const uint32_t row = row0 + i * 16 + n;
+      node[i] = row / a.grp;
+      const bool on = node[i] < k.e.nodes;
+      const size_t qrow = (size_t)k.b * a.tmax + (on ? node[i] : 0);
+      const float *q = a.q + (qrow * a.heads + (size_t)k.h * a.grp + (on ? row % a.grp : 0)) * HD + g * 16;
+      word[i] = k.masked && on ? kv8_word(a.mask[qrow], k.e.nodes) : 0;
+      float x[HD / 4], top = 0.0f;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float4 t = *(const float4 *)(q + c * 64 + j * 4);
+          float *y = x + c * 16 + j * 4;
+          y[0] = t.x; y[1] = t.y; y[2] = t.z; y[3] = t.w;
+        }
+#pragma unroll
+      for (int j = 0; j < HD / 4; j++) {
+        x[j] = on ? x[j] * a.coef : 0.0f;
+        top = fmaxf(top, fabsf(x[j]));
+      }
+      top = rows_max(top);
+      const int ex = top > 0.0f && top <= 3.4028234663852886e38f ? __builtin_amdgcn_frexp_expf(top) : 0;
+      rs[i] = ldexpf(1.0f, ex);
+#pragma unroll
+      for (int j = 0; j < HD / 4; j++) x[j] = ldexpf(x[j], -ex);
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        split8(x + c * 16, qh[i][2 * c], ql[i][2 * c]);
+        split8(x + c * 16 + 8, qh[i][2 * c + 1], ql[i][2 * c + 1]);
+      }
+      m[i] = -INFINITY;
+      z[i] = 0.0f;
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    vref = 0.0f;
+  }
+
+  // V scales in units of vref / 2^15: the probabilities times them, as halves,
+  // then use the type's whole range.  vs: this lane's of the step; returns what
+  // the contexts so far are to be multiplied by.
+  __device__ __forceinline__ float rescale(float &vs) {
+    float vtop = fabsf(vs);
+    vtop = vtop <= 3.4028234663852886e38f ? vtop : 0.0f;
+    vtop = nlg_wave_max_f32(vtop);
+    float f = 1.0f;
+    if (vtop > vref) {  // the same in every lane
+      const int e = __builtin_amdgcn_frexp_expf(vtop);
+      const float nv = ldexpf(1.0f, e < -100 ? -100 : e);
+      f = vref / nv;
+      vref = nv;
+    }
+    vs = vref > 0.0f ? vs * (32768.0f / vref) : vs;
+    return f;
+  }
+
+  // A step's scores of tile i (products of the codes with q) made probabilities:
+  // the running maximum and sum, the contexts rescaled, and the probabilities
+  // times the V scales as halves.
+  template <bool GEN>
+  __device__ __forceinline__ void soften(int i, const float4v *acc, float ks, float vs, float vresc, uint32_t bits,
+                                         half8v *ph, half8v *pl) {
+    float s[16];
+    each<16>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      s[j] = acc[j >> 2][j & 3] * row_lane<j>(ks);
+      if (GEN) s[j] = bits >> j & 1 ? s[j] : -INFINITY;
+    });
+    float top[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) top[j] = fmaxf(fmaxf(s[j], s[j + 4]), fmaxf(s[j + 8], s[j + 12]));
+    const float t = rows_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * rs[i];
+    const float mn = fmaxf(m[i], t);
+    const float ms = mn == -INFINITY ? 0.0f : mn;
+    const float al = nlg_exp2(m[i] - ms);
+    m[i] = mn;
+    float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+      s[j] = nlg_exp2(fmaf(s[j], rs[i], -ms));
+      zz[j & 3] = zz[j & 3] + s[j];
+    }
+    z[i] = fmaf(z[i], al, (zz[0] + zz[1]) + (zz[2] + zz[3]));
+    const float sc = al * vresc;
+    if (__any(sc != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;
+    }
+    each<16>([&](auto J) {
+      constexpr int j = decltype(J)::value;
+      s[j] = s[j] * row_lane<j>(vs);
+      if (GEN) s[j] = bits >> j & 1 ? s[j] : 0.0f;
+    });
+    split8(s, ph[0], pl[0]);
+    split8(s + 8, ph[1], pl[1]);
+  }
 };
 
-// One step: 64 positions, tile `tk` holding this lane's K row (4 positions of
-// each of the four tiles a time), tile `tv` its V columns and both scales.
-// GEN: some of the positions are masked, absent or past the end; bits[i]: which
-// of this lane's sixteen the query row of tile i attends; left: how many of
-// them exist.
+// The tiles of 1,024 positions from p0 on, one a lane.
+__device__ __forceinline__ uint32_t kv8_tiles(const Kv8Attn &a, const Kv8Work &k, uint32_t p0, int lane) {
+  const uint32_t mine = p0 + lane * KV8_TILE;
+  return mine < k.c1 ? kv8_tile(a.pg, k.b, k.h, mine / KV8_TILE) : KV8_NONE;
+}
+// Which bytes of a V column's sixteen exist.
+__device__ __forceinline__ uint4 kv8_keep(bool there, int left) {
+  uint32_t keep[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int k = left - 4 * i;
+    keep[i] = !there || k <= 0 ? 0u : k >= 4 ? 0xffffffffu : (1u << (8 * k)) - 1;
+  }
+  return make_uint4(keep[0], keep[1], keep[2], keep[3]);
+}
+__device__ __forceinline__ uint4 and4(uint4 x, uint4 m) { return make_uint4(x.x & m.x, x.y & m.y, x.z & m.z, x.w & m.w); }
+
+#define MFMA(x, y, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0)
+
+// One step of a wave on its own: 64 positions, tile `tk` holding this lane's K
+// row (4 positions of each of the four tiles a time), tile `tv` its V columns
+// and both scales.  GEN: some of the positions are masked, absent or past the
+// end; bits[i]: which of this lane's sixteen the query row of tile i attends;
+// left: how many of them exist.
 template <int HD, int FMT, int NT, bool GEN>
 __device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w, uint32_t tk, uint32_t tv,
                                          const uint32_t *bits, int left, int lane) {
   constexpr int C = HD / 64, D = HD / 16;
   const int g = lane >> 4, n = lane & 15;
   uint4 kr[4][C], vr[D];
-  float ks, vs;
-  {
-    const bool hk = !GEN || tk != KV8_NONE, hv = !GEN || tv != KV8_NONE;
-    const uint8_t *kp = a.kpool + (size_t)(hk ? tk : 0) * kv8_tile_bytes(HD) + (lane & 3) * HD + g * 16;
-    const size_t vt = (size_t)(hv ? tv : 0) * kv8_tile_bytes(HD);
-    const uint8_t *vp = a.vpool + vt;
-    ks = *(const float *)(a.kpool + vt + kv8_scale_byte(HD, n));
-    vs = *(const float *)(vp + kv8_scale_byte(HD, n));
+  const bool hk = !GEN || tk != KV8_NONE, hv = !GEN || tv != KV8_NONE;
+  const uint8_t *kp = a.kpool + (size_t)(hk ? tk : 0) * kv8_tile_bytes(HD) + (lane & 3) * HD + g * 16;
+  const size_t vt = (size_t)(hv ? tv : 0) * kv8_tile_bytes(HD);
+  const uint8_t *vp = a.vpool + vt;
+  float ks = *(const float *)(a.kpool + vt + kv8_scale_byte(HD, n));
+  float vs = *(const float *)(vp + kv8_scale_byte(HD, n));
 #pragma unroll
-    for (int t = 0; t < 4; t++)
+  for (int t = 0; t < 4; t++)
 #pragma unroll
-      for (int c = 0; c < C; c++) kr[t][c] = *(const uint4 *)(kp + t * 4 * HD + c * 64);
+    for (int c = 0; c < C; c++) kr[t][c] = *(const uint4 *)(kp + t * 4 * HD + c * 64);
 #pragma unroll
-    for (int i = 0; i < D; i++) vr[i] = *(const uint4 *)(vp + i * 256 + n * 16);
-    if (GEN) {
-      // absent tiles read as zero rows; what lies past the end is not used
-      if (!hk)
+  for (int i = 0; i < D; i++) vr[i] = *(const uint4 *)(vp + i * 256 + n * 16);
+  if (GEN) {
+    // absent tiles read as zero rows; what lies past the end is not used
+    if (!hk)
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+      for (int t = 0; t < 4; t++)
 #pragma unroll
-          for (int c = 0; c < C; c++) kr[t][c] = make_uint4(0, 0, 0, 0);
-      uint32_t keep[4];
+        for (int c = 0; c < C; c++) kr[t][c] = make_uint4(0, 0, 0, 0);
+    const uint4 keep = kv8_keep(hv, left);
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int k = left - 4 * i;
-        keep[i] = !hv || k <= 0 ? 0u : k >= 4 ? 0xffffffffu : (1u << (8 * k)) - 1;
-      }
-#pragma unroll
-      for (int i = 0; i < D; i++) {
-        vr[i].x &= keep[0]; vr[i].y &= keep[1]; vr[i].z &= keep[2]; vr[i].w &= keep[3];
-      }
-      if (!hv || n >= left) ks = vs = 0.0f;
-    }
+    for (int i = 0; i < D; i++) vr[i] = and4(vr[i], keep);
+    if (!hv || n >= left) ks = vs = 0.0f;
   }
-  // V scales in units of vref / 2^15: the probabilities times them, as halves,
-  // then use the type's whole range
-  float vtop = fabsf(vs);
-  vtop = vtop <= 3.4028234663852886e38f ? vtop : 0.0f;
-  vtop = nlg_wave_max_f32(vtop);
-  float vresc = 1.0f;
-  if (vtop > w.vref) {  // the same in every lane
-    const int e = __builtin_amdgcn_frexp_expf(vtop);
-    const float nv = ldexpf(1.0f, e < -100 ? -100 : e);
-    vresc = w.vref / nv;
-    w.vref = nv;
-  }
-  vs = w.vref > 0.0f ? vs * (32768.0f / w.vref) : vs;
+  const float vresc = w.rescale(vs);
 #pragma unroll
   for (int i = 0; i < NT; i++) {
-    float s[16];
     float4v acc[4];
 #pragma unroll
     for (int t = 0; t < 4; t++) {
@@ -399,144 +601,51 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w,
 #pragma unroll
       for (int c = 0; c < C; c++) {
         const half8v k0 = kv8_half8<FMT>(kr[t][c].x, kr[t][c].y), k1 = kv8_half8<FMT>(kr[t][c].z, kr[t][c].w);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, w.ql[i][2 * c], acc[t], 0, 0, 0);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, w.ql[i][2 * c + 1], acc[t], 0, 0, 0);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, w.qh[i][2 * c], acc[t], 0, 0, 0);
-        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, w.qh[i][2 * c + 1], acc[t], 0, 0, 0);
+        acc[t] = MFMA(k0, w.ql[i][2 * c], acc[t]);
+        acc[t] = MFMA(k1, w.ql[i][2 * c + 1], acc[t]);
+        acc[t] = MFMA(k0, w.qh[i][2 * c], acc[t]);
+        acc[t] = MFMA(k1, w.qh[i][2 * c + 1], acc[t]);
       }
     }
-    each<16>([&](auto J) {
-      constexpr int j = decltype(J)::value;
-      s[j] = acc[j >> 2][j & 3] * row_lane<j>(ks);
-      if (GEN) s[j] = bits[i] >> j & 1 ? s[j] : -INFINITY;
-    });
-    float top = s[0];
-#pragma unroll
-    for (int j = 1; j < 16; j++) top = fmaxf(top, s[j]);
-    top = rows_max(top) * w.rs[i];
-    const float mn = fmaxf(w.m[i], top);
-    const float ms = mn == -INFINITY ? 0.0f : mn;
-    const float al = nlg_exp2(w.m[i] - ms);
-    w.m[i] = mn;
-    float zz = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 16; j++) {
-      s[j] = nlg_exp2(fmaf(s[j], w.rs[i], -ms));
-      zz = zz + s[j];
-    }
-    w.z[i] = fmaf(w.z[i], al, zz);
-    const float sc = al * vresc;
-    if (__any(sc != 1.0f)) {
-#pragma unroll
-      for (int d = 0; d < D; d++) w.o[i][d] = w.o[i][d] * sc;
-    }
-    each<16>([&](auto J) {
-      constexpr int j = decltype(J)::value;
-      s[j] = s[j] * row_lane<j>(vs);
-      if (GEN) s[j] = bits[i] >> j & 1 ? s[j] : 0.0f;
-    });
     half8v ph[2], pl[2];
-    split8(s, ph[0], pl[0]);
-    split8(s + 8, ph[1], pl[1]);
+    w.template soften<GEN>(i, acc, ks, vs, vresc, GEN ? bits[i] : 0, ph, pl);
 #pragma unroll
     for (int d = 0; d < D; d++) {
       const half8v v0 = kv8_half8<FMT>(vr[d].x, vr[d].y), v1 = kv8_half8<FMT>(vr[d].z, vr[d].w);
-      w.o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], w.o[i][d], 0, 0, 0);
-      w.o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], w.o[i][d], 0, 0, 0);
-      w.o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], w.o[i][d], 0, 0, 0);
-      w.o[i][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], w.o[i][d], 0, 0, 0);
+      w.o[i][d] = MFMA(v0, pl[0], w.o[i][d]);
+      w.o[i][d] = MFMA(v1, pl[1], w.o[i][d]);
+      w.o[i][d] = MFMA(v0, ph[0], w.o[i][d]);
+      w.o[i][d] = MFMA(v1, ph[1], w.o[i][d]);
     }
   }
 }
 
-// The positions of sequence b.
-template <bool TREE>
-__device__ __forceinline__ Kv8Extent kv8_of(const Kv8Attn &a, uint32_t b) {
-  return kv8_extent(TREE, a.base[b], TREE && a.nodes ? a.nodes[b] : (int32_t)a.tmax, a.tmax,
-                    a.pg.mbps * a.pg.bpt * KV8_TILE);
-}
-
+// Up to 32 rows (16 NT): the workgroup's waves take its positions in turn, 64 at
+// a time, straight from memory into the matrix cores' operands, and meet in LDS.
 template <int HD, int FMT, int NT, bool TREE>
 __global__ __launch_bounds__(64 * KV8_WAVES) void k_attn_q8(Kv8Attn a) {
-  constexpr int C = HD / 64, D = HD / 16;
+  constexpr int D = HD / 16;
   __shared__ float4v s_o[KV8_WAVES][D][64];
   __shared__ float s_m[KV8_WAVES][16], s_z[KV8_WAVES][16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
-  uint32_t id = blockIdx.x;
-  const uint32_t chunk = id % a.nchunk;
-  id /= a.nchunk;
-  const uint32_t grp = id % a.groups;
-  id /= a.groups;
-  const uint32_t h = id % a.pg.kvheads, b = id / a.pg.kvheads;
-  const Kv8Extent e = kv8_of<TREE>(a, b);
-  if (!e.on) return;
-  const uint32_t row0 = grp * (NT * 16);
-  if (row0 >= (uint64_t)e.nodes * a.grp) return;
-  const uint32_t c0 = chunk * a.chunk;
-  if (c0 >= e.end && chunk) return;
-  const bool masked = TREE && a.mask;
-  // a causal group of rows ends at its last node
-  const uint32_t stop = TREE && !masked ? kv8_stop(e, (row0 + NT * 16 - 1) / a.grp) : e.end;
-  const uint32_t c1 = kv8_chunk_end(c0, stop, a.chunk);
-
+  Kv8Work k;
+  if (!kv8_work<TREE>(a, NT * 16, lane, k)) return;
   WaveState<HD, NT> w;
-  uint32_t node[NT];
-  uint64_t word[NT];
-#pragma unroll
-  for (int i = 0; i < NT; i++) {
-    const uint32_t row = row0 + i * 16 + n;
-    node[i] = row / a.grp;
-    const bool on = node[i] < e.nodes;
-    const float *q = a.q + ((size_t)b * a.tmax + (on ? node[i] : 0)) * a.heads * HD +
-                     (size_t)(h * a.grp + (on ? row % a.grp : 0)) * HD + g * 16;
-    word[i] = masked && on ? kv8_word(a.mask[(size_t)b * a.tmax + node[i]], e.nodes) : 0;
-    float x[HD / 4], top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const float4 t = *(const float4 *)(q + c * 64 + k * 4);
-        float *y = x + c * 16 + k * 4;
-        y[0] = t.x; y[1] = t.y; y[2] = t.z; y[3] = t.w;
-      }
-#pragma unroll
-    for (int k = 0; k < HD / 4; k++) {
-      x[k] = on ? x[k] * a.coef : 0.0f;
-      top = fmaxf(top, fabsf(x[k]));
-    }
-    top = rows_max(top);
-    const int ex = top > 0.0f && top <= 3.4028234663852886e38f ? __builtin_amdgcn_frexp_expf(top) : 0;
-    w.rs[i] = ldexpf(1.0f, ex);
-#pragma unroll
-    for (int k = 0; k < HD / 4; k++) x[k] = ldexpf(x[k], -ex);
-#pragma unroll
-    for (int c = 0; c < C; c++) {
-      split8(x + c * 16, w.qh[i][2 * c], w.ql[i][2 * c]);
-      split8(x + c * 16 + 8, w.qh[i][2 * c + 1], w.ql[i][2 * c + 1]);
-    }
-    w.m[i] = -INFINITY;
-    w.z[i] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < D; d++) w.o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  w.vref = 0.0f;
-
-  for (uint32_t p0 = c0; p0 < c1; p0 += 64 * KV8_TILE) {
-    // the tiles of the next 1,024 positions, one a lane
-    const uint32_t mine = p0 + lane * KV8_TILE;
-    const uint32_t tid = mine < c1 ? kv8_tile(a.pg, b, h, mine / KV8_TILE) : KV8_NONE;
-    const uint32_t p1 = c1 - p0 < 64 * KV8_TILE ? c1 : p0 + 64 * KV8_TILE;
+  w.begin(a, k, k.row0, lane);
+  const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;  // no mask below this position
+  for (uint32_t p0 = k.c0; p0 < k.c1; p0 += 64 * KV8_TILE) {
+    const uint32_t tid = kv8_tiles(a, k, p0, lane);
+    const uint32_t p1 = k.c1 - p0 < 64 * KV8_TILE ? k.c1 : p0 + 64 * KV8_TILE;
     for (uint32_t p = p0 + wv * KV8_STEP; p < p1; p += KV8_WAVES * KV8_STEP) {
       const int t0 = (int)(p - p0) / KV8_TILE;
       const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
-      const bool gen = p + KV8_STEP > (e.base < stop ? e.base : stop) || __any(tv == KV8_NONE);
-      if (gen) {
+      if (p + KV8_STEP > whole || __any(tv == KV8_NONE)) {
         uint32_t bits[NT];
         const uint32_t q0 = p + g * KV8_TILE;  // this lane's first position
-        const int left = kv8_left(e, q0);
+        const int left = kv8_left(k.e, q0);
 #pragma unroll
         for (int i = 0; i < NT; i++)
-          bits[i] = TREE ? kv8_bits(e, masked, node[i], word[i], q0) : (1u << left) - 1;
+          bits[i] = TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], q0) : (1u << left) - 1;
         kv8_step<HD, FMT, NT, true>(a, w, tk, tv, bits, left, lane);
       } else {
         kv8_step<HD, FMT, NT, false>(a, w, tk, tv, nullptr, 16, lane);
@@ -559,63 +668,228 @@ __global__ __launch_bounds__(64 * KV8_WAVES) void k_attn_q8(Kv8Attn a) {
     __syncthreads();
     float mm = s_m[0][n];
 #pragma unroll
-    for (int k = 1; k < KV8_WAVES; k++) mm = fmaxf(mm, s_m[k][n]);
+    for (int j = 1; j < KV8_WAVES; j++) mm = fmaxf(mm, s_m[j][n]);
     const float ms = mm == -INFINITY ? 0.0f : mm;
     float f[KV8_WAVES], zz = 0.0f;
 #pragma unroll
-    for (int k = 0; k < KV8_WAVES; k++) {
-      f[k] = nlg_exp2(s_m[k][n] - ms);
-      zz = fmaf(s_z[k][n], f[k], zz);
+    for (int j = 0; j < KV8_WAVES; j++) {
+      f[j] = nlg_exp2(s_m[j][n] - ms);
+      zz = fmaf(s_z[j][n], f[j], zz);
     }
-    const uint32_t row = row0 + i * 16 + n;
-    if (row < (uint64_t)e.nodes * a.grp) {
-      const uint64_t part = (((uint64_t)b * a.pg.kvheads + h) * a.nchunk + chunk) * a.rows + row;
-      if (a.nchunk > 1 && wv == 0 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(mm, zz);
-      const float inv = a.nchunk > 1 ? 1.0f : zz > 0.0f || zz != zz ? 1.0f / zz : 0.0f;
-      float *o = a.nchunk > 1 ? a.pctx + part * HD
-                              : a.out + (((size_t)b * a.tmax + row / a.grp) * a.heads + h * a.grp + row % a.grp) * HD;
-  #pragma unroll
+    const uint32_t row = k.row0 + i * 16 + n;
+    if (row < (uint64_t)k.e.nodes * a.grp) {
+      const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rows + row;
+      if (k.chunks > 1 && wv == 0 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(mm, zz);
+      const float inv = k.chunks > 1 ? 1.0f : zz > 0.0f || zz != zz ? 1.0f / zz : 0.0f;
+      float *o = k.chunks > 1 ? a.pctx + part * HD
+                              : a.out + (((size_t)k.b * a.tmax + row / a.grp) * a.heads + k.h * a.grp + row % a.grp) * HD;
+#pragma unroll
       for (int d = wv; d < D; d += KV8_WAVES) {
         float4v t = s_o[0][d][lane] * f[0];
-  #pragma unroll
-        for (int k = 1; k < KV8_WAVES; k++) t = t + s_o[k][d][lane] * f[k];
+#pragma unroll
+        for (int j = 1; j < KV8_WAVES; j++) t = t + s_o[j][d][lane] * f[j];
         *(float4v *)(o + d * 16 + g * 4) = t * inv;
       }
     }
   }
 }
 
-// The chunks' parts of each output row, joined.
-template <bool TREE>
-__global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint64_t total) {
-  const uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const uint32_t per = hd / 4, d = (uint32_t)(i % per) * 4;
-  const uint64_t r = i / per;
-  const uint32_t head = (uint32_t)(r % a.heads);
-  const uint64_t bn = r / a.heads;
-  const uint32_t node = (uint32_t)(bn % a.tmax), b = (uint32_t)(bn / a.tmax);
-  const Kv8Extent e = kv8_of<TREE>(a, b);
-  if (!e.on || node >= e.nodes) return;
-  uint32_t live = (uint32_t)(((uint64_t)e.end + a.chunk - 1) / a.chunk);
-  live = live ? live : 1;
-  const uint32_t h = head / a.grp, row = node * a.grp + head % a.grp;
-  const uint64_t p0 = ((uint64_t)b * a.pg.kvheads + h) * a.nchunk * a.rows + row;
-  const float2 *mz = (const float2 *)a.pmz;
-  float mm = -INFINITY;
-  for (uint32_t c = 0; c < live; c++) mm = fmaxf(mm, mz[p0 + (uint64_t)c * a.rows].x);
-  const float ms = mm == -INFINITY ? 0.0f : mm;
-  float z = 0.0f;
-  float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (uint32_t c = 0; c < live; c++) {
-    const uint64_t p = p0 + (uint64_t)c * a.rows;
-    const float2 t = mz[p];
-    const float f = nlg_exp2(t.x - ms);
-    z = fmaf(t.y, f, z);
-    o = o + *(const float4v *)(a.pctx + p * hd + d) * f;
+// More rows: each wave has 16 NT of its own, all walk the same positions, and K
+// and V are made halves once for the workgroup, in LDS, in the order in which
+// the waves' operands lie (a fragment's 64 lanes side by side: no bank is asked
+// twice).  While a step is computed the next one's halves are written and the
+// one's after it are on their way from memory.
+template <int HD, int FMT, int NT, bool TREE>
+__global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
+  constexpr int C = HD / 64, D = HD / 16, DW = D / KV8_WAVES;
+  __shared__ half8v s_k[2][4][2 * C][64], s_v[2][D][2][64];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
+  Kv8Work k;
+  if (!kv8_work<TREE>(a, KV8_WAVES * NT * 16, lane, k)) return;
+  const uint32_t row0 = k.row0 + wv * (NT * 16);
+  const bool rows = row0 < (uint64_t)k.e.nodes * a.grp;
+  // where this wave's rows stop attending
+  const uint32_t stop = TREE && !k.masked ? kv8_stop(k.e, (row0 + NT * 16 - 1) / a.grp) : k.e.end;
+  WaveState<HD, NT> w;
+  w.begin(a, k, row0, lane);
+  const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;
+
+  // this wave's share of a step: tile wv's K, DW sixteens of V's dimensions
+  uint4 kr[C], vr[DW];
+  float ks, vs;
+  uint32_t tid = KV8_NONE, tid0 = 0xffffffffu;
+  auto load = [&](uint32_t p) {
+    const uint32_t p0 = k.c0 + (p - k.c0) / (64 * KV8_TILE) * (64 * KV8_TILE);
+    if (p0 != tid0) {
+      tid0 = p0;
+      tid = kv8_tiles(a, k, p0, lane);
+    }
+    const int t0 = (int)(p - p0) / KV8_TILE;
+    const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
+    const bool hk = tk != KV8_NONE, hv = tv != KV8_NONE;
+    const uint8_t *kp = a.kpool + (size_t)(hk ? tk : 0) * kv8_tile_bytes(HD) + (wv * 4 + (lane & 3)) * HD + g * 16;
+    const size_t vt = (size_t)(hv ? tv : 0) * kv8_tile_bytes(HD);
+    const uint8_t *vp = a.vpool + vt + wv * DW * 256 + n * 16;
+    ks = *(const float *)(a.kpool + vt + kv8_scale_byte(HD, n));
+    vs = *(const float *)(a.vpool + vt + kv8_scale_byte(HD, n));
+#pragma unroll
+    for (int c = 0; c < C; c++) kr[c] = *(const uint4 *)(kp + c * 64);
+#pragma unroll
+    for (int d = 0; d < DW; d++) vr[d] = *(const uint4 *)(vp + d * 256);
+    const int left = kv8_left(k.e, p + g * KV8_TILE);
+    if (__any(!hv || left < 16)) {
+      if (!hk)
+#pragma unroll
+        for (int c = 0; c < C; c++) kr[c] = make_uint4(0, 0, 0, 0);
+      const uint4 keep = kv8_keep(hv, left);
+#pragma unroll
+      for (int d = 0; d < DW; d++) vr[d] = and4(vr[d], keep);
+      if (!hv || n >= left) ks = vs = 0.0f;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      s_k[buf][wv][2 * c][lane] = kv8_half8<FMT>(kr[c].x, kr[c].y);
+      s_k[buf][wv][2 * c + 1][lane] = kv8_half8<FMT>(kr[c].z, kr[c].w);
+    }
+#pragma unroll
+    for (int d = 0; d < DW; d++) {
+      s_v[buf][wv * DW + d][0][lane] = kv8_half8<FMT>(vr[d].x, vr[d].y);
+      s_v[buf][wv * DW + d][1][lane] = kv8_half8<FMT>(vr[d].z, vr[d].w);
+    }
+  };
+  auto compute = [&](auto GENV, int buf, float ksc, float vsc, uint32_t p) {
+    constexpr bool GEN = decltype(GENV)::value != 0;
+    const float vresc = w.rescale(vsc);
+    float4v acc[NT][4];
+#pragma unroll
+    for (int t = 0; t < 4; t++) {
+#pragma unroll
+      for (int i = 0; i < NT; i++) acc[i][t] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int c = 0; c < 2 * C; c++) {
+        const half8v f = s_k[buf][t][c][lane];
+#pragma unroll
+        for (int i = 0; i < NT; i++) {
+          acc[i][t] = MFMA(f, w.ql[i][c], acc[i][t]);
+          acc[i][t] = MFMA(f, w.qh[i][c], acc[i][t]);
+        }
+      }
+    }
+    half8v ph[NT][2], pl[NT][2];
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      const uint32_t bits = GEN ? TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], p + g * KV8_TILE)
+                                       : (1u << kv8_left(k.e, p + g * KV8_TILE)) - 1
+                                : 0u;
+      w.template soften<GEN>(i, acc[i], ksc, vsc, vresc, bits, ph[i], pl[i]);
+    }
+#pragma unroll
+    for (int d = 0; d < D; d++) {
+      const half8v v0 = s_v[buf][d][0][lane], v1 = s_v[buf][d][1][lane];
+#pragma unroll
+      for (int i = 0; i < NT; i++) {
+        w.o[i][d] = MFMA(v0, pl[i][0], w.o[i][d]);
+        w.o[i][d] = MFMA(v1, pl[i][1], w.o[i][d]);
+        w.o[i][d] = MFMA(v0, ph[i][0], w.o[i][d]);
+        w.o[i][d] = MFMA(v1, ph[i][1], w.o[i][d]);
+      }
+    }
+  };
+  if (k.c0 < k.c1) {
+    load(k.c0);
+    store(0);
+    float ksc = ks, vsc = vs;
+    if (k.c1 - k.c0 > KV8_STEP) load(k.c0 + KV8_STEP);
+    __syncthreads();
+    int buf = 0;
+    for (uint32_t p = k.c0; p < k.c1; p += KV8_STEP, buf ^= 1) {
+      float ksn = 0.0f, vsn = 0.0f;
+      if (k.c1 - p > KV8_STEP) {
+        store(buf ^ 1);
+        ksn = ks;
+        vsn = vs;
+        if (k.c1 - p > 2 * KV8_STEP) load(p + 2 * KV8_STEP);
+      }
+      if (rows && p < stop) {
+        if (p + KV8_STEP > whole) compute(Int<1>{}, buf, ksc, vsc, p);
+        else compute(Int<0>{}, buf, ksc, vsc, p);
+      }
+      __syncthreads();
+      ksc = ksn;
+      vsc = vsn;
+    }
   }
+  if (!rows) return;
+  const float vu = w.vref > 0.0f ? w.vref * (1.0f / 32768.0f) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < NT; i++) {
+    const float z = rows_sum(w.z[i]);
+    const uint32_t row = row0 + i * 16 + n;
+    if (row >= (uint64_t)k.e.nodes * a.grp) continue;
+    const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rows + row;
+    if (k.chunks > 1 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(w.m[i], z);
+    const float f = k.chunks > 1 ? vu : z > 0.0f || z != z ? vu / z : 0.0f;
+    float *o = k.chunks > 1 ? a.pctx + part * HD
+                            : a.out + (((size_t)k.b * a.tmax + row / a.grp) * a.heads + k.h * a.grp + row % a.grp) * HD;
+#pragma unroll
+    for (int d = 0; d < D; d++) *(float4v *)(o + d * 16 + g * 4) = w.o[i][d] * f;
+  }
+}
+
+// The chunks' parts of each output row, joined: SUBS groups of hd / 4 threads
+// walk a row's chunks.  A workgroup's rows are of one sequence.
+template <bool TREE, int SUBS>
+__global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint32_t blocks) {
+  __shared__ float4v s_o[256];
+  __shared__ float2 s_mz[256];
+  const uint32_t per = hd / 4, t = threadIdx.x, b = blockIdx.x / blocks;
+  const uint32_t r = blockIdx.x % blocks * (256 / per / SUBS) + t / (per * SUBS), sub = t / per % SUBS, d = t % per * 4;
+  const Kv8Plan<TREE> plan(a, t & 63);
+  uint32_t chunks;
+  const uint32_t slot = plan.first(a, b, t & 63, chunks);
+  if (chunks < 2) return;  // (none, or written already)
+  const Kv8Extent e = kv8_of<TREE>(a, b);
+  const uint32_t node = r / a.heads, head = r % a.heads;
+  const bool on = node < e.nodes;
+  const uint64_t p0 = ((uint64_t)slot * a.pg.kvheads + head / a.grp) * a.rows + (uint64_t)node * a.grp + head % a.grp;
+  const uint64_t step = (uint64_t)a.pg.kvheads * a.rows;
+  float m = -INFINITY, z = 0.0f;
+  float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (on)
+    for (uint32_t c = sub; c < chunks; c += SUBS) {
+      const uint64_t p = p0 + c * step;
+      const float2 x = *(const float2 *)(a.pmz + p * 2);
+      const float4v y = *(const float4v *)(a.pctx + p * hd + d);
+      const float mn = fmaxf(m, x.x), ms = mn == -INFINITY ? 0.0f : mn;
+      const float f = nlg_exp2(m - ms), fx = nlg_exp2(x.x - ms);
+      m = mn;
+      z = fmaf(z, f, x.y * fx);
+      o = o * f + y * fx;
+    }
+  if (SUBS > 1) {
+    s_mz[t] = make_float2(m, z);
+    s_o[t] = o;
+    __syncthreads();
+    if (sub) return;
+    float mm = m;
+#pragma unroll
+    for (int i = 1; i < SUBS; i++) mm = fmaxf(mm, s_mz[t + i * per].x);
+    const float ms = mm == -INFINITY ? 0.0f : mm, f = nlg_exp2(m - ms);
+    z = z * f;
+    o = o * f;
+#pragma unroll
+    for (int i = 1; i < SUBS; i++) {
+      const float2 x = s_mz[t + i * per];
+      const float fx = nlg_exp2(x.x - ms);
+      z = fmaf(x.y, fx, z);
+      o = o + s_o[t + i * per] * fx;
+    }
+  }
+  if (!on) return;
   const float inv = z > 0.0f || z != z ? 1.0f / z : 0.0f;
-  *(float4v *)(a.out + r * hd + d) = o * inv;
+  *(float4v *)(a.out + (((size_t)b * a.tmax + node) * a.heads + head) * hd + d) = o * inv;
 }
 
 // ------------------------------------------------------------------ commit
@@ -858,8 +1132,8 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
 }
 
 // The partials' bytes: contexts, then (maximum, sum) pairs; 0 where one chunk needs none.
-static uint64_t kv8_partials(const Kv8Split &s, uint32_t batch, uint64_t rows, uint32_t kvheads, uint32_t hd) {
-  return s.nchunk < 2 ? 0 : (uint64_t)batch * kvheads * s.nchunk * rows * (hd + 2) * 4;
+static uint64_t kv8_partials(const Kv8Split &s, uint64_t rows, uint32_t kvheads, uint32_t hd) {
+  return s.one ? 0 : s.slots * kvheads * rows * (hd + 2) * 4;
 }
 // Sizes an attention call can have at all (0: none).
 static uint64_t kv8_rows(uint32_t tmax, uint32_t heads, uint32_t kvheads) {
@@ -874,8 +1148,7 @@ extern "C" size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax
   if (!batch || !rows || !bs || bs % KV8_TILE || !mbps || (uint64_t)bs * mbps > 0x7fffffffull ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, (uint64_t)bs * mbps), batch, rows, kvheads,
-                              head_dim);
+  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, (uint64_t)bs * mbps), rows, kvheads, head_dim);
 }
 extern "C" size_t nlg_decode_attn_paged_q8_workspace(uint32_t batch, uint32_t heads, uint32_t kvheads,
                                                      uint32_t head_dim, uint32_t bs, uint32_t mbps) {
@@ -896,9 +1169,12 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   if (mask && tmax > KV8_TREE) return nlg_fail("%s: %u nodes under a mask (at most %d)", what, tmax, KV8_TREE);
   if (mask && ((uintptr_t)mask & 7)) return nlg_fail("%s: the masks must be 8-byte aligned", what);
   const Kv8Split s = kv8_split(batch, (uint32_t)rows, kvheads, (uint64_t)bs * mbps);
-  const uint64_t need = kv8_partials(s, batch, rows, kvheads, hd);
-  const uint64_t total = (uint64_t)batch * tmax * heads * (hd / 4);
-  if (!nlg_fits(s.blocks, 64 * KV8_WAVES) || !nlg_fits((total + 255) / 256, 256))
+  const uint64_t need = kv8_partials(s, rows, kvheads, hd);
+  // joining: eight groups of threads a row while its rows would not fill the card with one
+  const uint64_t orows = (uint64_t)tmax * heads;
+  const bool subs = orows * batch * (hd / 4) < 256 * 2048;
+  const uint64_t oper = 256 / (hd / 4) / (subs ? 8 : 1), oblocks = (orows + oper - 1) / oper;
+  if (!nlg_fits(s.blocks, 64 * KV8_WAVES) || !nlg_fits(oblocks * batch, 256) || orows > 0xffffffffull)
     return nlg_fail("%s: too many queries for one launch", what);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -909,18 +1185,23 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   KV8_SCOPE(what);
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
   a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads; a.rows = (uint32_t)rows;
-  a.groups = s.groups; a.chunk = s.chunk; a.nchunk = s.nchunk;
+  a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
   a.pctx = (float *)workspace;
-  a.pmz = need ? a.pctx + (uint64_t)batch * kvheads * s.nchunk * rows * hd : nullptr;
+  a.pmz = need ? a.pctx + s.slots * kvheads * rows * hd : nullptr;
   a.coef = NLG_LOG2E / sqrtf((float)hd);
   const dim3 grid((uint32_t)s.blocks), blk(64 * KV8_WAVES);
   hipStream_t st = nlg_stream(stream);
-#define GO(HD, F)                                                                               \
-  do {                                                                                          \
-    if (!tree && s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, false>), grid, blk, 0, st, a); \
-    else if (!tree) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, false>), grid, blk, 0, st, a);      \
-    else if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, true>), grid, blk, 0, st, a); \
-    else hipLaunchKernelGGL((k_attn_q8<HD, F, 2, true>), grid, blk, 0, st, a);                  \
+#define GO3(HD, F, T)                                                                            \
+  do {                                                                                           \
+    if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, T>), grid, blk, 0, st, a);      \
+    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, T>), grid, blk, 0, st, a); \
+    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1, T>), grid, blk, 0, st, a); \
+    else hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 2, T>), grid, blk, 0, st, a);                 \
+  } while (0)
+#define GO(HD, F)               \
+  do {                          \
+    if (tree) GO3(HD, F, true); \
+    else GO3(HD, F, false);     \
   } while (0)
   if (hd == 128) {
     if (fmt == NLG_KV_I8) GO(128, NLG_KV_I8); else GO(128, NLG_KV_E4M3);
@@ -928,11 +1209,15 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
     if (fmt == NLG_KV_I8) GO(64, NLG_KV_I8); else GO(64, NLG_KV_E4M3);
   }
 #undef GO
+#undef GO3
   NLG_LAUNCHED(what);
   if (need) {
-    const dim3 mg((uint32_t)((total + 255) / 256));
-    if (tree) hipLaunchKernelGGL(k_attn_q8_merge<true>, mg, dim3(256), 0, st, a, hd, total);
-    else hipLaunchKernelGGL(k_attn_q8_merge<false>, mg, dim3(256), 0, st, a, hd, total);
+    const dim3 mg((uint32_t)(oblocks * batch));
+    const uint32_t ob = (uint32_t)oblocks;
+    if (tree && subs) hipLaunchKernelGGL((k_attn_q8_merge<true, 8>), mg, dim3(256), 0, st, a, hd, ob);
+    else if (tree) hipLaunchKernelGGL((k_attn_q8_merge<true, 1>), mg, dim3(256), 0, st, a, hd, ob);
+    else if (subs) hipLaunchKernelGGL((k_attn_q8_merge<false, 8>), mg, dim3(256), 0, st, a, hd, ob);
+    else hipLaunchKernelGGL((k_attn_q8_merge<false, 1>), mg, dim3(256), 0, st, a, hd, ob);
     NLG_LAUNCHED(what);
   }
   return NLG_OK;

@@ -35,53 +35,73 @@ static int layout(uint32_t hd) {
   }
   return 0;
 }
-// one call: what the workgroups and waves attend, by row and position
-static int call(bool tree, bool masked, int32_t at, int32_t nodes, uint32_t tmax, uint32_t grp, uint32_t bs, uint32_t mbps,
-                uint32_t batch, uint32_t kvheads) {
-  const uint32_t cap = bs * mbps, rows = tmax * grp;
+// one call: what the workgroups and waves attend, by sequence, row and position
+static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int32_t> nodes, uint32_t tmax, uint32_t grp,
+                uint32_t bs, uint32_t mbps, uint32_t kvheads) {
+  const uint32_t cap = bs * mbps, rows = tmax * grp, batch = at.size();
   const Kv8Split s = kv8_split(batch, rows, kvheads, cap);
-  CHECK(s.chunk % (KV8_STEP * KV8_WAVES) == 0 && s.nchunk >= 1 && (uint64_t)s.chunk * s.nchunk >= cap);
-  CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows);
-  CHECK(s.blocks == (uint64_t)batch * kvheads * s.groups * s.nchunk);
-  const Kv8Extent e = kv8_extent(tree, at, nodes, tmax, cap);
-  CHECK(e.end <= cap);
-  std::vector<uint64_t> mask(tmax);
-  for (auto &m : mask) m = (uint64_t)rnd(1u << 31) << 33 ^ (uint64_t)rnd(1u << 31) << 10 ^ rnd(1024);
-  const int64_t nn = !tree ? 1 : nodes < 0 ? 0 : nodes > (int64_t)tmax ? tmax : nodes;
-  CHECK(e.on == (!tree || (at >= 0 && nn > 0)));
-  if (!e.on) return 0;
-  for (uint32_t g = 0; g < s.groups; g++)
-    for (uint32_t r = g * s.rowsper; r < (g + 1) * s.rowsper && r < rows; r++) {
+  CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows && s.want >= 1);
+  // every (slot, kv head, group) is some workgroup's, as the kernels number them
+  std::vector<int> seen((size_t)s.slots * kvheads * s.groups);
+  for (uint64_t i = 0; i < s.blocks; i++) {
+    const uint64_t u = i / (8 * s.groups) * 8 + i % 8, g = i / 8 % s.groups;
+    if (u < (uint64_t)s.slots * kvheads) seen[u * s.groups + g]++;
+  }
+  for (int n : seen) CHECK(n == 1);
+  std::vector<Kv8Extent> e(batch);
+  uint64_t total = 0, slots = 0;
+  for (uint32_t b = 0; b < batch; b++) {
+    e[b] = kv8_extent(tree, at[b], nodes[b], tmax, cap);
+    CHECK(e[b].end <= cap);
+    total += kv8_steps(e[b]);
+  }
+  const uint32_t per = kv8_per(total, s.want, s.least, s.unit);
+  CHECK(per % s.unit == 0 && per >= s.least);
+  for (uint32_t b = 0; b < batch; b++) {
+    const int64_t nn = !tree ? 1 : nodes[b] < 0 ? 0 : nodes[b] > (int64_t)tmax ? tmax : nodes[b];
+    CHECK(e[b].on == (!tree || (at[b] >= 0 && nn > 0)));
+    const uint32_t steps = kv8_steps(e[b]), chunks = kv8_chunks(steps, per);
+    slots += chunks;
+    CHECK(chunks == 0 ? !e[b].on : (s.one ? chunks == 1 : true));
+    if (!chunks) continue;
+    const uint32_t share = kv8_share(steps, chunks, s.unit);
+    CHECK(share % s.unit == 0 && share <= per && (uint64_t)share * chunks >= steps && share * (chunks - 1) < steps);
+    std::vector<uint64_t> mask(tmax);
+    for (auto &m : mask) m = (uint64_t)rnd(1u << 31) << 33 ^ (uint64_t)rnd(1u << 31) << 10 ^ rnd(1024);
+    for (uint32_t r = 0; r < rows; r += 1 + rnd(3)) {
       const uint32_t node = r / grp;
       if (node >= nn) continue;
       std::vector<int> seen(cap + 64);
-      const uint32_t stop = tree && !masked ? kv8_stop(e, (g * s.rowsper + s.rowsper - 1) / grp) : e.end;
-      for (uint32_t c = 0; c < s.nchunk; c++) {
-        const uint32_t c0 = c * s.chunk;
-        if (c0 >= e.end && c) continue;
-        const uint32_t c1 = kv8_chunk_end(c0, stop, s.chunk);
+      const uint32_t g0 = r / s.rowsper * s.rowsper;
+      const uint32_t stop = tree && !masked ? kv8_stop(e[b], (g0 + s.rowsper - 1) / grp) : e[b].end;
+      const uint32_t mine = tree && !masked ? kv8_stop(e[b], node) : e[b].end;
+      for (uint32_t c = 0; c < chunks; c++) {
+        const uint32_t c0 = c * share * KV8_STEP;
+        const uint32_t c1 = c0 >= stop ? c0 : stop - c0 < share * KV8_STEP ? stop : c0 + share * KV8_STEP;
+        const uint32_t whole = e[b].base < c1 ? e[b].base : c1;
         for (uint32_t p = c0; p < c1; p += KV8_STEP)
           for (uint32_t t = 0; t < 4; t++) {
             const uint32_t q0 = p + t * 16;
-            const bool whole = p + KV8_STEP <= (e.base < stop ? e.base : stop);
-            const uint32_t bits = whole ? 0xffffu
-                                  : tree ? kv8_bits(e, masked, node, masked ? kv8_word(mask[node], e.nodes) : 0, q0)
-                                         : (1u << kv8_left(e, q0)) - 1;
-            CHECK(bits < 65536);
+            const uint32_t bits = p + KV8_STEP <= whole ? 0xffffu
+                                  : tree ? kv8_bits(e[b], masked, node, masked ? kv8_word(mask[node], e[b].nodes) : 0, q0)
+                                         : (1u << kv8_left(e[b], q0)) - 1;
+            CHECK(bits < 65536 && (p < mine || !bits));
             for (uint32_t j = 0; j < 16; j++) seen[q0 + j < cap + 63 ? q0 + j : cap + 63] += bits >> j & 1;
           }
       }
       for (uint32_t p = 0; p < cap + 64; p++) {
         int want;
         if (p >= cap) want = 0;
-        else if (!tree) want = (int64_t)p <= at;
-        else if ((int64_t)p < at) want = 1;
-        else if ((int64_t)p >= at + nn) want = 0;
-        else if (masked) want = mask[node] >> (p - at) & 1;
-        else want = p - at <= node;
+        else if (!tree) want = (int64_t)p <= at[b];
+        else if ((int64_t)p < at[b]) want = 1;
+        else if ((int64_t)p >= at[b] + nn) want = 0;
+        else if (masked) want = mask[node] >> (p - at[b]) & 1;
+        else want = p - at[b] <= node;
         CHECK(seen[p] == want);
       }
     }
+  }
+  CHECK(slots <= s.slots);
   return 0;
 }
 int main(void) {
@@ -92,24 +112,31 @@ int main(void) {
   CHECK(kv8_tile(g, 0, 4, 1) == (3 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 4) == 0);
   CHECK(kv8_tile(g, 0, 0, 2) == KV8_NONE && kv8_tile(g, 0, 0, 6) == KV8_NONE && kv8_tile(g, 1, 0, 0) == KV8_NONE);
   CHECK(kv8_tile(g, 1, 0, 3) == KV8_NONE && kv8_tile(g, 1, 4, 5) == (1 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 0xffffffffu) == KV8_NONE);
-  for (int i = 0; i < 400; i++) {
-    const uint32_t bs = 16 * (1 + rnd(4)), mbps = 1 + rnd(20), cap = bs * mbps;
-    const uint32_t grp = 1 + rnd(9), kvh = 1 + rnd(3), batch = 1 + rnd(40);
-    if (call(false, false, (int32_t)rnd(cap + 20) - 2, 1, 1, grp, bs, mbps, batch, kvh)) return 1;
+  for (int i = 0; i < 300; i++) {
+    const uint32_t bs = 16 * (1 + rnd(4)), mbps = 1 + rnd(i % 10 ? 20 : 300), cap = bs * mbps;
+    const uint32_t grp = 1 + rnd(9), kvh = 1 + rnd(i % 3 ? 8 : 300), batch = 1 + rnd(i % 4 ? 4 : 90);
     const uint32_t tm = 1 + rnd(64), tc = 1 + rnd(90);
-    if (call(true, true, (int32_t)rnd(cap + 4) - 2, (int32_t)rnd(tm + 4) - 1, tm, grp, bs, mbps, batch, kvh)) return 1;
-    if (call(true, false, (int32_t)rnd(cap + 4) - 2, (int32_t)rnd(tc + 4) - 1, tc, grp, bs, mbps, batch, kvh)) return 1;
+    std::vector<int32_t> at, nm, nc;
+    for (uint32_t b = 0; b < batch; b++) {
+      at.push_back((int32_t)rnd(cap + 20) - 2);
+      nm.push_back((int32_t)rnd(tm + 4) - 1);
+      nc.push_back((int32_t)rnd(tc + 4) - 1);
+    }
+    if (call(false, false, at, nm, 1, grp, bs, mbps, kvh)) return 1;
+    if (call(true, true, at, nm, tm, grp, bs, mbps, kvh)) return 1;
+    if (call(true, false, at, nc, tc, grp, bs, mbps, kvh)) return 1;
   }
   // extremes
-  if (call(false, false, 2147483647, 1, 1, 1, 16, 1, 1, 1) || call(true, false, 2147483647, 5, 5, 1, 16, 2, 1, 1)) return 1;
+  if (call(false, false, {2147483647}, {1}, 1, 1, 16, 1, 1) || call(true, false, {2147483647}, {5}, 5, 1, 16, 2, 1)) return 1;
   const Kv8Extent e = kv8_extent(true, 2147483647, 2147483647, 2147483647u, 2147483632u);
   CHECK(e.end == 2147483632u && e.base == 2147483647u && kv8_left(e, 2147483616u) == 16);
+  CHECK(kv8_steps(e) == (1u << 25) && kv8_per(65535ull << 25, 1, 4, 4) == 0x7ffffffcu);
   for (uint64_t pos : {16ull, 4096ull, 2147483632ull})
-    for (uint32_t batch : {1u, 65535u})
-      for (uint32_t rows : {1u, 16u, 17u, 2147483647u}) {
+    for (uint32_t batch : {1u, 65535u, 4294967295u})
+      for (uint32_t rows : {1u, 16u, 17u, 33u, 65u, 2147483647u}) {
         const Kv8Split s = kv8_split(batch, rows, 8, pos);
-        CHECK((uint64_t)s.chunk * s.nchunk >= pos && (uint64_t)s.chunk * (s.nchunk - 1) < pos);
-        CHECK((uint64_t)s.groups * s.rowsper >= rows);
+        CHECK((uint64_t)s.groups * s.rowsper >= rows && s.slots >= 1);
+        CHECK(s.one == (pos <= 256) && s.blocks >= (uint64_t)s.slots * 8 * s.groups);
       }
   printf("ok\n");
   return 0;
@@ -158,6 +185,7 @@ def test_workspace_bytes():
     """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
     w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
     assert w(1, 20, 5, 128, 16, 16) == 0 and w(1, 20, 5, 128, 16, 17) == 5 * 2 * 4 * 130 * 4
+    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5 + 3) * 5 * 4 * 130 * 4
     assert w(1, 20, 5, 128, 16, 17) == t(1, 1, 20, 5, 128, 16, 17)
     for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
                 (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
