@@ -419,7 +419,7 @@ int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const
  * zero; positions past the block table are not attended; table entries
  * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
  * and carry 22 bits of q and of the probabilities.  V rows
- * whose scales lie more than 2^18 below the largest in a chunk lose bits.
+ * whose scales lie more than 2^12 below the largest in a chunk lose bits.
  * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0 bytes: none is read), as
  * below; calls that share one run in stream order. */
 int nlg_decode_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt,

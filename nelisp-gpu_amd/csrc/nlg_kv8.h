@@ -102,27 +102,27 @@ NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 
 // of a kv head) come in groups of `rowsper`; up to 32 of them a workgroup's
 // waves share (they split the positions), from 33 on each wave has its own
 // (`wide`: they share K and V).  Positions are split by the lengths that the
-// kernel finds on the device: of all sequences' steps (64 positions) a chunk
-// takes 1 / want, at least `least`, in multiples of `unit`; a sequence's chunks
-// are of one size.  want fills the card once (two workgroups a CU), so there
-// are at most `slots` = want + batch chunks for each kv head and group.
+// kernel finds on the device (kv8_per); a sequence's chunks are of one size.
+// want: the chunks that fill the card once (two workgroups a CU) for each kv
+// head and group; slots: the most there can be.
 struct Kv8Split {
   uint32_t rowsper, groups, want, least, unit;
   uint64_t slots;
   bool wide, one;   // one: no sequence can have two chunks
   uint64_t blocks;  // workgroups
 };
-inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint64_t positions) {
+inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint32_t hd, uint64_t positions) {
   Kv8Split s;
   s.wide = rows > 32;
-  s.rowsper = rows > 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
+  s.rowsper = rows > 64 && hd == 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
   s.groups = (uint32_t)(((uint64_t)rows + s.rowsper - 1) / s.rowsper);
   s.unit = s.wide ? 1 : KV8_WAVES;
   s.least = 4;
   const uint64_t units = (uint64_t)kvheads * s.groups, most = (positions + KV8_STEP - 1) / KV8_STEP;
-  const uint64_t want = 512 / units ? 512 / units : 1, all = batch * ((most + s.least - 1) / s.least);
+  const uint64_t fill = s.wide ? 1024 : 512, want = fill / units ? fill / units : 1, all = batch * ((most + s.least - 1) / s.least);
   s.want = (uint32_t)want;
-  s.slots = want + batch < all ? want + batch : all;
+  const uint64_t upto = batch <= want / 2 ? want : 2 * want + batch;
+  s.slots = upto < all ? upto : all;
   s.one = most <= s.least;
   // (a multiple of eight of (slot, kv head)s: the groups of one lie on one XCD)
   s.blocks = (s.slots * kvheads + 7) / 8 * 8 * s.groups;
@@ -133,8 +133,13 @@ inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint6
 NLG_KV8_HD uint32_t kv8_steps(const Kv8Extent &e) {
   return !e.on ? 0u : e.end ? (e.end - 1) / KV8_STEP + 1 : 1u;
 }
-NLG_KV8_HD uint32_t kv8_per(uint64_t total, uint32_t want, uint32_t least, uint32_t unit) {
-  uint64_t per = (total + want - 1) / want;
+// A sequence's last chunk may be a small one, so total / per + batch of them
+// bound the chunks: few sequences are split so that this is want, and all
+// workgroups run at once; with many (batch over want / 2) there are several
+// rounds anyway, and the chunks are made small against the last one's tail.
+NLG_KV8_HD uint32_t kv8_per(uint64_t total, uint32_t batch, uint32_t want, uint32_t least, uint32_t unit) {
+  const uint64_t over = batch <= want / 2 ? want - batch : 2ull * want;
+  uint64_t per = (total + over - 1) / over;
   if (per < least) per = least;
   per = (per + unit - 1) / unit * unit;
   return per > 0x7fffffffu ? 0x7fffffffu / unit * unit : (uint32_t)per;

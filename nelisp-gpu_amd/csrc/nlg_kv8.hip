@@ -276,6 +276,8 @@ __device__ __forceinline__ half8v kv8_half8(uint32_t w0, uint32_t w1) {
 }
 // Eight f32 as halves hi + lo, each rounded to nearest: 22 bits together.
 __device__ __forceinline__ void split8(const float *w, half8v &hi, half8v &lo) {
+  float minus = -1.0f;  // (a factor the compiler does not see: one mixed FMA a remainder, not two instructions)
+  asm("" : "+s"(minus));
   union {
     half8v v;
     half2v p[4];
@@ -284,7 +286,7 @@ __device__ __forceinline__ void split8(const float *w, half8v &hi, half8v &lo) {
   for (int i = 0; i < 4; i++) {
     const float2v t = {w[2 * i], w[2 * i + 1]};
     a.p[i] = __builtin_convertvector(t, half2v);
-    const float2v r = {fmaf((float)a.p[i][0], -1.0f, t[0]), fmaf((float)a.p[i][1], -1.0f, t[1])};
+    const float2v r = {fmaf((float)a.p[i][0], minus, t[0]), fmaf((float)a.p[i][1], minus, t[1])};
     b.p[i] = __builtin_convertvector(r, half2v);
   }
   hi = a.v;
@@ -306,11 +308,18 @@ __device__ __forceinline__ void each(F &&f) {
     each<N, I + 1>(f);
   }
 }
+// (fmaxf would make each operand quiet first; a NaN may lose against any value:
+// the sums take it up again)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+  return r;
+}
 __device__ __forceinline__ float rows_max(float v) {  // over lanes 16, 32 and 48 apart
   float2 r = nlg_pair_f32<16>(v);
-  v = fmaxf(r.x, r.y);
+  v = max3(r.x, r.y, r.y);
   r = nlg_pair_f32<32>(v);
-  return fmaxf(r.x, r.y);
+  return max3(r.x, r.y, r.y);
 }
 __device__ __forceinline__ float rows_sum(float v) {
   float2 r = nlg_pair_f32<16>(v);
@@ -345,17 +354,19 @@ struct Kv8Plan {
     mine = of(a, 0, lane);
     uint64_t total = kv8_steps(mine);
     for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += kv8_steps(of(a, b0, lane));
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor((unsigned long long)total, o);
-    per = kv8_per(total, a.want, a.least, a.unit);
+    // (in two halves of 32 bits: a lane's part is below 2^42)
+    total = (uint64_t)(uint32_t)nlg_wave_sum_i32((int)(total & 0xffffff)) +
+            ((uint64_t)(uint32_t)nlg_wave_sum_i32((int)(total >> 24)) << 24);
+    per = kv8_per(total, a.batch, a.want, a.least, a.unit);
   }
   // inclusive sums over the lanes
-  static __device__ __forceinline__ uint32_t sums(uint32_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = __shfl_up(v, o);
-      if (lane >= o) v += u;
-    }
+  static __device__ __forceinline__ uint32_t sums(uint32_t v) {
+    v += (uint32_t)nlg_dpp<0x111>((int)v);       // row_shr:1
+    v += (uint32_t)nlg_dpp<0x112>((int)v);       // row_shr:2
+    v += (uint32_t)nlg_dpp<0x114>((int)v);       // row_shr:4
+    v += (uint32_t)nlg_dpp<0x118>((int)v);       // row_shr:8
+    v += (uint32_t)nlg_dpp<0x142, 0xa>((int)v);  // row_bcast:15 into rows 1, 3
+    v += (uint32_t)nlg_dpp<0x143, 0xc>((int)v);  // row_bcast:31 into rows 2, 3
     return v;
   }
   // The sequence and chunk of slot x; false: there are fewer.
@@ -364,7 +375,7 @@ struct Kv8Plan {
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
       const Kv8Extent l = at(a, b0, lane);
-      const uint32_t n = kv8_chunks(kv8_steps(l), per), to = sums(n, lane);
+      const uint32_t n = kv8_chunks(kv8_steps(l), per), to = sums(n);
       const uint64_t past = __ballot(before + to > x);
       if (past) {
         const int i = __builtin_ctzll(past);
@@ -385,7 +396,7 @@ struct Kv8Plan {
   __device__ __forceinline__ uint32_t first(const Kv8Attn &a, uint32_t b, int lane, uint32_t &chunks) const {
     uint32_t before = 0;
     for (uint32_t b0 = 0;; b0 += 64) {
-      const uint32_t n = kv8_chunks(kv8_steps(at(a, b0, lane)), per), to = sums(n, lane);
+      const uint32_t n = kv8_chunks(kv8_steps(at(a, b0, lane)), per), to = sums(n);
       if (b < b0 + 64) {
         chunks = __builtin_amdgcn_readlane(n, b - b0);
         return before + __builtin_amdgcn_readlane(to, b - b0) - chunks;
@@ -421,6 +432,15 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, uint32_t rowsper, int
   return true;
 }
 
+// A row's maximum m is a reference only: it moves when a score is more than
+// KV8_SLACK (in base 2) above it, so after a row's first steps its contexts are
+// hardly ever rescaled; the probabilities are below 2^KV8_SLACK, and times the V
+// scales in units of vref / 2^(15 - KV8_SLACK) they stay within fp16.
+#define KV8_SLACK 6.0f
+#define KV8_VUNIT 512.0f  // 2^(15 - KV8_SLACK)
+// The maximum of no score: finite, so that no difference of two is a NaN.
+#define KV8_FLOOR -1.7e38f
+
 // A wave's running state over NT tiles of sixteen query rows.  A lane holds the
 // query row n = lane & 15 of each tile, and of its scores the sixteen positions
 // of the step's tile g = lane >> 4.
@@ -429,8 +449,8 @@ struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
   float rs[NT];            // what the row's q was divided by (a power of two)
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
-  float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^15 / vref
-  float vref;              // a power of two no V scale so far exceeds, or 0
+  float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times KV8_VUNIT / vref
+  float vref, vinv;        // a power of two no V scale so far exceeds, or 0; KV8_VUNIT / vref
   uint32_t node[NT];
   uint64_t word[NT];       // the node's mask
 
@@ -469,29 +489,29 @@ struct WaveState {
         split8(x + c * 16, qh[i][2 * c], ql[i][2 * c]);
         split8(x + c * 16 + 8, qh[i][2 * c + 1], ql[i][2 * c + 1]);
       }
-      m[i] = -INFINITY;
+      m[i] = KV8_FLOOR;
       z[i] = 0.0f;
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
-    vref = 0.0f;
+    vref = vinv = 0.0f;
   }
 
-  // V scales in units of vref / 2^15: the probabilities times them, as halves,
-  // then use the type's whole range.  vs: this lane's of the step; returns what
+  // V scales in units of vref / KV8_VUNIT: the probabilities times them, as
+  // halves, then use the type's whole range.  vs: this lane's of the step; returns what
   // the contexts so far are to be multiplied by.
   __device__ __forceinline__ float rescale(float &vs) {
-    float vtop = fabsf(vs);
-    vtop = vtop <= 3.4028234663852886e38f ? vtop : 0.0f;
-    vtop = nlg_wave_max_f32(vtop);
     float f = 1.0f;
-    if (vtop > vref) {  // the same in every lane
-      const int e = __builtin_amdgcn_frexp_expf(vtop);
-      const float nv = ldexpf(1.0f, e < -100 ? -100 : e);
-      f = vref / nv;
+    const float mag = fabsf(vs) <= 3.4028234663852886e38f ? fabsf(vs) : 0.0f;
+    if (__any(mag > vref)) {
+      const int e = __builtin_amdgcn_frexp_expf(nlg_wave_max_f32(mag));
+      const int ne = e < -100 ? -100 : e;
+      const float nv = ldexpf(1.0f, ne);
+      f = vref > 0.0f ? vref * ldexpf(1.0f, -ne) : 0.0f;
       vref = nv;
+      vinv = ldexpf(KV8_VUNIT, -ne);
     }
-    vs = vref > 0.0f ? vs * (32768.0f / vref) : vs;
+    vs = vs * vinv;
     return f;
   }
 
@@ -507,26 +527,27 @@ struct WaveState {
       s[j] = acc[j >> 2][j & 3] * row_lane<j>(ks);
       if (GEN) s[j] = bits >> j & 1 ? s[j] : -INFINITY;
     });
-    float top[4];
+    float top = max3(s[0], s[1], s[2]);
 #pragma unroll
-    for (int j = 0; j < 4; j++) top[j] = fmaxf(fmaxf(s[j], s[j + 4]), fmaxf(s[j + 8], s[j + 12]));
-    const float t = rows_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))) * rs[i];
-    const float mn = fmaxf(m[i], t);
-    const float ms = mn == -INFINITY ? 0.0f : mn;
-    const float al = nlg_exp2(m[i] - ms);
-    m[i] = mn;
-    float zz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 3; j < 15; j += 2) top = max3(top, s[j], s[j + 1]);
+    top = max3(top, s[15], s[15]) * rs[i];
+    if (__any(top > m[i] + KV8_SLACK || vresc != 1.0f)) {
+      top = rows_max(top);
+      const float mn = top > m[i] + KV8_SLACK ? top : m[i];
+      const float al = nlg_exp2(m[i] - mn), sc = al * vresc;
+      m[i] = mn;
+      z[i] = z[i] * al;
+#pragma unroll
+      for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;
+    }
+    const float ms = m[i];
+    float zz[4] = {z[i], 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       s[j] = nlg_exp2(fmaf(s[j], rs[i], -ms));
       zz[j & 3] = zz[j & 3] + s[j];
     }
-    z[i] = fmaf(z[i], al, (zz[0] + zz[1]) + (zz[2] + zz[3]));
-    const float sc = al * vresc;
-    if (__any(sc != 1.0f)) {
-#pragma unroll
-      for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;
-    }
+    z[i] = (zz[0] + zz[1]) + (zz[2] + zz[3]);
     each<16>([&](auto J) {
       constexpr int j = decltype(J)::value;
       s[j] = s[j] * row_lane<j>(vs);
@@ -556,18 +577,17 @@ __device__ __forceinline__ uint4 and4(uint4 x, uint4 m) { return make_uint4(x.x 
 
 #define MFMA(x, y, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0)
 
-// One step of a wave on its own: 64 positions, tile `tk` holding this lane's K
-// row (4 positions of each of the four tiles a time), tile `tv` its V columns
-// and both scales.  GEN: some of the positions are masked, absent or past the
-// end; bits[i]: which of this lane's sixteen the query row of tile i attends;
-// left: how many of them exist.
-template <int HD, int FMT, int NT, bool GEN>
-__device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w, uint32_t tk, uint32_t tv,
-                                         const uint32_t *bits, int left, int lane) {
+// One step of a wave on its own: 64 positions from p on, tile `tk` holding this
+// lane's K row (4 positions of each of the four tiles a time), tile `tv` its V
+// columns and both scales.  GEN: some of the positions are masked or past the
+// end.
+template <int HD, int FMT, int NT, bool GEN, bool TREE>
+__device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, WaveState<HD, NT> &w, uint32_t tk,
+                                         uint32_t tv, uint32_t p, int lane) {
   constexpr int C = HD / 64, D = HD / 16;
   const int g = lane >> 4, n = lane & 15;
   uint4 kr[4][C], vr[D];
-  const bool hk = !GEN || tk != KV8_NONE, hv = !GEN || tv != KV8_NONE;
+  const bool hk = tk != KV8_NONE, hv = tv != KV8_NONE;
   const uint8_t *kp = a.kpool + (size_t)(hk ? tk : 0) * kv8_tile_bytes(HD) + (lane & 3) * HD + g * 16;
   const size_t vt = (size_t)(hv ? tv : 0) * kv8_tile_bytes(HD);
   const uint8_t *vp = a.vpool + vt;
@@ -579,7 +599,9 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w,
     for (int c = 0; c < C; c++) kr[t][c] = *(const uint4 *)(kp + t * 4 * HD + c * 64);
 #pragma unroll
   for (int i = 0; i < D; i++) vr[i] = *(const uint4 *)(vp + i * 256 + n * 16);
-  if (GEN) {
+  const uint32_t q0 = p + g * KV8_TILE;  // this lane's first position
+  const int left = GEN ? kv8_left(k.e, q0) : 16;
+  if (__any(!hv || left < 16)) {
     // absent tiles read as zero rows; what lies past the end is not used
     if (!hk)
 #pragma unroll
@@ -594,67 +616,71 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, WaveState<HD, NT> &w,
   const float vresc = w.rescale(vs);
 #pragma unroll
   for (int i = 0; i < NT; i++) {
+    // (four sums side by side: a product waits for the one before it on its sum)
     float4v acc[4];
+    const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      acc[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 2 * C; c++) {
+      half8v f[4];
 #pragma unroll
-      for (int c = 0; c < C; c++) {
-        const half8v k0 = kv8_half8<FMT>(kr[t][c].x, kr[t][c].y), k1 = kv8_half8<FMT>(kr[t][c].z, kr[t][c].w);
-        acc[t] = MFMA(k0, w.ql[i][2 * c], acc[t]);
-        acc[t] = MFMA(k1, w.ql[i][2 * c + 1], acc[t]);
-        acc[t] = MFMA(k0, w.qh[i][2 * c], acc[t]);
-        acc[t] = MFMA(k1, w.qh[i][2 * c + 1], acc[t]);
-      }
+      for (int t = 0; t < 4; t++)
+        f[t] = c & 1 ? kv8_half8<FMT>(kr[t][c / 2].z, kr[t][c / 2].w) : kv8_half8<FMT>(kr[t][c / 2].x, kr[t][c / 2].y);
+#pragma unroll
+      for (int t = 0; t < 4; t++) acc[t] = MFMA(f[t], w.ql[i][c], c ? acc[t] : none);
+#pragma unroll
+      for (int t = 0; t < 4; t++) acc[t] = MFMA(f[t], w.qh[i][c], acc[t]);
     }
     half8v ph[2], pl[2];
-    w.template soften<GEN>(i, acc, ks, vs, vresc, GEN ? bits[i] : 0, ph, pl);
+    const uint32_t bits = GEN ? TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], q0) : (1u << left) - 1 : 0u;
+    w.template soften<GEN>(i, acc, ks, vs, vresc, bits, ph, pl);
 #pragma unroll
-    for (int d = 0; d < D; d++) {
-      const half8v v0 = kv8_half8<FMT>(vr[d].x, vr[d].y), v1 = kv8_half8<FMT>(vr[d].z, vr[d].w);
-      w.o[i][d] = MFMA(v0, pl[0], w.o[i][d]);
-      w.o[i][d] = MFMA(v1, pl[1], w.o[i][d]);
-      w.o[i][d] = MFMA(v0, ph[0], w.o[i][d]);
-      w.o[i][d] = MFMA(v1, ph[1], w.o[i][d]);
-    }
+    for (int d = 0; d < D; d += 4)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        half8v f[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          f[j] = u ? kv8_half8<FMT>(vr[d + j].z, vr[d + j].w) : kv8_half8<FMT>(vr[d + j].x, vr[d + j].y);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.o[i][d + j] = MFMA(f[j], pl[u], w.o[i][d + j]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.o[i][d + j] = MFMA(f[j], ph[u], w.o[i][d + j]);
+      }
   }
 }
 
 // Up to 32 rows (16 NT): the workgroup's waves take its positions in turn, 64 at
 // a time, straight from memory into the matrix cores' operands, and meet in LDS.
 template <int HD, int FMT, int NT, bool TREE>
-__global__ __launch_bounds__(64 * KV8_WAVES) void k_attn_q8(Kv8Attn a) {
+__global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 2 : 1, 2))) void k_attn_q8(Kv8Attn a) {
   constexpr int D = HD / 16;
   __shared__ float4v s_o[KV8_WAVES][D][64];
   __shared__ float s_m[KV8_WAVES][16], s_z[KV8_WAVES][16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
   if (!kv8_work<TREE>(a, NT * 16, lane, k)) return;
+  uint32_t tid = kv8_tiles(a, k, k.c0, lane);
   WaveState<HD, NT> w;
   w.begin(a, k, k.row0, lane);
   const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;  // no mask below this position
-  for (uint32_t p0 = k.c0; p0 < k.c1; p0 += 64 * KV8_TILE) {
-    const uint32_t tid = kv8_tiles(a, k, p0, lane);
-    const uint32_t p1 = k.c1 - p0 < 64 * KV8_TILE ? k.c1 : p0 + 64 * KV8_TILE;
-    for (uint32_t p = p0 + wv * KV8_STEP; p < p1; p += KV8_WAVES * KV8_STEP) {
-      const int t0 = (int)(p - p0) / KV8_TILE;
-      const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
-      if (p + KV8_STEP > whole || __any(tv == KV8_NONE)) {
-        uint32_t bits[NT];
-        const uint32_t q0 = p + g * KV8_TILE;  // this lane's first position
-        const int left = kv8_left(k.e, q0);
-#pragma unroll
-        for (int i = 0; i < NT; i++)
-          bits[i] = TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], q0) : (1u << left) - 1;
-        kv8_step<HD, FMT, NT, true>(a, w, tk, tv, bits, left, lane);
-      } else {
-        kv8_step<HD, FMT, NT, false>(a, w, tk, tv, nullptr, 16, lane);
-      }
+  uint32_t p0 = k.c0;  // tid: the tiles from here on
+  uint32_t p = k.c0 + wv * KV8_STEP;
+  auto step = [&](auto GENV) {
+    const uint32_t from = k.c0 + (p - k.c0) / (64 * KV8_TILE) * (64 * KV8_TILE);
+    if (from != p0) {
+      p0 = from;
+      tid = kv8_tiles(a, k, p0, lane);
     }
-  }
+    const int t0 = (int)(p - p0) / KV8_TILE;
+    const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
+    kv8_step<HD, FMT, NT, decltype(GENV)::value != 0, TREE>(a, k, w, tk, tv, p, lane);
+    p += KV8_WAVES * KV8_STEP;
+  };
+  while (p + KV8_STEP <= whole) step(Int<0>{});
+  while (p < k.c1) step(Int<1>{});
 
   // the waves' parts meet, one tile of rows at a time
-  const float vs = w.vref > 0.0f ? w.vref * (1.0f / 32768.0f) : 0.0f;
+  const float vs = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NT; i++) {
     if (i) __syncthreads();
@@ -669,11 +695,10 @@ __global__ __launch_bounds__(64 * KV8_WAVES) void k_attn_q8(Kv8Attn a) {
     float mm = s_m[0][n];
 #pragma unroll
     for (int j = 1; j < KV8_WAVES; j++) mm = fmaxf(mm, s_m[j][n]);
-    const float ms = mm == -INFINITY ? 0.0f : mm;
     float f[KV8_WAVES], zz = 0.0f;
 #pragma unroll
     for (int j = 0; j < KV8_WAVES; j++) {
-      f[j] = nlg_exp2(s_m[j][n] - ms);
+      f[j] = nlg_exp2(s_m[j][n] - mm);
       zz = fmaf(s_z[j][n], f[j], zz);
     }
     const uint32_t row = k.row0 + i * 16 + n;
@@ -694,14 +719,16 @@ __global__ __launch_bounds__(64 * KV8_WAVES) void k_attn_q8(Kv8Attn a) {
   }
 }
 
-// More rows: each wave has 16 NT of its own, all walk the same positions, and K
-// and V are made halves once for the workgroup, in LDS, in the order in which
-// the waves' operands lie (a fragment's 64 lanes side by side: no bank is asked
-// twice).  While a step is computed the next one's halves are written and the
-// one's after it are on their way from memory.
+// More rows: each of the waves has 16 NT of its own, all walk the same positions,
+// and K and V are made halves once for the workgroup, in LDS, in the order in
+// which the waves' operands lie (a fragment's 64 lanes side by side: no bank is
+// asked twice).  While a step is computed the next one's halves are written and
+// the one's after it are on their way from memory.  Two waves a SIMD: the
+// matrix cores work for one while the other is at its softmax.
 template <int HD, int FMT, int NT, bool TREE>
-__global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
-  constexpr int C = HD / 64, D = HD / 16, DW = D / KV8_WAVES;
+__global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void k_attn_wide_q8(Kv8Attn a) {
+  constexpr int C = HD / 64, D = HD / 16, DW = D / 4;
   __shared__ half8v s_k[2][4][2 * C][64], s_v[2][D][2][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
@@ -733,9 +760,9 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
     ks = *(const float *)(a.kpool + vt + kv8_scale_byte(HD, n));
     vs = *(const float *)(a.vpool + vt + kv8_scale_byte(HD, n));
 #pragma unroll
-    for (int c = 0; c < C; c++) kr[c] = *(const uint4 *)(kp + c * 64);
+      for (int c = 0; c < C; c++) kr[c] = *(const uint4 *)(kp + c * 64);
 #pragma unroll
-    for (int d = 0; d < DW; d++) vr[d] = *(const uint4 *)(vp + d * 256);
+      for (int d = 0; d < DW; d++) vr[d] = *(const uint4 *)(vp + d * 256);
     const int left = kv8_left(k.e, p + g * KV8_TILE);
     if (__any(!hv || left < 16)) {
       if (!hk)
@@ -749,34 +776,41 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
   };
   auto store = [&](int buf) {
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-      s_k[buf][wv][2 * c][lane] = kv8_half8<FMT>(kr[c].x, kr[c].y);
-      s_k[buf][wv][2 * c + 1][lane] = kv8_half8<FMT>(kr[c].z, kr[c].w);
-    }
+      for (int c = 0; c < C; c++) {
+        s_k[buf][wv][2 * c][lane] = kv8_half8<FMT>(kr[c].x, kr[c].y);
+        s_k[buf][wv][2 * c + 1][lane] = kv8_half8<FMT>(kr[c].z, kr[c].w);
+      }
 #pragma unroll
-    for (int d = 0; d < DW; d++) {
-      s_v[buf][wv * DW + d][0][lane] = kv8_half8<FMT>(vr[d].x, vr[d].y);
-      s_v[buf][wv * DW + d][1][lane] = kv8_half8<FMT>(vr[d].z, vr[d].w);
-    }
+      for (int d = 0; d < DW; d++) {
+        s_v[buf][wv * DW + d][0][lane] = kv8_half8<FMT>(vr[d].x, vr[d].y);
+        s_v[buf][wv * DW + d][1][lane] = kv8_half8<FMT>(vr[d].z, vr[d].w);
+      }
   };
   auto compute = [&](auto GENV, int buf, float ksc, float vsc, uint32_t p) {
     constexpr bool GEN = decltype(GENV)::value != 0;
     const float vresc = w.rescale(vsc);
     float4v acc[NT][4];
+    const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
+    half8v f[2][4];
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
+    for (int t = 0; t < 4; t++) f[0][t] = s_k[buf][t][0][lane];
 #pragma unroll
-      for (int i = 0; i < NT; i++) acc[i][t] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c = 0; c < 2 * C; c++) {
 #pragma unroll
-      for (int c = 0; c < 2 * C; c++) {
-        const half8v f = s_k[buf][t][c][lane];
+      for (int t = 0; t < 4; t++)
+        if (c + 1 < 2 * C) f[(c + 1) & 1][t] = s_k[buf][t][c + 1][lane];
 #pragma unroll
-        for (int i = 0; i < NT; i++) {
-          acc[i][t] = MFMA(f, w.ql[i][c], acc[i][t]);
-          acc[i][t] = MFMA(f, w.qh[i][c], acc[i][t]);
-        }
-      }
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[i][t] = MFMA(f[c & 1][t], w.ql[i][c], c ? acc[i][t] : none);
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int t = 0; t < 4; t++) acc[i][t] = MFMA(f[c & 1][t], w.qh[i][c], acc[i][t]);
+      __builtin_amdgcn_sched_barrier(0);
     }
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[0][j] = s_v[buf][j][0][lane];
     half8v ph[NT][2], pl[NT][2];
 #pragma unroll
     for (int i = 0; i < NT; i++) {
@@ -786,15 +820,20 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
       w.template soften<GEN>(i, acc[i], ksc, vsc, vresc, bits, ph[i], pl[i]);
     }
 #pragma unroll
-    for (int d = 0; d < D; d++) {
-      const half8v v0 = s_v[buf][d][0][lane], v1 = s_v[buf][d][1][lane];
+    for (int r = 0; r < D / 2; r++) {  // four sixteens of dimensions, half of the positions
+      const int d = r / 2 * 4, u = r & 1;
 #pragma unroll
-      for (int i = 0; i < NT; i++) {
-        w.o[i][d] = MFMA(v0, pl[i][0], w.o[i][d]);
-        w.o[i][d] = MFMA(v1, pl[i][1], w.o[i][d]);
-        w.o[i][d] = MFMA(v0, ph[i][0], w.o[i][d]);
-        w.o[i][d] = MFMA(v1, ph[i][1], w.o[i][d]);
-      }
+      for (int j = 0; j < 4; j++)
+        if (r + 1 < D / 2) f[(r + 1) & 1][j] = s_v[buf][(r + 1) / 2 * 4 + j][(r + 1) & 1][lane];
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.o[i][d + j] = MFMA(f[r & 1][j], pl[i][u], w.o[i][d + j]);
+#pragma unroll
+      for (int i = 0; i < NT; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) w.o[i][d + j] = MFMA(f[r & 1][j], ph[i][u], w.o[i][d + j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   if (k.c0 < k.c1) {
@@ -804,7 +843,8 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
     if (k.c1 - k.c0 > KV8_STEP) load(k.c0 + KV8_STEP);
     __syncthreads();
     int buf = 0;
-    for (uint32_t p = k.c0; p < k.c1; p += KV8_STEP, buf ^= 1) {
+    uint32_t p = k.c0;
+    auto turn = [&](auto &&work) {
       float ksn = 0.0f, vsn = 0.0f;
       if (k.c1 - p > KV8_STEP) {
         store(buf ^ 1);
@@ -812,17 +852,22 @@ __global__ __launch_bounds__(64 * KV8_WAVES, 2) void k_attn_wide_q8(Kv8Attn a) {
         vsn = vs;
         if (k.c1 - p > 2 * KV8_STEP) load(p + 2 * KV8_STEP);
       }
-      if (rows && p < stop) {
-        if (p + KV8_STEP > whole) compute(Int<1>{}, buf, ksc, vsc, p);
-        else compute(Int<0>{}, buf, ksc, vsc, p);
-      }
+      work();
       __syncthreads();
       ksc = ksn;
       vsc = vsn;
+      buf ^= 1;
+      p += KV8_STEP;
+    };
+    // (loops of their own, not branches of one: where two ways meet, the contexts are copied)
+    if (rows) {
+      while (p + KV8_STEP <= whole) turn([&] { compute(Int<0>{}, buf, ksc, vsc, p); });
+      while (p < stop && p < k.c1) turn([&] { compute(Int<1>{}, buf, ksc, vsc, p); });
     }
+    while (p < k.c1) turn([] {});
   }
   if (!rows) return;
-  const float vu = w.vref > 0.0f ? w.vref * (1.0f / 32768.0f) : 0.0f;
+  const float vu = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NT; i++) {
     const float z = rows_sum(w.z[i]);
@@ -855,15 +900,15 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
   const bool on = node < e.nodes;
   const uint64_t p0 = ((uint64_t)slot * a.pg.kvheads + head / a.grp) * a.rows + (uint64_t)node * a.grp + head % a.grp;
   const uint64_t step = (uint64_t)a.pg.kvheads * a.rows;
-  float m = -INFINITY, z = 0.0f;
+  float m = KV8_FLOOR, z = 0.0f;
   float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (on)
     for (uint32_t c = sub; c < chunks; c += SUBS) {
       const uint64_t p = p0 + c * step;
       const float2 x = *(const float2 *)(a.pmz + p * 2);
       const float4v y = *(const float4v *)(a.pctx + p * hd + d);
-      const float mn = fmaxf(m, x.x), ms = mn == -INFINITY ? 0.0f : mn;
-      const float f = nlg_exp2(m - ms), fx = nlg_exp2(x.x - ms);
+      const float mn = fmaxf(m, x.x);
+      const float f = nlg_exp2(m - mn), fx = nlg_exp2(x.x - mn);
       m = mn;
       z = fmaf(z, f, x.y * fx);
       o = o * f + y * fx;
@@ -876,13 +921,13 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
     float mm = m;
 #pragma unroll
     for (int i = 1; i < SUBS; i++) mm = fmaxf(mm, s_mz[t + i * per].x);
-    const float ms = mm == -INFINITY ? 0.0f : mm, f = nlg_exp2(m - ms);
+    const float f = nlg_exp2(m - mm);
     z = z * f;
     o = o * f;
 #pragma unroll
     for (int i = 1; i < SUBS; i++) {
       const float2 x = s_mz[t + i * per];
-      const float fx = nlg_exp2(x.x - ms);
+      const float fx = nlg_exp2(x.x - mm);
       z = fmaf(x.y, fx, z);
       o = o + s_o[t + i * per] * fx;
     }
@@ -1148,7 +1193,7 @@ extern "C" size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax
   if (!batch || !rows || !bs || bs % KV8_TILE || !mbps || (uint64_t)bs * mbps > 0x7fffffffull ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, (uint64_t)bs * mbps), rows, kvheads, head_dim);
+  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, head_dim, (uint64_t)bs * mbps), rows, kvheads, head_dim);
 }
 extern "C" size_t nlg_decode_attn_paged_q8_workspace(uint32_t batch, uint32_t heads, uint32_t kvheads,
                                                      uint32_t head_dim, uint32_t bs, uint32_t mbps) {
@@ -1168,13 +1213,13 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   if (!rows) return nlg_fail("%s: %u heads over %u kv heads, %u queries", what, heads, kvheads, tmax);
   if (mask && tmax > KV8_TREE) return nlg_fail("%s: %u nodes under a mask (at most %d)", what, tmax, KV8_TREE);
   if (mask && ((uintptr_t)mask & 7)) return nlg_fail("%s: the masks must be 8-byte aligned", what);
-  const Kv8Split s = kv8_split(batch, (uint32_t)rows, kvheads, (uint64_t)bs * mbps);
+  const Kv8Split s = kv8_split(batch, (uint32_t)rows, kvheads, hd, (uint64_t)bs * mbps);
   const uint64_t need = kv8_partials(s, rows, kvheads, hd);
   // joining: eight groups of threads a row while its rows would not fill the card with one
   const uint64_t orows = (uint64_t)tmax * heads;
-  const bool subs = orows * batch * (hd / 4) < 256 * 2048;
+  const bool subs = orows * batch * (hd / 4) < 65536;
   const uint64_t oper = 256 / (hd / 4) / (subs ? 8 : 1), oblocks = (orows + oper - 1) / oper;
-  if (!nlg_fits(s.blocks, 64 * KV8_WAVES) || !nlg_fits(oblocks * batch, 256) || orows > 0xffffffffull)
+  if (!nlg_fits(s.blocks, 256) || !nlg_fits(oblocks * batch, 256) || orows > 0xffffffffull)
     return nlg_fail("%s: too many queries for one launch", what);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -1189,14 +1234,14 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   a.pctx = (float *)workspace;
   a.pmz = need ? a.pctx + s.slots * kvheads * rows * hd : nullptr;
   a.coef = NLG_LOG2E / sqrtf((float)hd);
-  const dim3 grid((uint32_t)s.blocks), blk(64 * KV8_WAVES);
+  const dim3 grid((uint32_t)s.blocks);
   hipStream_t st = nlg_stream(stream);
-#define GO3(HD, F, T)                                                                            \
-  do {                                                                                           \
-    if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, T>), grid, blk, 0, st, a);      \
-    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, T>), grid, blk, 0, st, a); \
-    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1, T>), grid, blk, 0, st, a); \
-    else hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 2, T>), grid, blk, 0, st, a);                 \
+#define GO3(HD, F, T)                                                                                 \
+  do {                                                                                                \
+    if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, T>), grid, dim3(256), 0, st, a);     \
+    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, T>), grid, dim3(256), 0, st, a); \
+    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1, T>), grid, dim3(256), 0, st, a); \
+    else hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 2, T>), grid, dim3(256), 0, st, a);                \
   } while (0)
 #define GO(HD, F)               \
   do {                          \

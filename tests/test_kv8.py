@@ -39,7 +39,7 @@ static int layout(uint32_t hd) {
 static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int32_t> nodes, uint32_t tmax, uint32_t grp,
                 uint32_t bs, uint32_t mbps, uint32_t kvheads) {
   const uint32_t cap = bs * mbps, rows = tmax * grp, batch = at.size();
-  const Kv8Split s = kv8_split(batch, rows, kvheads, cap);
+  const Kv8Split s = kv8_split(batch, rows, kvheads, rnd(2) ? 64 : 128, cap);
   CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows && s.want >= 1);
   // every (slot, kv head, group) is some workgroup's, as the kernels number them
   std::vector<int> seen((size_t)s.slots * kvheads * s.groups);
@@ -55,7 +55,7 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
     CHECK(e[b].end <= cap);
     total += kv8_steps(e[b]);
   }
-  const uint32_t per = kv8_per(total, s.want, s.least, s.unit);
+  const uint32_t per = kv8_per(total, batch, s.want, s.least, s.unit);
   CHECK(per % s.unit == 0 && per >= s.least);
   for (uint32_t b = 0; b < batch; b++) {
     const int64_t nn = !tree ? 1 : nodes[b] < 0 ? 0 : nodes[b] > (int64_t)tmax ? tmax : nodes[b];
@@ -130,11 +130,11 @@ int main(void) {
   if (call(false, false, {2147483647}, {1}, 1, 1, 16, 1, 1) || call(true, false, {2147483647}, {5}, 5, 1, 16, 2, 1)) return 1;
   const Kv8Extent e = kv8_extent(true, 2147483647, 2147483647, 2147483647u, 2147483632u);
   CHECK(e.end == 2147483632u && e.base == 2147483647u && kv8_left(e, 2147483616u) == 16);
-  CHECK(kv8_steps(e) == (1u << 25) && kv8_per(65535ull << 25, 1, 4, 4) == 0x7ffffffcu);
+  CHECK(kv8_steps(e) == (1u << 25) && kv8_per(65535ull << 25, 1, 1, 4, 4) == 0x7ffffffcu);
   for (uint64_t pos : {16ull, 4096ull, 2147483632ull})
     for (uint32_t batch : {1u, 65535u, 4294967295u})
       for (uint32_t rows : {1u, 16u, 17u, 33u, 65u, 2147483647u}) {
-        const Kv8Split s = kv8_split(batch, rows, 8, pos);
+        const Kv8Split s = kv8_split(batch, rows, 8, 64, pos);
         CHECK((uint64_t)s.groups * s.rowsper >= rows && s.slots >= 1);
         CHECK(s.one == (pos <= 256) && s.blocks >= (uint64_t)s.slots * 8 * s.groups);
       }
@@ -185,7 +185,7 @@ def test_workspace_bytes():
     """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
     w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
     assert w(1, 20, 5, 128, 16, 16) == 0 and w(1, 20, 5, 128, 16, 17) == 5 * 2 * 4 * 130 * 4
-    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5 + 3) * 5 * 4 * 130 * 4
+    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 4 * 130 * 4
     assert w(1, 20, 5, 128, 16, 17) == t(1, 1, 20, 5, 128, 16, 17)
     for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
                 (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
