@@ -37,42 +37,51 @@ inline uint64_t kv8_pool_bytes(uint32_t npool, uint32_t bs, uint32_t kvheads, ui
   return tiles * kv8_tile_bytes(hd);
 }
 
+// Division of n < 2^31 by a number that the host knows: n * mul / 2^shift, mul
+// the quotient 2^shift / d rounded up with shift = 31 + ceil(log2 d), so that
+// its error, below 1 / 2^31 of a step, never reaches the next quotient.
+struct Kv8Div {
+  uint32_t d, mul, shift;
+};
+inline Kv8Div kv8_div(uint32_t d) {
+  uint32_t l = 0;
+  while (l < 31 && (1ull << l) < d) l++;
+  return Kv8Div{d, (uint32_t)(((1ull << (31 + l)) + d - 1) / d), 31 + l};
+}
+NLG_KV8_HD uint32_t kv8_quot(const Kv8Div &v, uint32_t n) { return (uint32_t)(((uint64_t)n * v.mul) >> v.shift); }
+
 // What finds a position's tile.
 struct Kv8Pages {
-  const int32_t *table;                // [batch][mbps]
-  uint32_t npool, mbps, bpt, kvheads;  // bpt: tiles of a block
+  const int32_t *table;          // [batch][mbps]
+  uint32_t npool, mbps, kvheads;
+  Kv8Div bpt;                    // tiles of a block
 };
 #define KV8_NONE 0xffffffffu
-// The tile of sequence b's tile number t (position / 16) and kv head h, or
+// The tile of sequence b's tile number t (position / 16, below 2^31) and kv head h, or
 // KV8_NONE outside the table or the pool.
 NLG_KV8_HD uint32_t kv8_tile(const Kv8Pages &g, uint32_t b, uint32_t h, uint32_t t) {
-  const uint32_t blk = t / g.bpt;
+  const uint32_t blk = kv8_quot(g.bpt, t);
   if (blk >= g.mbps) return KV8_NONE;
   const int32_t ph = g.table[(uint64_t)b * g.mbps + blk];
   if (ph < 0 || (uint32_t)ph >= g.npool) return KV8_NONE;
-  return ((uint32_t)ph * g.kvheads + h) * g.bpt + t % g.bpt;
+  return ((uint32_t)ph * g.kvheads + h) * g.bpt.d + (t - blk * g.bpt.d);
 }
 
 // The positions of a sequence: those below `base` all rows attend, those from
-// base to end hold nodes (none without a tree); on: it takes part at all.
+// base to end hold nodes; on: it takes part at all.  A decoded token is one
+// node at the last position.
 struct Kv8Extent {
   uint32_t base, end, nodes;
   bool on;
 };
-// at: the last position, or with a tree the slot of node 0; cap: the block table's positions.
+// at: the slot of node 0; cap: the block table's positions.  A sequence without
+// a slot or nodes takes no part in a tree; a decoded one attends nothing.
 NLG_KV8_HD Kv8Extent kv8_extent(bool tree, int32_t at, int32_t nodes, uint32_t tmax, uint32_t cap) {
   Kv8Extent e;
-  if (!tree) {
-    e.end = at < 0 ? 0u : (uint32_t)at >= cap ? cap : (uint32_t)at + 1;
-    e.base = e.end;
-    e.nodes = 1;
-    e.on = true;
-  } else {
-    e.nodes = nodes < 0 ? 0u : (uint32_t)nodes > tmax ? tmax : (uint32_t)nodes;
-    e.base = at < 0 ? 0u : (uint32_t)at;
-    e.end = e.base + e.nodes < cap ? e.base + e.nodes : cap;
-    e.on = at >= 0 && e.nodes;
-  }
+  e.nodes = nodes < 0 ? 0u : (uint32_t)nodes > tmax ? tmax : (uint32_t)nodes;
+  e.base = at < 0 ? 0u : (uint32_t)at;
+  e.end = at < 0 ? 0u : e.base + e.nodes < cap ? e.base + e.nodes : cap;
+  e.on = !tree || (at >= 0 && e.nodes);
   return e;
 }
 // Where the rows of nodes up to `last` stop attending, without a mask.
@@ -103,12 +112,12 @@ NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 
 // waves share (they split the positions), from 33 on each wave has its own
 // (`wide`: they share K and V).  Positions are split by the lengths that the
 // kernel finds on the device (kv8_per); a sequence's chunks are of one size.
-// want: the chunks that fill the card once (two workgroups a CU) for each kv
-// head and group; slots: the most there can be.
+// want: the chunks that fill the card for each kv head and group; slots: the
+// most there can be.  one: no sequence is split, and its slot is its number.
 struct Kv8Split {
   uint32_t rowsper, groups, want, least, unit;
   uint64_t slots;
-  bool wide, one;   // one: no sequence can have two chunks
+  bool wide, one;
   uint64_t blocks;  // workgroups
 };
 inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint32_t hd, uint64_t positions) {
@@ -119,11 +128,13 @@ inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint3
   s.unit = s.wide ? 1 : KV8_WAVES;
   s.least = 4;
   const uint64_t units = (uint64_t)kvheads * s.groups, most = (positions + KV8_STEP - 1) / KV8_STEP;
-  const uint64_t fill = s.wide ? 1024 : 512, want = fill / units ? fill / units : 1, all = batch * ((most + s.least - 1) / s.least);
+  // two workgroups a CU at once; wide ones, whose steps cost more than their loads, in two rounds
+  const uint64_t fill = s.wide ? 1024 : 512, want = fill / units ? fill / units : 1;
+  const uint64_t all = batch * ((most + s.least - 1) / s.least), upto = batch <= want / 2 ? want : 2 * want + batch;
   s.want = (uint32_t)want;
-  const uint64_t upto = batch <= want / 2 ? want : 2 * want + batch;
-  s.slots = upto < all ? upto : all;
-  s.one = most <= s.least;
+  // (eight waves to a workgroup take 1,024 positions in two steps each: less than a second launch)
+  s.one = most <= (s.rowsper == 16 ? 16 : s.least);
+  s.slots = s.one ? batch : upto < all ? upto : all;
   // (a multiple of eight of (slot, kv head)s: the groups of one lie on one XCD)
   s.blocks = (s.slots * kvheads + 7) / 8 * 8 * s.groups;
   return s;
@@ -138,8 +149,8 @@ NLG_KV8_HD uint32_t kv8_steps(const Kv8Extent &e) {
 // workgroups run at once; with many (batch over want / 2) there are several
 // rounds anyway, and the chunks are made small against the last one's tail.
 NLG_KV8_HD uint32_t kv8_per(uint64_t total, uint32_t batch, uint32_t want, uint32_t least, uint32_t unit) {
-  const uint64_t over = batch <= want / 2 ? want - batch : 2ull * want;
-  uint64_t per = (total + over - 1) / over;
+  const uint32_t over = batch <= want / 2 ? want - batch : 2 * want;
+  uint64_t per = total >> 32 ? total / over + 1 : ((uint32_t)total - 1u) / over + 1u;  // (total is not 0)
   if (per < least) per = least;
   per = (per + unit - 1) / unit * unit;
   return per > 0x7fffffffu ? 0x7fffffffu / unit * unit : (uint32_t)per;

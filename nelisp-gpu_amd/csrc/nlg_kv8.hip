@@ -245,6 +245,8 @@ struct Kv8Attn {
   float *out, *pctx, *pmz;  // partials: [slots][kvheads][rows][hd], [slots][kvheads][rows][2]
   uint32_t batch, tmax, heads, grp, rows;  // rows = tmax * grp
   uint32_t groups, want, least, unit, slots;  // Kv8Split
+  Kv8Div by8groups, bykvheads, bygrp;
+  bool tree, one;
   float coef;  // log2(e) / sqrt(hd): scores in base 2
 };
 
@@ -286,9 +288,29 @@ __device__ __forceinline__ void split8(const float *w, half8v &hi, half8v &lo) {
   for (int i = 0; i < 4; i++) {
     const float2v t = {w[2 * i], w[2 * i + 1]};
     a.p[i] = __builtin_convertvector(t, half2v);
-    const float2v r = {fmaf((float)a.p[i][0], minus, t[0]), fmaf((float)a.p[i][1], minus, t[1])};
-    b.p[i] = __builtin_convertvector(r, half2v);
+    b.p[i] = {(_Float16)fmaf((float)a.p[i][0], minus, t[0]), (_Float16)fmaf((float)a.p[i][1], minus, t[1])};
   }
+  hi = a.v;
+  lo = b.v;
+}
+// Eight products of f32 as halves: rounded, and what that left, rounded (exact
+// where it is representable).  Written out: each is one mixed FMA that leaves its
+// half in place, where the compiler takes two instructions.  (The first wait is for an
+// exponential that was issued just before.)
+__device__ __forceinline__ void split_products(const float *x, const float *y, half8v &hi, half8v &lo) {
+  union {
+    half8v v;
+    uint32_t u[4];
+  } a, b;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    asm("s_nop 0\n\t"
+        "v_fma_mixlo_f16 %0, %2, %4, 0\n\t"
+        "v_fma_mixhi_f16 %0, %3, %5, 0\n\t"
+        "v_fma_mixlo_f16 %1, %2, %4, -%0 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+        "v_fma_mixhi_f16 %1, %3, %5, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
+        : "=&v"(a.u[i]), "=&v"(b.u[i])
+        : "v"(x[2 * i]), "v"(x[2 * i + 1]), "v"(y[2 * i]), "v"(y[2 * i + 1]));
   hi = a.v;
   lo = b.v;
 }
@@ -329,14 +351,12 @@ __device__ __forceinline__ float rows_sum(float v) {
 }
 
 // The positions of sequence b.
-template <bool TREE>
 __device__ __forceinline__ Kv8Extent kv8_of(const Kv8Attn &a, uint32_t b) {
-  return kv8_extent(TREE, a.base[b], TREE && a.nodes ? a.nodes[b] : (int32_t)a.tmax, a.tmax,
-                    a.pg.mbps * a.pg.bpt * KV8_TILE);
+  return kv8_extent(a.tree, a.base[b], a.nodes ? a.nodes[b] : (int32_t)a.tmax, a.tmax,
+                    a.pg.mbps * a.pg.bpt.d * KV8_TILE);
 }
 
 // A wave's view of the split: lanes hold 64 sequences at a time.
-template <bool TREE>
 struct Kv8Plan {
   uint32_t per;
   Kv8Extent mine;  // of sequence `lane`
@@ -346,7 +366,7 @@ struct Kv8Plan {
     return of(a, b0, lane);
   }
   static __device__ __forceinline__ Kv8Extent of(const Kv8Attn &a, uint32_t b0, int lane) {
-    Kv8Extent e = kv8_of<TREE>(a, b0 + lane < a.batch ? b0 + lane : a.batch - 1);
+    Kv8Extent e = kv8_of(a, b0 + lane < a.batch ? b0 + lane : a.batch - 1);
     e.on = e.on && b0 + lane < a.batch;
     return e;
   }
@@ -412,22 +432,32 @@ struct Kv8Work {
   Kv8Extent e;
   bool masked;
 };
-template <bool TREE>
 __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, uint32_t rowsper, int lane, Kv8Work &w) {
-  const uint32_t u = blockIdx.x / (8 * a.groups) * 8 + blockIdx.x % 8, grp = blockIdx.x / 8 % a.groups;
-  w.slot = u / a.pg.kvheads;
-  w.h = u % a.pg.kvheads;
+  const uint32_t u8 = kv8_quot(a.by8groups, blockIdx.x), in8 = blockIdx.x - u8 * a.by8groups.d;
+  const uint32_t u = u8 * 8 + in8 % 8, grp = in8 / 8;
+  w.slot = kv8_quot(a.bykvheads, u);
+  w.h = u - w.slot * a.pg.kvheads;
   if (w.slot >= a.slots) return false;
-  const Kv8Plan<TREE> plan(a, lane);
-  uint32_t chunk;
-  if (!plan.find(a, w.slot, lane, w.b, w.e, chunk, w.chunks)) return false;
+  uint32_t share;
+  if (a.one) {
+    w.b = w.slot;
+    w.chunks = 1;
+    w.e = kv8_of(a, w.b);
+    w.c0 = 0;
+    share = 0xffffffffu;
+    if (!w.e.on) return false;
+  } else {
+    const Kv8Plan plan(a, lane);
+    uint32_t chunk;
+    if (!plan.find(a, w.slot, lane, w.b, w.e, chunk, w.chunks)) return false;
+    share = kv8_share(kv8_steps(w.e), w.chunks, a.unit) * KV8_STEP;
+    w.c0 = chunk * share;
+  }
   w.row0 = grp * rowsper;
   if (w.row0 >= (uint64_t)w.e.nodes * a.grp) return false;
-  w.masked = TREE && a.mask;
+  w.masked = a.mask;
   // a causal group of rows ends at its last node
-  const uint32_t stop = TREE && !w.masked ? kv8_stop(w.e, (w.row0 + rowsper - 1) / a.grp) : w.e.end;
-  const uint32_t share = kv8_share(kv8_steps(w.e), w.chunks, a.unit) * KV8_STEP;
-  w.c0 = chunk * share;
+  const uint32_t stop = w.masked ? w.e.end : kv8_stop(w.e, kv8_quot(a.bygrp, w.row0 + rowsper - 1));
   w.c1 = w.c0 >= stop ? w.c0 : stop - w.c0 < share ? stop : w.c0 + share;
   return true;
 }
@@ -460,10 +490,10 @@ struct WaveState {
 #pragma unroll
     for (int i = 0; i < NT; i++) {
       const uint32_t row = row0 + i * 16 + n;
-      node[i] = row / a.grp;
+      node[i] = kv8_quot(a.bygrp, row);
       const bool on = node[i] < k.e.nodes;
       const size_t qrow = (size_t)k.b * a.tmax + (on ? node[i] : 0);
-      const float *q = a.q + (qrow * a.heads + (size_t)k.h * a.grp + (on ? row % a.grp : 0)) * HD + g * 16;
+      const float *q = a.q + (qrow * a.heads + (size_t)k.h * a.grp + (on ? row - node[i] * a.grp : 0)) * HD + g * 16;
       word[i] = k.masked && on ? kv8_word(a.mask[qrow], k.e.nodes) : 0;
       float x[HD / 4], top = 0.0f;
 #pragma unroll
@@ -498,13 +528,22 @@ struct WaveState {
   }
 
   // V scales in units of vref / KV8_VUNIT: the probabilities times them, as
-  // halves, then use the type's whole range.  vs: this lane's of the step; returns what
-  // the contexts so far are to be multiplied by.
-  __device__ __forceinline__ float rescale(float &vs) {
+  // halves, then use the type's whole range.  vs: this lane's of the step; one
+  // that is no number counts as 0 there and is named in `odd`, a bit for each of
+  // this lane's sixteen positions (any: of the whole wave).  Returns what the
+  // contexts so far are to be multiplied by.
+  __device__ __forceinline__ float rescale(float &vs, uint32_t &odd, bool &any, int lane) {
     float f = 1.0f;
-    const float mag = fabsf(vs) <= 3.4028234663852886e38f ? fabsf(vs) : 0.0f;
-    if (__any(mag > vref)) {
-      const int e = __builtin_amdgcn_frexp_expf(nlg_wave_max_f32(mag));
+    const bool bad = !(fabsf(vs) <= 3.4028234663852886e38f);
+    const uint64_t all = __ballot(bad);
+    any = all != 0;
+    odd = 0;
+    if (any) {
+      odd = (uint32_t)(all >> (lane & 48)) & 0xffffu;
+      vs = bad ? 0.0f : vs;
+    }
+    if (__any(fabsf(vs) > vref)) {
+      const int e = __builtin_amdgcn_frexp_expf(nlg_wave_max_f32(fabsf(vs)));
       const int ne = e < -100 ? -100 : e;
       const float nv = ldexpf(1.0f, ne);
       f = vref > 0.0f ? vref * ldexpf(1.0f, -ne) : 0.0f;
@@ -517,15 +556,20 @@ struct WaveState {
 
   // A step's scores of tile i (products of the codes with q) made probabilities:
   // the running maximum and sum, the contexts rescaled, and the probabilities
-  // times the V scales as halves.
+  // times the V scales (vb, all sixteen) as halves hi + lo: the product rounded,
+  // and what that left, 22 bits together.
   template <bool GEN>
-  __device__ __forceinline__ void soften(int i, const float4v *acc, float ks, float vs, float vresc, uint32_t bits,
-                                         half8v *ph, half8v *pl) {
+  __device__ __forceinline__ void soften(int i, const float4v *acc, float ks, const float *vb, float vresc,
+                                         uint32_t bits, uint32_t odd, bool any, half8v *ph, half8v *pl) {
     float s[16];
     each<16>([&](auto J) {
       constexpr int j = decltype(J)::value;
       s[j] = acc[j >> 2][j & 3] * row_lane<j>(ks);
-      if (GEN) s[j] = bits >> j & 1 ? s[j] : -INFINITY;
+      // (the bit as a word of ones or zeros: no comparison)
+      if (GEN) {
+        const uint32_t on = (uint32_t)((int32_t)(bits << (31 - j)) >> 31);
+        s[j] = __uint_as_float((__float_as_uint(s[j]) & on) | (0xff800000u & ~on));
+      }
     });
     float top = max3(s[0], s[1], s[2]);
 #pragma unroll
@@ -548,13 +592,10 @@ struct WaveState {
       zz[j & 3] = zz[j & 3] + s[j];
     }
     z[i] = (zz[0] + zz[1]) + (zz[2] + zz[3]);
-    each<16>([&](auto J) {
-      constexpr int j = decltype(J)::value;
-      s[j] = s[j] * row_lane<j>(vs);
-      if (GEN) s[j] = bits >> j & 1 ? s[j] : 0.0f;
-    });
-    split8(s, ph[0], pl[0]);
-    split8(s + 8, ph[1], pl[1]);
+    // a row that attends a V row which is no number is none either
+    if (any) z[i] = odd & (GEN ? bits : 0xffffu) ? __uint_as_float(0x7fc00000u) : z[i];
+    split_products(s, vb, ph[0], pl[0]);
+    split_products(s + 8, vb + 8, ph[1], pl[1]);
   }
 };
 
@@ -581,7 +622,7 @@ __device__ __forceinline__ uint4 and4(uint4 x, uint4 m) { return make_uint4(x.x 
 // lane's K row (4 positions of each of the four tiles a time), tile `tv` its V
 // columns and both scales.  GEN: some of the positions are masked or past the
 // end.
-template <int HD, int FMT, int NT, bool GEN, bool TREE>
+template <int HD, int FMT, int NT, bool GEN>
 __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, WaveState<HD, NT> &w, uint32_t tk,
                                          uint32_t tv, uint32_t p, int lane) {
   constexpr int C = HD / 64, D = HD / 16;
@@ -613,7 +654,11 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
     for (int i = 0; i < D; i++) vr[i] = and4(vr[i], keep);
     if (!hv || n >= left) ks = vs = 0.0f;
   }
-  const float vresc = w.rescale(vs);
+  uint32_t odd;
+  bool any;
+  const float vresc = w.rescale(vs, odd, any, lane);
+  float vb[16];
+  each<16>([&](auto J) { vb[decltype(J)::value] = row_lane<decltype(J)::value>(vs); });
 #pragma unroll
   for (int i = 0; i < NT; i++) {
     // (four sums side by side: a product waits for the one before it on its sum)
@@ -631,8 +676,8 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
       for (int t = 0; t < 4; t++) acc[t] = MFMA(f[t], w.qh[i][c], acc[t]);
     }
     half8v ph[2], pl[2];
-    const uint32_t bits = GEN ? TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], q0) : (1u << left) - 1 : 0u;
-    w.template soften<GEN>(i, acc, ks, vs, vresc, bits, ph, pl);
+    const uint32_t bits = GEN ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], q0) : 0u;
+    w.template soften<GEN>(i, acc, ks, vb, vresc, bits, odd, any, ph, pl);
 #pragma unroll
     for (int d = 0; d < D; d += 4)
 #pragma unroll
@@ -649,16 +694,18 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
   }
 }
 
-// Up to 32 rows (16 NT): the workgroup's waves take its positions in turn, 64 at
-// a time, straight from memory into the matrix cores' operands, and meet in LDS.
-template <int HD, int FMT, int NT, bool TREE>
-__global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 ? 2 : 1, 2))) void k_attn_q8(Kv8Attn a) {
+// Up to 32 rows (16 NT): the workgroup's W waves take its positions in turn, 64
+// at a time, straight from memory into the matrix cores' operands, and meet in
+// LDS.
+template <int HD, int FMT, int NT, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD * NT > 128 ? 1 : 2, HD * NT > 128 ? 1 : 2)))
+void k_attn_q8(Kv8Attn a) {
   constexpr int D = HD / 16;
-  __shared__ float4v s_o[KV8_WAVES][D][64];
-  __shared__ float s_m[KV8_WAVES][16], s_z[KV8_WAVES][16];
+  __shared__ float4v s_o[W][D][64];
+  __shared__ float s_m[W][16], s_z[W][16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
-  if (!kv8_work<TREE>(a, NT * 16, lane, k)) return;
+  if (!kv8_work(a, NT * 16, lane, k)) return;
   uint32_t tid = kv8_tiles(a, k, k.c0, lane);
   WaveState<HD, NT> w;
   w.begin(a, k, k.row0, lane);
@@ -673,8 +720,8 @@ __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(
     }
     const int t0 = (int)(p - p0) / KV8_TILE;
     const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
-    kv8_step<HD, FMT, NT, decltype(GENV)::value != 0, TREE>(a, k, w, tk, tv, p, lane);
-    p += KV8_WAVES * KV8_STEP;
+    kv8_step<HD, FMT, NT, decltype(GENV)::value != 0>(a, k, w, tk, tv, p, lane);
+    p += W * KV8_STEP;
   };
   while (p + KV8_STEP <= whole) step(Int<0>{});
   while (p < k.c1) step(Int<1>{});
@@ -694,10 +741,10 @@ __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(
     __syncthreads();
     float mm = s_m[0][n];
 #pragma unroll
-    for (int j = 1; j < KV8_WAVES; j++) mm = fmaxf(mm, s_m[j][n]);
-    float f[KV8_WAVES], zz = 0.0f;
+    for (int j = 1; j < W; j++) mm = fmaxf(mm, s_m[j][n]);
+    float f[W], zz = 0.0f;
 #pragma unroll
-    for (int j = 0; j < KV8_WAVES; j++) {
+    for (int j = 0; j < W; j++) {
       f[j] = nlg_exp2(s_m[j][n] - mm);
       zz = fmaf(s_z[j][n], f[j], zz);
     }
@@ -707,12 +754,12 @@ __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(
       if (k.chunks > 1 && wv == 0 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(mm, zz);
       const float inv = k.chunks > 1 ? 1.0f : zz > 0.0f || zz != zz ? 1.0f / zz : 0.0f;
       float *o = k.chunks > 1 ? a.pctx + part * HD
-                              : a.out + (((size_t)k.b * a.tmax + row / a.grp) * a.heads + k.h * a.grp + row % a.grp) * HD;
+                              : a.out + (((size_t)k.b * a.tmax + w.node[i]) * a.heads + k.h * a.grp + row - w.node[i] * a.grp) * HD;
 #pragma unroll
-      for (int d = wv; d < D; d += KV8_WAVES) {
+      for (int d = wv; d < D; d += W) {
         float4v t = s_o[0][d][lane] * f[0];
 #pragma unroll
-        for (int j = 1; j < KV8_WAVES; j++) t = t + s_o[j][d][lane] * f[j];
+        for (int j = 1; j < W; j++) t = t + s_o[j][d][lane] * f[j];
         *(float4v *)(o + d * 16 + g * 4) = t * inv;
       }
     }
@@ -725,18 +772,18 @@ __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(
 // asked twice).  While a step is computed the next one's halves are written and
 // the one's after it are on their way from memory.  Two waves a SIMD: the
 // matrix cores work for one while the other is at its softmax.
-template <int HD, int FMT, int NT, bool TREE>
+template <int HD, int FMT, int NT>
 __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_wide_q8(Kv8Attn a) {
   constexpr int C = HD / 64, D = HD / 16, DW = D / 4;
   __shared__ half8v s_k[2][4][2 * C][64], s_v[2][D][2][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
-  if (!kv8_work<TREE>(a, KV8_WAVES * NT * 16, lane, k)) return;
+  if (!kv8_work(a, KV8_WAVES * NT * 16, lane, k)) return;
   const uint32_t row0 = k.row0 + wv * (NT * 16);
   const bool rows = row0 < (uint64_t)k.e.nodes * a.grp;
   // where this wave's rows stop attending
-  const uint32_t stop = TREE && !k.masked ? kv8_stop(k.e, (row0 + NT * 16 - 1) / a.grp) : k.e.end;
+  const uint32_t stop = k.masked ? k.e.end : kv8_stop(k.e, kv8_quot(a.bygrp, row0 + NT * 16 - 1));
   WaveState<HD, NT> w;
   w.begin(a, k, row0, lane);
   const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;
@@ -788,7 +835,9 @@ void k_attn_wide_q8(Kv8Attn a) {
   };
   auto compute = [&](auto GENV, int buf, float ksc, float vsc, uint32_t p) {
     constexpr bool GEN = decltype(GENV)::value != 0;
-    const float vresc = w.rescale(vsc);
+    uint32_t odd;
+    bool any;
+    const float vresc = w.rescale(vsc, odd, any, lane);
     float4v acc[NT][4];
     const float4v none = {0.0f, 0.0f, 0.0f, 0.0f};
     half8v f[2][4];
@@ -812,12 +861,12 @@ void k_attn_wide_q8(Kv8Attn a) {
 #pragma unroll
     for (int j = 0; j < 4; j++) f[0][j] = s_v[buf][j][0][lane];
     half8v ph[NT][2], pl[NT][2];
+    float vb[16];
+    each<16>([&](auto J) { vb[decltype(J)::value] = row_lane<decltype(J)::value>(vsc); });
 #pragma unroll
     for (int i = 0; i < NT; i++) {
-      const uint32_t bits = GEN ? TREE ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], p + g * KV8_TILE)
-                                       : (1u << kv8_left(k.e, p + g * KV8_TILE)) - 1
-                                : 0u;
-      w.template soften<GEN>(i, acc[i], ksc, vsc, vresc, bits, ph[i], pl[i]);
+      const uint32_t bits = GEN ? kv8_bits(k.e, k.masked, w.node[i], w.word[i], p + g * KV8_TILE) : 0u;
+      w.template soften<GEN>(i, acc[i], ksc, vb, vresc, bits, odd, any, ph[i], pl[i]);
     }
 #pragma unroll
     for (int r = 0; r < D / 2; r++) {  // four sixteens of dimensions, half of the positions
@@ -877,7 +926,7 @@ void k_attn_wide_q8(Kv8Attn a) {
     if (k.chunks > 1 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(w.m[i], z);
     const float f = k.chunks > 1 ? vu : z > 0.0f || z != z ? vu / z : 0.0f;
     float *o = k.chunks > 1 ? a.pctx + part * HD
-                            : a.out + (((size_t)k.b * a.tmax + row / a.grp) * a.heads + k.h * a.grp + row % a.grp) * HD;
+                            : a.out + (((size_t)k.b * a.tmax + w.node[i]) * a.heads + k.h * a.grp + row - w.node[i] * a.grp) * HD;
 #pragma unroll
     for (int d = 0; d < D; d++) *(float4v *)(o + d * 16 + g * 4) = w.o[i][d] * f;
   }
@@ -885,17 +934,17 @@ void k_attn_wide_q8(Kv8Attn a) {
 
 // The chunks' parts of each output row, joined: SUBS groups of hd / 4 threads
 // walk a row's chunks.  A workgroup's rows are of one sequence.
-template <bool TREE, int SUBS>
+template <int SUBS>
 __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint32_t blocks) {
   __shared__ float4v s_o[256];
   __shared__ float2 s_mz[256];
   const uint32_t per = hd / 4, t = threadIdx.x, b = blockIdx.x / blocks;
   const uint32_t r = blockIdx.x % blocks * (256 / per / SUBS) + t / (per * SUBS), sub = t / per % SUBS, d = t % per * 4;
-  const Kv8Plan<TREE> plan(a, t & 63);
+  const Kv8Plan plan(a, t & 63);
   uint32_t chunks;
   const uint32_t slot = plan.first(a, b, t & 63, chunks);
   if (chunks < 2) return;  // (none, or written already)
-  const Kv8Extent e = kv8_of<TREE>(a, b);
+  const Kv8Extent e = kv8_of(a, b);
   const uint32_t node = r / a.heads, head = r % a.heads;
   const bool on = node < e.nodes;
   const uint64_t p0 = ((uint64_t)slot * a.pg.kvheads + head / a.grp) * a.rows + (uint64_t)node * a.grp + head % a.grp;
@@ -1112,7 +1161,7 @@ static int kv8_check(const char *what, const void *kpool, const void *vpool, con
                      int fmt, uint32_t batch, uint32_t kvheads, uint32_t hd, uint32_t bs, uint32_t mbps, Kv8Pages &pg) {
   if (!kpool || !vpool || !table) return nlg_fail("%s: null pointer", what);
   if (((uintptr_t)kpool & 15) || ((uintptr_t)vpool & 15)) return nlg_fail("%s: pools must be 16-byte aligned", what);
-  if (((uintptr_t)table & 3)) return nlg_fail("%s: the block table must be 4-byte aligned", what);
+  if ((uintptr_t)table & 3) return nlg_fail("%s: the block table must be 4-byte aligned", what);
   if (fmt != NLG_KV_I8 && fmt != NLG_KV_E4M3) return nlg_fail("%s: unknown cache format %d", what, fmt);
   if (hd != 64 && hd != 128) return nlg_fail("%s: head_dim %u (64 or 128)", what, hd);
   if (!kvheads) return nlg_fail("%s: kvheads must be nonzero", what);
@@ -1120,7 +1169,8 @@ static int kv8_check(const char *what, const void *kpool, const void *vpool, con
     return nlg_fail("%s: block size %u (a multiple of %d), %u blocks a sequence (fewer than 2^31 positions)", what, bs,
                     KV8_TILE, mbps);
   if (!kv8_pool_bytes(npool, bs, kvheads, hd)) return nlg_fail("%s: bad pool of %u blocks", what, npool);
-  pg.table = table; pg.npool = npool; pg.mbps = mbps; pg.bpt = bs / KV8_TILE; pg.kvheads = kvheads;
+  pg.table = table; pg.npool = npool; pg.mbps = mbps; pg.bpt = kv8_div(bs / KV8_TILE);
+  pg.kvheads = kvheads;
   return NLG_OK;
 }
 // (after the checks of arguments: those need no device)
@@ -1219,7 +1269,7 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   const uint64_t orows = (uint64_t)tmax * heads;
   const bool subs = orows * batch * (hd / 4) < 65536;
   const uint64_t oper = 256 / (hd / 4) / (subs ? 8 : 1), oblocks = (orows + oper - 1) / oper;
-  if (!nlg_fits(s.blocks, 256) || !nlg_fits(oblocks * batch, 256) || orows > 0xffffffffull)
+  if (!nlg_fits(s.blocks, 512) || !nlg_fits(oblocks * batch, 256) || orows > 0xffffffffull)
     return nlg_fail("%s: too many queries for one launch", what);
   if (need) {
     if (!workspace || workspace_bytes < need)
@@ -1231,22 +1281,20 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
   a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads; a.rows = (uint32_t)rows;
   a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
+  a.by8groups = kv8_div(8 * s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
+  a.tree = tree; a.one = s.one;
   a.pctx = (float *)workspace;
   a.pmz = need ? a.pctx + s.slots * kvheads * rows * hd : nullptr;
   a.coef = NLG_LOG2E / sqrtf((float)hd);
   const dim3 grid((uint32_t)s.blocks);
   hipStream_t st = nlg_stream(stream);
-#define GO3(HD, F, T)                                                                                 \
-  do {                                                                                                \
-    if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, T>), grid, dim3(256), 0, st, a);     \
-    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, T>), grid, dim3(256), 0, st, a); \
-    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1, T>), grid, dim3(256), 0, st, a); \
-    else hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 2, T>), grid, dim3(256), 0, st, a);                \
-  } while (0)
-#define GO(HD, F)               \
-  do {                          \
-    if (tree) GO3(HD, F, true); \
-    else GO3(HD, F, false);     \
+#define GO(HD, F)                                                                                          \
+  do {                                                                                                     \
+    if (s.rowsper == 16 && s.one) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 8>), grid, dim3(512), 0, st, a); \
+    else if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 4>), grid, dim3(256), 0, st, a);     \
+    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, 4>), grid, dim3(256), 0, st, a);     \
+    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1>), grid, dim3(256), 0, st, a);   \
+    else hipLaunchKernelGGL((k_attn_wide_q8<64, F, 2>), grid, dim3(256), 0, st, a);                        \
   } while (0)
   if (hd == 128) {
     if (fmt == NLG_KV_I8) GO(128, NLG_KV_I8); else GO(128, NLG_KV_E4M3);
@@ -1254,15 +1302,12 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
     if (fmt == NLG_KV_I8) GO(64, NLG_KV_I8); else GO(64, NLG_KV_E4M3);
   }
 #undef GO
-#undef GO3
   NLG_LAUNCHED(what);
   if (need) {
     const dim3 mg((uint32_t)(oblocks * batch));
     const uint32_t ob = (uint32_t)oblocks;
-    if (tree && subs) hipLaunchKernelGGL((k_attn_q8_merge<true, 8>), mg, dim3(256), 0, st, a, hd, ob);
-    else if (tree) hipLaunchKernelGGL((k_attn_q8_merge<true, 1>), mg, dim3(256), 0, st, a, hd, ob);
-    else if (subs) hipLaunchKernelGGL((k_attn_q8_merge<false, 8>), mg, dim3(256), 0, st, a, hd, ob);
-    else hipLaunchKernelGGL((k_attn_q8_merge<false, 1>), mg, dim3(256), 0, st, a, hd, ob);
+    if (subs) hipLaunchKernelGGL(k_attn_q8_merge<8>, mg, dim3(256), 0, st, a, hd, ob);
+    else hipLaunchKernelGGL(k_attn_q8_merge<1>, mg, dim3(256), 0, st, a, hd, ob);
     NLG_LAUNCHED(what);
   }
   return NLG_OK;

@@ -24,6 +24,16 @@ static uint64_t seed = 1;
 static uint32_t rnd(uint32_t n) { seed = seed * 6364136223846793005ull + 1442695040888963407ull; return (uint32_t)(seed >> 33) % n; }
 #define CHECK(c) do { if (!(c)) { printf("line %d: %s\n", __LINE__, #c); return 1; } } while (0)
 // the layout: each byte of a tile once
+static int division() {
+  for (uint32_t d : {1u, 2u, 3u, 5u, 7u, 8u, 40u, 48u, 65535u, 65537u, 1u << 20, (1u << 27) - 1, 0x7fffffffu, 0x80000000u, 0xffffffffu}) {
+    const Kv8Div v = kv8_div(d);
+    for (int i = 0; i < 20000; i++) {
+      const uint32_t n = i < 5 ? i : i < 10 ? 0x7fffffffu - i : i % 2 ? rnd(1u << 31) : (uint32_t)((uint64_t)d * rnd(0x7fffffffu / d + 1) - i / 2 % 2) & 0x7fffffffu;
+      CHECK(kv8_quot(v, n) == n / d);
+    }
+  }
+  return 0;
+}
 static int layout(uint32_t hd) {
   for (int v = 0; v < 2; v++) {
     std::vector<int> seen(kv8_tile_bytes(hd));
@@ -60,12 +70,14 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
   for (uint32_t b = 0; b < batch; b++) {
     const int64_t nn = !tree ? 1 : nodes[b] < 0 ? 0 : nodes[b] > (int64_t)tmax ? tmax : nodes[b];
     CHECK(e[b].on == (!tree || (at[b] >= 0 && nn > 0)));
-    const uint32_t steps = kv8_steps(e[b]), chunks = kv8_chunks(steps, per);
-    slots += chunks;
-    CHECK(chunks == 0 ? !e[b].on : (s.one ? chunks == 1 : true));
+    const uint32_t steps = kv8_steps(e[b]);
+    uint32_t chunks = kv8_chunks(steps, per);
+    slots += s.one ? 1 : chunks;
+    CHECK((chunks == 0) == !e[b].on);
     if (!chunks) continue;
-    const uint32_t share = kv8_share(steps, chunks, s.unit);
-    CHECK(share % s.unit == 0 && share <= per && (uint64_t)share * chunks >= steps && share * (chunks - 1) < steps);
+    if (s.one) chunks = 1;
+    const uint32_t share = s.one ? 1u << 25 : kv8_share(steps, chunks, s.unit);
+    CHECK(s.one || (share % s.unit == 0 && share <= per && (uint64_t)share * chunks >= steps && share * (chunks - 1) < steps));
     std::vector<uint64_t> mask(tmax);
     for (auto &m : mask) m = (uint64_t)rnd(1u << 31) << 33 ^ (uint64_t)rnd(1u << 31) << 10 ^ rnd(1024);
     for (uint32_t r = 0; r < rows; r += 1 + rnd(3)) {
@@ -73,8 +85,8 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
       if (node >= nn) continue;
       std::vector<int> seen(cap + 64);
       const uint32_t g0 = r / s.rowsper * s.rowsper;
-      const uint32_t stop = tree && !masked ? kv8_stop(e[b], (g0 + s.rowsper - 1) / grp) : e[b].end;
-      const uint32_t mine = tree && !masked ? kv8_stop(e[b], node) : e[b].end;
+      const uint32_t stop = masked ? e[b].end : kv8_stop(e[b], (g0 + s.rowsper - 1) / grp);
+      const uint32_t mine = masked ? e[b].end : kv8_stop(e[b], node);
       for (uint32_t c = 0; c < chunks; c++) {
         const uint32_t c0 = c * share * KV8_STEP;
         const uint32_t c1 = c0 >= stop ? c0 : stop - c0 < share * KV8_STEP ? stop : c0 + share * KV8_STEP;
@@ -83,8 +95,7 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
           for (uint32_t t = 0; t < 4; t++) {
             const uint32_t q0 = p + t * 16;
             const uint32_t bits = p + KV8_STEP <= whole ? 0xffffu
-                                  : tree ? kv8_bits(e[b], masked, node, masked ? kv8_word(mask[node], e[b].nodes) : 0, q0)
-                                         : (1u << kv8_left(e[b], q0)) - 1;
+                                  : kv8_bits(e[b], masked, node, masked ? kv8_word(mask[node], e[b].nodes) : 0, q0);
             CHECK(bits < 65536 && (p < mine || !bits));
             for (uint32_t j = 0; j < 16; j++) seen[q0 + j < cap + 63 ? q0 + j : cap + 63] += bits >> j & 1;
           }
@@ -105,13 +116,13 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
   return 0;
 }
 int main(void) {
-  if (layout(64) || layout(128)) return 1;
+  if (division() || layout(64) || layout(128)) return 1;
   // pages: entries outside the pool, positions behind the table
   const int32_t table[6] = {3, -1, 0, 7, 2147483647, 1};
-  const Kv8Pages g = {table, 7, 3, 2, 5};
+  const Kv8Pages g = {table, 7, 3, 5, kv8_div(2)};
   CHECK(kv8_tile(g, 0, 4, 1) == (3 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 4) == 0);
   CHECK(kv8_tile(g, 0, 0, 2) == KV8_NONE && kv8_tile(g, 0, 0, 6) == KV8_NONE && kv8_tile(g, 1, 0, 0) == KV8_NONE);
-  CHECK(kv8_tile(g, 1, 0, 3) == KV8_NONE && kv8_tile(g, 1, 4, 5) == (1 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 0xffffffffu) == KV8_NONE);
+  CHECK(kv8_tile(g, 1, 0, 3) == KV8_NONE && kv8_tile(g, 1, 4, 5) == (1 * 5 + 4) * 2 + 1 && kv8_tile(g, 0, 0, 0x7fffffffu) == KV8_NONE);
   for (int i = 0; i < 300; i++) {
     const uint32_t bs = 16 * (1 + rnd(4)), mbps = 1 + rnd(i % 10 ? 20 : 300), cap = bs * mbps;
     const uint32_t grp = 1 + rnd(9), kvh = 1 + rnd(i % 3 ? 8 : 300), batch = 1 + rnd(i % 4 ? 4 : 90);
@@ -122,7 +133,7 @@ int main(void) {
       nm.push_back((int32_t)rnd(tm + 4) - 1);
       nc.push_back((int32_t)rnd(tc + 4) - 1);
     }
-    if (call(false, false, at, nm, 1, grp, bs, mbps, kvh)) return 1;
+    if (call(false, false, at, std::vector<int32_t>(batch, 1), 1, grp, bs, mbps, kvh)) return 1;
     if (call(true, true, at, nm, tm, grp, bs, mbps, kvh)) return 1;
     if (call(true, false, at, nc, tc, grp, bs, mbps, kvh)) return 1;
   }
@@ -136,7 +147,7 @@ int main(void) {
       for (uint32_t rows : {1u, 16u, 17u, 33u, 65u, 2147483647u}) {
         const Kv8Split s = kv8_split(batch, rows, 8, 64, pos);
         CHECK((uint64_t)s.groups * s.rowsper >= rows && s.slots >= 1);
-        CHECK(s.one == (pos <= 256) && s.blocks >= (uint64_t)s.slots * 8 * s.groups);
+        CHECK(s.one == (pos <= (rows > 16 ? 256 : 1024)) && s.blocks >= (uint64_t)s.slots * 8 * s.groups);
       }
   printf("ok\n");
   return 0;
@@ -184,9 +195,10 @@ def test_pool_bytes():
 def test_workspace_bytes():
     """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
     w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
-    assert w(1, 20, 5, 128, 16, 16) == 0 and w(1, 20, 5, 128, 16, 17) == 5 * 2 * 4 * 130 * 4
+    assert w(1, 20, 5, 128, 16, 64) == 0 and w(1, 20, 5, 128, 16, 65) == 5 * 5 * 4 * 130 * 4
+    assert t(1, 8, 20, 5, 128, 16, 16) == 0 and t(1, 8, 20, 5, 128, 16, 17) == 2 * 5 * 32 * 130 * 4
     assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 4 * 130 * 4
-    assert w(1, 20, 5, 128, 16, 17) == t(1, 1, 20, 5, 128, 16, 17)
+    assert w(1, 20, 5, 128, 16, 65) == t(1, 1, 20, 5, 128, 16, 65)
     for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
                 (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
                 (1, 1, 20, 5, 128, 20, 64), (1, 1, 20, 5, 128, 16, 0), (1, 1, 20, 5, 128, 16, 1 << 27),
@@ -233,7 +245,7 @@ def test_append_refuses(bad, words):
     refused(nlgpu.qk_norm_rope_append_paged_q8, dict(kw, **bad), words)
 
 
-ATTN = dict(CACHE, q=GOOD, out=GOOD, heads=8, workspace=GOOD)
+ATTN = dict(CACHE, mbps=128, q=GOOD, out=GOOD, heads=8, workspace=GOOD)
 BAD_ATTN = BAD_CACHE + [
     (dict(fmt=2), "format"), (dict(q=At(None)), "null"), (dict(out=At(None)), "null"), (dict(heads=9), "heads"),
     (dict(heads=0), "heads"), (dict(q=ODD), "aligned"), (dict(out=ODD), "aligned"), (dict(workspace=ODD), "aligned"),
