@@ -110,12 +110,14 @@ NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 
 // How an attention call is laid over workgroups.  Rows (queries x query heads
 // of a kv head) come in groups of `rowsper`; up to 32 of them a workgroup's
 // waves share (they split the positions), from 33 on each wave has its own
-// (`wide`: they share K and V).  Positions are split by the lengths that the
-// kernel finds on the device (kv8_per); a sequence's chunks are of one size.
-// want: the chunks that fill the card for each kv head and group; slots: the
-// most there can be.  one: no sequence is split, and its slot is its number.
+// (`wide`: they share K and V).  A slot is a sequence, a group of its rows and a
+// chunk of its positions; every kv head has all of them.  How many there are,
+// and how long, follows from the lengths and node counts that the kernel finds
+// on the device (kv8_per); a sequence's chunks are of one size.  want: the slots
+// that fill the card once, two workgroups a CU; slots: the most there can be.
+// one: no sequence is split, and a slot is its sequence and group.
 struct Kv8Split {
-  uint32_t rowsper, groups, want, least, unit;
+  uint32_t rowsper, rowslog, groups, want, least, unit;
   uint64_t slots;
   bool wide, one;
   uint64_t blocks;  // workgroups
@@ -124,36 +126,59 @@ inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint3
   Kv8Split s;
   s.wide = rows > 32;
   s.rowsper = rows > 64 && hd == 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
+  s.rowslog = s.rowsper == 16 ? 4 : s.rowsper == 32 ? 5 : s.rowsper == 64 ? 6 : 7;
   s.groups = (uint32_t)(((uint64_t)rows + s.rowsper - 1) / s.rowsper);
   s.unit = s.wide ? 1 : KV8_WAVES;
-  s.least = 4;
-  const uint64_t units = (uint64_t)kvheads * s.groups, most = (positions + KV8_STEP - 1) / KV8_STEP;
-  // two workgroups a CU at once; wide ones, whose steps cost more than their loads, in two rounds
-  const uint64_t fill = s.wide ? 1024 : 512, want = fill / units ? fill / units : 1;
-  const uint64_t all = batch * ((most + s.least - 1) / s.least), upto = batch <= want / 2 ? want : 2 * want + batch;
-  s.want = (uint32_t)want;
+  s.least = s.wide ? 2 : KV8_WAVES;
+  const uint64_t most = (positions + KV8_STEP - 1) / KV8_STEP, pairs = (uint64_t)batch * s.groups;
+  s.want = 512 / kvheads ? 512 / kvheads : 1;
   // (eight waves to a workgroup take 1,024 positions in two steps each: less than a second launch)
   s.one = most <= (s.rowsper == 16 ? 16 : s.least);
-  s.slots = s.one ? batch : upto < all ? upto : all;
-  // (a multiple of eight of (slot, kv head)s: the groups of one lie on one XCD)
-  s.blocks = (s.slots * kvheads + 7) / 8 * 8 * s.groups;
+  const uint64_t all = pairs * ((most + s.least - 1) / s.least);
+  const uint64_t upto = pairs <= s.want / 2 ? s.want : 2ull * s.want + pairs;
+  s.slots = s.one ? pairs : upto < all ? upto : all;
+  s.blocks = s.slots * kvheads;
   return s;
 }
-// Steps of a sequence; of a chunk, with `total` steps in all sequences; and a
-// sequence's chunks, each of kv8_share steps (the last what is left).
+// A sequence's steps and groups.
 NLG_KV8_HD uint32_t kv8_steps(const Kv8Extent &e) {
   return !e.on ? 0u : e.end ? (e.end - 1) / KV8_STEP + 1 : 1u;
 }
-// A sequence's last chunk may be a small one, so total / per + batch of them
-// bound the chunks: few sequences are split so that this is want, and all
-// workgroups run at once; with many (batch over want / 2) there are several
-// rounds anyway, and the chunks are made small against the last one's tail.
-NLG_KV8_HD uint32_t kv8_per(uint64_t total, uint32_t batch, uint32_t want, uint32_t least, uint32_t unit) {
-  const uint32_t over = batch <= want / 2 ? want - batch : 2 * want;
-  uint64_t per = total >> 32 ? total / over + 1 : ((uint32_t)total - 1u) / over + 1u;  // (total is not 0)
+NLG_KV8_HD uint32_t kv8_groups(const Kv8Extent &e, uint32_t grp, uint32_t rowslog) {
+  return e.on ? (e.nodes * grp + (1u << rowslog) - 1) >> rowslog : 0u;  // (a sequence's rows are below 2^31)
+}
+// Steps of a chunk: a first guess, from the steps of all groups of rows and
+// their number, and the largest that is taken.  The last chunk of each may be a
+// small one, so total / per + pairs bound the slots: few pairs are split so that
+// there are no more than want, and all workgroups run at once; with many (over
+// want / 2) there are several rounds anyway, and the chunks are made small
+// against the last one's tail.
+struct Kv8Per {
+  uint32_t first, last;
+};
+NLG_KV8_HD uint32_t kv8_ceil_to(uint64_t per, uint32_t least, uint32_t unit) {
   if (per < least) per = least;
   per = (per + unit - 1) / unit * unit;
   return per > 0x7fffffffu ? 0x7fffffffu / unit * unit : (uint32_t)per;
+}
+// At least n / d, 0 < n < 2^48 (from 2^32 on not the least: no 64-bit division).
+NLG_KV8_HD uint64_t kv8_div_up(uint64_t n, uint32_t d) {
+  return n >> 32 ? ((uint64_t)((uint32_t)(n >> 16) / d) + 1) << 16 : ((uint32_t)n - 1u) / d + 1u;
+}
+NLG_KV8_HD Kv8Per kv8_per(uint64_t total, uint64_t pairs, uint32_t want, uint32_t least, uint32_t unit) {
+  const bool few = pairs <= want / 2;
+  Kv8Per p;
+  p.last = kv8_ceil_to(kv8_div_up(total, few ? want - (uint32_t)pairs : 2 * want), least, unit);
+  p.first = few ? kv8_ceil_to(kv8_div_up(total, want), least, unit) : p.last;
+  return p;
+}
+// The next guess, where `per` gave `slots` > want.
+NLG_KV8_HD uint32_t kv8_more(uint32_t per, uint32_t slots, uint32_t want, uint32_t last, uint32_t unit) {
+  if ((uint64_t)per * slots >> 32) return last;
+  uint64_t next = kv8_div_up((uint64_t)per * slots, want);
+  next = (next > per ? next : per + 1) + unit - 1;
+  next = next / unit * unit;
+  return next < last ? (uint32_t)next : last;
 }
 NLG_KV8_HD uint32_t kv8_chunks(uint32_t steps, uint32_t per) { return (steps + per - 1) / per; }
 NLG_KV8_HD uint32_t kv8_share(uint32_t steps, uint32_t chunks, uint32_t unit) {

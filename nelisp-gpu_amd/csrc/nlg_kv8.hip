@@ -242,10 +242,10 @@ struct Kv8Attn {
   const int32_t *nodes;   // tree: [batch] or null
   const uint64_t *mask;   // tree: [batch][tmax] or null
   Kv8Pages pg;
-  float *out, *pctx, *pmz;  // partials: [slots][kvheads][rows][hd], [slots][kvheads][rows][2]
+  float *out, *pctx, *pmz;  // partials: [slots][kvheads][rowsper][hd], [slots][kvheads][rowsper][2]
   uint32_t batch, tmax, heads, grp, rows;  // rows = tmax * grp
-  uint32_t groups, want, least, unit, slots;  // Kv8Split
-  Kv8Div by8groups, bykvheads, bygrp;
+  uint32_t rowsper, rowslog, groups, want, least, unit, slots;  // Kv8Split
+  Kv8Div bykvheads, bygrp, bygroups;
   bool tree, one;
   float coef;  // log2(e) / sqrt(hd): scores in base 2
 };
@@ -370,14 +370,37 @@ struct Kv8Plan {
     e.on = e.on && b0 + lane < a.batch;
     return e;
   }
+  static __device__ __forceinline__ uint64_t sum(uint64_t v) {  // (lanes below 2^42 each)
+    return (uint64_t)(uint32_t)nlg_wave_sum_i32((int)(v & 0xffffff)) +
+           ((uint64_t)(uint32_t)nlg_wave_sum_i32((int)(v >> 24)) << 24);
+  }
+  __device__ __forceinline__ uint32_t slots(const Kv8Attn &a, const Kv8Extent &e) const {
+    return kv8_groups(e, a.grp, a.rowslog) * kv8_chunks(kv8_steps(e), per);
+  }
   __device__ __forceinline__ Kv8Plan(const Kv8Attn &a, int lane) {
     mine = of(a, 0, lane);
-    uint64_t total = kv8_steps(mine);
-    for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) total += kv8_steps(of(a, b0, lane));
-    // (in two halves of 32 bits: a lane's part is below 2^42)
-    total = (uint64_t)(uint32_t)nlg_wave_sum_i32((int)(total & 0xffffff)) +
-            ((uint64_t)(uint32_t)nlg_wave_sum_i32((int)(total >> 24)) << 24);
-    per = kv8_per(total, a.batch, a.want, a.least, a.unit);
+    uint32_t g = kv8_groups(mine, a.grp, a.rowslog);
+    uint64_t total = (uint64_t)g * kv8_steps(mine), pairs = g;
+    for (uint32_t b0 = 64; b0 < a.batch; b0 += 64) {
+      const Kv8Extent e = of(a, b0, lane);
+      g = kv8_groups(e, a.grp, a.rowslog);
+      total += (uint64_t)g * kv8_steps(e);
+      pairs += g;
+    }
+    total = sum(total);
+    pairs = sum(pairs);
+    const Kv8Per p = kv8_per(total ? total : 1, pairs, a.want, a.least, a.unit);
+    per = p.first;
+    // (a better fit than the bound, for up to 64 sequences)
+    for (int i = 0; i < 4 && per < p.last; i++) {
+      if (a.batch > 64 || i == 3) {
+        per = p.last;
+        break;
+      }
+      const uint32_t n = (uint32_t)nlg_wave_sum_i32((int)slots(a, mine));
+      if (n <= a.want) break;
+      per = kv8_more(per, n, a.want, p.last, a.unit);
+    }
   }
   // inclusive sums over the lanes
   static __device__ __forceinline__ uint32_t sums(uint32_t v) {
@@ -389,23 +412,25 @@ struct Kv8Plan {
     v += (uint32_t)nlg_dpp<0x143, 0xc>((int)v);  // row_bcast:31 into rows 2, 3
     return v;
   }
-  // The sequence and chunk of slot x; false: there are fewer.
-  __device__ __forceinline__ bool find(const Kv8Attn &a, uint32_t x, int lane, uint32_t &b, Kv8Extent &e, uint32_t &chunk,
-                                       uint32_t &chunks) const {
+  // The sequence, group and chunk of slot x; false: there are fewer.
+  __device__ __forceinline__ bool find(const Kv8Attn &a, uint32_t x, int lane, uint32_t &b, Kv8Extent &e, uint32_t &group,
+                                       uint32_t &chunk, uint32_t &chunks) const {
     uint32_t before = 0;
     for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
       const Kv8Extent l = at(a, b0, lane);
-      const uint32_t n = kv8_chunks(kv8_steps(l), per), to = sums(n);
+      const uint32_t n = slots(a, l), to = sums(n);
       const uint64_t past = __ballot(before + to > x);
       if (past) {
         const int i = __builtin_ctzll(past);
         b = b0 + i;
-        chunks = __builtin_amdgcn_readlane(n, i);
-        chunk = x - before - (__builtin_amdgcn_readlane(to, i) - chunks);
+        const uint32_t in = x - before - (__builtin_amdgcn_readlane(to, i) - __builtin_amdgcn_readlane(n, i));
         e.base = __builtin_amdgcn_readlane(l.base, i);
         e.end = __builtin_amdgcn_readlane(l.end, i);
         e.nodes = __builtin_amdgcn_readlane(l.nodes, i);
         e.on = true;
+        chunks = kv8_chunks(kv8_steps(e), per);
+        group = in / chunks;
+        chunk = in - group * chunks;
         return true;
       }
       before += __builtin_amdgcn_readlane(to, 63);
@@ -416,10 +441,11 @@ struct Kv8Plan {
   __device__ __forceinline__ uint32_t first(const Kv8Attn &a, uint32_t b, int lane, uint32_t &chunks) const {
     uint32_t before = 0;
     for (uint32_t b0 = 0;; b0 += 64) {
-      const uint32_t n = kv8_chunks(kv8_steps(at(a, b0, lane)), per), to = sums(n);
+      const Kv8Extent l = at(a, b0, lane);
+      const uint32_t n = slots(a, l), to = sums(n);
       if (b < b0 + 64) {
-        chunks = __builtin_amdgcn_readlane(n, b - b0);
-        return before + __builtin_amdgcn_readlane(to, b - b0) - chunks;
+        chunks = __builtin_amdgcn_readlane(kv8_chunks(kv8_steps(l), per), b - b0);
+        return before + __builtin_amdgcn_readlane(to, b - b0) - __builtin_amdgcn_readlane(n, b - b0);
       }
       before += __builtin_amdgcn_readlane(to, 63);
     }
@@ -432,32 +458,29 @@ struct Kv8Work {
   Kv8Extent e;
   bool masked;
 };
-__device__ __forceinline__ bool kv8_work(const Kv8Attn &a, uint32_t rowsper, int lane, Kv8Work &w) {
-  const uint32_t u8 = kv8_quot(a.by8groups, blockIdx.x), in8 = blockIdx.x - u8 * a.by8groups.d;
-  const uint32_t u = u8 * 8 + in8 % 8, grp = in8 / 8;
-  w.slot = kv8_quot(a.bykvheads, u);
-  w.h = u - w.slot * a.pg.kvheads;
-  if (w.slot >= a.slots) return false;
-  uint32_t share;
+__device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w) {
+  w.slot = kv8_quot(a.bykvheads, blockIdx.x);
+  w.h = blockIdx.x - w.slot * a.pg.kvheads;
+  uint32_t share, group;
   if (a.one) {
-    w.b = w.slot;
+    w.b = kv8_quot(a.bygroups, w.slot);
+    group = w.slot - w.b * a.groups;
     w.chunks = 1;
     w.e = kv8_of(a, w.b);
     w.c0 = 0;
     share = 0xffffffffu;
-    if (!w.e.on) return false;
+    if (group >= kv8_groups(w.e, a.grp, a.rowslog)) return false;
   } else {
     const Kv8Plan plan(a, lane);
     uint32_t chunk;
-    if (!plan.find(a, w.slot, lane, w.b, w.e, chunk, w.chunks)) return false;
+    if (!plan.find(a, w.slot, lane, w.b, w.e, group, chunk, w.chunks)) return false;
     share = kv8_share(kv8_steps(w.e), w.chunks, a.unit) * KV8_STEP;
     w.c0 = chunk * share;
   }
-  w.row0 = grp * rowsper;
-  if (w.row0 >= (uint64_t)w.e.nodes * a.grp) return false;
+  w.row0 = group * a.rowsper;
   w.masked = a.mask;
   // a causal group of rows ends at its last node
-  const uint32_t stop = w.masked ? w.e.end : kv8_stop(w.e, kv8_quot(a.bygrp, w.row0 + rowsper - 1));
+  const uint32_t stop = w.masked ? w.e.end : kv8_stop(w.e, kv8_quot(a.bygrp, w.row0 + a.rowsper - 1));
   w.c1 = w.c0 >= stop ? w.c0 : stop - w.c0 < share ? stop : w.c0 + share;
   return true;
 }
@@ -705,7 +728,7 @@ void k_attn_q8(Kv8Attn a) {
   __shared__ float s_m[W][16], s_z[W][16];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
-  if (!kv8_work(a, NT * 16, lane, k)) return;
+  if (!kv8_work(a, lane, k)) return;
   uint32_t tid = kv8_tiles(a, k, k.c0, lane);
   WaveState<HD, NT> w;
   w.begin(a, k, k.row0, lane);
@@ -750,7 +773,7 @@ void k_attn_q8(Kv8Attn a) {
     }
     const uint32_t row = k.row0 + i * 16 + n;
     if (row < (uint64_t)k.e.nodes * a.grp) {
-      const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rows + row;
+      const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rowsper + row - k.row0;
       if (k.chunks > 1 && wv == 0 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(mm, zz);
       const float inv = k.chunks > 1 ? 1.0f : zz > 0.0f || zz != zz ? 1.0f / zz : 0.0f;
       float *o = k.chunks > 1 ? a.pctx + part * HD
@@ -779,13 +802,12 @@ void k_attn_wide_q8(Kv8Attn a) {
   __shared__ half8v s_k[2][4][2 * C][64], s_v[2][D][2][64];
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, n = lane & 15;
   Kv8Work k;
-  if (!kv8_work(a, KV8_WAVES * NT * 16, lane, k)) return;
+  if (!kv8_work(a, lane, k)) return;
   const uint32_t row0 = k.row0 + wv * (NT * 16);
   const bool rows = row0 < (uint64_t)k.e.nodes * a.grp;
   // where this wave's rows stop attending
   const uint32_t stop = k.masked ? k.e.end : kv8_stop(k.e, kv8_quot(a.bygrp, row0 + NT * 16 - 1));
   WaveState<HD, NT> w;
-  w.begin(a, k, row0, lane);
   const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;
 
   // this wave's share of a step: tile wv's K, DW sixteens of V's dimensions
@@ -885,8 +907,9 @@ void k_attn_wide_q8(Kv8Attn a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
+  if (k.c0 < k.c1) load(k.c0);  // (under way while the queries are made ready)
+  w.begin(a, k, row0, lane);
   if (k.c0 < k.c1) {
-    load(k.c0);
     store(0);
     float ksc = ks, vsc = vs;
     if (k.c1 - k.c0 > KV8_STEP) load(k.c0 + KV8_STEP);
@@ -922,7 +945,7 @@ void k_attn_wide_q8(Kv8Attn a) {
     const float z = rows_sum(w.z[i]);
     const uint32_t row = row0 + i * 16 + n;
     if (row >= (uint64_t)k.e.nodes * a.grp) continue;
-    const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rows + row;
+    const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rowsper + row - k.row0;
     if (k.chunks > 1 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(w.m[i], z);
     const float f = k.chunks > 1 ? vu : z > 0.0f || z != z ? vu / z : 0.0f;
     float *o = k.chunks > 1 ? a.pctx + part * HD
@@ -947,8 +970,9 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
   const Kv8Extent e = kv8_of(a, b);
   const uint32_t node = r / a.heads, head = r % a.heads;
   const bool on = node < e.nodes;
-  const uint64_t p0 = ((uint64_t)slot * a.pg.kvheads + head / a.grp) * a.rows + (uint64_t)node * a.grp + head % a.grp;
-  const uint64_t step = (uint64_t)a.pg.kvheads * a.rows;
+  const uint32_t h = kv8_quot(a.bygrp, head), row = node * a.grp + head - h * a.grp, group = row >> a.rowslog;
+  const uint64_t p0 = ((uint64_t)(slot + group * chunks) * a.pg.kvheads + h) * a.rowsper + (row & (a.rowsper - 1));
+  const uint64_t step = (uint64_t)a.pg.kvheads * a.rowsper;
   float m = KV8_FLOOR, z = 0.0f;
   float4v o = {0.0f, 0.0f, 0.0f, 0.0f};
   if (on)
@@ -1227,8 +1251,8 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
 }
 
 // The partials' bytes: contexts, then (maximum, sum) pairs; 0 where one chunk needs none.
-static uint64_t kv8_partials(const Kv8Split &s, uint64_t rows, uint32_t kvheads, uint32_t hd) {
-  return s.one ? 0 : s.slots * kvheads * rows * (hd + 2) * 4;
+static uint64_t kv8_partials(const Kv8Split &s, uint32_t kvheads, uint32_t hd) {
+  return s.one ? 0 : s.slots * kvheads * s.rowsper * (hd + 2) * 4;
 }
 // Sizes an attention call can have at all (0: none).
 static uint64_t kv8_rows(uint32_t tmax, uint32_t heads, uint32_t kvheads) {
@@ -1243,7 +1267,7 @@ extern "C" size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax
   if (!batch || !rows || !bs || bs % KV8_TILE || !mbps || (uint64_t)bs * mbps > 0x7fffffffull ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, head_dim, (uint64_t)bs * mbps), rows, kvheads, head_dim);
+  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, head_dim, (uint64_t)bs * mbps), kvheads, head_dim);
 }
 extern "C" size_t nlg_decode_attn_paged_q8_workspace(uint32_t batch, uint32_t heads, uint32_t kvheads,
                                                      uint32_t head_dim, uint32_t bs, uint32_t mbps) {
@@ -1264,7 +1288,7 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   if (mask && tmax > KV8_TREE) return nlg_fail("%s: %u nodes under a mask (at most %d)", what, tmax, KV8_TREE);
   if (mask && ((uintptr_t)mask & 7)) return nlg_fail("%s: the masks must be 8-byte aligned", what);
   const Kv8Split s = kv8_split(batch, (uint32_t)rows, kvheads, hd, (uint64_t)bs * mbps);
-  const uint64_t need = kv8_partials(s, rows, kvheads, hd);
+  const uint64_t need = kv8_partials(s, kvheads, hd);
   // joining: eight groups of threads a row while its rows would not fill the card with one
   const uint64_t orows = (uint64_t)tmax * heads;
   const bool subs = orows * batch * (hd / 4) < 65536;
@@ -1280,11 +1304,11 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   KV8_SCOPE(what);
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
   a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads; a.rows = (uint32_t)rows;
-  a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
-  a.by8groups = kv8_div(8 * s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
+  a.rowsper = s.rowsper; a.rowslog = s.rowslog; a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
+  a.bygroups = kv8_div(s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
   a.tree = tree; a.one = s.one;
   a.pctx = (float *)workspace;
-  a.pmz = need ? a.pctx + s.slots * kvheads * rows * hd : nullptr;
+  a.pmz = need ? a.pctx + s.slots * kvheads * s.rowsper * hd : nullptr;
   a.coef = NLG_LOG2E / sqrtf((float)hd);
   const dim3 grid((uint32_t)s.blocks);
   hipStream_t st = nlg_stream(stream);

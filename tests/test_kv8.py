@@ -50,29 +50,40 @@ static int call(bool tree, bool masked, std::vector<int32_t> at, std::vector<int
                 uint32_t bs, uint32_t mbps, uint32_t kvheads) {
   const uint32_t cap = bs * mbps, rows = tmax * grp, batch = at.size();
   const Kv8Split s = kv8_split(batch, rows, kvheads, rnd(2) ? 64 : 128, cap);
-  CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows && s.want >= 1);
-  // every (slot, kv head, group) is some workgroup's, as the kernels number them
-  std::vector<int> seen((size_t)s.slots * kvheads * s.groups);
-  for (uint64_t i = 0; i < s.blocks; i++) {
-    const uint64_t u = i / (8 * s.groups) * 8 + i % 8, g = i / 8 % s.groups;
-    if (u < (uint64_t)s.slots * kvheads) seen[u * s.groups + g]++;
-  }
-  for (int n : seen) CHECK(n == 1);
+  CHECK((uint64_t)s.groups * s.rowsper >= rows && (s.groups - 1) * s.rowsper < rows && s.want >= 1 && 1u << s.rowslog == s.rowsper);
+  CHECK(kv8_div_up((1ull << 47) + 12345, 7) * 7 >= (1ull << 47) + 12345);
   std::vector<Kv8Extent> e(batch);
-  uint64_t total = 0, slots = 0;
+  uint64_t total = 0, slots = 0, pairs = 0;
   for (uint32_t b = 0; b < batch; b++) {
     e[b] = kv8_extent(tree, at[b], nodes[b], tmax, cap);
     CHECK(e[b].end <= cap);
-    total += kv8_steps(e[b]);
+    const uint32_t g = kv8_groups(e[b], grp, s.rowslog);
+    CHECK(g <= s.groups && (g == 0) == !e[b].on && (uint64_t)g * s.rowsper >= (e[b].on ? (uint64_t)e[b].nodes * grp : 0));
+    total += (uint64_t)g * kv8_steps(e[b]);
+    pairs += g;
   }
-  const uint32_t per = kv8_per(total, batch, s.want, s.least, s.unit);
-  CHECK(per % s.unit == 0 && per >= s.least);
+  CHECK(s.blocks == s.slots * kvheads);
+  const Kv8Per range = kv8_per(total ? total : 1, pairs, s.want, s.least, s.unit);
+  CHECK(range.first <= range.last && range.first % s.unit == 0 && range.last % s.unit == 0 && range.first >= s.least);
+  uint32_t per = range.first;
+  for (int i = 0; i < 4 && per < range.last; i++) {  // as the kernel does
+    if (batch > 64 || i == 3) {
+      per = range.last;
+      break;
+    }
+    uint64_t n = 0;
+    for (uint32_t b = 0; b < batch; b++) n += kv8_groups(e[b], grp, s.rowslog) * kv8_chunks(kv8_steps(e[b]), per);
+    if (n <= s.want) break;
+    const uint32_t next = kv8_more(per, n, s.want, range.last, s.unit);
+    CHECK(next > per && next % s.unit == 0);
+    per = next;
+  }
   for (uint32_t b = 0; b < batch; b++) {
     const int64_t nn = !tree ? 1 : nodes[b] < 0 ? 0 : nodes[b] > (int64_t)tmax ? tmax : nodes[b];
     CHECK(e[b].on == (!tree || (at[b] >= 0 && nn > 0)));
     const uint32_t steps = kv8_steps(e[b]);
     uint32_t chunks = kv8_chunks(steps, per);
-    slots += s.one ? 1 : chunks;
+    slots += s.one ? s.groups : kv8_groups(e[b], grp, s.rowslog) * chunks;
     CHECK((chunks == 0) == !e[b].on);
     if (!chunks) continue;
     if (s.one) chunks = 1;
@@ -141,13 +152,13 @@ int main(void) {
   if (call(false, false, {2147483647}, {1}, 1, 1, 16, 1, 1) || call(true, false, {2147483647}, {5}, 5, 1, 16, 2, 1)) return 1;
   const Kv8Extent e = kv8_extent(true, 2147483647, 2147483647, 2147483647u, 2147483632u);
   CHECK(e.end == 2147483632u && e.base == 2147483647u && kv8_left(e, 2147483616u) == 16);
-  CHECK(kv8_steps(e) == (1u << 25) && kv8_per(65535ull << 25, 1, 1, 4, 4) == 0x7ffffffcu);
+  CHECK(kv8_steps(e) == (1u << 25) && kv8_per(65535ull << 25, 1, 1, 4, 4).last == 0x7ffffffcu);
   for (uint64_t pos : {16ull, 4096ull, 2147483632ull})
     for (uint32_t batch : {1u, 65535u, 4294967295u})
       for (uint32_t rows : {1u, 16u, 17u, 33u, 65u, 2147483647u}) {
         const Kv8Split s = kv8_split(batch, rows, 8, 64, pos);
         CHECK((uint64_t)s.groups * s.rowsper >= rows && s.slots >= 1);
-        CHECK(s.one == (pos <= (rows > 16 ? 256 : 1024)) && s.blocks >= (uint64_t)s.slots * 8 * s.groups);
+        CHECK(s.one == (pos <= (rows > 32 ? 128 : rows > 16 ? 256 : 1024)) && s.blocks == s.slots * 8);
       }
   printf("ok\n");
   return 0;
@@ -195,9 +206,9 @@ def test_pool_bytes():
 def test_workspace_bytes():
     """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
     w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
-    assert w(1, 20, 5, 128, 16, 64) == 0 and w(1, 20, 5, 128, 16, 65) == 5 * 5 * 4 * 130 * 4
+    assert w(1, 20, 5, 128, 16, 64) == 0 and w(1, 20, 5, 128, 16, 65) == 5 * 5 * 16 * 130 * 4
     assert t(1, 8, 20, 5, 128, 16, 16) == 0 and t(1, 8, 20, 5, 128, 16, 17) == 2 * 5 * 32 * 130 * 4
-    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 4 * 130 * 4
+    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 16 * 130 * 4
     assert w(1, 20, 5, 128, 16, 65) == t(1, 1, 20, 5, 128, 16, 65)
     for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
                 (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
