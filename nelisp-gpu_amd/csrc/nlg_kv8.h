@@ -125,7 +125,7 @@ struct Kv8Split {
 inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint32_t hd, uint64_t positions) {
   Kv8Split s;
   s.wide = rows > 32;
-  s.rowsper = rows > 64 && hd == 64 ? 128 : rows > 32 ? 64 : rows > 16 ? 32 : 16;
+  s.rowsper = rows > 64 && hd == 64 ? 128 : rows > 32 ? 64 : rows > 16 && hd == 64 ? 32 : 16;
   s.rowslog = s.rowsper == 16 ? 4 : s.rowsper == 32 ? 5 : s.rowsper == 64 ? 6 : 7;
   s.groups = (uint32_t)(((uint64_t)rows + s.rowsper - 1) / s.rowsper);
   s.unit = s.wide ? 1 : KV8_WAVES;

@@ -41,6 +41,7 @@ struct AppendArgs {
   double eps;
   uint64_t rows;
   uint32_t batch, heads, trows, qblocks;
+  bool past;  // q is stored past the caches
 };
 
 template <int CTRL>
@@ -219,8 +220,15 @@ __global__ __launch_bounds__(256) void k_append_q8(AppendArgs a) {
   }
   if (h < a.heads) {
     float *q = a.q + (row * a.heads + h) * HD;
-    *(float4 *)(q + d0) = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
-    *(float4 *)(q + d1) = make_float4((float)y[4], (float)y[5], (float)y[6], (float)y[7]);
+    const float4 q0 = make_float4((float)y[0], (float)y[1], (float)y[2], (float)y[3]);
+    const float4 q1 = make_float4((float)y[4], (float)y[5], (float)y[6], (float)y[7]);
+    if (a.past) {
+      nlg_st_stream_f4((float4 *)(q + d0), q0);
+      nlg_st_stream_f4((float4 *)(q + d1), q1);
+    } else {
+      *(float4 *)(q + d0) = q0;
+      *(float4 *)(q + d1) = q1;
+    }
     return;
   }
   uint2 code;
@@ -243,6 +251,7 @@ struct Kv8Attn {
   const uint64_t *mask;   // tree: [batch][tmax] or null
   Kv8Pages pg;
   float *out, *pctx, *pmz;  // partials: [slots][kvheads][rowsper][hd], [slots][kvheads][rowsper][2]
+  uint2 *pfirst;            // [batch]: a sequence's first slot, its chunks
   uint32_t batch, tmax, heads, grp, rows;  // rows = tmax * grp
   uint32_t rowsper, rowslog, groups, want, least, unit, slots;  // Kv8Split
   Kv8Div bykvheads, bygrp, bygroups;
@@ -437,19 +446,6 @@ struct Kv8Plan {
     }
     return false;
   }
-  // Sequence b's first slot and its chunks.
-  __device__ __forceinline__ uint32_t first(const Kv8Attn &a, uint32_t b, int lane, uint32_t &chunks) const {
-    uint32_t before = 0;
-    for (uint32_t b0 = 0;; b0 += 64) {
-      const Kv8Extent l = at(a, b0, lane);
-      const uint32_t n = slots(a, l), to = sums(n);
-      if (b < b0 + 64) {
-        chunks = __builtin_amdgcn_readlane(kv8_chunks(kv8_steps(l), per), b - b0);
-        return before + __builtin_amdgcn_readlane(to, b - b0) - __builtin_amdgcn_readlane(n, b - b0);
-      }
-      before += __builtin_amdgcn_readlane(to, 63);
-    }
-  }
 };
 
 // What a workgroup does: which rows of which sequence and kv head over which positions.
@@ -476,6 +472,8 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
     if (!plan.find(a, w.slot, lane, w.b, w.e, group, chunk, w.chunks)) return false;
     share = kv8_share(kv8_steps(w.e), w.chunks, a.unit) * KV8_STEP;
     w.c0 = chunk * share;
+    // for the launch that joins the chunks
+    if (!group && !chunk && !w.h && threadIdx.x == 0) a.pfirst[w.b] = make_uint2(w.slot, w.chunks);
   }
   w.row0 = group * a.rowsper;
   w.masked = a.mask;
@@ -641,11 +639,18 @@ __device__ __forceinline__ uint4 and4(uint4 x, uint4 m) { return make_uint4(x.x 
 
 #define MFMA(x, y, c) __builtin_amdgcn_mfma_f32_16x16x32_f16(x, y, c, 0, 0, 0)
 
+// PAST: past the caches, for K and V that they will not hold until they are read
+// again.
+template <bool PAST>
+__device__ __forceinline__ uint4 load16(const uint8_t *p) {
+  return PAST ? nlg_ld_stream((const uint4 *)p) : *(const uint4 *)p;
+}
+
 // One step of a wave on its own: 64 positions from p on, tile `tk` holding this
 // lane's K row (4 positions of each of the four tiles a time), tile `tv` its V
 // columns and both scales.  GEN: some of the positions are masked or past the
 // end.
-template <int HD, int FMT, int NT, bool GEN>
+template <int HD, int FMT, int NT, bool GEN, bool PAST>
 __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, WaveState<HD, NT> &w, uint32_t tk,
                                          uint32_t tv, uint32_t p, int lane) {
   constexpr int C = HD / 64, D = HD / 16;
@@ -660,9 +665,9 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
 #pragma unroll
   for (int t = 0; t < 4; t++)
 #pragma unroll
-    for (int c = 0; c < C; c++) kr[t][c] = *(const uint4 *)(kp + t * 4 * HD + c * 64);
+    for (int c = 0; c < C; c++) kr[t][c] = load16<PAST>(kp + t * 4 * HD + c * 64);
 #pragma unroll
-  for (int i = 0; i < D; i++) vr[i] = *(const uint4 *)(vp + i * 256 + n * 16);
+  for (int i = 0; i < D; i++) vr[i] = load16<PAST>(vp + i * 256 + n * 16);
   const uint32_t q0 = p + g * KV8_TILE;  // this lane's first position
   const int left = GEN ? kv8_left(k.e, q0) : 16;
   if (__any(!hv || left < 16)) {
@@ -720,8 +725,8 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
 // Up to 32 rows (16 NT): the workgroup's W waves take its positions in turn, 64
 // at a time, straight from memory into the matrix cores' operands, and meet in
 // LDS.
-template <int HD, int FMT, int NT, int W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(HD * NT > 128 ? 1 : 2, HD * NT > 128 ? 1 : 2)))
+template <int HD, int FMT, int NT, int W, bool PAST>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_q8(Kv8Attn a) {
   constexpr int D = HD / 16;
   __shared__ float4v s_o[W][D][64];
@@ -743,7 +748,7 @@ void k_attn_q8(Kv8Attn a) {
     }
     const int t0 = (int)(p - p0) / KV8_TILE;
     const uint32_t tv = __shfl(tid, t0 + g), tk = __shfl(tid, t0 + (n >> 2));
-    kv8_step<HD, FMT, NT, decltype(GENV)::value != 0>(a, k, w, tk, tv, p, lane);
+    kv8_step<HD, FMT, NT, decltype(GENV)::value != 0, PAST>(a, k, w, tk, tv, p, lane);
     p += W * KV8_STEP;
   };
   while (p + KV8_STEP <= whole) step(Int<0>{});
@@ -963,11 +968,10 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
   __shared__ float2 s_mz[256];
   const uint32_t per = hd / 4, t = threadIdx.x, b = blockIdx.x / blocks;
   const uint32_t r = blockIdx.x % blocks * (256 / per / SUBS) + t / (per * SUBS), sub = t / per % SUBS, d = t % per * 4;
-  const Kv8Plan plan(a, t & 63);
-  uint32_t chunks;
-  const uint32_t slot = plan.first(a, b, t & 63, chunks);
-  if (chunks < 2) return;  // (none, or written already)
   const Kv8Extent e = kv8_of(a, b);
+  const uint2 f = a.pfirst[b];
+  const uint32_t slot = f.x, chunks = f.y;
+  if (!e.on || chunks < 2) return;  // (one: its workgroup has written the row)
   const uint32_t node = r / a.heads, head = r % a.heads;
   const bool on = node < e.nodes;
   const uint32_t h = kv8_quot(a.bygrp, head), row = node * a.grp + head - h * a.grp, group = row >> a.rowslog;
@@ -1099,6 +1103,15 @@ struct Columns {
 __device__ __forceinline__ uint32_t kv8_pick(uint64_t lo, uint64_t hi, uint32_t at) {
   return (uint32_t)((at < 8 ? lo : hi) >> 8 * (at & 7)) & 0xffu;
 }
+// Rows that no cache will hold until they are read are stored past it (many rows
+// only: 20,384 of 8 heads of 128 33 -> 26 us).
+template <bool NT>
+__device__ __forceinline__ void store16(void *p, uint4 v) {
+  typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+  const v4u t = {v.x, v.y, v.z, v.w};
+  if (NT) __builtin_nontemporal_store(t, (v4u *)p);
+  else *(v4u *)p = t;
+}
 // A wave reads N rows of one kv head: sixteen, or four where there are too few
 // rows to fill the card.  K: HD / 8 lanes a row.  V: a lane holds the sixteen
 // positions of two (HD 128) or one dimensions of a tile, and gives each of its
@@ -1159,8 +1172,12 @@ __global__ __launch_bounds__(256) void k_read_q8(ReadArgs a) {
     uint32_t pair = kv8_pick(c.a0, c.a1, fa) | (DV == 2 ? kv8_pick(c.b0, c.b1, fa) << 8 : 0u);
     if (from == KV8_NONE) pair = 0;
     const half2v v = kv8_value2<FMT, 0>(pair, s);
-    if (DV == 2) *(half2v *)(a.v + o) = v;
-    else *(_Float16 *)(a.v + o) = v[0];
+    if (DV == 2) {
+      if (N > 1) __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, v), (uint32_t *)(a.v + o));
+      else *(half2v *)(a.v + o) = v;
+    } else {
+      *(_Float16 *)(a.v + o) = v[0];
+    }
   }
 #pragma unroll
   for (int p = 0; p < N / RP; p++) {
@@ -1174,7 +1191,7 @@ __global__ __launch_bounds__(256) void k_read_q8(ReadArgs a) {
     o.h[1] = kv8_value2<FMT, 1>(k[p].x, ks[p]);
     o.h[2] = kv8_value2<FMT, 0>(k[p].y, ks[p]);
     o.h[3] = kv8_value2<FMT, 1>(k[p].y, ks[p]);
-    *(uint4 *)(a.k + ((r0 + i) * a.pg.kvheads + h) * HD + m * 8) = o.u;
+    store16<(N > 1)>(a.k + ((r0 + i) * a.pg.kvheads + h) * HD + m * 8, o.u);
   }
 }
 
@@ -1233,6 +1250,8 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   a.qkv = qkv; a.qgain = qgain; a.kgain = kgain; a.co = rope_cos; a.si = rope_sin;
   a.seq = seq; a.slot = slot; a.rpos = rpos; a.q = q; a.kpool = kpool; a.vpool = vpool;
   a.eps = eps; a.rows = rows; a.batch = batch; a.heads = heads; a.trows = trows; a.qblocks = (uint32_t)qb;
+  // queries that outgrow the L2 caches are not kept in them (4,731 rows of 32 heads of 128: 51 -> 45 us)
+  a.past = (uint64_t)rows * heads * head_dim * 4 > (32u << 20);
   const dim3 grid((uint32_t)(qb + vb)), blk(256);
   hipStream_t st = nlg_stream(stream);
 #define GO(HD, F)                                                                          \
@@ -1250,9 +1269,9 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   return NLG_OK;
 }
 
-// The partials' bytes: contexts, then (maximum, sum) pairs; 0 where one chunk needs none.
-static uint64_t kv8_partials(const Kv8Split &s, uint32_t kvheads, uint32_t hd) {
-  return s.one ? 0 : s.slots * kvheads * s.rowsper * (hd + 2) * 4;
+// The partials' bytes: contexts, (maximum, sum) pairs, where each sequence's are; 0 where one chunk needs none.
+static uint64_t kv8_partials(const Kv8Split &s, uint32_t batch, uint32_t kvheads, uint32_t hd) {
+  return s.one ? 0 : s.slots * kvheads * s.rowsper * (hd + 2) * 4 + 8ull * batch;
 }
 // Sizes an attention call can have at all (0: none).
 static uint64_t kv8_rows(uint32_t tmax, uint32_t heads, uint32_t kvheads) {
@@ -1267,7 +1286,7 @@ extern "C" size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax
   if (!batch || !rows || !bs || bs % KV8_TILE || !mbps || (uint64_t)bs * mbps > 0x7fffffffull ||
       (head_dim != 64 && head_dim != 128))
     return 0;
-  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, head_dim, (uint64_t)bs * mbps), kvheads, head_dim);
+  return (size_t)kv8_partials(kv8_split(batch, (uint32_t)rows, kvheads, head_dim, (uint64_t)bs * mbps), batch, kvheads, head_dim);
 }
 extern "C" size_t nlg_decode_attn_paged_q8_workspace(uint32_t batch, uint32_t heads, uint32_t kvheads,
                                                      uint32_t head_dim, uint32_t bs, uint32_t mbps) {
@@ -1288,7 +1307,7 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   if (mask && tmax > KV8_TREE) return nlg_fail("%s: %u nodes under a mask (at most %d)", what, tmax, KV8_TREE);
   if (mask && ((uintptr_t)mask & 7)) return nlg_fail("%s: the masks must be 8-byte aligned", what);
   const Kv8Split s = kv8_split(batch, (uint32_t)rows, kvheads, hd, (uint64_t)bs * mbps);
-  const uint64_t need = kv8_partials(s, kvheads, hd);
+  const uint64_t need = kv8_partials(s, batch, kvheads, hd);
   // joining: eight groups of threads a row while its rows would not fill the card with one
   const uint64_t orows = (uint64_t)tmax * heads;
   const bool subs = orows * batch * (hd / 4) < 65536;
@@ -1309,16 +1328,22 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   a.tree = tree; a.one = s.one;
   a.pctx = (float *)workspace;
   a.pmz = need ? a.pctx + s.slots * kvheads * s.rowsper * hd : nullptr;
+  a.pfirst = need ? (uint2 *)(a.pmz + s.slots * kvheads * s.rowsper * 2) : nullptr;
   a.coef = NLG_LOG2E / sqrtf((float)hd);
   const dim3 grid((uint32_t)s.blocks);
   hipStream_t st = nlg_stream(stream);
-#define GO(HD, F)                                                                                          \
-  do {                                                                                                     \
-    if (s.rowsper == 16 && s.one) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 8>), grid, dim3(512), 0, st, a); \
-    else if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 4>), grid, dim3(256), 0, st, a);     \
-    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<HD, F, 2, 4>), grid, dim3(256), 0, st, a);     \
-    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1>), grid, dim3(256), 0, st, a);   \
-    else hipLaunchKernelGGL((k_attn_wide_q8<64, F, 2>), grid, dim3(256), 0, st, a);                        \
+  // K and V of more than the 256 MB MALL are gone from it before the next call
+  // reads them (eight sequences at 24,000-32,768 of 8 heads of 128, 480 MB: 94 ->
+  // 88 us; 32 at up to 4,096 of 5, 87 MB: 25.4 us kept, 27.0 past)
+  const bool past = (uint64_t)batch * mbps * bs * kvheads * 2 * (hd + 4) > (256u << 20);
+#define GO(HD, F)                                                                                                 \
+  do {                                                                                                            \
+    if (s.rowsper == 16 && s.one) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 8, false>), grid, dim3(512), 0, st, a); \
+    else if (s.rowsper == 16 && past) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 4, true>), grid, dim3(256), 0, st, a); \
+    else if (s.rowsper == 16) hipLaunchKernelGGL((k_attn_q8<HD, F, 1, 4, false>), grid, dim3(256), 0, st, a);     \
+    else if (s.rowsper == 32) hipLaunchKernelGGL((k_attn_q8<64, F, 2, 4, false>), grid, dim3(256), 0, st, a);     \
+    else if (s.rowsper == 64) hipLaunchKernelGGL((k_attn_wide_q8<HD, F, 1>), grid, dim3(256), 0, st, a);          \
+    else hipLaunchKernelGGL((k_attn_wide_q8<64, F, 2>), grid, dim3(256), 0, st, a);                               \
   } while (0)
   if (hd == 128) {
     if (fmt == NLG_KV_I8) GO(128, NLG_KV_I8); else GO(128, NLG_KV_E4M3);

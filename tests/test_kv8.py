@@ -206,9 +206,9 @@ def test_pool_bytes():
 def test_workspace_bytes():
     """0 where one chunk needs none and for sizes that are refused; the bytes of all partials else."""
     w, t = nlgpu.decode_attn_paged_q8_workspace, nlgpu.tree_attn_paged_q8_workspace
-    assert w(1, 20, 5, 128, 16, 64) == 0 and w(1, 20, 5, 128, 16, 65) == 5 * 5 * 16 * 130 * 4
-    assert t(1, 8, 20, 5, 128, 16, 16) == 0 and t(1, 8, 20, 5, 128, 16, 17) == 2 * 5 * 32 * 130 * 4
-    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 16 * 130 * 4
+    assert w(1, 20, 5, 128, 16, 64) == 0 and w(1, 20, 5, 128, 16, 65) == 5 * 5 * 16 * 130 * 4 + 8
+    assert t(1, 8, 20, 5, 64, 16, 16) == 0 and t(1, 8, 20, 5, 64, 16, 17) == 2 * 5 * 32 * 66 * 4 + 8
+    assert w(3, 20, 5, 128, 16, 1 << 20) == (512 // 5) * 5 * 16 * 130 * 4 + 24
     assert w(1, 20, 5, 128, 16, 65) == t(1, 1, 20, 5, 128, 16, 65)
     for bad in ((0, 1, 20, 5, 128, 16, 64), (1, 0, 20, 5, 128, 16, 64), (1, 1, 20, 3, 128, 16, 64),
                 (1, 1, 20, 0, 128, 16, 64), (1, 1, 0, 5, 128, 16, 64), (1, 1, 20, 5, 96, 16, 64),
