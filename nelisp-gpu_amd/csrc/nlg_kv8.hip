@@ -505,8 +505,12 @@ struct WaveState {
   uint32_t node[NT];
   uint64_t word[NT];       // the node's mask
 
-  __device__ __forceinline__ void begin(const Kv8Attn &a, const Kv8Work &k, uint32_t row0, int lane) {
-    constexpr int C = HD / 64;
+  // The rows' queries asked for, and made ready (what is loaded between the two
+  // arrives while they are).
+  struct Queries {
+    float4 x[NT][HD / 16];
+  };
+  __device__ __forceinline__ void fetch(const Kv8Attn &a, const Kv8Work &k, uint32_t row0, int lane, Queries &f) {
     const int g = lane >> 4, n = lane & 15;
 #pragma unroll
     for (int i = 0; i < NT; i++) {
@@ -515,16 +519,23 @@ struct WaveState {
       const bool on = node[i] < k.e.nodes;
       const size_t qrow = (size_t)k.b * a.tmax + (on ? node[i] : 0);
       const float *q = a.q + (qrow * a.heads + (size_t)k.h * a.grp + (on ? row - node[i] * a.grp : 0)) * HD + g * 16;
-      word[i] = k.masked && on ? kv8_word(a.mask[qrow], k.e.nodes) : 0;
+      word[i] = k.masked && on ? a.mask[qrow] : 0;
+#pragma unroll
+      for (int j = 0; j < HD / 16; j++) f.x[i][j] = *(const float4 *)(q + j / 4 * 64 + j % 4 * 4);
+    }
+  }
+  __device__ __forceinline__ void begin(const Kv8Attn &a, const Kv8Work &k, const Queries &f) {
+    constexpr int C = HD / 64;
+#pragma unroll
+    for (int i = 0; i < NT; i++) {
+      const bool on = node[i] < k.e.nodes;
+      word[i] = kv8_word(word[i], k.e.nodes);
       float x[HD / 4], top = 0.0f;
 #pragma unroll
-      for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float4 t = *(const float4 *)(q + c * 64 + j * 4);
-          float *y = x + c * 16 + j * 4;
-          y[0] = t.x; y[1] = t.y; y[2] = t.z; y[3] = t.w;
-        }
+      for (int j = 0; j < HD / 16; j++) {
+        float *y = x + j * 4;
+        y[0] = f.x[i][j].x; y[1] = f.x[i][j].y; y[2] = f.x[i][j].z; y[3] = f.x[i][j].w;
+      }
 #pragma unroll
       for (int j = 0; j < HD / 4; j++) {
         x[j] = on ? x[j] * a.coef : 0.0f;
@@ -736,7 +747,9 @@ void k_attn_q8(Kv8Attn a) {
   if (!kv8_work(a, lane, k)) return;
   uint32_t tid = kv8_tiles(a, k, k.c0, lane);
   WaveState<HD, NT> w;
-  w.begin(a, k, k.row0, lane);
+  typename WaveState<HD, NT>::Queries qx;
+  w.fetch(a, k, k.row0, lane, qx);
+  w.begin(a, k, qx);
   const uint32_t whole = k.e.base < k.c1 ? k.e.base : k.c1;  // no mask below this position
   uint32_t p0 = k.c0;  // tid: the tiles from here on
   uint32_t p = k.c0 + wv * KV8_STEP;
@@ -912,8 +925,10 @@ void k_attn_wide_q8(Kv8Attn a) {
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  if (k.c0 < k.c1) load(k.c0);  // (under way while the queries are made ready)
-  w.begin(a, k, row0, lane);
+  typename WaveState<HD, NT>::Queries qx;
+  w.fetch(a, k, row0, lane, qx);
+  if (k.c0 < k.c1) load(k.c0);
+  w.begin(a, k, qx);
   if (k.c0 < k.c1) {
     store(0);
     float ksc = ks, vsc = vs;
