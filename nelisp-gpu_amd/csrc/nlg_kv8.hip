@@ -116,13 +116,17 @@ __device__ __forceinline__ void load8(const float *p, const float *q, double *y)
   y[4] = b.x; y[5] = b.y; y[6] = b.z; y[7] = b.w;
 }
 
-// All in 64 bits: a code then depends on the inputs alone and not on the order
-// of a sum, so a prefix cached twice holds the same bytes.  They cost little
-// only where lanes share a row's root and quotients: a head row is on HD / 8
-// lanes, eight values (four rotation pairs) each.  The first qblocks workgroups
-// take the q and k heads; the others V, a wave sixteen rows of one head, whose
-// codes pass through LDS: a position's bytes of a tile lie sixteen apart, and a
-// store then runs over 64 dimensions (8 lines) instead of one byte a line.
+// y = x / sqrt(mean(x^2) + eps) * gain, rotated; codes of y / scale.  All in 64
+// bits: a code then depends on the inputs alone and not on the order of a sum, so
+// a prefix cached twice holds the same bytes.  They cost little only where lanes
+// share a row's root and quotients: a head row is on HD / 8 lanes, eight values
+// (four rotation pairs) each (on all 64 of a wave 97 us at 4,731 rows of 32/8
+// heads of 128, 51 so).  The first qblocks workgroups take the q and
+// k heads; the others V, a wave sixteen rows of one head, whose codes pass
+// through LDS: a position's bytes of a tile lie sixteen apart, and a store then
+// runs over 64 dimensions (8 lines) instead of one byte a line.  Bound by the
+// bytes where there are many: 48 us there, 204 MB, 4.2 TB/s; one row of 20/5
+// heads, 3.1 us, by the chain slot -> block -> store.
 template <int HD, int FMT, bool HALF>
 __global__ __launch_bounds__(256) void k_append_q8(AppendArgs a) {
   constexpr int L = HD / 8, RP = 64 / L;  // lanes a row, rows at once
@@ -252,7 +256,7 @@ struct Kv8Attn {
   Kv8Pages pg;
   float *out, *pctx, *pmz;  // partials: [slots][kvheads][rowsper][hd], [slots][kvheads][rowsper][2]
   uint2 *pfirst;            // [batch]: a sequence's first slot, its chunks
-  uint32_t batch, tmax, heads, grp, rows;  // rows = tmax * grp
+  uint32_t batch, tmax, heads, grp;  // grp: query heads of a kv head; a sequence's rows: tmax * grp
   uint32_t rowsper, rowslog, groups, want, least, unit, slots;  // Kv8Split
   Kv8Div bykvheads, bygrp, bygroups;
   bool tree, one;
@@ -304,22 +308,36 @@ __device__ __forceinline__ void split8(const float *w, half8v &hi, half8v &lo) {
 }
 // Eight products of f32 as halves: rounded, and what that left, rounded (exact
 // where it is representable).  Written out: each is one mixed FMA that leaves its
-// half in place, where the compiler takes two instructions.  (The first wait is for an
-// exponential that was issued just before.)
+// half in place, where the compiler takes two instructions.  It does not look
+// inside, so the waits are here too: before, for an exponential issued just
+// ahead (one state); after, for a matrix instruction that reads the result (two).
 __device__ __forceinline__ void split_products(const float *x, const float *y, half8v &hi, half8v &lo) {
   union {
     half8v v;
     uint32_t u[4];
   } a, b;
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-    asm("s_nop 0\n\t"
-        "v_fma_mixlo_f16 %0, %2, %4, 0\n\t"
-        "v_fma_mixhi_f16 %0, %3, %5, 0\n\t"
-        "v_fma_mixlo_f16 %1, %2, %4, -%0 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
-        "v_fma_mixhi_f16 %1, %3, %5, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]"
-        : "=&v"(a.u[i]), "=&v"(b.u[i])
-        : "v"(x[2 * i]), "v"(x[2 * i + 1]), "v"(y[2 * i]), "v"(y[2 * i + 1]));
+  asm("s_nop 0\n\t"
+      "v_fma_mixlo_f16 %0, %8, %16, 0\n\t"
+      "v_fma_mixhi_f16 %0, %9, %17, 0\n\t"
+      "v_fma_mixlo_f16 %1, %10, %18, 0\n\t"
+      "v_fma_mixhi_f16 %1, %11, %19, 0\n\t"
+      "v_fma_mixlo_f16 %2, %12, %20, 0\n\t"
+      "v_fma_mixhi_f16 %2, %13, %21, 0\n\t"
+      "v_fma_mixlo_f16 %3, %14, %22, 0\n\t"
+      "v_fma_mixhi_f16 %3, %15, %23, 0\n\t"
+      "v_fma_mixlo_f16 %4, %8, %16, -%0 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %4, %9, %17, -%0 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %5, %10, %18, -%1 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %5, %11, %19, -%1 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %6, %12, %20, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %6, %13, %21, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixlo_f16 %7, %14, %22, -%3 op_sel:[0,0,0] op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %7, %15, %23, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "s_nop 1"
+      : "=&v"(a.u[0]), "=&v"(a.u[1]), "=&v"(a.u[2]), "=&v"(a.u[3]), "=&v"(b.u[0]), "=&v"(b.u[1]), "=&v"(b.u[2]),
+        "=&v"(b.u[3])
+      : "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]), "v"(y[0]), "v"(y[1]),
+        "v"(y[2]), "v"(y[3]), "v"(y[4]), "v"(y[5]), "v"(y[6]), "v"(y[7]));
   hi = a.v;
   lo = b.v;
 }
@@ -733,9 +751,16 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
   }
 }
 
-// Up to 32 rows (16 NT): the workgroup's W waves take its positions in turn, 64
-// at a time, straight from memory into the matrix cores' operands, and meet in
-// LDS.
+// Few rows (16 NT a group): the workgroup's W waves take its positions in turn,
+// 64 at a time, straight from memory into the matrix cores' operands, and meet
+// in LDS.  S^T = K q^T and O^T = V^T p^T: a lane then holds one query row and, as
+// the scores come out, the very sixteen positions that the second product wants
+// of it, with K's rows dealt to the first so (4 of each tile a time); nothing is
+// exchanged but maxima and sums.  One pass over the cache, bound by its bytes:
+// 8 sequences at 24,000-32,768, 32/8 heads of 128, 480 MB: 85 us, 5.7 TB/s; 32
+// of up to 4,096, 20/5 heads, 87 MB: 22 us, 4.0 TB/s, the chain lengths -> table
+// -> K, V before it and chunks of unequal lengths; 640 positions of one sequence
+// (eight waves, no second launch): 9.2 us, that chain and the waves' meeting.
 template <int HD, int FMT, int NT, int W, bool PAST>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_q8(Kv8Attn a) {
@@ -811,8 +836,15 @@ void k_attn_q8(Kv8Attn a) {
 // and K and V are made halves once for the workgroup, in LDS, in the order in
 // which the waves' operands lie (a fragment's 64 lanes side by side: no bank is
 // asked twice).  While a step is computed the next one's halves are written and
-// the one's after it are on their way from memory.  Two waves a SIMD: the
-// matrix cores work for one while the other is at its softmax.
+// the one's after it are on their way from memory.  Bound by issue: two chunks
+// of 500-512 tokens over 1,024-2,047, 32/8 heads of 64, take 58 us, 256 TFLOP/s
+// (each product counted once; it is done twice, for hi and lo).  When they took
+// 68 with the join, 22 were left without any step, 28 with only the loads and the
+// halves in LDS; the softmax was 20, the second product 5, waiting for memory 4.
+// 16 trees of up to 32 nodes over up to 4,000, 20/5 heads of 128: 31 us (of 46
+// with the join, 20 without steps, 6 for the softmax).  Two waves a SIMD: three at
+// head dim 64, with 64 rows a workgroup, took 69 us for 60; eight waves a
+// workgroup 85 for 76.
 template <int HD, int FMT, int NT>
 __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_wide_q8(Kv8Attn a) {
@@ -975,7 +1007,7 @@ void k_attn_wide_q8(Kv8Attn a) {
   }
 }
 
-// The chunks' parts of each output row, joined: SUBS groups of hd / 4 threads
+// The chunks' parts of each output row, joined by their maxima: SUBS groups of hd / 4 threads
 // walk a row's chunks.  A workgroup's rows are of one sequence.
 template <int SUBS>
 __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint32_t blocks) {
@@ -1040,7 +1072,8 @@ struct CommitArgs {
   uint32_t tmax;
 };
 // A workgroup moves the rows of one sequence, kv head and pool: all are read
-// before the first is written.
+// before the first is written.  A few kilobytes: the chain path -> block -> bytes
+// -> store bounds it, 5 us for one sequence as for 64.
 template <int HD>
 __global__ __launch_bounds__(256) void k_commit_q8(CommitArgs a) {
   __shared__ uint32_t s_from[KV8_TREE], s_to[KV8_TREE];
@@ -1265,7 +1298,8 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   a.qkv = qkv; a.qgain = qgain; a.kgain = kgain; a.co = rope_cos; a.si = rope_sin;
   a.seq = seq; a.slot = slot; a.rpos = rpos; a.q = q; a.kpool = kpool; a.vpool = vpool;
   a.eps = eps; a.rows = rows; a.batch = batch; a.heads = heads; a.trows = trows; a.qblocks = (uint32_t)qb;
-  // queries that outgrow the L2 caches are not kept in them (4,731 rows of 32 heads of 128: 51 -> 45 us)
+  // queries that outgrow the L2 caches are not kept in them (4,731 rows of 32 heads of 128, with
+  // the codes read back: 62 -> 57 us)
   a.past = (uint64_t)rows * heads * head_dim * 4 > (32u << 20);
   const dim3 grid((uint32_t)(qb + vb)), blk(256);
   hipStream_t st = nlg_stream(stream);
@@ -1337,7 +1371,7 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   }
   KV8_SCOPE(what);
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
-  a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads; a.rows = (uint32_t)rows;
+  a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads;
   a.rowsper = s.rowsper; a.rowslog = s.rowslog; a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
   a.bygroups = kv8_div(s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
   a.tree = tree; a.one = s.one;
