@@ -628,3 +628,98 @@ def test_offsets_past_four_gib():
     for d, which in ((rk, "k"), (rv, "v")):
         row = want.row(local, 0, 90, which).astype(F32).astype(np.float16)
         assert np.array_equal(down(d, np.float16, (2, hd)), np.concatenate([row, row]))
+
+
+# ------------------------------------------------------------------ how the work is laid out
+
+@pytest.mark.parametrize("batch,tmax,heads,kvh,hd", [(150, 1, 8, 2, 64), (70, 5, 8, 2, 64), (65, 17, 4, 2, 128)])
+def test_many_sequences(batch, tmax, heads, kvh, hd):
+    """More sequences than a wave has lanes, few of them long: the layout is counted over several rounds of 64."""
+    rng = np.random.default_rng(batch)
+    bs, mbps = 16, 70
+    base = rng.integers(-1, 90, batch)
+    base[[0, 63, 64, batch - 1]] = [1119 - tmax, 700, 1100 - tmax, 300]
+    pools, table = cached(rng, base + tmax, kvh, hd, bs, mbps, ref.I8)
+    if tmax == 1:
+        q = rng.standard_normal((batch, heads * hd)).astype(F32)
+        check_decode(pools, table, q, base.astype(np.int32))
+        return
+    q = rng.standard_normal((batch, tmax, heads * hd)).astype(F32)
+    nodes = rng.integers(0, tmax + 1, batch).astype(np.int32)
+    nodes[[0, 63, 64]] = tmax
+    check_tree(pools, table, q, base.astype(np.int32), nodes, words(rng, batch, tmax), rows=(0, tmax - 1))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tmax", [1, 40])
+def test_long_chunks(fmt, tmax):
+    """So many kv heads that a chunk of one sequence is longer than the 1,024 positions whose tiles a wave looks up at
+    once; five heads are compared."""
+    rng = np.random.default_rng(13 + tmax)
+    kvh, hd, bs, n = 256, 64, 16, 2350
+    pools = ref.Pools(150, kvh, hd, bs, fmt)
+    table = rng.permutation(150)[:148].reshape(1, 148).astype(np.int32)
+    for p in (pools.k, pools.v):
+        c = rng.integers(0, 255, p.shape[:3] + (16 * hd,)).astype(np.uint8)
+        # (any int8 but -128; any e4m3 but the NaN codes, and none over 30)
+        c = np.where(c == 0x80, 0, c) if fmt == ref.I8 else (c & 0x80) | (c & 0x7f) % 0x5f
+        p[..., :16 * hd] = c
+        s = rng.uniform(0.5, 1.5, p.shape[:3] + (16,)) / (74.0 if fmt == ref.I8 else 8.0)
+        p[..., 16 * hd:] = np.ascontiguousarray(s.astype(F32)).view(np.uint8)
+    q = rng.standard_normal((1, tmax, kvh * hd)).astype(F32)
+    base = np.array([n - tmax], np.int32)
+    got = decode(pools, table, q[0], base)[None] if tmax == 1 else tree(pools, table, q, base, None, None)
+    some = [0, 1, 100, 254, 255]
+    part = ref.Pools(150, len(some), hd, bs, fmt)
+    part.k, part.v = (np.ascontiguousarray(p[:, some]) for p in (pools.k, pools.v))
+    k, v = (part.rows(table, 0, n, w) for w in "kv")
+    for i in {0, tmax // 2, tmax - 1}:
+        g, x = (t[0, i].reshape(kvh, hd)[some].reshape(-1) for t in (got, q))
+        close(g, x, k, v, np.arange(n) <= n - tmax + i, (i, n))
+
+
+@pytest.mark.parametrize("fmt,hd,bs,mbps", [(ref.I8, 64, 16, 1 << 15), (ref.E4M3, 128, 64, 1 << 12)])
+def test_table_of_many_blocks(fmt, hd, bs, mbps):
+    """A table whose positions would be over 256 MB, of which few have blocks: those without one are zero rows."""
+    rng = np.random.default_rng(mbps)
+    heads, kvh, batch = 16, 4, 2
+    n = 1280 // bs
+    pools = ref.Pools(2 * n, kvh, hd, bs, fmt, fill=0xff)
+    table = np.full((batch, mbps), -1, np.int32)
+    table[:, :n] = rng.permutation(2 * n).reshape(2, n)
+    lens = np.array([1279, 1500], np.int32)
+    for b in range(batch):
+        pools.fill_rows(table, b, range(1280), rng)
+    assert batch * mbps * bs * kvh * 2 * (hd + 4) > 1 << 28
+    check_decode(pools, table, rng.standard_normal((batch, heads * hd)).astype(F32), lens)
+
+
+def test_two_graphs_of_one_workspace():
+    """Two captured calls that share a workspace, replayed in turn on one stream, give the bits of calls alone."""
+    rng = np.random.default_rng(17)
+    heads, kvh, hd, bs, mbps, batch = 20, 5, 128, 16, 80, 3
+    lens = np.array([1250, 30, 800], np.int32)
+    pools, table = cached(rng, lens + 1, kvh, hd, bs, mbps, ref.I8)
+    qs = [rng.standard_normal((batch, heads * hd)).astype(F32) for _ in range(2)]
+    want = [decode(pools, table, q, lens) for q in qs]
+    st = nlgpu.lib().nlg_stream_create()
+    dk, dv, dt, dl = up(pools.k), up(pools.v), up(table), up(lens)
+    need = nlgpu.decode_attn_paged_q8_workspace(batch, heads, kvh, hd, bs, mbps)
+    ws, dq, outs = nlgpu.DeviceArray(need), [up(q) for q in qs], [nlgpu.DeviceArray(q.nbytes) for q in qs]
+    assert need > 0
+    graphs = []
+    for i in range(2):
+        nlgpu.graph_begin(st)
+        nlgpu.decode_attn_paged_q8(dq[i], dk, dv, dl, dt, pools.npool, outs[i], batch, heads, kvh, hd, bs, mbps, ws,
+                                   stream=st)
+        graphs.append(nlgpu.graph_end(st))
+    for _ in range(3):
+        for o in outs:
+            o.zero(st)
+        for g in graphs:
+            nlgpu.graph_launch(g, st)
+        nlgpu.sync(st)
+        assert all(same(down(o, F32, w.shape), w) for o, w in zip(outs, want))
+    for g in graphs:
+        nlgpu.graph_destroy(g)
+    nlgpu.lib().nlg_stream_destroy(st)
