@@ -380,13 +380,13 @@ int nlg_block_copy_f16(uint16_t *kpool, uint16_t *vpool, const int32_t *pairs, u
  *                (ties to even), an int8
  *   NLG_KV_E4M3  scale = a/448, code = x/scale to the nearest e4m3 (finite)
  * with a the row's largest magnitude (f32) and one scale a position and kv
- * head.  A row with a value that is not finite (in f32) is stored as codes 0 and scale
- * NaN, and so reads as NaN; a zero row has scale 0.
+ * head.  A row with a value that is not finite (in f32) is stored as codes 0
+ * and scale NaN, and so reads as NaN; a zero row has scale 0.
  * nlg_block_copy_f16 copies blocks of these pools when it is given kvdim =
  * kvheads * (head_dim + 4) / 2.  nlg_kv_q8_pool_bytes: bytes of one pool (0:
  * sizes that the cache does not take).  head_dim is 64 or 128, heads any
- * multiple of kvheads; pools are 16-byte aligned.  Nothing here allocates, so every call may be
- * captured into a graph.
+ * multiple of kvheads; pools are 16-byte aligned.  Nothing here allocates, so
+ * every call may be captured into a graph.
  * ---------------------------------------------------------------------- */
 #define NLG_KV_I8 0
 #define NLG_KV_E4M3 1
@@ -403,8 +403,8 @@ size_t nlg_kv_q8_pool_bytes(uint32_t npool, uint32_t kvheads, uint32_t head_dim,
  * the queries; k and v are quantised into position slot[r] of the sequence.
  * Rows whose sequence, slot or block is out of range (a negative slot:
  * padding) cache nothing.  qkv, q, gains and tables are 16-byte aligned; the
- * rows of one call name distinct positions; q does not overlap qkv.  All is computed in 64 bits, so a row's codes depend
- * on its inputs alone.  For drafted tokens rpos is the node's depth behind
+ * rows of one call name distinct positions; q does not overlap qkv.  All is computed in 64
+ * bits, so a row's codes depend on its inputs alone.  For drafted tokens rpos is the node's depth behind
  * the context, and slot the node's place. */
 int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const float *kgain, float eps,
                                      const float *rope_cos, const float *rope_sin, uint32_t trows, int rope_half,
@@ -415,13 +415,14 @@ int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const
 
 /* Single-query attention of every sequence over its positions 0..lens[b]
  * (nlg_decode_attn_paged_f16's, with K and V from the 8-bit pools): out and q
- * [batch x heads*head_dim], 16-byte aligned.  lens[b] < 0: nothing is attended and the row is
- * zero; positions past the block table are not attended; table entries
+ * [batch x heads*head_dim], 16-byte aligned.  lens[b] < 0: nothing is attended
+ * and the row is zero; positions past the block table are not attended; table entries
  * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
- * and carry 22 bits of q and of the probabilities.  V rows
- * whose scales lie more than 2^12 below the largest in a chunk lose bits.
- * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0 bytes: none is read), as
- * below; calls that share one run in stream order. */
+ * and carry 22 bits of q and of the probabilities.  Of the V rows
+ * that a query attends, those whose scales lie more than 2^12 below the
+ * largest lose bits (what is masked does not count, up to 2^60 above).
+ * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0
+ * bytes: none is read), as below; calls that share one run in stream order. */
 int nlg_decode_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt,
                              const int32_t *lens, const int32_t *table, uint32_t npool, float *out, uint32_t batch,
                              uint32_t heads, uint32_t kvheads, uint32_t head_dim, uint32_t bs, uint32_t mbps,
@@ -448,8 +449,8 @@ size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax, uint32_t 
 
 /* A tree's accepted path moved behind the context: for i < accepted[b] (at
  * most tmax <= 64) the cached row of node path[b*tmax + i], position base[b] +
- * path[..], goes to position base[b] + i, as if all of a sequence's rows were read before
- * any is written.  Entries outside [0, tmax), and rows whose source or
+ * path[..], goes to position base[b] + i, as if all of a sequence's rows
+ * were read before any is written.  Entries outside [0, tmax), and rows whose source or
  * destination has no block, move nothing; sequences with base[b] < 0 are
  * left alone.  Blocks written here belong to one sequence. */
 int nlg_tree_commit_paged_q8(uint8_t *kpool, uint8_t *vpool, const int32_t *base, const int32_t *path,

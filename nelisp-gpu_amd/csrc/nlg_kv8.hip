@@ -507,6 +507,12 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 // scales in units of vref / 2^(15 - KV8_SLACK) they stay within fp16.
 #define KV8_SLACK 6.0f
 #define KV8_VUNIT 512.0f  // 2^(15 - KV8_SLACK)
+// V scales this many binades below vref keep 22 bits of the products; how far a
+// row is lifted at most (its sum stays in 32 bits); the distance of a row that has
+// attended nothing yet (negative: of a row that is none).
+#define KV8_NEAR 8.0f
+#define KV8_UP 60.0f
+#define KV8_NEVER 1e6f
 // The maximum of no score: finite, so that no difference of two is a NaN.
 #define KV8_FLOOR -1.7e38f
 
@@ -518,7 +524,8 @@ struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
   float rs[NT];            // what the row's q was divided by (a power of two)
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
-  float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times KV8_VUNIT / vref
+  float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest V scale
+  float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^up KV8_VUNIT / vref
   float vref, vinv;        // a power of two no V scale so far exceeds, or 0; KV8_VUNIT / vref
   uint32_t node[NT];
   uint64_t word[NT];       // the node's mask
@@ -570,7 +577,8 @@ struct WaveState {
         split8(x + c * 16 + 8, qh[i][2 * c + 1], ql[i][2 * c + 1]);
       }
       m[i] = KV8_FLOOR;
-      z[i] = 0.0f;
+      z[i] = up[i] = 0.0f;
+      far[i] = on ? KV8_NEVER : -KV8_NEVER;
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -604,6 +612,24 @@ struct WaveState {
     return f;
   }
 
+  // vref is of all positions, those too that a row does not attend (another
+  // branch's, a later token's).  A row whose own V scales are far below it has its
+  // probabilities, sum and context carry 2^up, so that no masked row, however
+  // large, takes their products' bits.  Returns what up has grown by, as a factor.
+  template <bool GEN>
+  __device__ __forceinline__ float near(int i, const float *vb, float vresc, uint32_t bits) {
+    float v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; j++) v = fmaxf(v, !GEN || bits >> j & 1 ? fabsf(vb[j]) : 0.0f);
+    v = rows_max(v);
+    if (vresc > 0.0f) far[i] = far[i] + (float)(1 - __builtin_amdgcn_frexp_expf(vresc));
+    if (v > 0.0f) far[i] = fminf(far[i], (float)(9 - __builtin_amdgcn_frexp_expf(v)));
+    const float now = far[i] > KV8_NEAR && far[i] < KV8_NEVER ? fminf(far[i], KV8_UP) : 0.0f;
+    const float lift = ldexpf(1.0f, (int)(now - up[i]));
+    up[i] = now;
+    return lift;
+  }
+
   // A step's scores of tile i (products of the codes with q) made probabilities:
   // the running maximum and sum, the contexts rescaled, and the probabilities
   // times the V scales (vb, all sixteen) as halves hi + lo: the product rounded,
@@ -625,16 +651,17 @@ struct WaveState {
 #pragma unroll
     for (int j = 3; j < 15; j += 2) top = max3(top, s[j], s[j + 1]);
     top = max3(top, s[15], s[15]) * rs[i];
-    if (__any(top > m[i] + KV8_SLACK || vresc != 1.0f)) {
+    if (__any(top > m[i] + KV8_SLACK || vresc != 1.0f || far[i] > KV8_NEAR)) {
       top = rows_max(top);
       const float mn = top > m[i] + KV8_SLACK ? top : m[i];
-      const float al = nlg_exp2(m[i] - mn), sc = al * vresc;
+      const float al = nlg_exp2(m[i] - mn);
       m[i] = mn;
-      z[i] = z[i] * al;
+      const float lift = near<GEN>(i, vb, vresc, bits), sc = al * (vresc * lift);
+      z[i] = z[i] * (al * lift);
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;
     }
-    const float ms = m[i];
+    const float ms = m[i] - up[i];
     float zz[4] = {z[i], 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 16; j++) {
@@ -797,13 +824,13 @@ void k_attn_q8(Kv8Attn a) {
 #pragma unroll
   for (int i = 0; i < NT; i++) {
     if (i) __syncthreads();
-    const float z = rows_sum(w.z[i]);
+    const float unit = ldexpf(1.0f, -(int)w.up[i]), z = rows_sum(w.z[i]) * unit, vu = vs * unit;
     if (g == 0) {
       s_m[wv][n] = w.m[i];
       s_z[wv][n] = z;
     }
 #pragma unroll
-    for (int d = 0; d < D; d++) s_o[wv][d][lane] = w.o[i][d] * vs;
+    for (int d = 0; d < D; d++) s_o[wv][d][lane] = w.o[i][d] * vu;
     __syncthreads();
     float mm = s_m[0][n];
 #pragma unroll
@@ -991,10 +1018,10 @@ void k_attn_wide_q8(Kv8Attn a) {
     while (p < k.c1) turn([] {});
   }
   if (!rows) return;
-  const float vu = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
+  const float vall = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NT; i++) {
-    const float z = rows_sum(w.z[i]);
+    const float unit = ldexpf(1.0f, -(int)w.up[i]), z = rows_sum(w.z[i]) * unit, vu = vall * unit;
     const uint32_t row = row0 + i * 16 + n;
     if (row >= (uint64_t)k.e.nodes * a.grp) continue;
     const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rowsper + row - k.row0;

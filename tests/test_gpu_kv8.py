@@ -367,6 +367,28 @@ def test_tree_masks(fmt):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("huge", [1e4, 1e9, 1e17])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,base", [(4, 2, 64, 12, 0), (8, 2, 64, 6, 70), (8, 2, 64, 20, 1000),
+                                                    (8, 1, 64, 30, 130), (2, 2, 128, 9, 1200), (20, 5, 128, 16, 61)])
+def test_masked_rows_of_any_size(fmt, huge, heads, kvh, hd, tmax, base):
+    """V rows, however large, that a node does not attend (another branch's, a later token's) leave its output alone:
+    the tolerance is of the rows attended."""
+    rng = np.random.default_rng(tmax)
+    bs, mbps = 16, (base + tmax + 15) // 16
+    pools, table = cached(rng, [base + tmax], kvh, hd, bs, mbps, fmt)
+    big = tmax // 2
+    for i, f in ((big, huge), (big + 1, huge ** 0.5), (tmax - 1, huge * 100)):
+        codes, scale = ref.quantise(rng.standard_normal((kvh, hd)) * f, fmt)
+        pools.write(table, 0, base + i, "v", codes, scale)
+    q = rng.standard_normal((1, tmax, heads * hd)).astype(F32)
+    at = np.array([base], np.int32)
+    check_tree(pools, table, q, at, None, None)
+    mask = words(rng, 1, tmax)
+    mask[0, big + 2:tmax - 1] &= ~np.uint64(3 << big)
+    check_tree(pools, table, q, at, None, mask)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("heads,kvh,hd,bs,mbps,tmax,base,nodes", [
     (20, 5, 128, 16, 24, 130, [200, 0, 17], [130, 129, 3]), (8, 8, 64, 16, 20, 97, [100, 3], None),
     (4, 1, 128, 32, 30, 300, [600, 0], [300, 257]), (2, 2, 64, 16, 80, 1200, [0], None)])
