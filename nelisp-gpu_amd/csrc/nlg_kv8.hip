@@ -787,7 +787,7 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
 // 8 sequences at 24,000-32,768, 32/8 heads of 128, 480 MB: 85 us, 5.7 TB/s; 32
 // of up to 4,096, 20/5 heads, 87 MB: 22 us, 4.0 TB/s, the chain lengths -> table
 // -> K, V before it and chunks of unequal lengths; 640 positions of one sequence
-// (eight waves, no second launch): 9.2 us, that chain and the waves' meeting.
+// (eight waves, no second launch): 9.6 us, that chain and the waves' meeting.
 template <int HD, int FMT, int NT, int W, bool PAST>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_q8(Kv8Attn a) {
@@ -864,11 +864,11 @@ void k_attn_q8(Kv8Attn a) {
 // which the waves' operands lie (a fragment's 64 lanes side by side: no bank is
 // asked twice).  While a step is computed the next one's halves are written and
 // the one's after it are on their way from memory.  Bound by issue: two chunks
-// of 500-512 tokens over 1,024-2,047, 32/8 heads of 64, take 58 us, 256 TFLOP/s
+// of 500-512 tokens over 1,024-2,047, 32/8 heads of 64, take 60 us, 249 TFLOP/s
 // (each product counted once; it is done twice, for hi and lo).  When they took
 // 68 with the join, 22 were left without any step, 28 with only the loads and the
 // halves in LDS; the softmax was 20, the second product 5, waiting for memory 4.
-// 16 trees of up to 32 nodes over up to 4,000, 20/5 heads of 128: 31 us (of 46
+// 16 trees of up to 32 nodes over up to 4,000, 20/5 heads of 128: 32 us (of 46
 // with the join, 20 without steps, 6 for the softmax).  Two waves a SIMD: three at
 // head dim 64, with 64 rows a workgroup, took 69 us for 60; eight waves a
 // workgroup 85 for 76.
@@ -1034,8 +1034,10 @@ void k_attn_wide_q8(Kv8Attn a) {
   }
 }
 
-// The chunks' parts of each output row, joined by their maxima: SUBS groups of hd / 4 threads
-// walk a row's chunks.  A workgroup's rows are of one sequence.
+// The chunks' parts of each output row, joined by their maxima: SUBS groups of
+// hd / 4 threads walk a row's chunks.  A workgroup's rows are of one sequence.  4-6
+// us traced: eight groups where one each would leave the
+// card empty and walk tens of chunks one after another.
 template <int SUBS>
 __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint32_t blocks) {
   __shared__ float4v s_o[256];
@@ -1399,7 +1401,8 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   KV8_SCOPE(what);
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
   a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads;
-  a.rowsper = s.rowsper; a.rowslog = s.rowslog; a.groups = s.groups; a.want = s.want; a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
+  a.rowsper = s.rowsper; a.rowslog = s.rowslog; a.groups = s.groups; a.want = s.want;
+  a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
   a.bygroups = kv8_div(s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
   a.tree = tree; a.one = s.one;
   a.pctx = (float *)workspace;
