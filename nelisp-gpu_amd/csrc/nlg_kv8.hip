@@ -254,7 +254,9 @@ struct Kv8Attn {
   const int32_t *nodes;   // tree: [batch] or null
   const uint64_t *mask;   // tree: [batch][tmax] or null
   Kv8Pages pg;
-  float *out, *pctx, *pmz;  // partials: [slots][kvheads][rowsper][hd], [slots][kvheads][rowsper][2]
+  // partials: averages of V [slots][kvheads][rowsper][hd] (sums of them with their weights
+  // could pass f32's end where V is large), maxima and sums [slots][kvheads][rowsper][2]
+  float *out, *pctx, *pmz;
   uint2 *pfirst;            // [batch]: a sequence's first slot, its chunks
   uint32_t batch, tmax, heads, grp;  // grp: query heads of a kv head; a sequence's rows: tmax * grp
   uint32_t rowsper, rowslog, groups, want, least, unit, slots;  // Kv8Split
@@ -376,6 +378,10 @@ __device__ __forceinline__ float rows_sum(float v) {
   r = nlg_pair_f32<32>(v);
   return r.x + r.y;
 }
+
+// What a row's context is divided by: its sum; where it has attended nothing, the
+// context is zero.
+__device__ __forceinline__ float kv8_inverse(float z) { return z > 0.0f || z != z ? 1.0f / z : 0.0f; }
 
 // The positions of sequence b.
 __device__ __forceinline__ Kv8Extent kv8_of(const Kv8Attn &a, uint32_t b) {
@@ -819,18 +825,18 @@ void k_attn_q8(Kv8Attn a) {
   while (p + KV8_STEP <= whole) step(Int<0>{});
   while (p < k.c1) step(Int<1>{});
 
-  // the waves' parts meet, one tile of rows at a time
+  // the waves' parts meet, one tile of rows at a time, as averages of V with a weight each
   const float vs = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NT; i++) {
     if (i) __syncthreads();
-    const float unit = ldexpf(1.0f, -(int)w.up[i]), z = rows_sum(w.z[i]) * unit, vu = vs * unit;
+    const float z = rows_sum(w.z[i]), inv = kv8_inverse(z);
     if (g == 0) {
       s_m[wv][n] = w.m[i];
-      s_z[wv][n] = z;
+      s_z[wv][n] = ldexpf(z, -(int)w.up[i]);
     }
 #pragma unroll
-    for (int d = 0; d < D; d++) s_o[wv][d][lane] = w.o[i][d] * vu;
+    for (int d = 0; d < D; d++) s_o[wv][d][lane] = (w.o[i][d] * inv) * vs;
     __syncthreads();
     float mm = s_m[0][n];
 #pragma unroll
@@ -838,22 +844,22 @@ void k_attn_q8(Kv8Attn a) {
     float f[W], zz = 0.0f;
 #pragma unroll
     for (int j = 0; j < W; j++) {
-      f[j] = nlg_exp2(s_m[j][n] - mm);
-      zz = fmaf(s_z[j][n], f[j], zz);
+      f[j] = s_z[j][n] * nlg_exp2(s_m[j][n] - mm);
+      zz = zz + f[j];
     }
+    const float share = kv8_inverse(zz);
     const uint32_t row = k.row0 + i * 16 + n;
     if (row < (uint64_t)k.e.nodes * a.grp) {
       const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rowsper + row - k.row0;
       if (k.chunks > 1 && wv == 0 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(mm, zz);
-      const float inv = k.chunks > 1 ? 1.0f : zz > 0.0f || zz != zz ? 1.0f / zz : 0.0f;
       float *o = k.chunks > 1 ? a.pctx + part * HD
                               : a.out + (((size_t)k.b * a.tmax + w.node[i]) * a.heads + k.h * a.grp + row - w.node[i] * a.grp) * HD;
 #pragma unroll
       for (int d = wv; d < D; d += W) {
-        float4v t = s_o[0][d][lane] * f[0];
+        float4v t = s_o[0][d][lane] * (f[0] * share);
 #pragma unroll
-        for (int j = 1; j < W; j++) t = t + s_o[j][d][lane] * f[j];
-        *(float4v *)(o + d * 16 + g * 4) = t * inv;
+        for (int j = 1; j < W; j++) t = t + s_o[j][d][lane] * (f[j] * share);
+        *(float4v *)(o + d * 16 + g * 4) = t;
       }
     }
   }
@@ -1021,21 +1027,21 @@ void k_attn_wide_q8(Kv8Attn a) {
   const float vall = w.vref > 0.0f ? w.vref * (1.0f / KV8_VUNIT) : 0.0f;
 #pragma unroll
   for (int i = 0; i < NT; i++) {
-    const float unit = ldexpf(1.0f, -(int)w.up[i]), z = rows_sum(w.z[i]) * unit, vu = vall * unit;
+    const float z = rows_sum(w.z[i]), inv = kv8_inverse(z);
     const uint32_t row = row0 + i * 16 + n;
     if (row >= (uint64_t)k.e.nodes * a.grp) continue;
     const uint64_t part = ((uint64_t)k.slot * a.pg.kvheads + k.h) * a.rowsper + row - k.row0;
-    if (k.chunks > 1 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(w.m[i], z);
-    const float f = k.chunks > 1 ? vu : z > 0.0f || z != z ? vu / z : 0.0f;
+    if (k.chunks > 1 && g == 0) *(float2 *)(a.pmz + part * 2) = make_float2(w.m[i], ldexpf(z, -(int)w.up[i]));
     float *o = k.chunks > 1 ? a.pctx + part * HD
                             : a.out + (((size_t)k.b * a.tmax + w.node[i]) * a.heads + k.h * a.grp + row - w.node[i] * a.grp) * HD;
 #pragma unroll
-    for (int d = 0; d < D; d++) *(float4v *)(o + d * 16 + g * 4) = w.o[i][d] * f;
+    for (int d = 0; d < D; d++) *(float4v *)(o + d * 16 + g * 4) = (w.o[i][d] * inv) * vall;
   }
 }
 
-// The chunks' parts of each output row, joined by their maxima: SUBS groups of
-// hd / 4 threads walk a row's chunks.  A workgroup's rows are of one sequence.  4-6
+// The chunks' parts of each output row, joined by their maxima and sums: SUBS
+// groups of hd / 4 threads walk a row's chunks.  The sum of averages times weights is
+// held in units of the weights' sum's power of two, no larger than the largest V.  A workgroup's rows are of one sequence.  4-6
 // us traced: eight groups where one each would leave the
 // card empty and walk tens of chunks one after another.
 template <int SUBS>
@@ -1061,10 +1067,12 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
       const float2 x = *(const float2 *)(a.pmz + p * 2);
       const float4v y = *(const float4v *)(a.pctx + p * hd + d);
       const float mn = fmaxf(m, x.x);
-      const float f = nlg_exp2(m - mn), fx = nlg_exp2(x.x - mn);
+      const float f = nlg_exp2(m - mn), wx = x.y * nlg_exp2(x.x - mn);
+      const int e = __builtin_amdgcn_frexp_expf(z);
       m = mn;
-      z = fmaf(z, f, x.y * fx);
-      o = o * f + y * fx;
+      z = fmaf(z, f, wx);
+      const int ne = __builtin_amdgcn_frexp_expf(z);
+      o = o * ldexpf(f, e - ne) + y * ldexpf(wx, -ne);
     }
   if (SUBS > 1) {
     s_mz[t] = make_float2(m, z);
@@ -1075,19 +1083,21 @@ __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, u
 #pragma unroll
     for (int i = 1; i < SUBS; i++) mm = fmaxf(mm, s_mz[t + i * per].x);
     const float f = nlg_exp2(m - mm);
+    const int e = __builtin_amdgcn_frexp_expf(z);
     z = z * f;
-    o = o * f;
+#pragma unroll
+    for (int i = 1; i < SUBS; i++) z = fmaf(s_mz[t + i * per].y, nlg_exp2(s_mz[t + i * per].x - mm), z);
+    const int ne = __builtin_amdgcn_frexp_expf(z);
+    o = o * ldexpf(f, e - ne);
 #pragma unroll
     for (int i = 1; i < SUBS; i++) {
       const float2 x = s_mz[t + i * per];
-      const float fx = nlg_exp2(x.x - mm);
-      z = fmaf(x.y, fx, z);
-      o = o + s_o[t + i * per] * fx;
+      o = o + s_o[t + i * per] * ldexpf(nlg_exp2(x.x - mm), __builtin_amdgcn_frexp_expf(x.y) - ne);
     }
   }
   if (!on) return;
-  const float inv = z > 0.0f || z != z ? 1.0f / z : 0.0f;
-  *(float4v *)(a.out + (((size_t)b * a.tmax + node) * a.heads + head) * hd + d) = o * inv;
+  *(float4v *)(a.out + (((size_t)b * a.tmax + node) * a.heads + head) * hd + d) =
+      o * kv8_inverse(ldexpf(z, -__builtin_amdgcn_frexp_expf(z)));
 }
 
 // ------------------------------------------------------------------ commit

@@ -1,0 +1,96 @@
+"""Attention over the 8-bit paged KV cache where sizes lie far apart or near the
+ends of the f32 range, against 64 bits and relative to what the output itself is
+made of."""
+import math
+
+import numpy as np
+import pytest
+
+import kv8_ref as ref
+import nlgpu
+from test_gpu_kv8 import cached, decode, tree, words
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+FORMATS = [ref.I8, ref.E4M3]
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    nlgpu.init()
+    yield
+
+
+# heads, kv heads, head dim, queries, positions: one query in one launch and in chunks, its group of 16 rows half
+# and quite full; 32 rows sharing waves; 64 and 128 rows to a workgroup, the last with a row's chunks joined by one thread each.
+LAYOUTS = [(20, 5, 128, 1, 300), (8, 2, 64, 1, 1300), (32, 2, 128, 1, 64), (8, 2, 64, 6, 700), (8, 2, 128, 20, 400),
+           (8, 2, 64, 40, 200), (32, 4, 64, 150, 330)]
+
+
+def attended(q, k, v):
+    """One query head row [hd] over k, v [n, hd]: the output in 64 bits; the weighted sum of the rows' largest |v|; the
+    largest root of sum (q k)^2 / hd."""
+    qq = q.astype(np.float64)
+    s = k @ qq / math.sqrt(q.size)
+    p = np.exp(s - s.max())
+    p /= p.sum()
+    return p @ v, float(p @ np.abs(v).max(axis=1)), float(np.sqrt(((k * qq) ** 2).sum(axis=1) / q.size).max())
+
+
+def close(got, q, k, v, label):
+    """The query row's error against a bound relative to its own products.  Scores, exponentials and sums as in
+    kv8_ref.tolerance, but each moves its own product p |v| alone, so their weighted sum stands for the largest |v|.
+    A product of a probability and a V scale is two halves, the second with steps of 2^-24: half a step, where the
+    row's largest is at least 1, is 2^-25 of it for each of n positions."""
+    hd = k.shape[2]
+    heads = q.size // hd
+    q, got = q.reshape(heads, hd), got.reshape(heads, hd).astype(np.float64)
+    n = k.shape[0]
+    for h in range(heads):
+        g = h // (heads // k.shape[1])
+        want, size, amp = attended(q[h], k[:, g], v[:, g])
+        tol = 2.0 ** -24 * (150.0 * amp + 64.0 + 4.0 * math.sqrt(n) + n) * size + 2.0 ** -149
+        err = np.abs(got[h] - want).max()
+        assert np.isfinite(got[h]).all() and err <= tol, (label, h, err, tol, size)
+
+
+def check(pools, table, q, n):
+    """q [1, tmax, heads * hd], the queries at positions n - tmax .. n - 1, as a decoded token, a causal chunk and a
+    masked tree."""
+    tmax = q.shape[1]
+    k, v = pools.rows(table, 0, n, "k"), pools.rows(table, 0, n, "v")
+    base = np.array([n - tmax], np.int32)
+    if tmax == 1:
+        close(decode(pools, table, q[0], base)[0], q[0, 0], k, v, "decode")
+        return
+    rows = sorted({0, 1, tmax // 2, tmax - 1} | set(range(0, tmax, 7)))
+    got = tree(pools, table, q, base, None, None)
+    for i in rows:
+        close(got[0, i], q[0, i], k[:n - tmax + i + 1], v[:n - tmax + i + 1], ("causal", i))
+    if tmax > 64:
+        return
+    mask = words(np.random.default_rng(1), 1, tmax)
+    got = tree(pools, table, q, base, None, mask)
+    for i in rows:
+        on = np.array([p < n - tmax or int(mask[0, i]) >> (p - n + tmax) & 1 for p in range(n)], bool)
+        close(got[0, i], q[0, i], k[on], v[on], ("masked", i))
+
+
+def put(pools, table, pos, which, row):
+    """One position's row [kvheads, hd], quantised."""
+    c, s = ref.quantise(row, pools.fmt)
+    pools.write(table, 0, pos, which, c, s)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [3e38, 1e37, 1e-20, 1e-30, 1e-35])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_values_of_any_size(fmt, size, heads, kvh, hd, tmax, n):
+    """V up to the largest f32 numbers, under flat scores that many positions share: no sum on the way overflows; V of
+    next to nothing keeps its bits.  (The largest magnitude of a row is 3/4 of `size`.)"""
+    rng = np.random.default_rng(n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    for pos in range(n):
+        put(pools, table, pos, "v", rng.uniform(-0.75, 0.75, (kvh, hd)) * size)
+    q = (0.1 * rng.standard_normal((1, tmax, heads * hd))).astype(F32)
+    check(pools, table, q, n)
