@@ -418,9 +418,10 @@ int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const
  * [batch x heads*head_dim], 16-byte aligned.  lens[b] < 0: nothing is attended
  * and the row is zero; positions past the block table are not attended; table entries
  * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
- * and carry 22 bits of q and of the probabilities.  Of the V rows
- * that a query attends, those whose scales lie more than 2^12 below the
- * largest lose bits (what is masked does not count, up to 2^60 above).
+ * and carry 22 bits of q and of the probabilities.  A V row that a query
+ * masks, or gives next to no weight, takes no bits of what makes its output
+ * as long as its scale is below 2^96 times the query's largest product of a
+ * probability and a V scale.
  * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0
  * bytes: none is read), as below; calls that share one run in stream order. */
 int nlg_decode_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt,

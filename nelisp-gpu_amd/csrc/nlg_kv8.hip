@@ -513,11 +513,12 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 // scales in units of vref / 2^(15 - KV8_SLACK) they stay within fp16.
 #define KV8_SLACK 6.0f
 #define KV8_VUNIT 512.0f  // 2^(15 - KV8_SLACK)
-// V scales this many binades below vref keep 22 bits of the products; how far a
-// row is lifted at most (its sum stays in 32 bits); the distance of a row that has
-// attended nothing yet (negative: of a row that is none).
+// Products of a probability and a V scale this many binades below vref keep their
+// bits (at least 1 in those units, the halves' last step is 2^-24 of it); how far a
+// row is lifted at most (its sum of 2^31 times 2^(KV8_UP + KV8_SLACK) stays in 32
+// bits); from this distance on a row has no product yet.
 #define KV8_NEAR 8.0f
-#define KV8_UP 60.0f
+#define KV8_UP 90.0f
 #define KV8_NEVER 1e6f
 // The maximum of no score: finite, so that no difference of two is a NaN.
 #define KV8_FLOOR -1.7e38f
@@ -530,7 +531,7 @@ struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
   float rs[NT];            // what the row's q was divided by (a power of two)
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
-  float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest V scale
+  float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest product with a V scale
   float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^up KV8_VUNIT / vref
   float vref, vinv;        // a power of two no V scale so far exceeds, or 0; KV8_VUNIT / vref
   uint32_t node[NT];
@@ -584,7 +585,7 @@ struct WaveState {
       }
       m[i] = KV8_FLOOR;
       z[i] = up[i] = 0.0f;
-      far[i] = on ? KV8_NEVER : -KV8_NEVER;
+      far[i] = on ? KV8_NEVER : -INFINITY;  // (a row that is none: never lifted)
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -618,19 +619,30 @@ struct WaveState {
     return f;
   }
 
-  // vref is of all positions, those too that a row does not attend (another
-  // branch's, a later token's).  A row whose own V scales are far below it has its
-  // probabilities, sum and context carry 2^up, so that no masked row, however
-  // large, takes their products' bits.  Returns what up has grown by, as a factor.
-  template <bool GEN>
-  __device__ __forceinline__ float near(int i, const float *vb, float vresc, uint32_t bits) {
-    float v = 0.0f;
+  // vref is of all positions: of those that a row does not attend (another
+  // branch's, a later token's) and of those that it gives next to no weight.  A row
+  // whose own products p V are all far below it has its probabilities, sum and context
+  // carry 2^up, so that no such V row, however large, takes the bits of those that
+  // make its output.  s: the step's scores, top: their largest; by: how far the
+  // maximum has moved.  Returns what up has grown by, as a factor.
+  __device__ __forceinline__ float raise(int i, const float *s, float top, const float *vb, float by, float vresc) {
+    // earlier products are smaller by both
+    far[i] = far[i] + (fminf(by, KV8_NEVER) + (vresc > 0.0f ? (float)(1 - __builtin_amdgcn_frexp_expf(vresc)) : KV8_NEVER));
+    // most often the step's largest probability times its smallest V scale is near
+    // enough, and says so without an exponential for each position
+    float low = fabsf(vb[0]);
 #pragma unroll
-    for (int j = 0; j < 16; j++) v = fmaxf(v, !GEN || bits >> j & 1 ? fabsf(vb[j]) : 0.0f);
-    v = rows_max(v);
-    if (vresc > 0.0f) far[i] = far[i] + (float)(1 - __builtin_amdgcn_frexp_expf(vresc));
+    for (int j = 1; j < 16; j++) low = fminf(low, fabsf(vb[j]));
+    low = -rows_max(-low);
+    float v = nlg_exp2(top - m[i]) * low;
+    if (__any(far[i] > KV8_NEAR && !(v >= 1.0f))) {
+      v = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 16; j++) v = fmaxf(v, nlg_exp2(fmaf(s[j], rs[i], -m[i])) * fabsf(vb[j]));
+      v = rows_max(v);
+    }
     if (v > 0.0f) far[i] = fminf(far[i], (float)(9 - __builtin_amdgcn_frexp_expf(v)));
-    const float now = far[i] > KV8_NEAR && far[i] < KV8_NEVER ? fminf(far[i], KV8_UP) : 0.0f;
+    const float now = far[i] > KV8_NEAR && far[i] < KV8_NEVER ? fminf(floorf(far[i]), KV8_UP) : 0.0f;
     const float lift = ldexpf(1.0f, (int)(now - up[i]));
     up[i] = now;
     return lift;
@@ -660,9 +672,9 @@ struct WaveState {
     if (__any(top > m[i] + KV8_SLACK || vresc != 1.0f || far[i] > KV8_NEAR)) {
       top = rows_max(top);
       const float mn = top > m[i] + KV8_SLACK ? top : m[i];
-      const float al = nlg_exp2(m[i] - mn);
+      const float by = mn - m[i], al = nlg_exp2(-by);
       m[i] = mn;
-      const float lift = near<GEN>(i, vb, vresc, bits), sc = al * (vresc * lift);
+      const float lift = raise(i, s, top, vb, by, vresc), sc = al * (vresc * lift);
       z[i] = z[i] * (al * lift);
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;

@@ -94,3 +94,35 @@ def test_values_of_any_size(fmt, size, heads, kvh, hd, tmax, n):
         put(pools, table, pos, "v", rng.uniform(-0.75, 0.75, (kvh, hd)) * size)
     q = (0.1 * rng.standard_normal((1, tmax, heads * hd))).astype(F32)
     check(pools, table, q, n)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("binades", [12, 20, 28, 40, 66, 90])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_large_rows_of_no_weight(fmt, binades, heads, kvh, hd, tmax, n):
+    """V rows 2^binades above the others, attended with a probability near 2^-100: the first position, some in the
+    middle, the last below the queries."""
+    rng = np.random.default_rng(binades + n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    low = 100 * math.log(2) / math.sqrt(hd)
+    for pos in {0, n // 3, n // 3 + 1, n - tmax - 1}:
+        put(pools, table, pos, "k", np.full((kvh, hd), -low))
+        put(pools, table, pos, "v", rng.standard_normal((kvh, hd)) * 2.0 ** binades)
+    q = (1 + 0.1 * rng.standard_normal((1, tmax, heads * hd))).astype(F32)
+    check(pools, table, q, n)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("nats", [12, 25, 60])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_a_heavy_position_without_value(fmt, nats, heads, kvh, hd, tmax, n):
+    """The position that takes nearly all the weight has a V row of zeros (or a tiny one): the output is what the others
+    leave."""
+    rng = np.random.default_rng(nats + n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    put(pools, table, 0, "k", np.full((kvh, hd), nats / math.sqrt(hd)))
+    put(pools, table, 0, "v", np.zeros((kvh, hd)))
+    put(pools, table, n // 2, "k", np.full((kvh, hd), nats / math.sqrt(hd)))
+    put(pools, table, n // 2, "v", rng.standard_normal((kvh, hd)) * 2.0 ** -90)
+    q = (1 + 0.1 * rng.standard_normal((1, tmax, heads * hd))).astype(F32)
+    check(pools, table, q, n)
