@@ -520,8 +520,11 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 #define KV8_NEAR 8.0f
 #define KV8_UP 90.0f
 #define KV8_NEVER 1e6f
-// The maximum of no score: finite, so that no difference of two is a NaN.
-#define KV8_FLOOR -1.7e38f
+// The maximum of no score: below all that there are, and finite, so that no
+// difference of two is a NaN.
+#define KV8_FLOOR -3.4028234663852886e38f
+// Queries are multiplied as numbers below 2^KV8_QTOP.
+#define KV8_QTOP 2
 
 // A wave's running state over NT tiles of sixteen query rows.  A lane holds the
 // query row n = lane & 15 of each tile, and of its scores the sixteen positions
@@ -529,7 +532,8 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 template <int HD, int NT>
 struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
-  float rs[NT];            // what the row's q was divided by (a power of two)
+  float rs[NT];            // what the row's q was divided by (a power of two, a normal number)
+  int ke;                  // no K scale so far exceeds 2^ke
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
   float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest product with a V scale
   float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^up KV8_VUNIT / vref
@@ -570,14 +574,15 @@ struct WaveState {
       }
 #pragma unroll
       for (int j = 0; j < HD / 4; j++) {
-        x[j] = on ? x[j] * a.coef : 0.0f;
+        x[j] = on ? x[j] : 0.0f;
         top = fmaxf(top, fabsf(x[j]));
       }
       top = rows_max(top);
-      const int ex = top > 0.0f && top <= 3.4028234663852886e38f ? __builtin_amdgcn_frexp_expf(top) : 0;
+      const int e = top > 0.0f && top <= 3.4028234663852886e38f ? __builtin_amdgcn_frexp_expf(top) - KV8_QTOP : 0;
+      const int ex = e < -126 ? -126 : e;
       rs[i] = ldexpf(1.0f, ex);
 #pragma unroll
-      for (int j = 0; j < HD / 4; j++) x[j] = ldexpf(x[j], -ex);
+      for (int j = 0; j < HD / 4; j++) x[j] = ldexpf(x[j], -ex) * a.coef;
 #pragma unroll
       for (int c = 0; c < C; c++) {
         split8(x + c * 16, qh[i][2 * c], ql[i][2 * c]);
@@ -590,6 +595,23 @@ struct WaveState {
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
     vref = vinv = 0.0f;
+    ke = -100;
+  }
+
+  // K scales in units of 2^ke, which no score's product of a code's sum and a scale
+  // then passes f32's end with, and what the rows' scores are to be multiplied by
+  // for it: 2^ke rs, kept where -infinity times it is that, and 0 is 0.
+  __device__ __forceinline__ float rescale_k(float ks) {
+    float u = ldexpf(ks, -ke);
+    if (__any(fabsf(u) > 1.0f)) {
+      const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(nlg_wave_max_f32(fabsf(ks))));
+      ke = e < -100 ? -100 : e;
+      u = ldexpf(ks, -ke);
+    }
+    return u;
+  }
+  __device__ __forceinline__ float unit(int i) const {
+    return __builtin_amdgcn_fmed3f(ldexpf(rs[i], ke), 1.17549435e-38f, 1.70141183e38f);
   }
 
   // V scales in units of vref / KV8_VUNIT: the probabilities times them, as
@@ -623,9 +645,9 @@ struct WaveState {
   // branch's, a later token's) and of those that it gives next to no weight.  A row
   // whose own products p V are all far below it has its probabilities, sum and context
   // carry 2^up, so that no such V row, however large, takes the bits of those that
-  // make its output.  s: the step's scores, top: their largest; by: how far the
+  // make its output.  s: the step's scores in units of su, top: their largest; by: how far the
   // maximum has moved.  Returns what up has grown by, as a factor.
-  __device__ __forceinline__ float raise(int i, const float *s, float top, const float *vb, float by, float vresc) {
+  __device__ __forceinline__ float raise(int i, const float *s, float su, float top, const float *vb, float by, float vresc) {
     // earlier products are smaller by both
     far[i] = far[i] + (fminf(by, KV8_NEVER) + (vresc > 0.0f ? (float)(1 - __builtin_amdgcn_frexp_expf(vresc)) : KV8_NEVER));
     // most often the step's largest probability times its smallest V scale is near
@@ -638,7 +660,7 @@ struct WaveState {
     if (__any(far[i] > KV8_NEAR && !(v >= 1.0f))) {
       v = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 16; j++) v = fmaxf(v, nlg_exp2(fmaf(s[j], rs[i], -m[i])) * fabsf(vb[j]));
+      for (int j = 0; j < 16; j++) v = fmaxf(v, nlg_exp2(fmaf(s[j], su, -m[i])) * fabsf(vb[j]));
       v = rows_max(v);
     }
     if (v > 0.0f) far[i] = fminf(far[i], (float)(9 - __builtin_amdgcn_frexp_expf(v)));
@@ -655,6 +677,7 @@ struct WaveState {
   template <bool GEN>
   __device__ __forceinline__ void soften(int i, const float4v *acc, float ks, const float *vb, float vresc,
                                          uint32_t bits, uint32_t odd, bool any, half8v *ph, half8v *pl) {
+    const float su = unit(i);
     float s[16];
     each<16>([&](auto J) {
       constexpr int j = decltype(J)::value;
@@ -668,13 +691,13 @@ struct WaveState {
     float top = max3(s[0], s[1], s[2]);
 #pragma unroll
     for (int j = 3; j < 15; j += 2) top = max3(top, s[j], s[j + 1]);
-    top = max3(top, s[15], s[15]) * rs[i];
+    top = max3(top, s[15], s[15]) * su;
     if (__any(top > m[i] + KV8_SLACK || vresc != 1.0f || far[i] > KV8_NEAR)) {
       top = rows_max(top);
       const float mn = top > m[i] + KV8_SLACK ? top : m[i];
       const float by = mn - m[i], al = nlg_exp2(-by);
       m[i] = mn;
-      const float lift = raise(i, s, top, vb, by, vresc), sc = al * (vresc * lift);
+      const float lift = raise(i, s, su, top, vb, by, vresc), sc = al * (vresc * lift);
       z[i] = z[i] * (al * lift);
 #pragma unroll
       for (int d = 0; d < HD / 16; d++) o[i][d] = o[i][d] * sc;
@@ -683,7 +706,7 @@ struct WaveState {
     float zz[4] = {z[i], 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 16; j++) {
-      s[j] = nlg_exp2(fmaf(s[j], rs[i], -ms));
+      s[j] = nlg_exp2(fmaf(s[j], su, -ms));
       zz[j & 3] = zz[j & 3] + s[j];
     }
     z[i] = (zz[0] + zz[1]) + (zz[2] + zz[3]);
@@ -756,6 +779,7 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
     for (int i = 0; i < D; i++) vr[i] = and4(vr[i], keep);
     if (!hv || n >= left) ks = vs = 0.0f;
   }
+  ks = w.rescale_k(ks);
   uint32_t odd;
   bool any;
   const float vresc = w.rescale(vs, odd, any, lane);
@@ -952,6 +976,7 @@ void k_attn_wide_q8(Kv8Attn a) {
   };
   auto compute = [&](auto GENV, int buf, float ksc, float vsc, uint32_t p) {
     constexpr bool GEN = decltype(GENV)::value != 0;
+    ksc = w.rescale_k(ksc);
     uint32_t odd;
     bool any;
     const float vresc = w.rescale(vsc, odd, any, lane);

@@ -126,3 +126,45 @@ def test_a_heavy_position_without_value(fmt, nats, heads, kvh, hd, tmax, n):
     put(pools, table, n // 2, "v", rng.standard_normal((kvh, hd)) * 2.0 ** -90)
     q = (1 + 0.1 * rng.standard_normal((1, tmax, heads * hd))).astype(F32)
     check(pools, table, q, n)
+
+
+def fill(pools, table, n, which, rows):
+    """All n positions of a side: rows [n, kvheads, hd]."""
+    c, s = ref.quantise(rows, pools.fmt)
+    for pos in range(n):
+        pools.write(table, 0, pos, which, c[pos], s[pos])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("size", [3e38, 4e37, 1e30, 1e-30, 1e-35])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_keys_of_any_size(fmt, size, heads, kvh, hd, tmax, n):
+    """K of any size with queries that make ordinary scores of it."""
+    rng = np.random.default_rng(n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    fill(pools, table, n, "k", rng.uniform(-0.75, 0.75, (n, kvh, hd)) * size)
+    q = (rng.standard_normal((1, tmax, heads * hd)) * (6 / size)).astype(F32)
+    check(pools, table, q, n)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("sign", [1, -1, 0])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_scores_near_the_end_of_f32(fmt, sign, heads, kvh, hd, tmax, n):
+    """Equal scores of 3e38 in base 2, all positive, all negative, or every third positive: the weight is shared by the
+    largest.  (K of one magnitude and q of one value: the sums are exact and the scores the same.)"""
+    rng = np.random.default_rng(n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    side = np.where(np.arange(n) % 3 == 0, 1.0, -1.0) if sign == 0 else np.full(n, float(sign))
+    fill(pools, table, n, "k", np.broadcast_to(side[:, None, None] * 1e38, (n, kvh, hd)))
+    q = np.full((1, tmax, heads * hd), 3e38 / (1e38 * math.sqrt(hd) * math.log2(math.e)), F32)
+    v = pools.rows(table, 0, n, "v")
+    base = np.array([n - tmax], np.int32)
+    got = decode(pools, table, q[0], base)[None] if tmax == 1 else tree(pools, table, q, base, None, None)
+    for i in {0, tmax // 2, tmax - 1}:
+        on = np.flatnonzero(side[:n - tmax + i + 1] == side[0])
+        want = v[on].mean(axis=0)
+        # as in close(), with weights that are exact
+        tol = 2.0 ** -24 * (64.0 + 4.0 * math.sqrt(n) + n) * np.abs(v[on]).max(axis=2).mean(axis=0)
+        err = np.abs(got[0, i].reshape(kvh, heads // kvh, hd) - want[:, None]).max(axis=(1, 2))
+        assert (err <= tol).all(), (i, err.max(), tol.min())
