@@ -418,7 +418,9 @@ int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const
  * [batch x heads*head_dim], 16-byte aligned.  lens[b] < 0: nothing is attended
  * and the row is zero; positions past the block table are not attended; table entries
  * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
- * and carry 22 bits of q and of the probabilities.  A V row that a query
+ * and carry 22 bits of the probabilities and of q (of its elements down to
+ * 2^-14 of a head's largest; smaller ones are held in steps of 2^-36 of
+ * that).  A V row that a query
  * masks, or gives next to no weight, takes no bits of what makes its output
  * as long as its scale is below 2^96 times the query's largest product of a
  * probability and a V scale.

@@ -523,8 +523,10 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 // The maximum of no score: below all that there are, and finite, so that no
 // difference of two is a NaN.
 #define KV8_FLOOR -3.4028234663852886e38f
-// Queries are multiplied as numbers below 2^KV8_QTOP.
-#define KV8_QTOP 2
+// Queries are multiplied as numbers whose largest is 2^(KV8_QTOP - 1) or more, times
+// coef (0.13, 0.18): well below fp16's end, so that elements down to 2^-14 of a row's
+// largest keep 22 bits in two halves (with 2 in place of 16, down to 1).
+#define KV8_QTOP 16
 
 // A wave's running state over NT tiles of sixteen query rows.  A lane holds the
 // query row n = lane & 15 of each tile, and of its scores the sixteen positions

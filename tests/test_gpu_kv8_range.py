@@ -168,3 +168,20 @@ def test_scores_near_the_end_of_f32(fmt, sign, heads, kvh, hd, tmax, n):
         tol = 2.0 ** -24 * (64.0 + 4.0 * math.sqrt(n) + n) * np.abs(v[on]).max(axis=2).mean(axis=0)
         err = np.abs(got[0, i].reshape(kvh, heads // kvh, hd) - want[:, None]).max(axis=(1, 2))
         assert (err <= tol).all(), (i, err.max(), tol.min())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("binades", [8, 14, 18])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_queries_of_one_large_element(fmt, binades, heads, kvh, hd, tmax, n):
+    """An element of q 2^binades above the others, where K is zero: the others make the scores.  They are multiplied as
+    two halves whose last step is 2^-24 where the largest is some 2^12: half a step is 2^-37 of it, 2^-19 of an element
+    of size 1 at most, against the 2^-24 * 150 amp of the bound, amp about 1; over hd products it grows as the root."""
+    rng = np.random.default_rng(n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    k = rng.standard_normal((n, kvh, hd))
+    k[:, :, 3] = 0
+    fill(pools, table, n, "k", k)
+    q = rng.standard_normal((1, tmax, heads, hd))
+    q[..., 3] = 2.0 ** binades
+    check(pools, table, q.reshape(1, tmax, -1).astype(F32), n)
