@@ -1340,6 +1340,11 @@ static int kv8_check(const char *what, const void *kpool, const void *vpool, con
   pg.kvheads = kvheads;
   return NLG_OK;
 }
+// Arrays of 32-bit numbers, those that may be null among them.
+template <class... P>
+static bool kv8_words(P... p) {
+  return ((... | (uintptr_t)p) & 3) == 0;
+}
 // (after the checks of arguments: those need no device)
 #define KV8_SCOPE(what)                                       \
   if (nlg_ensure_init()) return NLG_ERR;                      \
@@ -1366,6 +1371,7 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   if (((uintptr_t)qkv & 15) || ((uintptr_t)q & 15) || ((uintptr_t)rope_cos & 15) || ((uintptr_t)rope_sin & 15) ||
       ((uintptr_t)qgain & 15) || ((uintptr_t)kgain & 15))
     return nlg_fail("%s: qkv, q, gains and rotation tables must be 16-byte aligned", what);
+  if (!kv8_words(seq, slot, rpos)) return nlg_fail("%s: seq, slot and rpos must be 4-byte aligned", what);
   if (!seq && rows > batch) return nlg_fail("%s: %u rows without a sequence each, batch %u", what, rows, batch);
   const uint64_t per = (uint64_t)heads + 2ull * kvheads;
   const uint64_t qb = ((uint64_t)rows * (heads + (uint64_t)kvheads) * (head_dim / 8) + 255) / 256;
@@ -1429,6 +1435,8 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   if (kv8_check(what, kpool, vpool, table, npool, fmt, batch, kvheads, hd, bs, mbps, a.pg)) return NLG_ERR;
   if (!q || !base || !out) return nlg_fail("%s: null pointer", what);
   if (((uintptr_t)q & 15) || ((uintptr_t)out & 15)) return nlg_fail("%s: q and out must be 16-byte aligned", what);
+  if (!kv8_words(base, nodes))
+    return nlg_fail("%s: %s must be 4-byte aligned", what, tree ? "base and nodes" : "lens");
   const uint64_t rows = kv8_rows(tmax, heads, kvheads);
   if (!rows) return nlg_fail("%s: %u heads over %u kv heads, %u queries", what, heads, kvheads, tmax);
   if (mask && tmax > KV8_TREE) return nlg_fail("%s: %u nodes under a mask (at most %d)", what, tmax, KV8_TREE);
@@ -1517,6 +1525,7 @@ extern "C" int nlg_tree_commit_paged_q8(uint8_t *kpool, uint8_t *vpool, const in
   CommitArgs a;
   if (kv8_check(what, kpool, vpool, table, npool, NLG_KV_I8, batch, kvheads, head_dim, bs, mbps, a.pg)) return NLG_ERR;
   if (!base || !path || !accepted) return nlg_fail("%s: null pointer", what);
+  if (!kv8_words(base, path, accepted)) return nlg_fail("%s: base, path and accepted must be 4-byte aligned", what);
   if (tmax > KV8_TREE) return nlg_fail("%s: paths of %u nodes (at most %d)", what, tmax, KV8_TREE);
   if (batch > 65535 || !nlg_fits(2ull * kvheads, 256)) return nlg_fail("%s: batch %u x %u kv heads", what, batch, kvheads);
   KV8_SCOPE(what);
@@ -1539,6 +1548,7 @@ extern "C" int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpoo
   if (!slot || !k || !v) return nlg_fail("%s: null pointer", what);
   if (!batch) return nlg_fail("%s: batch must be nonzero", what);
   if (((uintptr_t)k & 15) || ((uintptr_t)v & 15)) return nlg_fail("%s: k and v must be 16-byte aligned", what);
+  if (!kv8_words(seq, slot)) return nlg_fail("%s: seq and slot must be 4-byte aligned", what);
   if (!seq && rows > batch) return nlg_fail("%s: %u rows without a sequence each, batch %u", what, rows, batch);
   const bool few = (uint64_t)rows * kvheads < 16384;  // (2,000 rows of 8 heads of 128: 7.9 us, 8.1 in sixteens; 480: 4.1, 6.7; 16,000: 48, 24)
   const uint64_t per = few ? 1 : 16, blocks = (((uint64_t)rows + per - 1) / per * kvheads + 3) / 4;

@@ -301,3 +301,19 @@ def test_nothing_to_do_is_no_error():
     nlgpu.tree_attn_paged_q8(q=n, base=n, out=n, heads=0, workspace=None, batch=4, tmax=0, **kw)
     nlgpu.tree_commit_paged_q8(base=n, path=n, accepted=n, batch=0, tmax=4, **kw)
     nlgpu.cache_read_paged_q8(slot=n, k=n, v=n, rows=0, batch=0, **kw)
+
+
+HALF = At((1 << 20) + 2)
+
+
+@pytest.mark.parametrize("call,kw,names", [
+    (nlgpu.qk_norm_rope_append_paged_q8,
+     dict(CACHE, qkv=GOOD, qgain=None, kgain=None, eps=1e-6, co=GOOD, si=GOOD, trows=10, slot=GOOD, q=At(1 << 24), rows=2,
+          heads=8, seq=GOOD, rpos=GOOD), ("seq", "slot", "rpos")),
+    (nlgpu.decode_attn_paged_q8, dict(ATTN, lens=GOOD), ("lens",)),
+    (nlgpu.tree_attn_paged_q8, dict(ATTN, base=GOOD, nodes=GOOD, tmax=8), ("base", "nodes")),
+    (nlgpu.tree_commit_paged_q8, dict(CACHE, base=GOOD, path=GOOD, accepted=GOOD, tmax=8), ("base", "path", "accepted")),
+    (nlgpu.cache_read_paged_q8, dict(CACHE, slot=GOOD, k=GOOD, v=GOOD, rows=2, seq=GOOD), ("seq", "slot"))])
+def test_number_arrays_are_aligned(call, kw, names):
+    for n in names:
+        refused(call, dict(kw, **{n: HALF}), "4-byte aligned|" + n)
