@@ -403,7 +403,7 @@ size_t nlg_kv_q8_pool_bytes(uint32_t npool, uint32_t kvheads, uint32_t head_dim,
  * the queries; k and v are quantised into position slot[r] of the sequence.
  * Rows whose sequence, slot or block is out of range (a negative slot:
  * padding) cache nothing.  qkv, q, gains and tables are 16-byte aligned; the
- * rows of one call name distinct positions; q does not overlap qkv.  All is computed in 64
+ * rows of one call name distinct positions; a q that overlaps qkv is refused.  All is computed in 64
  * bits, so a row's codes depend on its inputs alone.  For drafted tokens rpos is the node's depth behind
  * the context, and slot the node's place. */
 int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const float *kgain, float eps,

@@ -1378,6 +1378,10 @@ extern "C" int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *q
   const uint64_t vb = (((uint64_t)rows + 15) / 16 * kvheads + 3) / 4;
   if (per > 0xffffffffull || !nlg_fits(qb + vb, 256))
     return nlg_fail("%s: too many rows and heads (%u x %llu) for one launch", what, rows, (unsigned long long)per);
+  // (head rows are read by some workgroups while others store queries)
+  const uintptr_t x0 = (uintptr_t)qkv, q0 = (uintptr_t)q;
+  if (x0 < q0 + (uint64_t)rows * heads * head_dim * 4 && q0 < x0 + (uint64_t)rows * per * head_dim * 4)
+    return nlg_fail("%s: q overlaps qkv", what);
   KV8_SCOPE(what);
   a.qkv = qkv; a.qgain = qgain; a.kgain = kgain; a.co = rope_cos; a.si = rope_sin;
   a.seq = seq; a.slot = slot; a.rpos = rpos; a.q = q; a.kpool = kpool; a.vpool = vpool;

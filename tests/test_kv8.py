@@ -317,3 +317,12 @@ HALF = At((1 << 20) + 2)
 def test_number_arrays_are_aligned(call, kw, names):
     for n in names:
         refused(call, dict(kw, **{n: HALF}), "4-byte aligned|" + n)
+
+
+@pytest.mark.parametrize("q,qkv", [(1 << 20, 1 << 20), ((1 << 20) + 16, 1 << 20), (1 << 20, (1 << 20) + 8192 - 16),
+                                   ((1 << 20) + 16384 - 16, 1 << 20)])
+def test_append_refuses_queries_over_its_input(q, qkv):
+    """Two rows of 16 heads of 128: 16,384 bytes of input, 8,192 of them queries."""
+    kw = dict(CACHE, qkv=At(qkv), qgain=None, kgain=None, eps=1e-6, co=GOOD, si=GOOD, trows=10, slot=GOOD, q=At(q), rows=2,
+              heads=8, seq=GOOD)
+    refused(nlgpu.qk_norm_rope_append_paged_q8, kw, "overlaps")
