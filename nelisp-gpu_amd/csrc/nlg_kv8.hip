@@ -527,6 +527,9 @@ __device__ __forceinline__ bool kv8_work(const Kv8Attn &a, int lane, Kv8Work &w)
 // coef (0.13, 0.18): well below fp16's end, so that elements down to 2^-14 of a row's
 // largest keep 22 bits in two halves (with 2 in place of 16, down to 1).
 #define KV8_QTOP 16
+// K scales are multiplied as numbers up to 2^KV8_KTOP: they then keep their bits down
+// to 2^-190 of the largest met (a masked row's).
+#define KV8_KTOP 64
 
 // A wave's running state over NT tiles of sixteen query rows.  A lane holds the
 // query row n = lane & 15 of each tile, and of its scores the sixteen positions
@@ -535,7 +538,7 @@ template <int HD, int NT>
 struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
   float rs[NT];            // what the row's q was divided by (a power of two, a normal number)
-  int ke;                  // no K scale so far exceeds 2^ke
+  int ke;                  // no K scale so far exceeds 2^(ke + KV8_KTOP)
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
   float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest product with a V scale
   float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^up KV8_VUNIT / vref
@@ -597,17 +600,18 @@ struct WaveState {
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
     vref = vinv = 0.0f;
-    ke = -100;
+    ke = -100 - KV8_KTOP;
   }
 
-  // K scales in units of 2^ke, which no score's product of a code's sum and a scale
-  // then passes f32's end with, and what the rows' scores are to be multiplied by
-  // for it: 2^ke rs, kept where -infinity times it is that, and 0 is 0.
+  // K scales in units of 2^ke: a sum of codes times queries (below 2^28) times one
+  // stays within f32 where the score does.  unit: what the rows' scores are to be
+  // multiplied by for it, 2^ke rs, kept where -infinity times it is that and 0 is 0 (at
+  // the lower end scores are below 2^-34).
   __device__ __forceinline__ float rescale_k(float ks) {
     float u = ldexpf(ks, -ke);
-    if (__any(fabsf(u) > 1.0f)) {
+    if (__any(fabsf(u) > ldexpf(1.0f, KV8_KTOP))) {
       const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(nlg_wave_max_f32(fabsf(ks))));
-      ke = e < -100 ? -100 : e;
+      ke = (e < -100 ? -100 : e) - KV8_KTOP;
       u = ldexpf(ks, -ke);
     }
     return u;

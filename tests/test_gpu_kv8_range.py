@@ -185,3 +185,31 @@ def test_queries_of_one_large_element(fmt, binades, heads, kvh, hd, tmax, n):
     q = rng.standard_normal((1, tmax, heads, hd))
     q[..., 3] = 2.0 ** binades
     check(pools, table, q.reshape(1, tmax, -1).astype(F32), n)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("small", [1.0, 1e-4, 1e-10, 1e-18])
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", [x for x in LAYOUTS if x[3] > 1])
+def test_masked_keys_of_any_size(fmt, small, heads, kvh, hd, tmax, n):
+    """K rows near the end of f32 that a node does not attend (another branch's, a later token's) beside ordinary and
+    very small ones that it does."""
+    rng = np.random.default_rng(n)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    k = rng.standard_normal((n, kvh, hd)) * small
+    big = n - tmax // 2
+    k[big] = rng.uniform(-3e38, 3e38, (kvh, hd))
+    fill(pools, table, n, "k", k)
+    q = (rng.standard_normal((1, tmax, heads * hd)) * 3 / small).astype(F32)
+    base = np.array([n - tmax], np.int32)
+    k, v = pools.rows(table, 0, n, "k"), pools.rows(table, 0, n, "v")
+    node = big - (n - tmax)
+    got = tree(pools, table, q, base, None, None)
+    for i in range(0, node, 3):
+        close(got[0, i], q[0, i], k[:n - tmax + i + 1], v[:n - tmax + i + 1], ("causal", i))
+    if tmax > 64:
+        return
+    mask = words(rng, 1, tmax) & ~np.uint64(1 << node)
+    got = tree(pools, table, q, base, None, mask)
+    for i in range(0, tmax, 3):
+        on = np.array([p < n - tmax or int(mask[0, i]) >> (p - n + tmax) & 1 for p in range(n)], bool)
+        close(got[0, i], q[0, i], k[on], v[on], ("masked", i))
