@@ -538,7 +538,7 @@ template <int HD, int NT>
 struct WaveState {
   half8v qh[NT][HD / 32], ql[NT][HD / 32];
   float rs[NT];            // what the row's q was divided by (a power of two, a normal number)
-  int ke;                  // no K scale so far exceeds 2^(ke + KV8_KTOP)
+  int ke;                  // no K scale so far exceeds 2^(ke + KV8_KTOP), 1 at first
   float m[NT], z[NT];      // running maximum; this lane's part of the sum
   float up[NT], far[NT];   // probabilities carry 2^up; binades from vref down to the row's largest product with a V scale
   float4v o[NT][HD / 16];  // out[dim 16 i + 4 g + r][query n], times 2^up KV8_VUNIT / vref
@@ -600,7 +600,7 @@ struct WaveState {
       for (int d = 0; d < HD / 16; d++) o[i][d] = {0.0f, 0.0f, 0.0f, 0.0f};
     }
     vref = vinv = 0.0f;
-    ke = -100 - KV8_KTOP;
+    ke = -KV8_KTOP;
   }
 
   // K scales in units of 2^ke: a sum of codes times queries (below 2^28) times one
@@ -610,8 +610,7 @@ struct WaveState {
   __device__ __forceinline__ float rescale_k(float ks) {
     float u = ldexpf(ks, -ke);
     if (__any(fabsf(u) > ldexpf(1.0f, KV8_KTOP))) {
-      const int e = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(nlg_wave_max_f32(fabsf(ks))));
-      ke = (e < -100 ? -100 : e) - KV8_KTOP;
+      ke = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(nlg_wave_max_f32(fabsf(ks)))) - KV8_KTOP;
       u = ldexpf(ks, -ke);
     }
     return u;
