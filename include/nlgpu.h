@@ -403,9 +403,10 @@ size_t nlg_kv_q8_pool_bytes(uint32_t npool, uint32_t kvheads, uint32_t head_dim,
  * the queries; k and v are quantised into position slot[r] of the sequence.
  * Rows whose sequence, slot or block is out of range (a negative slot:
  * padding) cache nothing.  qkv, q, gains and tables are 16-byte aligned; the
- * rows of one call name distinct positions; a q that overlaps qkv is refused.  All is computed in 64
- * bits, so a row's codes depend on its inputs alone.  For drafted tokens rpos is the node's depth behind
- * the context, and slot the node's place. */
+ * rows of one call name distinct positions; a q that overlaps qkv is refused.
+ * All is computed in 64 bits, so a row's codes depend on its inputs alone.
+ * For drafted tokens rpos is the node's depth behind the context, and slot
+ * the node's place. */
 int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const float *kgain, float eps,
                                      const float *rope_cos, const float *rope_sin, uint32_t trows, int rope_half,
                                      const int32_t *seq, const int32_t *slot, const int32_t *rpos,
@@ -420,11 +421,9 @@ int nlg_qk_norm_rope_append_paged_q8(const float *qkv, const float *qgain, const
  * outside [0, npool) read as zero K/V rows.  Products are exact in the codes
  * and carry 22 bits of the probabilities and of q (of its elements down to
  * 2^-14 of a head's largest; smaller ones are held in steps of 2^-36 of
- * that).  A V row that a query
- * masks, or gives next to no weight, takes no bits of what makes its output
- * as long as its scale is below 2^96 times the query's largest product of a
- * probability and a V scale.
- * Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0
+ * that).  A V row that a query masks, or gives next to no weight, takes no
+ * bits of what makes its output as long as its scale is below 2^96 times the
+ * query's largest product of a probability and a V scale.  Workspace from nlg_decode_attn_paged_q8_workspace (16-byte aligned; 0
  * bytes: none is read), as below; calls that share one run in stream order. */
 int nlg_decode_attn_paged_q8(const float *q, const uint8_t *kpool, const uint8_t *vpool, int fmt,
                              const int32_t *lens, const int32_t *table, uint32_t npool, float *out, uint32_t batch,
@@ -455,7 +454,7 @@ size_t nlg_tree_attn_paged_q8_workspace(uint32_t batch, uint32_t tmax, uint32_t 
  * path[..], goes to position base[b] + i, as if all of a sequence's rows
  * were read before any is written.  Entries outside [0, tmax), and rows whose source or
  * destination has no block, move nothing; sequences with base[b] < 0 are
- * left alone.  Blocks written here belong to one sequence. */
+ * left alone.  At most 65,535 sequences.  Blocks written here belong to one sequence. */
 int nlg_tree_commit_paged_q8(uint8_t *kpool, uint8_t *vpool, const int32_t *base, const int32_t *path,
                              const int32_t *accepted, const int32_t *table, uint32_t npool, uint32_t batch,
                              uint32_t tmax, uint32_t kvheads, uint32_t head_dim, uint32_t bs, uint32_t mbps,

@@ -20,7 +20,7 @@
 
 #define KV8_TILE 16  // positions of a tile
 #define KV8_STEP 64  // positions that a wave attends at once
-#define KV8_WAVES 4  // waves of an attention workgroup
+#define KV8_WAVES 4  // waves of an attention workgroup that takes a chunk (eight where a sequence is one)
 
 NLG_KV8_HD constexpr uint32_t kv8_tile_bytes(uint32_t hd) { return KV8_TILE * (hd + 4); }
 // Byte of position `at` (0..15), dimension d in a tile; of its scale.
@@ -114,7 +114,7 @@ NLG_KV8_HD uint64_t kv8_word(uint64_t mask, uint32_t nodes) { return nodes < 64 
 // chunk of its positions; every kv head has all of them.  How many there are,
 // and how long, follows from the lengths and node counts that the kernel finds
 // on the device (kv8_per); a sequence's chunks are of one size.  want: the slots
-// that fill the card once, two workgroups a CU; slots: the most there can be.
+// that fill the card once, two workgroups on each of its 256 CUs; slots: the most there can be.
 // one: no sequence is split, and a slot is its sequence and group.
 struct Kv8Split {
   uint32_t rowsper, rowslog, groups, want, least, unit;
@@ -134,7 +134,8 @@ inline Kv8Split kv8_split(uint32_t batch, uint32_t rows, uint32_t kvheads, uint3
   s.least = s.wide ? 2 : KV8_WAVES;
   const uint64_t most = (positions + KV8_STEP - 1) / KV8_STEP, pairs = (uint64_t)batch * s.groups;
   s.want = 512 / kvheads ? 512 / kvheads : 1;
-  // (eight waves to a workgroup take 1,024 positions in two steps each: less than a second launch)
+  // (eight waves to a workgroup take 1,024 positions in two steps each: less than a second launch.  By the table's
+  // positions, as the lengths are on the device: 640 in a table for more take the two launches, 11.0 us for 9.6)
   s.one = most <= (s.rowsper == 16 ? 16 : s.least);
   const uint64_t all = pairs * ((most + s.least - 1) / s.least);
   const uint64_t upto = pairs <= s.want / 2 ? s.want : 2ull * s.want + pairs;

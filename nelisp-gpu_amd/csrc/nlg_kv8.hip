@@ -125,7 +125,7 @@ __device__ __forceinline__ void load8(const float *p, const float *q, double *y)
 // k heads; the others V, a wave sixteen rows of one head, whose codes pass
 // through LDS: a position's bytes of a tile lie sixteen apart, and a store then
 // runs over 64 dimensions (8 lines) instead of one byte a line.  Bound by the
-// bytes where there are many: 48 us there, 204 MB, 4.2 TB/s; one row of 20/5
+// bytes where there are many: 48 us there, 204 MB, 4.2 TB/s, in either format; one row of 20/5
 // heads, 3.1 us, by the chain slot -> block -> store.
 template <int HD, int FMT, bool HALF>
 __global__ __launch_bounds__(256) void k_append_q8(AppendArgs a) {
@@ -259,7 +259,7 @@ struct Kv8Attn {
   float *out, *pctx, *pmz;
   uint2 *pfirst;            // [batch]: a sequence's first slot, its chunks
   uint32_t batch, tmax, heads, grp;  // grp: query heads of a kv head; a sequence's rows: tmax * grp
-  uint32_t rowsper, rowslog, groups, want, least, unit, slots;  // Kv8Split
+  uint32_t rowsper, rowslog, groups, want, least, unit;  // Kv8Split
   Kv8Div bykvheads, bygrp, bygroups;
   bool tree, one;
   float coef;  // log2(e) / sqrt(hd): scores in base 2
@@ -831,10 +831,13 @@ __device__ __forceinline__ void kv8_step(const Kv8Attn &a, const Kv8Work &k, Wav
 // the scores come out, the very sixteen positions that the second product wants
 // of it, with K's rows dealt to the first so (4 of each tile a time); nothing is
 // exchanged but maxima and sums.  One pass over the cache, bound by its bytes:
-// 8 sequences at 24,000-32,768, 32/8 heads of 128, 480 MB: 85 us, 5.7 TB/s; 32
-// of up to 4,096, 20/5 heads, 87 MB: 22 us, 4.0 TB/s, the chain lengths -> table
-// -> K, V before it and chunks of unequal lengths; 640 positions of one sequence
-// (eight waves, no second launch): 9.6 us, that chain and the waves' meeting.
+// 8 sequences at 24,000-32,768, 32/8 heads of 128, 480 MB: 84 us, 5.7 TB/s; 32
+// of up to 4,096, 20/5 heads, 87 MB: 21.5 us, 4.0 TB/s (25.5 with the join), chunks
+// of unequal lengths and a step's loads that wait for the step before (42% of a
+// wave's cycles wait for something, 27% for their turn to issue).  One sequence
+// (eight waves, no second launch), 20/5 heads: 6.4 us at 64 positions, one step of
+// one wave; 8.7 at 512, one of each; 9.6 at 640; 11.7 at 1,024, two: five
+// workgroups, each wave's second step asked for after its first.
 template <int HD, int FMT, int NT, int W, bool PAST>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void k_attn_q8(Kv8Attn a) {
@@ -910,14 +913,18 @@ void k_attn_q8(Kv8Attn a) {
 // and K and V are made halves once for the workgroup, in LDS, in the order in
 // which the waves' operands lie (a fragment's 64 lanes side by side: no bank is
 // asked twice).  While a step is computed the next one's halves are written and
-// the one's after it are on their way from memory.  Bound by issue: two chunks
-// of 500-512 tokens over 1,024-2,047, 32/8 heads of 64, take 60 us, 249 TFLOP/s
-// (each product counted once; it is done twice, for hi and lo).  When they took
-// 68 with the join, 22 were left without any step, 28 with only the loads and the
-// halves in LDS; the softmax was 20, the second product 5, waiting for memory 4.
-// 16 trees of up to 32 nodes over up to 4,000, 20/5 heads of 128: 32 us (of 46
-// with the join, 20 without steps, 6 for the softmax).  Two waves a SIMD: three at
-// head dim 64, with 64 rows a workgroup, took 69 us for 60; eight waves a
+// the one's after it are on their way from memory.  Two chunks of 500-512 tokens
+// over 1,024-2,047, 32/8 heads of 64: 60 us, 62.5 with the join, 238 TFLOP/s (each
+// product counted once; it is done twice, for hi and lo), bound by issue: a wave
+// issues vector arithmetic in 36% of its cycles, two waves a SIMD.  16 us are left
+// without any step (the join 6, the partials' stores 4, launch, plan and queries
+// 6), 25 with only the loads and the halves in LDS, 41 without the softmax, 62
+// without the second product, 58 without waiting for memory.  16 trees of up to 32
+// nodes over up to 4,000, 20/5 heads of 128: 32 us, 37 with the join: 15 without
+// any step (the join 5, the partials 3), 22 with the loads and halves alone, 31
+// without the softmax, 36 without the second product; a wave waits in 45% of its
+// cycles, for memory or the other waves, and issues arithmetic in 24%.  Three waves a
+// SIMD at head dim 64, with 64 rows a workgroup, took 69 us for 60; eight waves a
 // workgroup 85 for 76.
 template <int HD, int FMT, int NT>
 __global__ __launch_bounds__(64 * KV8_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -1083,9 +1090,9 @@ void k_attn_wide_q8(Kv8Attn a) {
 
 // The chunks' parts of each output row, joined by their maxima and sums: SUBS
 // groups of hd / 4 threads walk a row's chunks.  The sum of averages times weights is
-// held in units of the weights' sum's power of two, no larger than the largest V.  A workgroup's rows are of one sequence.  4-6
-// us traced: eight groups where one each would leave the
-// card empty and walk tens of chunks one after another.
+// held in units of the weights' sum's power of two, no larger than the largest V.  A
+// workgroup's rows are of one sequence.  4-6.5 us traced: eight groups where one
+// each would leave the card empty and walk tens of chunks one after another.
 template <int SUBS>
 __global__ __launch_bounds__(256) void k_attn_q8_merge(Kv8Attn a, uint32_t hd, uint32_t blocks) {
   __shared__ float4v s_o[256];
@@ -1241,7 +1248,7 @@ __device__ __forceinline__ void store16(void *p, uint4 v) {
   if (NT) __builtin_nontemporal_store(t, (v4u *)p);
   else *(v4u *)p = t;
 }
-// A wave reads N rows of one kv head: sixteen, or four where there are too few
+// A wave reads N rows of one kv head: sixteen, or one where there are too few
 // rows to fill the card.  K: HD / 8 lanes a row.  V: a lane holds the sixteen
 // positions of two (HD 128) or one dimensions of a tile, and gives each of its
 // rows that lie there theirs; of rows that follow each other in a sequence the
@@ -1466,7 +1473,7 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   a.q = q; a.kpool = kpool; a.vpool = vpool; a.base = base; a.nodes = nodes; a.mask = mask; a.out = out;
   a.batch = batch; a.tmax = tmax; a.heads = heads; a.grp = heads / kvheads;
   a.rowsper = s.rowsper; a.rowslog = s.rowslog; a.groups = s.groups; a.want = s.want;
-  a.least = s.least; a.unit = s.unit; a.slots = (uint32_t)s.slots;
+  a.least = s.least; a.unit = s.unit;
   a.bygroups = kv8_div(s.groups); a.bykvheads = kv8_div(kvheads); a.bygrp = kv8_div(a.grp);
   a.tree = tree; a.one = s.one;
   a.pctx = (float *)workspace;
@@ -1477,7 +1484,10 @@ static int kv8_attend(const char *what, bool tree, const float *q, const uint8_t
   hipStream_t st = nlg_stream(stream);
   // K and V of more than the 256 MB MALL are gone from it before the next call
   // reads them (eight sequences at 24,000-32,768 of 8 heads of 128, 480 MB: 94 ->
-  // 88 us; 32 at up to 4,096 of 5, 87 MB: 25.4 us kept, 27.0 past)
+  // 88 us).  By the table's capacity: the lengths are on the device.  Where they are
+  // far below it that matters little (32 at up to 4,096 of 5, 87 MB: kept and past
+  // 24.9 and 25.6 us replayed alone, 25.4 and 27.1 over three layers' pools, 28.7 and
+  // 28.5 over eight; at up to 600 13.8 and 14.2, 15.5 and 15.2 over forty)
   const bool past = (uint64_t)batch * mbps * bs * kvheads * 2 * (hd + 4) > (256u << 20);
 #define GO(HD, F)                                                                                                 \
   do {                                                                                                            \
