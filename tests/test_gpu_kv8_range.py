@@ -213,3 +213,19 @@ def test_masked_keys_of_any_size(fmt, small, heads, kvh, hd, tmax, n):
     for i in range(0, tmax, 3):
         on = np.array([p < n - tmax or int(mask[0, i]) >> (p - n + tmax) & 1 for p in range(n)], bool)
         close(got[0, i], q[0, i], k[on], v[on], ("masked", i))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("seed", range(4))
+@pytest.mark.parametrize("heads,kvh,hd,tmax,n", LAYOUTS)
+def test_rows_of_all_sizes(fmt, seed, heads, kvh, hd, tmax, n):
+    """Each position's K, V and each query of its own random size, over 2^72 for V, scores up to some 60 and next to
+    nothing, zero rows among them."""
+    rng = np.random.default_rng(100 * n + seed)
+    pools, table = cached(rng, [n], kvh, hd, 16, (n + 15) // 16, fmt)
+    for which, span in (("k", 4), ("v", 25)):
+        rows = rng.standard_normal((n, kvh, hd)) * np.exp(rng.uniform(-span, span if which == "v" else 2, (n, kvh, 1)))
+        rows[rng.random(n) < 0.05] = 0
+        fill(pools, table, n, which, rows)
+    q = rng.standard_normal((1, tmax, heads, hd)) * np.exp(rng.uniform(-3, 1, (1, tmax, heads, 1)))
+    check(pools, table, q.reshape(1, tmax, -1).astype(F32), n)
