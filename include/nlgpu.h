@@ -469,6 +469,49 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
                             uint32_t rows, uint32_t batch, uint32_t kvheads, uint32_t head_dim, uint32_t bs,
                             uint32_t mbps, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Losses over a ternary LM head, without its logits.  The reference ends at
+ * the logits (rmsnorm-fwd, pack-act-rows, bitlinear-dp4a-1f) and takes input
+ * gradients with ternary-rows-t; these have no counterpart there.
+ *
+ * x [rows x cols] are the head's input rows (normed; f32), rounded to int8 as
+ * nlg_ternary_linear does; z[s,o] = bias[o] + (beta[b] * gamma[s]) * acc[s,o]
+ * are its logits over `vocab` rows of w2, computed a tile at a time (twice
+ * with a gradient) and never kept.  dx [rows x cols] (NULL: no gradient)
+ * receives dloss[s] (NULL: 1) times the gradient of loss[s] with respect to
+ * the rounded rows gamma*q, which passes straight through the rounding; it is
+ * overwritten.  lse [rows] (may be NULL) receives log(sum(exp(z/temperature))).
+ * Logits of -inf (a bias that forbids a token) have no part in a row.  The
+ * probabilities carry 22 bits of those from 2^-15 on and steps of 2^-39
+ * below.  cols is a multiple of 64, at most 16384; x, w2 and dx are 16-byte
+ * aligned.  The workspace (16-byte aligned, nlg_*_workspace bytes, 0 for
+ * sizes that the calls do not take; grad: whether dx is wanted) holds the
+ * probabilities of a piece of the vocabulary; calls that share one run in
+ * stream order.  Nothing here allocates, so every call may be captured into a
+ * graph.  dx may not overlap x.
+ * ---------------------------------------------------------------------- */
+
+/* Softmax cross entropy: loss[s] = lse[s] - z[s, label[s]].  Rows whose label
+ * is outside [0, vocab) have loss 0 and a zero gradient (their lse is still
+ * written). */
+int nlg_ternary_xent(const float *x, const uint32_t *w2, const float *bias, const float *beta, int beta_per_row,
+                     const int32_t *label, const float *dloss, float *loss, float *lse, float *dx, uint32_t rows,
+                     uint32_t vocab, uint32_t cols, void *workspace, size_t workspace_bytes, void *stream);
+size_t nlg_ternary_xent_workspace(uint32_t rows, uint32_t vocab, uint32_t cols, int grad);
+
+/* Distillation from a teacher's `top` (1 to 1024) best logits of each row:
+ * loss[s] = sum_k t_k * (log(t_k) - (z[s, index[s,k]]/temperature - lse[s])),
+ * with t the softmax of teacher[s,:]/temperature over those entries, or with
+ * teacher_lse t_k = exp(teacher[s,k]/temperature - teacher_lse[s]) (the
+ * teacher's own log sum at that temperature; the t then need not add up to
+ * one).  Entries whose index is outside [0, vocab) have no part; an index
+ * that comes twice counts twice.  index and teacher are [rows x top]. */
+int nlg_ternary_distill(const float *x, const uint32_t *w2, const float *bias, const float *beta, int beta_per_row,
+                        const int32_t *index, const float *teacher, const float *teacher_lse, uint32_t top,
+                        float temperature, const float *dloss, float *loss, float *lse, float *dx, uint32_t rows,
+                        uint32_t vocab, uint32_t cols, void *workspace, size_t workspace_bytes, void *stream);
+size_t nlg_ternary_distill_workspace(uint32_t rows, uint32_t vocab, uint32_t cols, uint32_t top, int grad);
+
 /* The first of nlg_decode_attn_f16's two launches alone: per chunk of
  * positions and head, the chunk's maximum score m (in base 2: q.k/sqrt(hd)
  * times log2 e), its sum of 2^(s - m) and the matching weighted sum of V,

@@ -136,6 +136,11 @@ def lib() -> C.CDLL:
         "nlg_tree_attn_paged_q8_workspace": (sz, [u32, u32, u32, u32, u32, u32, u32]),
         "nlg_tree_commit_paged_q8": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, vp]),
         "nlg_cache_read_paged_q8": (i32, [vp, vp, i32, vp, vp, vp, u32, vp, vp, u32, u32, u32, u32, u32, u32, vp]),
+        "nlg_ternary_xent": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, u32, u32, u32, vp, sz, vp]),
+        "nlg_ternary_xent_workspace": (sz, [u32, u32, u32, i32]),
+        "nlg_ternary_distill": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, u32, C.c_float, vp, vp, vp, vp, u32, u32, u32,
+                                      vp, sz, vp]),
+        "nlg_ternary_distill_workspace": (sz, [u32, u32, u32, u32, i32]),
         "nlg_repack_packed_to_2bit": (i32, [vp, u32, u32, u32, u32, vp, vp, vp]),
         "nlg_ternary_tiled_register": (i32, [vp, u32, u32, vp]),
         "nlg_ternary_tiled_unregister": (i32, [vp]),
@@ -508,6 +513,32 @@ def cache_read_paged_q8(kpool, vpool, slot, table, npool, k, v, rows, batch, kvh
     _check(lib().nlg_cache_read_paged_q8(kpool.ptr, vpool.ptr, fmt, _ptr(seq), slot.ptr, table.ptr, npool, k.ptr,
                                          v.ptr, rows, batch, kvheads, head_dim, bs, mbps, stream),
            "cache_read_paged_q8")
+
+
+def ternary_xent_workspace(rows, vocab, cols, grad) -> int:
+    return int(lib().nlg_ternary_xent_workspace(rows, vocab, cols, int(grad)))
+
+
+def ternary_xent(x, w2, bias, beta, label, loss, lse, rows, vocab, cols, workspace, dx=None, dloss=None,
+                 beta_per_row=False, stream=None) -> None:
+    """Softmax cross entropy of rows x [rows][cols] through a ternary LM head (its logits are not kept), with its
+    gradient in dx if that is given."""
+    _check(lib().nlg_ternary_xent(x.ptr, w2.ptr, _ptr(bias), beta.ptr, int(beta_per_row), label.ptr, _ptr(dloss),
+                                  loss.ptr, _ptr(lse), _ptr(dx), rows, vocab, cols, workspace.ptr, workspace.nbytes,
+                                  stream), "ternary_xent")
+
+
+def ternary_distill_workspace(rows, vocab, cols, top, grad) -> int:
+    return int(lib().nlg_ternary_distill_workspace(rows, vocab, cols, top, int(grad)))
+
+
+def ternary_distill(x, w2, bias, beta, index, teacher, top, temperature, loss, lse, rows, vocab, cols, workspace,
+                    teacher_lse=None, dx=None, dloss=None, beta_per_row=False, stream=None) -> None:
+    """Divergence of a ternary LM head from a teacher's `top` best logits (index, teacher [rows][top]), with its
+    gradient in dx if that is given."""
+    _check(lib().nlg_ternary_distill(x.ptr, w2.ptr, _ptr(bias), beta.ptr, int(beta_per_row), index.ptr, teacher.ptr,
+                                     _ptr(teacher_lse), top, temperature, _ptr(dloss), loss.ptr, _ptr(lse), _ptr(dx),
+                                     rows, vocab, cols, workspace.ptr, workspace.nbytes, stream), "ternary_distill")
 
 
 def cache_append_ring_f16(src, pos, cache, batch, kvheads, head_dim, nsink, win, stream=None) -> None:
