@@ -470,6 +470,63 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
                             uint32_t mbps, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared linear.  No counterpart
+ * in the reference, whose linears (bitlinear-dp4a-1f, ternary-rows,
+ * kernels.el:619-746) these stand beside.
+ *
+ * `adapters` resident adapters, a [adapters][rmax][cols] and
+ * b [adapters][out][rmax], 16-bit floats of format NLG_LORA_F16 or
+ * NLG_LORA_BF16; adapter i has rank rank[i] (NULL: rmax) of at most rmax (a
+ * multiple of 8 up to 128; what lies behind rank[i] is not used) and the
+ * factor scale[i].  Request i's rows are start[i] .. start[i+1]-1 (start
+ * [requests + 1], not falling; NULL: request i is row i) and its adapter is
+ * adapter[i]; any number outside [0, adapters) means none, and so do rows of
+ * no request.  start, adapter, rank and scale are device arrays.
+ *   u[s,j] = sum_c a[j,c] x[s,c]    (0 behind the rank)
+ *   y[s,o] = res[s,o] + scale * sum_j b[o,j] u[s,j]
+ * in 32 bits.  x [seq x cols] f32; cols is a multiple of 8.  a, b, x, u and
+ * the workspace (nlg_*_workspace bytes; 0: sizes that are not taken) are
+ * 16-byte aligned; calls that share a workspace run in stream order.  Nothing
+ * here allocates, so every call may be captured into a graph (but for the
+ * column split of nlg_ternary_linear_lora's base, which goes without its
+ * scratch if a capture is the first call that wants it).
+ * ---------------------------------------------------------------------- */
+#define NLG_LORA_F16 0
+#define NLG_LORA_BF16 1
+/* y = res + the adapters' part (res NULL: that alone; res may be y).  u
+ * [seq x rmax] (NULL: kept in the workspace, which is not read otherwise)
+ * receives what the gradient needs. */
+int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t *b, int fmt, const float *scale,
+                    const int32_t *rank, const int32_t *start, const int32_t *adapter, uint32_t requests,
+                    uint32_t adapters, uint32_t rmax, const float *res, float *y, float *u, uint32_t seq, uint32_t out,
+                    uint32_t cols, void *workspace, size_t workspace_bytes, void *stream);
+size_t nlg_lora_linear_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests);
+/* nlg_ternary_linear with the adapters of its rows' requests: the shared
+ * projection on the rounded rows, the adapters on the rows as they are.
+ * cols is at most 16384; w2 is 16-byte aligned. */
+int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const float *bias, const float *beta, int beta_per_row,
+                            const uint16_t *a, const uint16_t *b, int fmt, const float *scale, const int32_t *rank,
+                            const int32_t *start, const int32_t *adapter, uint32_t requests, uint32_t adapters,
+                            uint32_t rmax, float *y, float *u, uint32_t seq, uint32_t out, uint32_t cols,
+                            void *workspace, size_t workspace_bytes, void *stream);
+size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests);
+/* The gradients of nlg_lora_linear for dy [seq x out]: da [adapters][rmax]
+ * [cols] and db [adapters][out][rmax] (overwritten; zero behind the rank and
+ * for adapters without rows), and dx = dres + the adapters' part (dx NULL: not
+ * wanted; dres NULL: that part alone; dres may be dx: the base's input gradient,
+ * as ternary-rows-t leaves it, goes there).  u: what the forward call left
+ * (NULL: computed again).  seq is nonzero.  No output may overlap another
+ * or an input.  Sums over rows run in an order of the sizes alone, so the same
+ * call gives the same bits. */
+int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a, const uint16_t *b, int fmt,
+                         const float *scale, const int32_t *rank, const int32_t *start, const int32_t *adapter,
+                         uint32_t requests, uint32_t adapters, uint32_t rmax, const float *dres, float *dx, float *da,
+                         float *db, uint32_t seq, uint32_t out, uint32_t cols, void *workspace, size_t workspace_bytes,
+                         void *stream);
+size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters, uint32_t rmax,
+                                      uint32_t requests);
+
+/* ------------------------------------------------------------------------
  * Losses over a ternary LM head, without its logits.  The reference ends at
  * the logits (rmsnorm-fwd, pack-act-rows, bitlinear-dp4a-1f) and takes input
  * gradients with ternary-rows-t; these have no counterpart there.

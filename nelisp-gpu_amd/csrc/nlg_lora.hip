@@ -1,0 +1,628 @@
+// nlg_lora.hip -- low-rank adapters of many requests beside a shared linear,
+// forward and backward.  No reference counterpart.
+//
+//   u[s, j]  = sum_c A[a][j][c] x[s, c]               (j < rank[a]; 0 from there on)
+//   y[s, o]  = res[s, o] + scale[a] sum_j B[a][o][j] u[s, j]
+//   du[s, j] = scale[a] sum_o B[a][o][j] dy[s, o]
+//   dx[s, c] = dres[s, c] + sum_j A[a][j][c] du[s, j]
+//   dA[a][j][c] = sum_{s of a} du[s, j] x[s, c],  dB[a][o][j] = scale[a] sum_{s of a} dy[s, o] u[s, j]
+//
+// with a the adapter of row s's request.  Rows and adapters' values meet in
+// 32 bits (16 x 16 x 4 f32 products; the 16-bit values are exact there).
+//
+// v_mfma_f32_16x16x4_f32: lane 16 g + i gives A[i][g] and B[g][i]; its result
+// r is C[4 g + r][i].
+#include <math.h>
+
+#include "nlg_quant.h"
+#include "nlg_scope.h"
+
+int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *attn_mz, uint32_t attn_nc, uint32_t hd,
+                     int pro, uint8_t *xq, float *gamma, uint32_t seq, uint32_t cols, hipStream_t st);
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+#define LORA_RANK 128            // most ranks of an adapter
+#define LORA_ROWS (65535u * 32)  // most rows (a grid's y dimension)
+
+struct LoraArgs {
+  const int32_t *start;     // [requests + 1] or null: request i is row i
+  const int32_t *adapter;   // [requests]
+  const int32_t *rank;      // [adapters] or null
+  const float *scale;       // [adapters]
+  const uint16_t *a, *b;    // [adapters][rmax][cols], [adapters][out][rmax]
+  uint32_t requests, adapters, rmax, seq;
+};
+
+__device__ __forceinline__ uint32_t lora_rank(const LoraArgs &l, int32_t ad) {
+  if (!l.rank) return l.rmax;
+  const int32_t r = l.rank[ad];
+  return r < 0 ? 0u : min((uint32_t)r, l.rmax);
+}
+
+// A wave finds the adapters of rows row0 .. row0 + n - 1 (n <= 64), lane i
+// row0 + i's; -1: none.  A row that two requests name belongs to the first.
+__device__ __forceinline__ int32_t lora_rows(const LoraArgs &l, uint32_t row0, uint32_t n, int lane) {
+  int32_t got = -1;
+  const uint32_t row = row0 + lane;
+  if (!l.start) {
+    if ((uint32_t)lane < n && row < l.seq && row < l.requests) got = l.adapter[row];
+  } else {
+    bool found = false;
+    for (uint32_t i0 = 0; i0 < l.requests; i0 += 64) {
+      const uint32_t i = i0 + lane;
+      const bool in = i < l.requests;
+      const int32_t s = in ? l.start[i] : 0, e = in ? l.start[i + 1] : 0, ad = in ? l.adapter[i] : -1;
+      // requests of this block that touch the rows, in order
+      uint64_t hit = __ballot(in && s < e && (int64_t)s < (int64_t)row0 + n && (int64_t)e > (int64_t)row0);
+      while (hit) {
+        const int k = __builtin_ctzll(hit);
+        hit &= hit - 1;
+        const int64_t ks = __builtin_amdgcn_readlane(s, k), ke = __builtin_amdgcn_readlane(e, k);
+        const int32_t ka = __builtin_amdgcn_readlane(ad, k);
+        if (!found && (int64_t)row >= ks && (int64_t)row < ke) {
+          got = ka;
+          found = true;
+        }
+      }
+      if (__all(found || (uint32_t)lane >= n || row >= l.seq)) break;
+    }
+    if ((uint32_t)lane >= n || row >= l.seq) got = -1;
+  }
+  return got >= 0 && (uint32_t)got < l.adapters ? got : -1;
+}
+
+template <bool BF>
+__device__ __forceinline__ float wide(uint32_t h) {  // a 16-bit value (low half)
+  return BF ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
+}
+
+template <bool VEC>
+__device__ __forceinline__ float4 load4(const float *p, uint32_t n) {  // n: how many of them there are
+  if (VEC) return n ? *(const float4 *)p : make_float4(0, 0, 0, 0);
+  return make_float4(n > 0 ? p[0] : 0, n > 1 ? p[1] : 0, n > 2 ? p[2] : 0, n > 3 ? p[3] : 0);
+}
+template <bool VEC>
+__device__ __forceinline__ void store4(float *p, uint32_t n, float4 v) {
+  if (VEC) {
+    if (n) *(float4 *)p = v;
+    return;
+  }
+  if (n > 0) p[0] = v.x;
+  if (n > 1) p[1] = v.y;
+  if (n > 2) p[2] = v.z;
+  if (n > 3) p[3] = v.w;
+}
+__device__ __forceinline__ float at4(float4 v, int e) { return e == 0 ? v.x : e == 1 ? v.y : e == 2 ? v.z : v.w; }
+
+// ------------------------------------------------------------------ down: to the ranks
+
+struct DownArgs {
+  LoraArgs l;
+  const float *x;   // [seq][k]
+  uint32_t k;
+  bool scaled;
+  float *u;         // [seq][rmax]
+};
+
+// Sixteen rows a workgroup, all ranks (NT blocks of sixteen), the contraction
+// split over its eight waves.  Each adapter among the rows is one pass.
+// KMAJOR: weights [k][rmax] (B, in the backward pass), else [rmax][k] (A).
+// A step is sixteen k: lane group g holds k = 4 g .. 4 g + 3 of both operands.
+// Weights [k][rmax] are read as NT neighbouring ranks a lane, so block t of
+// the ranks is then NT i + t.
+template <bool BF, bool KMAJOR, int NT, bool VEC>
+__global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
+  __shared__ float s_u[8][16][NT * 16 + 4];
+  __shared__ int32_t s_ad[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const uint32_t row0 = blockIdx.x * 16;
+  if (w == 0) {
+    const int32_t ad = lora_rows(a.l, row0, 16, lane);
+    if (lane < 16) s_ad[lane] = ad;
+  }
+  __syncthreads();
+  const uint32_t row = min(row0 + i, a.l.seq - 1);
+  const float *const xr = a.x + (size_t)row * a.k;
+  uint32_t todo = 0;
+  for (int r = 0; r < 16; r++) {
+    if (s_ad[r] >= 0) todo |= 1u << r;
+    else if (row0 + r < a.l.seq)
+      for (uint32_t j = threadIdx.x; j < a.l.rmax; j += 512) a.u[(size_t)(row0 + r) * a.l.rmax + j] = 0.0f;
+  }
+  while (todo) {
+    const int32_t ad = __builtin_amdgcn_readfirstlane(s_ad[__builtin_ctz(todo)]);
+    uint32_t mine = 0;
+    for (int r = 0; r < 16; r++) mine |= s_ad[r] == ad ? 1u << r : 0u;
+    todo &= ~mine;
+    const uint32_t rank = lora_rank(a.l, ad);
+    const uint16_t *const wt = (KMAJOR ? a.l.b : a.l.a) + (size_t)ad * a.l.rmax * a.k;
+    v4f acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = (v4f){0, 0, 0, 0};
+    for (uint32_t k0 = w * 16; k0 < a.k; k0 += 128) {
+      const uint32_t k = k0 + 4 * g, n = k < a.k ? min(4u, a.k - k) : 0u;
+      const float4 xv = load4<VEC>(xr + k, n);
+      float wv[NT][4];
+      if (KMAJOR) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          // ranks NT i .. NT i + NT - 1 (rmax is a multiple of 8, so they are all there or none is; NT is 1, 2, 4 or 8)
+          union {
+            uint32_t u[(NT + 1) / 2];
+            uint16_t h[NT + NT % 2];
+          } v = {};
+          if ((uint32_t)e < n && (uint32_t)(NT * i) < rank) {
+            const uint16_t *p = wt + (size_t)(k + e) * a.l.rmax + NT * i;
+            if (NT == 1) v.h[0] = *p;
+            else if (NT == 2) v.u[0] = *(const uint32_t *)p;
+            else if (NT == 4) *(uint2 *)v.u = *(const uint2 *)p;
+            else *(uint4 *)v.u = *(const uint4 *)p;
+          }
+#pragma unroll
+          for (int t = 0; t < NT; t++) wv[t][e] = (uint32_t)(NT * i + t) < rank ? wide<BF>(v.h[t]) : 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          uint2 v = make_uint2(0, 0);
+          if (n && (uint32_t)(16 * t + i) < rank) v = *(const uint2 *)(wt + (size_t)(16 * t + i) * a.k + k);
+          wv[t][0] = wide<BF>(v.x & 0xffff);
+          wv[t][1] = wide<BF>(v.x >> 16);
+          wv[t][2] = wide<BF>(v.y & 0xffff);
+          wv[t][3] = wide<BF>(v.y >> 16);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(at4(xv, e), wv[t][e], acc[t], 0, 0, 0);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) s_u[w][4 * g + r][KMAJOR ? NT * i + t : 16 * t + i] = acc[t][r];
+    __syncthreads();
+    const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
+    for (uint32_t p = threadIdx.x; p < 16 * a.l.rmax; p += 512) {
+      const uint32_t r = p / a.l.rmax, j = p % a.l.rmax;
+      if (mine >> r & 1) {
+        float v = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 8; q++) v += s_u[q][r][j];
+        a.u[(size_t)(row0 + r) * a.l.rmax + j] = j < rank ? v * sc : 0.0f;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------ up: from the ranks
+
+struct UpArgs {
+  LoraArgs l;
+  const float *u;    // [seq][rmax]
+  const float *res;  // [seq][n] or null
+  float *y;          // [seq][n] (may be res)
+  uint32_t n;
+  bool scaled;
+};
+
+// 32 rows x 256 columns a workgroup, a wave 64 columns: four neighbouring
+// columns a lane, in four blocks (block e of the columns is 4 i + e), so that
+// results are stored sixteen bytes a lane.
+// KMAJOR: weights [rmax][n] (A, in the backward pass), else [n][rmax] (B).
+template <bool BF, bool KMAJOR, bool VEC>
+__global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
+  __shared__ int32_t s_ad[32];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const uint32_t row0 = blockIdx.y * 32, col = blockIdx.x * 256 + w * 64 + 4 * i;
+  const uint32_t nc = col < a.n ? min(4u, a.n - col) : 0u;
+  if (w == 0) {
+    const int32_t ad = lora_rows(a.l, row0, 32, lane);
+    if (lane < 32) s_ad[lane] = ad;
+  }
+  __syncthreads();
+  uint32_t todo = 0;
+  for (int r = 0; r < 32; r++) {
+    if (s_ad[r] >= 0) todo |= 1u << r;
+  }
+  if (a.y != a.res) {  // rows without an adapter
+    for (int r = g; r < 32; r += 4)
+      if (s_ad[r] < 0 && row0 + r < a.l.seq) {
+        const size_t o = (size_t)(row0 + r) * a.n + col;
+        store4<VEC>(a.y + o, nc, a.res ? load4<VEC>(a.res + o, nc) : make_float4(0, 0, 0, 0));
+      }
+  }
+  while (todo) {
+    const int32_t ad = __builtin_amdgcn_readfirstlane(s_ad[__builtin_ctz(todo)]);
+    uint32_t mine = 0;
+    for (int r = 0; r < 32; r++) mine |= s_ad[r] == ad ? 1u << r : 0u;
+    todo &= ~mine;
+    const uint32_t rank = lora_rank(a.l, ad);
+    const uint16_t *const wt = (KMAJOR ? a.l.a : a.l.b) + (size_t)ad * a.l.rmax * a.n;
+    v4f acc[2][4];
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) acc[m][e] = (v4f){0, 0, 0, 0};
+    for (uint32_t j0 = 0; j0 < rank; j0 += 16) {
+      const uint32_t j = j0 + 4 * g;  // lane group g's ranks j .. j + 3
+      float4 uv[2];
+#pragma unroll
+      for (int m = 0; m < 2; m++) {
+        const uint32_t row = min(row0 + 16 * m + i, a.l.seq - 1);
+        uv[m] = j < a.l.rmax ? *(const float4 *)(a.u + (size_t)row * a.l.rmax + j) : make_float4(0, 0, 0, 0);
+      }
+      uint2 v[4];  // KMAJOR: rank j + q, columns col ..; else column col + q, ranks j ..
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        v[q] = make_uint2(0, 0);
+        if (KMAJOR) {
+          if (j + q < rank && nc) v[q] = *(const uint2 *)(wt + (size_t)(j + q) * a.n + col);
+        } else {
+          if (j < rank && (uint32_t)q < nc) v[q] = *(const uint2 *)(wt + (size_t)(col + q) * a.l.rmax + j);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < 4; s++) {  // rank j + s
+        const bool in = j + s < rank;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const uint2 p = v[KMAJOR ? s : e];
+          const int f = KMAJOR ? e : s;
+          const uint32_t h = (f & 2 ? p.y : p.x) >> (16 * (f & 1)) & 0xffff;
+          const float b = in ? wide<BF>(h) : 0.0f;
+#pragma unroll
+          for (int m = 0; m < 2; m++)
+            acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? at4(uv[m], s) : 0.0f, b, acc[m][e], 0, 0, 0);
+        }
+      }
+    }
+    const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t rr = 16 * m + 4 * g + r;
+        if (!(mine >> rr & 1)) continue;
+        const size_t o = (size_t)(row0 + rr) * a.n + col;
+        float4 v = a.res ? load4<VEC>(a.res + o, nc) : make_float4(0, 0, 0, 0);
+        v.x = fmaf(sc, acc[m][0][r], v.x);
+        v.y = fmaf(sc, acc[m][1][r], v.y);
+        v.z = fmaf(sc, acc[m][2][r], v.z);
+        v.w = fmaf(sc, acc[m][3][r], v.w);
+        store4<VEC>(a.y + o, nc, v);
+      }
+  }
+}
+
+// ------------------------------------------------------------------ the adapters' gradients
+
+struct OuterArgs {
+  LoraArgs l;
+  const float *p;    // [seq][rmax]
+  const float *q;    // [seq][n]
+  float *out;        // [adapters][rmax][n], or [adapters][n][rmax]
+  uint32_t n;
+  bool scaled;
+};
+
+// sum over an adapter's rows of p[s, j] q[s, c], 64 columns and 16 NT ranks a
+// workgroup, its requests' rows over its eight waves.  TURN: stored [c][j].
+template <int NT, bool TURN, bool VEC>
+__global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
+  __shared__ v4f s_acc[4][NT][4][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int32_t ad = blockIdx.y;
+  const uint32_t rank = lora_rank(a.l, ad);
+  const uint32_t col = blockIdx.x * 64 + 4 * i, nc = col < a.n ? min(4u, a.n - col) : 0u;
+  v4f acc[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[t][e] = (v4f){0, 0, 0, 0};
+  int64_t before = 0;  // rows that earlier requests have taken
+  for (uint32_t rq = 0; rq < a.l.requests; rq++) {
+    int64_t s0 = a.l.start ? (int64_t)a.l.start[rq] : (int64_t)rq;
+    int64_t s1 = a.l.start ? (int64_t)a.l.start[rq + 1] : (int64_t)rq + 1;
+    if (s0 < before) s0 = before;
+    if (s1 > (int64_t)a.l.seq) s1 = a.l.seq;
+    if (s1 <= s0) continue;
+    before = s1;
+    if (a.l.adapter[rq] != ad) continue;
+    for (int64_t s = s0 + 4 * w; s < s1; s += 32) {
+      const int64_t row = s + g;
+      const bool in = row < s1;
+      const float4 qv = load4<VEC>(a.q + (size_t)(in ? row : s) * a.n + col, in ? nc : 0);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        const uint32_t j = 16 * t + i;
+        const float pv = in && j < rank ? a.p[(size_t)row * a.l.rmax + j] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv, at4(qv, e), acc[t][e], 0, 0, 0);
+      }
+    }
+  }
+  // the waves' sums, by halves
+#pragma unroll
+  for (int half = 4; half; half /= 2) {
+    if (w >= half && w < 2 * half)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s_acc[w - half][t][e][lane] = acc[t][e];
+    __syncthreads();
+    if (w < half)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[t][e] += s_acc[w][t][e][lane];
+    __syncthreads();
+  }
+  if (w) return;
+  const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
+  float *const o = a.out + (size_t)ad * a.l.rmax * a.n;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    if (TURN) {
+      const uint32_t j = 16 * t + 4 * g;
+      if (j >= a.l.rmax) continue;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if ((uint32_t)e < nc)
+          *(float4 *)(o + (size_t)(col + e) * a.l.rmax + j) =
+              make_float4(acc[t][e][0] * sc, acc[t][e][1] * sc, acc[t][e][2] * sc, acc[t][e][3] * sc);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t j = 16 * t + 4 * g + r;
+        if (j < a.l.rmax)
+          store4<VEC>(o + (size_t)j * a.n + col, nc,
+                      make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host side
+
+static int lora_check(const char *what, const void *a, const void *b, int fmt, const float *scale, const int32_t *rank,
+                      const int32_t *start, const int32_t *adapter, uint32_t requests, uint32_t adapters, uint32_t rmax,
+                      uint32_t seq, uint32_t out, uint32_t cols, LoraArgs &l) {
+  if (!a || !b || !scale || (requests && !adapter)) return nlg_fail("%s: null pointer", what);
+  if (fmt != NLG_LORA_F16 && fmt != NLG_LORA_BF16) return nlg_fail("%s: unknown adapter format %d", what, fmt);
+  if (!adapters) return nlg_fail("%s: adapters must be nonzero", what);
+  if (!rmax || rmax % 8 || rmax > LORA_RANK)
+    return nlg_fail("%s: rmax must be a multiple of 8 up to %d (got %u)", what, LORA_RANK, rmax);
+  if (!cols || cols % 8) return nlg_fail("%s: cols must be a multiple of 8 (got %u)", what, cols);
+  if (!out) return nlg_fail("%s: out must be nonzero", what);
+  if (seq > LORA_ROWS || out > 0x1000000u || cols > 0x1000000u || adapters > 65535 || requests > 0x1000000u)
+    return nlg_fail("%s: too many rows, columns, requests or adapters", what);
+  if (((uintptr_t)a & 15) || ((uintptr_t)b & 15)) return nlg_fail("%s: adapters must be 16-byte aligned", what);
+  if (((uintptr_t)scale | (uintptr_t)rank | (uintptr_t)start | (uintptr_t)adapter) & 3)
+    return nlg_fail("%s: scale, rank, start and adapter must be 4-byte aligned", what);
+  l.start = start; l.adapter = adapter; l.rank = rank; l.scale = scale;
+  l.a = (const uint16_t *)a; l.b = (const uint16_t *)b;
+  l.requests = requests; l.adapters = adapters; l.rmax = rmax; l.seq = seq;
+  return NLG_OK;
+}
+
+// sizes alone (the workspace functions have no pointers)
+static bool lora_sizes(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax) {
+  return seq && out && cols && cols % 8 == 0 && rmax && rmax % 8 == 0 && rmax <= LORA_RANK && seq <= LORA_ROWS &&
+         out <= 0x1000000u && cols <= 0x1000000u;
+}
+static size_t lora_round(size_t n) { return (n + 255) / 256 * 256; }
+static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && x < y + nb && y < x + na;
+}
+
+static int lora_down(const char *what, const DownArgs &d, bool bf, bool kmajor, hipStream_t st) {
+  const dim3 grid((d.l.seq + 15) / 16), blk(512);
+  const bool vec = d.k % 4 == 0 && ((uintptr_t)d.x & 15) == 0;
+  const uint32_t nt = (d.l.rmax + 15) / 16;
+#define GO(BF, KM, N)                                                                          \
+  do {                                                                                         \
+    if (vec) hipLaunchKernelGGL((k_lora_down<BF, KM, N, true>), grid, blk, 0, st, d);          \
+    else hipLaunchKernelGGL((k_lora_down<BF, KM, N, false>), grid, blk, 0, st, d);             \
+  } while (0)
+#define GO2(BF, KM)                  \
+  do {                               \
+    if (nt <= 1) GO(BF, KM, 1);      \
+    else if (nt <= 2) GO(BF, KM, 2); \
+    else if (nt <= 4) GO(BF, KM, 4); \
+    else GO(BF, KM, 8);              \
+  } while (0)
+  if (bf && kmajor) GO2(true, true);
+  else if (bf) GO2(true, false);
+  else if (kmajor) GO2(false, true);
+  else GO2(false, false);
+#undef GO2
+#undef GO
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipStream_t st) {
+  const dim3 grid((d.n + 255) / 256, (d.l.seq + 31) / 32), blk(256);
+  const bool vec = d.n % 4 == 0 && (((uintptr_t)d.y | (uintptr_t)d.res) & 15) == 0;
+#define GO(BF, KM)                                                                       \
+  do {                                                                                   \
+    if (vec) hipLaunchKernelGGL((k_lora_up<BF, KM, true>), grid, blk, 0, st, d);         \
+    else hipLaunchKernelGGL((k_lora_up<BF, KM, false>), grid, blk, 0, st, d);            \
+  } while (0)
+  if (bf && kmajor) GO(true, true);
+  else if (bf) GO(true, false);
+  else if (kmajor) GO(false, true);
+  else GO(false, false);
+#undef GO
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+static int lora_outer(const char *what, const OuterArgs &d, bool turn, hipStream_t st) {
+  const dim3 grid((d.n + 63) / 64, d.l.adapters), blk(512);
+  const bool vec = d.n % 4 == 0 && (((uintptr_t)d.q | (turn ? 0 : (uintptr_t)d.out)) & 15) == 0;
+  const uint32_t nt = (d.l.rmax + 15) / 16;
+#define GO(N, T)                                                                           \
+  do {                                                                                     \
+    if (vec) hipLaunchKernelGGL((k_lora_outer<N, T, true>), grid, blk, 0, st, d);          \
+    else hipLaunchKernelGGL((k_lora_outer<N, T, false>), grid, blk, 0, st, d);             \
+  } while (0)
+#define GO2(T)                  \
+  do {                          \
+    if (nt <= 1) GO(1, T);      \
+    else if (nt <= 2) GO(2, T); \
+    else if (nt <= 4) GO(4, T); \
+    else GO(8, T);              \
+  } while (0)
+  if (turn) GO2(true);
+  else GO2(false);
+#undef GO2
+#undef GO
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+extern "C" size_t nlg_lora_linear_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests) {
+  (void)requests;
+  return lora_sizes(seq, out, cols, rmax) ? lora_round((size_t)seq * rmax * 4) : 0;
+}
+
+extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t *b, int fmt, const float *scale,
+                               const int32_t *rank, const int32_t *start, const int32_t *adapter, uint32_t requests,
+                               uint32_t adapters, uint32_t rmax, const float *res, float *y, float *u, uint32_t seq,
+                               uint32_t out, uint32_t cols, void *workspace, size_t workspace_bytes, void *stream) {
+  const char *what = "lora linear";
+  if (!seq) return NLG_OK;
+  DownArgs d{};
+  if (lora_check(what, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, seq, out, cols, d.l)) return NLG_ERR;
+  if (!x || !y) return nlg_fail("%s: null pointer", what);
+  if (((uintptr_t)x | (uintptr_t)u) & 15) return nlg_fail("%s: x and u must be 16-byte aligned", what);
+  if (((uintptr_t)y | (uintptr_t)res) & 3) return nlg_fail("%s: y and res must be 4-byte aligned", what);
+  const size_t need = u ? 0 : nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
+  if (need && (!workspace || workspace_bytes < need))
+    return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
+  if (need && ((uintptr_t)workspace & 15)) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
+  const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nu = (uint64_t)seq * rmax * 4;
+  if (overlap(y, ny, x, nx) || overlap(u, nu, x, nx) || overlap(u, nu, y, ny) || (res != y && overlap(y, ny, res, ny)) ||
+      overlap(u, nu, res, ny))
+    return nlg_fail("%s: outputs overlap each other or an input (y may be res itself)", what);
+  NLG_SCOPE(what);
+  hipStream_t st = nlg_stream(stream);
+  d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
+  if (lora_down(what, d, fmt == NLG_LORA_BF16, false, st)) return NLG_ERR;
+  UpArgs p{};
+  p.l = d.l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
+  return lora_up(what, p, fmt == NLG_LORA_BF16, false, st);
+}
+
+extern "C" size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax,
+                                                    uint32_t requests) {
+  const size_t u = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
+  if (!u) return 0;
+  const size_t rows = nlg_ternary_linear_workspace(seq, cols), batched = nlg_batched_scratch_bytes(seq, cols);
+  return u + lora_round(rows > batched ? rows : batched);
+}
+
+extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const float *bias, const float *beta,
+                                       int beta_per_row, const uint16_t *a, const uint16_t *b, int fmt,
+                                       const float *scale, const int32_t *rank, const int32_t *start,
+                                       const int32_t *adapter, uint32_t requests, uint32_t adapters, uint32_t rmax,
+                                       float *y, float *u, uint32_t seq, uint32_t out, uint32_t cols, void *workspace,
+                                       size_t workspace_bytes, void *stream) {
+  const char *what = "ternary linear with adapters";
+  if (!seq) return NLG_OK;
+  LoraArgs l;
+  if (lora_check(what, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, seq, out, cols, l)) return NLG_ERR;
+  if (!x || !w2 || !beta || !y) return nlg_fail("%s: null pointer", what);
+  if (((uintptr_t)x | (uintptr_t)w2 | (uintptr_t)u) & 15) return nlg_fail("%s: x, w2 and u must be 16-byte aligned", what);
+  if (((uintptr_t)y | (uintptr_t)bias | (uintptr_t)beta) & 3)
+    return nlg_fail("%s: y, bias and beta must be 4-byte aligned", what);
+  if (cols > 16384) return nlg_fail("%s: cols must be at most 16384 (got %u)", what, cols);
+  const size_t nu = lora_round((size_t)seq * rmax * 4), need = nlg_ternary_linear_lora_workspace(seq, out, cols, rmax, requests);
+  if (!workspace || workspace_bytes < need)
+    return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
+  if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
+  const uint64_t bx = (uint64_t)seq * cols * 4, by = (uint64_t)seq * out * 4, bu = (uint64_t)seq * rmax * 4;
+  if (overlap(y, by, x, bx) || overlap(u, bu, x, bx) || overlap(u, bu, y, by))
+    return nlg_fail("%s: outputs overlap each other or x", what);
+  NLG_SCOPE(what);
+  hipStream_t st = nlg_stream(stream);
+  uint8_t *const more = (uint8_t *)workspace + nu;
+  if (nlg_batched(seq, cols)) {
+    float *const gamma = (float *)(more + ((size_t)seq * cols + 255) / 256 * 256);
+    if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st)) return NLG_ERR;
+    FusedArgs f{};
+    f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;
+    f.y = y; f.ystride = out;
+    if (nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st)) return NLG_ERR;
+  } else if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more,
+                                workspace_bytes - nu, (void *)st)) {
+    return NLG_ERR;
+  }
+  return nlg_lora_linear(x, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, y, y,
+                         u ? u : (float *)workspace, seq, out, cols, nullptr, 0, (void *)st);
+}
+
+extern "C" size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters,
+                                                 uint32_t rmax, uint32_t requests) {
+  (void)adapters;
+  (void)requests;
+  return lora_sizes(seq, out, cols, rmax) ? 2 * lora_round((size_t)seq * rmax * 4) : 0;
+}
+
+extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a,
+                                    const uint16_t *b, int fmt, const float *scale, const int32_t *rank,
+                                    const int32_t *start, const int32_t *adapter, uint32_t requests,
+                                    uint32_t adapters, uint32_t rmax, const float *dres, float *dx, float *da,
+                                    float *db, uint32_t seq, uint32_t out, uint32_t cols, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+  const char *what = "lora linear gradient";
+  if (!seq) return nlg_fail("%s: seq must be nonzero", what);
+  DownArgs d{};
+  if (lora_check(what, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, seq, out, cols, d.l)) return NLG_ERR;
+  if (!x || !dy || !da || !db) return nlg_fail("%s: null pointer", what);
+  if (((uintptr_t)x | (uintptr_t)u | (uintptr_t)da | (uintptr_t)db | (uintptr_t)dx | (uintptr_t)dres) & 15)
+    return nlg_fail("%s: x, u, dres, dx, da and db must be 16-byte aligned", what);
+  if ((uintptr_t)dy & 3) return nlg_fail("%s: dy must be 4-byte aligned", what);
+  const size_t nu = lora_round((size_t)seq * rmax * 4);
+  const size_t need = nlg_lora_linear_grad_workspace(seq, out, cols, adapters, rmax, requests);
+  if (!workspace || workspace_bytes < need)
+    return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
+  if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
+  // each output against the inputs and the outputs behind it
+  const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nr = (uint64_t)seq * rmax * 4;
+  const uint64_t na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out;
+  const struct { const void *p; uint64_t n; } in[] = {{x, nx}, {u, nr}, {dy, ny}, {a, 2 * na}, {b, 2 * nb},
+                                                      {dres == dx ? nullptr : dres, nx}, {dx, nx}, {da, 4 * na}, {db, 4 * nb}};
+  for (int o = 6; o < 9; o++)
+    for (int i = 0; i < 9; i++)
+      if (i < 6 || i > o)
+        if (overlap(in[o].p, in[o].n, in[i].p, in[i].n))
+          return nlg_fail("%s: outputs overlap each other or an input (dx may be dres itself)", what);
+  NLG_SCOPE(what);
+  hipStream_t st = nlg_stream(stream);
+  const bool bf = fmt == NLG_LORA_BF16;
+  float *const du = (float *)workspace;
+  if (!u) {
+    d.x = x; d.k = cols; d.scaled = false; d.u = (float *)((uint8_t *)workspace + nu);
+    u = d.u;
+    if (lora_down(what, d, bf, false, st)) return NLG_ERR;
+  }
+  d.x = dy; d.k = out; d.scaled = true; d.u = du;
+  if (lora_down(what, d, bf, true, st)) return NLG_ERR;
+  OuterArgs o{};
+  o.l = d.l;
+  o.p = u; o.q = dy; o.out = db; o.n = out; o.scaled = true;
+  if (lora_outer(what, o, true, st)) return NLG_ERR;
+  o.p = du; o.q = x; o.out = da; o.n = cols; o.scaled = false;
+  if (lora_outer(what, o, false, st)) return NLG_ERR;
+  if (!dx) return NLG_OK;
+  UpArgs p{};
+  p.l = d.l; p.u = du; p.res = dres; p.y = dx; p.n = cols; p.scaled = false;
+  return lora_up(what, p, bf, true, st);
+}

@@ -136,6 +136,14 @@ def lib() -> C.CDLL:
         "nlg_tree_attn_paged_q8_workspace": (sz, [u32, u32, u32, u32, u32, u32, u32]),
         "nlg_tree_commit_paged_q8": (i32, [vp, vp, vp, vp, vp, vp, u32, u32, u32, u32, u32, u32, u32, vp]),
         "nlg_cache_read_paged_q8": (i32, [vp, vp, i32, vp, vp, vp, u32, vp, vp, u32, u32, u32, u32, u32, u32, vp]),
+        "nlg_lora_linear": (i32, [vp, vp, vp, i32, vp, vp, vp, vp, u32, u32, u32, vp, vp, vp, u32, u32, u32, vp, sz, vp]),
+        "nlg_lora_linear_workspace": (sz, [u32, u32, u32, u32, u32]),
+        "nlg_ternary_linear_lora": (i32, [vp, vp, vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, u32, u32, u32, vp, vp, u32,
+                                          u32, u32, vp, sz, vp]),
+        "nlg_ternary_linear_lora_workspace": (sz, [u32, u32, u32, u32, u32]),
+        "nlg_lora_linear_grad": (i32, [vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, u32, u32, u32, vp, vp, vp, vp, u32, u32,
+                                       u32, vp, sz, vp]),
+        "nlg_lora_linear_grad_workspace": (sz, [u32, u32, u32, u32, u32, u32]),
         "nlg_ternary_xent": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, u32, u32, u32, vp, sz, vp]),
         "nlg_ternary_xent_workspace": (sz, [u32, u32, u32, i32]),
         "nlg_ternary_distill": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, u32, C.c_float, vp, vp, vp, vp, u32, u32, u32,
@@ -513,6 +521,47 @@ def cache_read_paged_q8(kpool, vpool, slot, table, npool, k, v, rows, batch, kvh
     _check(lib().nlg_cache_read_paged_q8(kpool.ptr, vpool.ptr, fmt, _ptr(seq), slot.ptr, table.ptr, npool, k.ptr,
                                          v.ptr, rows, batch, kvheads, head_dim, bs, mbps, stream),
            "cache_read_paged_q8")
+
+
+# The adapters' formats (NLG_LORA_* in nlgpu.h).
+LORA_F16, LORA_BF16 = 0, 1
+
+
+def lora_linear_workspace(seq, out, cols, rmax, requests) -> int:
+    return int(lib().nlg_lora_linear_workspace(seq, out, cols, rmax, requests))
+
+
+def lora_linear(x, a, b, scale, adapter, res, y, seq, out, cols, adapters, rmax, requests, workspace, start=None,
+                rank=None, u=None, fmt=LORA_F16, stream=None) -> None:
+    """y = res + each request's adapter's part (request i: rows start[i] .. start[i + 1] - 1, adapter[i])."""
+    _check(lib().nlg_lora_linear(x.ptr, a.ptr, b.ptr, fmt, scale.ptr, _ptr(rank), _ptr(start), adapter.ptr, requests,
+                                 adapters, rmax, _ptr(res), y.ptr, _ptr(u), seq, out, cols, _ptr(workspace),
+                                 workspace.nbytes if workspace is not None else 0, stream), "lora_linear")
+
+
+def ternary_linear_lora_workspace(seq, out, cols, rmax, requests) -> int:
+    return int(lib().nlg_ternary_linear_lora_workspace(seq, out, cols, rmax, requests))
+
+
+def ternary_linear_lora(x, w2, bias, beta, a, b, scale, adapter, y, seq, out, cols, adapters, rmax, requests, workspace,
+                        start=None, rank=None, u=None, fmt=LORA_F16, beta_per_row=False, stream=None) -> None:
+    """ternary_linear and each request's adapter's part beside it."""
+    _check(lib().nlg_ternary_linear_lora(x.ptr, w2.ptr, _ptr(bias), beta.ptr, int(beta_per_row), a.ptr, b.ptr, fmt,
+                                         scale.ptr, _ptr(rank), _ptr(start), adapter.ptr, requests, adapters, rmax,
+                                         y.ptr, _ptr(u), seq, out, cols, workspace.ptr, workspace.nbytes, stream),
+           "ternary_linear_lora")
+
+
+def lora_linear_grad_workspace(seq, out, cols, adapters, rmax, requests) -> int:
+    return int(lib().nlg_lora_linear_grad_workspace(seq, out, cols, adapters, rmax, requests))
+
+
+def lora_linear_grad(x, u, dy, a, b, scale, adapter, da, db, seq, out, cols, adapters, rmax, requests, workspace,
+                     dres=None, dx=None, start=None, rank=None, fmt=LORA_F16, stream=None) -> None:
+    """The gradients of lora_linear: da, db (every adapter's), and dx = dres + the adapters' part if it is given."""
+    _check(lib().nlg_lora_linear_grad(x.ptr, _ptr(u), dy.ptr, a.ptr, b.ptr, fmt, scale.ptr, _ptr(rank), _ptr(start),
+                                      adapter.ptr, requests, adapters, rmax, _ptr(dres), _ptr(dx), da.ptr, db.ptr, seq,
+                                      out, cols, workspace.ptr, workspace.nbytes, stream), "lora_linear_grad")
 
 
 def ternary_xent_workspace(rows, vocab, cols, grad) -> int:

@@ -1,0 +1,124 @@
+"""Low-rank adapters of many requests on the GPU against their form in 64 bits
+(lora_ref.py), within the bounds derived there."""
+import numpy as np
+import pytest
+
+import lora_ref as ref
+import nlgpu
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    nlgpu.init()
+    yield
+
+
+def up(a):
+    return nlgpu.to_device(a) if a is not None else None
+
+
+def close(got, want, name=""):
+    off = np.abs(got.astype(np.float64).reshape(want.value.shape) - want.value)
+    bad = off > want.off + 2.0 ** -140
+    assert not bad.any(), (name, np.argwhere(bad)[:3], off[bad][:3], want.off[bad][:3])
+
+
+class Case:
+    """Requests of the given lengths over rows that begin at `first`, each with its adapter."""
+
+    def __init__(self, lengths, adapter, adapters, rmax, out, cols, bf=False, mixed=False, first=0, behind=0, seed=0):
+        rng = np.random.default_rng([sum(lengths), adapters, rmax, out, cols, seed])
+        self.start = (first + np.concatenate([[0], np.cumsum(lengths)])).astype(np.int32)
+        self.seq, self.out, self.cols = int(self.start[-1]) + behind, out, cols
+        self.adapter = np.asarray(adapter, np.int32)
+        self.n, self.rmax, self.bf = adapters, rmax, bf
+        self.rank = (rng.integers(0, rmax + 1, adapters) if mixed else np.full(adapters, rmax)).astype(np.int32)
+        self.scale = rng.uniform(-2, 2, adapters).astype(F32)
+        self.a16, self.a = ref.to16(rng.standard_normal((adapters, rmax, cols)) * cols ** -0.5, bf)
+        self.b16, self.b = ref.to16(rng.standard_normal((adapters, out, rmax)) * 0.1, bf)
+        # what lies behind the ranks is not used: NaN
+        for k in range(adapters):
+            self.a16[k, self.rank[k]:] = 0x7fff
+            self.b16[k, :, self.rank[k]:] = 0x7fff
+        self.x = (rng.standard_normal((self.seq, cols)) * np.exp(rng.uniform(-3, 3, (self.seq, 1)))).astype(F32)
+        self.dy = (rng.standard_normal((self.seq, out)) * np.exp(rng.uniform(-3, 3, (self.seq, 1)))).astype(F32)
+        self.res = rng.standard_normal((self.seq, out)).astype(F32)
+        self.dres = rng.standard_normal((self.seq, cols)).astype(F32)
+        self.of = ref.owners(self.seq, self.start, self.adapter, adapters)
+        self.fmt = nlgpu.LORA_BF16 if bf else nlgpu.LORA_F16
+
+    def forward(self, res=True, inplace=False, keep=True, start=True, stream=None):
+        y = up(self.res if inplace else np.full((self.seq, self.out), np.nan, F32))
+        u = up(np.full((self.seq, self.rmax), np.nan, F32)) if keep else None
+        ws = nlgpu.DeviceArray(nlgpu.lora_linear_workspace(self.seq, self.out, self.cols, self.rmax, len(self.adapter)))
+        nlgpu.lora_linear(up(self.x), up(self.a16), up(self.b16), up(self.scale), up(self.adapter),
+                          y if inplace else up(self.res) if res else None, y, self.seq, self.out, self.cols, self.n,
+                          self.rmax, len(self.adapter), ws, start=up(self.start) if start else None, rank=up(self.rank),
+                          u=u, fmt=self.fmt, stream=stream)
+        nlgpu.sync(stream)
+        return y.download(F32), u.download(F32) if keep else None
+
+    def backward(self, u=None, dres=True, dx=True, inplace=False, stream=None):
+        da, db = (up(np.full(s, np.nan, F32)) for s in (self.a.shape, self.b.shape))
+        d = up(self.dres if inplace else np.full((self.seq, self.cols), np.nan, F32)) if dx else None
+        ws = nlgpu.DeviceArray(nlgpu.lora_linear_grad_workspace(self.seq, self.out, self.cols, self.n, self.rmax,
+                                                                len(self.adapter)))
+        nlgpu.lora_linear_grad(up(self.x), up(u), up(self.dy), up(self.a16), up(self.b16), up(self.scale),
+                               up(self.adapter), da, db, self.seq, self.out, self.cols, self.n, self.rmax,
+                               len(self.adapter), ws, dres=d if inplace else up(self.dres) if dres else None, dx=d,
+                               start=up(self.start), rank=up(self.rank), fmt=self.fmt, stream=stream)
+        nlgpu.sync(stream)
+        return d.download(F32) if dx else None, da.download(F32), db.download(F32)
+
+    def want(self, res=True):
+        return ref.forward(self.x.astype(float), self.a, self.b, self.scale.astype(float), self.rank, self.of,
+                           ref.Sums(self.res.astype(float)) if res else None)
+
+    def want_grad(self, u, dres=True):
+        return ref.backward(self.x.astype(float), u, self.dy.astype(float), self.a, self.b, self.scale.astype(float),
+                            self.rank, self.of, self.dres if dres else None)
+
+
+CASES = [dict(lengths=[1], adapter=[0], adapters=1, rmax=8, out=1, cols=8),
+         dict(lengths=[1] * 5, adapter=[2, 0, -1, 2, 7], adapters=3, rmax=16, out=257, cols=64, mixed=True),
+         dict(lengths=[1] * 70, adapter=[i % 9 for i in range(70)], adapters=9, rmax=64, out=300, cols=264, mixed=True),
+         dict(lengths=[17, 0, 40, 3, 1], adapter=[1, 0, 0, -5, 1], adapters=2, rmax=24, out=130, cols=200, first=3, behind=9),
+         dict(lengths=[100, 33], adapter=[0, 0], adapters=1, rmax=32, out=256, cols=512),
+         dict(lengths=[64, 64, 70], adapter=[3, 1, 3], adapters=5, rmax=128, out=72, cols=1000, mixed=True),
+         dict(lengths=[5, 6, 7], adapter=[0, 1, 2], adapters=3, rmax=40, out=333, cols=96, behind=40)]
+
+
+@pytest.mark.parametrize("bf", [False, True])
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_forward(i, bf):
+    c = Case(bf=bf, **CASES[i])
+    y, u = c.forward()
+    want, wu = c.want()
+    close(u, wu, "u")
+    close(y, want, "y")
+    assert np.array_equal(c.forward(inplace=True, keep=False)[0], y)  # y = res itself, u in the workspace
+    close(c.forward(res=False)[0], c.want(res=False)[0], "alone")
+
+
+@pytest.mark.parametrize("bf", [False, True])
+@pytest.mark.parametrize("i", range(len(CASES)))
+def test_backward(i, bf):
+    c = Case(bf=bf, **CASES[i])
+    u = c.want()[1]
+    given = u.value.astype(F32)
+    got = c.backward(u=given)
+    for g, w, n in zip(got, c.want_grad(ref.Sums(given.astype(float))), ("dx", "da", "db")):
+        close(g, w, n)
+    for k in range(c.n):  # behind the ranks, and where no row is
+        assert not got[1].reshape(c.a.shape)[k, c.rank[k]:].any() and not got[2].reshape(c.b.shape)[k, :, c.rank[k]:].any()
+        if not (c.of == k).any():
+            assert not got[1].reshape(c.a.shape)[k].any() and not got[2].reshape(c.b.shape)[k].any()
+    again = c.backward(u=given, inplace=True)
+    assert all(np.array_equal(x, y) for x, y in zip(again, got))
+    # u computed again, no dres, no dx
+    for g, w, n in zip(c.backward(dres=False), c.want_grad(u, dres=False), ("dx", "da", "db")):
+        close(g, w, n)
+    assert c.backward(u=given, dx=False)[0] is None
