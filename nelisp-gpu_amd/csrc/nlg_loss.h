@@ -15,22 +15,37 @@ struct LossPlan {
   bool ok;
   uint32_t tiles;          // tiles of the vocabulary
   uint32_t bm;             // rows of a workgroup of the gradient's product
-  uint32_t rows_pad;       // rows of a piece's probabilities
-  uint32_t piece;          // vocabulary rows of a piece (a multiple of LOSS_TILE)
-  uint32_t pieces;
-  uint32_t splits;         // parts of a piece that meet at the end, each with sums of its own
-  uint32_t share;          // vocabulary rows of such a part
+  uint32_t chunk, chunks;  // rows whose probabilities are held at a time (a multiple of bm)
+  uint32_t splits;         // parts of the vocabulary whose sums meet at the end
+  uint32_t share;          // vocabulary rows of a part (a multiple of LOSS_TILE)
   // offsets into the workspace (256-byte aligned) and its size
-  uint64_t xq, gamma, part, bmax, lse, sum, weight, prob, acc, bytes;
+  uint64_t xq, gamma, part, bmax, lse, sum, weight, order, prob, acc, bytes;
 };
 
 static inline uint64_t loss_round(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
-// rows x vocab logits over cols columns, top targets a row (0 refused sizes: ok false)
+// How many parts the gradient's product takes its `tiles` tiles of vocabulary in: those of the shortest time by a
+// measured 1 us for 32 vocabulary rows of a 256 x 256 tile (as many such tiles as CUs side by side, smaller ones in
+// proportion), 6 us to begin and end one, and 4 TB/s for what the parts leave and is read again.
+static inline uint32_t loss_splits(uint32_t tiles, uint32_t bm, uint64_t workgroups, uint64_t values) {
+  uint32_t best = 1;
+  double least = 0;
+  for (uint32_t n = 1; n <= 64 && n <= tiles; n++) {
+    const double rounds = (double)((workgroups * n + 255) / 256), share = (double)((tiles + n - 1) / n);
+    const double t = rounds * (share * 8 * bm / 256 + 6) + (double)n * (double)values * 8 / 4e6;
+    if (n == 1 || t < least) {
+      least = t;
+      best = n;
+    }
+  }
+  return best;
+}
+
+// rows x vocab logits over cols columns, top targets a row (refused sizes: ok false)
 static inline LossPlan loss_plan(uint32_t rows, uint32_t vocab, uint32_t cols, uint32_t top, bool grad) {
   LossPlan p = {};
-  if (!rows || !vocab || !cols || cols % 64 || cols > LOSS_COLS || !top || top > LOSS_TOP || rows > 0x1000000u ||
-      vocab > 0x40000000u)
+  if (!rows || !vocab || !cols || cols % 64 || cols > LOSS_COLS || !top || top > LOSS_TOP || rows > 0xffffffu ||
+      vocab > 0x1000000u)
     return p;
   p.tiles = (uint32_t)((vocab + (uint64_t)LOSS_TILE - 1) / LOSS_TILE);
   uint64_t at = 0;
@@ -47,24 +62,21 @@ static inline LossPlan loss_plan(uint32_t rows, uint32_t vocab, uint32_t cols, u
   p.sum = take((uint64_t)rows * 4);
   p.weight = take((uint64_t)rows * top * 4);
   if (grad) {
+    p.order = take(((uint64_t)rows + 1) * 4);
     p.bm = rows > 128 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : 32;
-    p.rows_pad = (uint32_t)loss_round(rows, p.bm);
-    // a piece's probabilities (two f16 each) are at most 128 MB where a piece of 2,048 rows of the vocabulary is: they are
-    // read back from the 256 MB MALL
-    uint64_t most = (128ull << 20) / (4ull * p.rows_pad) / LOSS_TILE * LOSS_TILE;
-    if (most < 2048) most = 2048;
-    p.pieces = (uint32_t)((vocab + most - 1) / most);
-    p.piece = (uint32_t)loss_round((vocab + p.pieces - 1) / p.pieces, LOSS_TILE);
-    p.pieces = (uint32_t)((vocab + (uint64_t)p.piece - 1) / p.piece);
-    // parts until every CU has a workgroup, of 256 vocabulary rows at least
-    const uint64_t tiles = (uint64_t)p.rows_pad / p.bm * ((cols + LOSS_CUT - 1) / LOSS_CUT);
-    uint64_t n = (256 + tiles - 1) / tiles;
-    const uint64_t most_parts = p.piece / LOSS_TILE;
-    if (n > most_parts) n = most_parts;
-    p.share = (uint32_t)loss_round((p.piece + n - 1) / n, LOSS_TILE);
-    p.splits = (uint32_t)((p.piece + (uint64_t)p.share - 1) / p.share);
-    p.prob = take((uint64_t)p.rows_pad * p.piece * 4);
-    p.acc = take((uint64_t)p.splits * rows * cols * 4);
+    // chunks of rows whose probabilities (two f16 each) are at most 512 MB, of 256 rows at least
+    const uint64_t row = 4ull * p.tiles * LOSS_TILE;
+    uint64_t most = (512ull << 20) / row / p.bm * p.bm;
+    if (most < p.bm) most = p.bm;
+    p.chunks = (uint32_t)((rows + most - 1) / most);
+    p.chunk = (uint32_t)loss_round((rows + (uint64_t)p.chunks - 1) / p.chunks, p.bm);
+    p.chunks = (uint32_t)((rows + (uint64_t)p.chunk - 1) / p.chunk);
+    const uint64_t workgroups = (uint64_t)(p.chunk / p.bm) * ((cols + LOSS_CUT - 1) / LOSS_CUT);
+    p.splits = loss_splits(p.tiles, p.bm, workgroups, (uint64_t)p.chunk * cols);
+    p.share = (p.tiles + p.splits - 1) / p.splits * LOSS_TILE;
+    p.splits = (uint32_t)(((uint64_t)p.tiles * LOSS_TILE + p.share - 1) / p.share);
+    p.prob = take(row * p.chunk);
+    p.acc = take((uint64_t)p.splits * p.chunk * cols * 4);
   }
   p.bytes = at;
   p.ok = true;

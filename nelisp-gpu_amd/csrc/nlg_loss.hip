@@ -16,11 +16,16 @@
 //    of each only every row's maximum and its sum of exponentials are kept.
 // 3. k_loss: a workgroup a row joins those, dots the row with its targets'
 //    weights, and leaves the loss.
-// Gradient, in pieces of the vocabulary whose probabilities fit the MALL:
-// 4. k_head<PROB>: the piece's logits again, as probabilities in two f16.
-// 5. k_back: their product with the piece's weights on the f16 matrix cores.
-// 6. k_dx: the parts' sums, less the targets' weights.
+// Gradient:
+// 4. k_order: the rows that have targets, ahead of those that have none.
+// and in chunks of those rows:
+// 5. k_head<PROB>: the chunk's logits again, as probabilities in two f16.
+// 6. k_back: their product with the weights on the f16 matrix cores, in
+//    parts of the vocabulary.
+// 7. k_dx: the parts' sums, less the targets' weights.
 #include <math.h>
+
+#include <type_traits>
 
 #include "nlg_loss.h"
 #include "nlg_quant.h"
@@ -54,17 +59,16 @@ struct HeadArgs {
   bool per_row;
   uint32_t rows, vocab, cols;
   float coef;           // log2(e) / tau
-  uint32_t vt0, vtiles; // tiles of this launch: vt0 .. vt0 + vtiles - 1
+  uint32_t tiles;       // of the vocabulary
   uint32_t ttiles, group; // token tiles, and of how many an XCD takes one vocabulary tile in a row
   // LOGSUM
   float2 *part;         // [rows][tiles]: the largest z2 = z coef, and the sum of 2^(z2 - it)
-  uint32_t tiles;
   float *bmax;          // [tiles]: the largest |beta|
   // PROB
   const float *lse;     // [rows], base 2
-  const float *sum;     // [rows]: T; rows of none need no probabilities
-  uint4 *prob;          // [piece / 8][2][rows_pad]: eight vocabulary rows of a row, rounded and left over
-  uint32_t rows_pad;
+  const int32_t *order; // [rows + 1] or null: the rows in order, then how many of them have targets
+  uint32_t first, chunk; // this chunk's
+  uint4 *prob;          // [tiles * 32][2][chunk]: eight vocabulary rows of a row, rounded and left over
 };
 
 // A maximum in which a NaN loses, so that it meets the sum and not the maximum.
@@ -109,21 +113,22 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
   // of the vocabulary, and of each tile up to sixteen token tiles in a row, so
   // that its L2 keeps those tokens and fetches each weight once for them.
   const uint32_t xcd = blockIdx.x % 8, j = blockIdx.x / 8;
-  const uint32_t mine = (a.vtiles + 7 - xcd) / 8;  // tiles of this XCD
-  const uint32_t group = a.group;
-  const uint32_t each = (a.vtiles + 7) / 8 * group, g0 = j / each, in = j % each;
-  const uint32_t here = min(group, a.ttiles - g0 * group);
-  const uint32_t vt = in / group, tt = in % group;
+  const uint32_t mine = (a.tiles + 7 - xcd) / 8;  // tiles of this XCD
+  const uint32_t each = (a.tiles + 7) / 8 * a.group, g0 = j / each, in = j % each;
+  const uint32_t here = min(a.group, a.ttiles - g0 * a.group);
+  const uint32_t vt = in / a.group, tt = in % a.group;
   if (vt >= mine || tt >= here) return;
-  const uint32_t vtile = a.vt0 + vt * 8 + xcd, tok0 = (g0 * group + tt) * MT;
+  const uint32_t vtile = vt * 8 + xcd, tok0 = (g0 * a.group + tt) * MT;
+  // tokens: of the call, or of the chunk and then by their order
+  const uint32_t count = MODE == PROB && a.order ? (uint32_t)a.order[a.rows] : a.rows;
+  const uint32_t first = MODE == PROB ? a.first : 0;
+  if (MODE == PROB && first + tok0 >= count) return;
+  const auto row_of = [&](uint32_t t) {
+    const uint32_t at = min(first + tok0 + t, count - 1);
+    return MODE == PROB && a.order ? (uint32_t)a.order[at] : at;
+  };
   const uint32_t vrow0 = vtile * LOSS_TILE, rbase = vrow0 + w * 64;
   const uint32_t steps = (a.cols + KC - 1) / KC, wng = a.cols / 16;
-  if (MODE == PROB) {
-    // tokens without targets have no gradient
-    const uint32_t tk = tok0 + lane;
-    const bool any = lane < MT && tk < a.rows && a.sum[tk] != 0.0f;
-    if (!__any(any)) return;
-  }
   uint32_t rc[NB];
   const uint4 *wp[NB];
 #pragma unroll
@@ -132,14 +137,16 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
     rc[nt] = r < a.vocab ? r : a.vocab - 1;
     wp[nt] = (const uint4 *)(a.w2 + (size_t)rc[nt] * wng) + 2 * lg;
   }
-  uint32_t xo[PI], xu[PI];
+  typename std::conditional<MODE == PROB, uint64_t, uint32_t>::type xo[PI];
+  uint32_t xu[PI];
 #pragma unroll
   for (int i = 0; i < PI; i++) {
-    const uint32_t k = 4 * (w * PI + i) + lane / 16, tk = tok0 + k < a.rows ? tok0 + k : a.rows - 1;
+    const uint32_t k = 4 * (w * PI + i) + lane / 16;
     xu[i] = 16 * ((lane % 16) ^ (k % 16));
-    xo[i] = (tk - tok0) * a.cols;
+    if (MODE == PROB) xo[i] = (uint64_t)row_of(k) * a.cols;
+    else xo[i] = (row_of(k) - tok0) * a.cols;
   }
-  const uint8_t *const xrow0 = a.xq + (size_t)tok0 * a.cols;
+  const uint8_t *const xrow0 = a.xq + (MODE == PROB ? 0 : (size_t)tok0 * a.cols);
   // (macros: register sets handed to a lambda end up in scratch)
 #define LOADW(c, dst)                                                                              \
   do {                                                                                             \
@@ -168,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
   const uint32_t vr = vrow0 + threadIdx.x;
   const float bo = a.bias && vr < a.vocab ? a.bias[vr] : 0.0f;
   const float be = a.beta[a.per_row ? min(vr, a.vocab - 1) : 0];
-  const uint32_t tkc = min(tok0 + threadIdx.x % MT, a.rows - 1);
+  const uint32_t tkc = row_of(threadIdx.x % MT);
   const float gm = a.gamma[tkc];
   const float ref = MODE == PROB ? a.lse[tkc] : 0.0f;
   wvec wA, wB, wC;
@@ -303,7 +310,7 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
 #pragma unroll
     for (int mt = 0; mt < MB; mt++) {
       const float g = s_gm[32 * mt + li] * c64, ls = s_ref[32 * mt + li];
-      const uint32_t tk = tok0 + 32 * mt + li;
+      const uint32_t tk = tok0 + 32 * mt + li;  // of the chunk
 #pragma unroll
       for (int nt = 0; nt < NB; nt++) {
 #pragma unroll
@@ -325,11 +332,11 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
             hi.h[e >> 1][e & 1] = h;
             lo.h[e >> 1][e & 1] = (_Float16)(p - (float)h);
           }
-          const uint32_t kg = ((vt * 8 + xcd) * LOSS_TILE + w * 64 + 32 * nt + 16 * b) / 8 + lg;
-          if (tk < a.rows_pad) {
-            uint4 *o = a.prob + (size_t)kg * 2 * a.rows_pad + tk;
+          const uint32_t kg = (vrow0 + w * 64 + 32 * nt + 16 * b) / 8 + lg;
+          if (tk < a.chunk) {
+            uint4 *o = a.prob + (size_t)kg * 2 * a.chunk + tk;
             o[0] = hi.u;
-            o[a.rows_pad] = lo.u;
+            o[a.chunk] = lo.u;
           }
         }
       }
@@ -367,21 +374,33 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
   const uint32_t wng = a.cols / 16;
   const uint4 *xr = (const uint4 *)(a.xq + (size_t)s * a.cols);
   const float gm = a.gamma[s];
-  for (uint32_t k = w; k < a.top; k += 4) {
-    const int32_t at = a.index[(size_t)s * a.top + k];
-    if (at < 0 || (uint32_t)at >= a.vocab) {
-      if (lane == 0) s_z[k] = 0.0f;
-      continue;
+  // four targets at a time a wave: their weights are on the way together
+  for (uint32_t k0 = 4 * w; k0 < a.top; k0 += 16) {
+    int32_t at[4];
+    const uint32_t *wr[4];
+    int q[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      at[e] = a.index[(size_t)s * a.top + min(k0 + e, a.top - 1)];
+      if (at[e] < 0 || (uint32_t)at[e] >= a.vocab) at[e] = 0;  // (has no part)
+      wr[e] = a.w2 + (size_t)at[e] * wng;
+      q[e] = 0;
     }
-    const uint32_t *wr = a.w2 + (size_t)at * wng;
-    int q = 0;
     for (uint32_t i = lane; i < wng; i += 64) {
       const uint4 y = xr[i];
-      q = wdot(wr[i], y.x, y.y, y.z, y.w, q);
+      uint32_t v[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = wr[e][i];
+#pragma unroll
+      for (int e = 0; e < 4; e++) q[e] = wdot(v[e], y.x, y.y, y.z, y.w, q[e]);
     }
-    q = nlg_wave_sum_i32(q);
-    const float b = a.bias ? a.bias[at] * a.coef : 0.0f;
-    if (lane == 0) s_z[k] = fmaf(a.beta[a.per_row ? at : 0] * (gm * (a.coef * 0.015625f)), (float)q, b);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int sum = nlg_wave_sum_i32(q[e]);
+      const float b = a.bias ? a.bias[at[e]] * a.coef : 0.0f;
+      if (lane == 0 && k0 + e < a.top)
+        s_z[k0 + e] = fmaf(a.beta[a.per_row ? at[e] : 0] * (gm * (a.coef * 0.015625f)), (float)sum, b);
+    }
   }
   // the tiles' parts
   float m = -INFINITY, l = 0.0f;
@@ -445,16 +464,42 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
   }
 }
 
+// The rows with targets in order, then those without; order[rows]: how many have.
+__global__ __launch_bounds__(1024) void k_order(const float *sum, int32_t *order, uint32_t rows) {
+  __shared__ uint32_t s_n[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  uint32_t have = 0;
+  for (int pass = 0; pass < 2; pass++) {
+    uint32_t at = pass ? have : 0;  // where the next rows of this pass go
+    for (uint32_t r0 = 0; r0 < rows; r0 += 1024) {
+      const uint32_t r = r0 + threadIdx.x;
+      const bool put = r < rows && (sum[r] != 0.0f) == (pass == 0);  // (a NaN has targets)
+      const uint64_t b = __ballot(put);
+      if (lane == 0) s_n[w] = __popcll(b);
+      __syncthreads();
+      uint32_t before = 0, all = 0;
+      for (int k = 0; k < 16; k++) {
+        if (k < w) before += s_n[k];
+        all += s_n[k];
+      }
+      if (put) order[at + before + __popcll(b & ((1ull << lane) - 1))] = (int32_t)r;
+      at += all;
+      __syncthreads();
+    }
+    if (!pass) have = at;
+  }
+  if (threadIdx.x == 0) order[rows] = (int32_t)have;
+}
+
 // ------------------------------------------------------------------ the gradient's product
 
 struct BackArgs {
-  const uint4 *prob;    // [piece / 8][2][rows_pad]
+  const uint4 *prob;    // [tiles * 32][2][chunk]
   const uint32_t *w2;   // [vocab][wng]
-  const float *sum;     // [rows]
-  float *acc;           // [splits][rows][cols]
-  uint32_t rows, rows_pad, cols, wng, vocab;
-  uint32_t v0, count, share, splits;  // the piece's first row, its rows (rounded up to 256), a part's
-  bool more;            // add to what an earlier piece left
+  const int32_t *order; // [rows + 1] or null
+  float *acc;           // [splits][chunk][cols]
+  uint32_t rows, first, chunk, cols, wng, vocab;
+  uint32_t count, share, splits;  // vocabulary rows (rounded up to 256), a part's
 };
 
 // 16 x 16 two-bit fields, words by rows, turned: field r of word f was field f of word r.
@@ -488,19 +533,22 @@ __device__ __forceinline__ void turn16(uint32_t (&w)[16]) {
     }
 }
 
-// Sums over a part of the piece's vocabulary rows of p W, for BM = 32 TM WM
-// rows x 256 columns a workgroup of 4 waves (WM x 4 / WM of them), in 32 x 32 x
-// 16 f16 products of the probabilities' two halves.  The weights are turned on
-// the way: a thread loads sixteen rows' words of sixteen columns, turns the 16
-// x 16 fields in registers and leaves a word a column in LDS, 256 vocabulary
-// rows at a time; a lane makes f16 of its eight fields with one byte
-// permutation a pair (the high byte of 0, +1, -2, -1).  Probabilities go from
-// memory to LDS directly, 32 vocabulary rows at a time, two stages.
-template <int WM, int TM>
-__global__ __launch_bounds__(256) void k_back(BackArgs a) {
-  constexpr int WN = 4 / WM, TN = 8 / WN, BM = 32 * TM * WM;
-  constexpr int STAGE = 4 * 2 * BM;  // 16-byte units of 32 vocabulary rows
-  constexpr int PI = STAGE / 64 / 4; // loads per wave and stage
+// Sums over a part of the vocabulary of p W, for BM = 32 TM WM rows x 256
+// columns a workgroup of 8 waves (WM x WN of them, each TM x TN blocks), in 32
+// x 32 x 16 f16 products of the probabilities' two halves.  The weights are
+// turned on the way: a thread loads sixteen rows' words of sixteen columns,
+// turns the 16 x 16 fields in registers and leaves a word a column in LDS, 256
+// vocabulary rows at a time (waves 0..3 the even ones, 4..7 the odd ones); a
+// lane makes f16 of its eight fields with one byte permutation a pair (the
+// high byte of 0, +1, -2, -1).  Probabilities go from memory to LDS directly,
+// 32 vocabulary rows at a time, two stages, the second loaded while the first
+// is multiplied.
+template <int WM, int TM, int TN>
+__global__ __launch_bounds__(512) void k_back(BackArgs a) {
+  constexpr int WN = 8 / WM, BM = 32 * TM * WM;
+  static_assert(WN * TN == 8, "256 columns");
+  constexpr int STAGE = 4 * 2 * BM;                        // 16-byte units of 32 vocabulary rows
+  constexpr int NL = STAGE / 64, PI = NL < 8 ? 1 : NL / 8; // loads a stage, a wave's
   __shared__ __align__(1024) uint4 s_p0[STAGE];
   __shared__ __align__(1024) uint4 s_p1[STAGE];
   __shared__ uint32_t s_w[2][16][256];
@@ -509,41 +557,37 @@ __global__ __launch_bounds__(256) void k_back(BackArgs a) {
   const int li = lane & 31, lg = lane >> 5;
   const int wm = w % WM, wn = w / WM;
   // the column tiles of one part and row tile on one XCD, in a row: its L2 then fetches the probabilities once
-  const uint32_t ncol = (a.cols + LOSS_CUT - 1) / LOSS_CUT, nrow = a.rows_pad / BM;
+  const uint32_t ncol = (a.cols + LOSS_CUT - 1) / LOSS_CUT, nrow = a.chunk / BM;
   const uint32_t xcd = blockIdx.x % 8, j = blockIdx.x / 8;
   const uint32_t pair = j / ncol * 8 + xcd, ct = j % ncol;
   if (pair >= nrow * a.splits) return;
-  const uint32_t rt = pair % nrow, part = pair / nrow;
-  const uint32_t row0 = rt * BM;
-  {
-    bool any = false;
-    for (uint32_t i = row0 + lane; i < row0 + BM && i < a.rows; i += 64) any |= a.sum[i] != 0.0f;
-    if (!__any(any)) return;
-  }
+  const uint32_t rt = pair % nrow, part = pair / nrow, row0 = rt * BM;
+  const uint32_t have = a.order ? (uint32_t)a.order[a.rows] : a.rows;
+  if (a.first + row0 >= have) return;
   const uint32_t k0 = part * a.share;
-  if (k0 >= a.count) return;
   const uint32_t chunks = min(a.share, a.count - k0) / 256, steps = chunks * 8;
-  // thread: words column wi of the tile, rows 16 wr .. 16 wr + 15 of a chunk
-  const uint32_t wi = threadIdx.x & 15, wr = threadIdx.x >> 4;
+  // thread: words column wi of the tile, rows 16 wr .. 16 wr + 15 of a 256-row block, the even or the odd ones
+  const uint32_t wi = threadIdx.x & 15, wr = threadIdx.x >> 4 & 15, odd = w / 4;
   const uint32_t wcol = min(ct * 16 + wi, a.wng - 1);
-  const auto loadw = [&](uint32_t chunk, uint32_t (&v)[16]) {
-    const uint32_t r0 = a.v0 + k0 + chunk * 256 + wr * 16;
+  uint32_t wv[16];
+  const auto loadw = [&](uint32_t block) {
+    const uint32_t r0 = k0 + block * 256 + wr * 16;
 #pragma unroll
-    for (int i = 0; i < 16; i++) v[i] = a.w2[(size_t)min(r0 + i, a.vocab - 1) * a.wng + wcol];
+    for (int i = 0; i < 16; i++) wv[i] = a.w2[(size_t)min(r0 + i, a.vocab - 1) * a.wng + wcol];
   };
-  const auto storew = [&](uint32_t buf, uint32_t (&v)[16]) {
-    turn16(v);
-    // columns 16 wi + f: four words at a time
+  const auto storew = [&] {
+    turn16(wv);
 #pragma unroll
     for (int q = 0; q < 4; q++)
-      *(uint4 *)&s_w[buf][wr][16 * wi + 4 * q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      *(uint4 *)&s_w[odd][wr][16 * wi + 4 * q] = make_uint4(wv[4 * q], wv[4 * q + 1], wv[4 * q + 2], wv[4 * q + 3]);
   };
-  const uint4 *const p0 = a.prob + (size_t)(k0 / 8) * 2 * a.rows_pad + row0;
+  const uint4 *const p0 = a.prob + (size_t)(k0 / 8) * 2 * a.chunk + row0;
   const auto loadp = [&](uint32_t step, uint4 *stage) {
+    if (NL < 8 && w >= NL) return;
 #pragma unroll
     for (int i = 0; i < PI; i++) {
       const uint32_t u = (w * PI + i) * 64, plane = (u + lane) / BM, r = (u + lane) % BM;
-      __builtin_amdgcn_global_load_lds((const void *)(p0 + ((size_t)step * 8 + plane) * a.rows_pad + r),
+      __builtin_amdgcn_global_load_lds((const void *)(p0 + ((size_t)step * 8 + plane) * a.chunk + r),
                                        (__attribute__((address_space(3))) void *)(stage + u), 16, 0, 0);
     }
   };
@@ -554,55 +598,63 @@ __global__ __launch_bounds__(256) void k_back(BackArgs a) {
     for (int n = 0; n < TN; n++) acc[m][n] = (v16f){};
   const auto mma = [&](uint32_t step, const uint4 *stage) {
     const uint32_t buf = step / 8 % 2, g = step % 8 * 2;
+    half8v p[2][TM][2];
+    uint32_t t[2][TN];
+    const auto read = [&](int h) {
+#pragma unroll
+      for (int n = 0; n < TN; n++) t[h][n] = s_w[buf][g + h][(wn * TN + n) * 32 + li];
+#pragma unroll
+      for (int m = 0; m < TM; m++)
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+          p[h][m][q] = __builtin_bit_cast(half8v, stage[((2 * h + lg) * 2 + q) * BM + (wm * TM + m) * 32 + li]);
+    };
+    read(0);
 #pragma unroll
     for (int h = 0; h < 2; h++) {  // sixteen vocabulary rows
-      half8v b[TN];
+      if (h == 0) read(1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < TN; n++) {
-        const uint32_t t = s_w[buf][g + h][(wn * TN + n) * 32 + li] >> (8 * lg);
+        const uint32_t f = t[h][n] >> (8 * lg);
         union {
           uint32_t u[4];
           half8v h;
-        } o;
+        } b;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-          o.u[e] = __builtin_amdgcn_perm(0u, 0xBCC03C00u, ((t << (8 - 2 * e)) & 0x03000300u) | 0x000c000cu);
-        b[n] = o.h;
-      }
+          b.u[e] = __builtin_amdgcn_perm(0u, 0xBCC03C00u, ((f << (8 - 2 * e)) & 0x03000300u) | 0x000c000cu);
 #pragma unroll
-      for (int m = 0; m < TM; m++) {
-        const int r = (wm * TM + m) * 32 + li;
-        union {
-          uint4 u;
-          half8v h;
-        } hi, lo;
-        hi.u = stage[((2 * h + lg) * 2 + 0) * BM + r];
-        lo.u = stage[((2 * h + lg) * 2 + 1) * BM + r];
+        for (int m = 0; m < TM; m++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[h][m][0], b.h, acc[m][n], 0, 0, 0);
 #pragma unroll
-        for (int n = 0; n < TN; n++) {
-          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi.h, b[n], acc[m][n], 0, 0, 0);
-          acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo.h, b[n], acc[m][n], 0, 0, 0);
-        }
+        for (int m = 0; m < TM; m++) acc[m][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(p[h][m][1], b.h, acc[m][n], 0, 0, 0);
       }
     }
   };
-  uint32_t wv[16];
-  loadw(0, wv);
-  loadp(0, s_p0);
-  storew(0, wv);
+  // the first two blocks' weights, each by its half of the waves
+  if (odd < chunks) {
+    loadw(odd);
+    loadp(0, s_p0);
+    storew();
+  } else {
+    loadp(0, s_p0);
+  }
   for (uint32_t s = 0; s < steps; s += 2) {
     WAIT_VM(0);
     __builtin_amdgcn_s_barrier();
     ORDER();
     loadp(s + 1, s_p1);
-    if (s % 8 == 0 && s + 8 < steps) loadw(s / 8 + 1, wv);
+    // while one block is multiplied, the half whose block is done loads its next one
+    const uint32_t block = s / 8, next = block + 1;
+    const bool turn = block > 0 && next < chunks && next % 2 == odd;
+    if (turn && s % 8 == 0) loadw(next);
     mma(s, s_p0);
     ORDER();
     WAIT_VM(0);
     __builtin_amdgcn_s_barrier();
     ORDER();
     if (s + 2 < steps) loadp(s + 2, s_p0);
-    if (s % 8 == 6 && s + 2 < steps) storew((s + 2) / 8 % 2, wv);
+    if (turn && s % 8 == 6) storew();
     mma(s + 1, s_p1);
     ORDER();
   }
@@ -612,60 +664,84 @@ __global__ __launch_bounds__(256) void k_back(BackArgs a) {
 #pragma unroll
     for (int n = 0; n < TN; n++) {
       const uint32_t col = ct * LOSS_CUT + (wn * TN + n) * 32 + li;
+      if (col >= a.cols) continue;
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const uint32_t row = row0 + (wm * TM + m) * 32 + (r % 4) + 8 * (r / 4) + 4 * lg;
-        if (row < a.rows && col < a.cols) {
-          float *o = a.acc + ((size_t)part * a.rows + row) * a.cols + col;
-          *o = a.more ? *o + acc[m][n][r] : acc[m][n][r];
-        }
+        a.acc[((size_t)part * a.chunk + row) * a.cols + col] = acc[m][n][r];
       }
     }
 }
 
 struct DxArgs {
-  const float *acc;      // [splits][rows][cols]
+  const float *acc;      // [splits][chunk][cols]
   const uint32_t *w2;
   const float *beta, *bmax, *sum, *weight, *dloss;
-  const int32_t *index;
+  const int32_t *index, *order;
   float *dx;
-  uint32_t rows, cols, wng, top, splits, vocab;
+  uint32_t first, chunk, cols, wng, top, splits;
   float itau;
   bool per_row;
 };
 
-// dx of a row: four columns a thread (a byte of the targets' words).
+// dx of 1,024 columns of a row: four a thread (a byte of the targets' words),
+// eight targets' loads and eight parts' at a time.
 __global__ __launch_bounds__(256) void k_dx(DxArgs a) {
-  const uint32_t s = blockIdx.x;
+  __shared__ float s_f[LOSS_TOP];
+  __shared__ uint32_t s_at[LOSS_TOP];
+  const uint32_t i = blockIdx.x, s = a.order ? (uint32_t)a.order[a.first + i] : a.first + i;
+  const uint32_t c = blockIdx.y * 256 + threadIdx.x, n4 = a.cols / 4;
   const float T = a.sum[s];
-  const float scale = (a.dloss ? a.dloss[s] : 1.0f) * a.itau;
-  float4 *o = (float4 *)(a.dx + (size_t)s * a.cols);
-  const float one = a.per_row ? 1.0f : a.beta[0];
-  const float tp = T / (PROB_SCALE * (a.per_row ? a.bmax[0] : 1.0f));
-  for (uint32_t c = threadIdx.x; c < a.cols / 4; c += 256) {
-    float4 v = make_float4(0, 0, 0, 0);
-    if (T != 0.0f) {
-      for (uint32_t i = 0; i < a.splits; i++) {
-        const float4 p = ((const float4 *)(a.acc + ((size_t)i * a.rows + s) * a.cols))[c];
-        v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
-      }
-      v.x *= tp; v.y *= tp; v.z *= tp; v.w *= tp;
-      for (uint32_t k = 0; k < a.top; k++) {
-        const float t = a.weight[(size_t)s * a.top + k];
-        if (t == 0.0f) continue;
-        const uint32_t at = (uint32_t)a.index[(size_t)s * a.top + k];
-        const float f = t * (a.per_row ? a.beta[at] : 1.0f);
-        const int b = ((const uint8_t *)(a.w2 + (size_t)at * a.wng))[c];
-        v.x = fmaf(-f, (float)((b << 30) >> 30), v.x);
-        v.y = fmaf(-f, (float)((b << 28) >> 30), v.y);
-        v.z = fmaf(-f, (float)((b << 26) >> 30), v.z);
-        v.w = fmaf(-f, (float)((b << 24) >> 30), v.w);
-      }
-      const float g = scale * one;
-      v.x *= g; v.y *= g; v.z *= g; v.w *= g;
-    }
-    o[c] = v;
+  float4 *const o = (float4 *)(a.dx + (size_t)s * a.cols);
+  if (T == 0.0f) {
+    if (c < n4) o[c] = make_float4(0, 0, 0, 0);
+    return;
   }
+  const uint32_t top8 = (a.top + 7) / 8 * 8;
+  for (uint32_t k = threadIdx.x; k < top8; k += 256) {
+    const float t = k < a.top ? a.weight[(size_t)s * a.top + k] : 0.0f;
+    const uint32_t at = t != 0.0f ? (uint32_t)a.index[(size_t)s * a.top + k] : 0u;  // (an index out of range has no weight)
+    s_at[k] = at;
+    s_f[k] = t * (a.per_row ? a.beta[at] : 1.0f);
+  }
+  __syncthreads();
+  if (c >= n4) return;
+  const float tp = T / (PROB_SCALE * (a.per_row ? a.bmax[0] : 1.0f));
+  const float4 *p = (const float4 *)(a.acc + (size_t)i * a.cols) + c;
+  const size_t stride = (size_t)a.chunk * n4;
+  float4 v = make_float4(0, 0, 0, 0);
+  uint32_t q = 0;
+  for (; q + 8 <= a.splits; q += 8, p += 8 * stride) {
+    float4 f[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) f[k] = p[k * stride];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      v.x += f[k].x; v.y += f[k].y; v.z += f[k].z; v.w += f[k].w;
+    }
+  }
+  for (; q < a.splits; q++, p += stride) {
+    const float4 f = *p;
+    v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+  }
+  v.x *= tp; v.y *= tp; v.z *= tp; v.w *= tp;
+  const uint8_t *const w = (const uint8_t *)a.w2 + c;
+  for (uint32_t k0 = 0; k0 < top8; k0 += 8) {
+    int b[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) b[k] = w[(size_t)s_at[k0 + k] * (a.wng * 4)];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const float f = s_f[k0 + k];
+      v.x = fmaf(-f, (float)((b[k] << 30) >> 30), v.x);
+      v.y = fmaf(-f, (float)((b[k] << 28) >> 30), v.y);
+      v.z = fmaf(-f, (float)((b[k] << 26) >> 30), v.z);
+      v.w = fmaf(-f, (float)((b[k] << 24) >> 30), v.w);
+    }
+  }
+  const float g = (a.dloss ? a.dloss[s] : 1.0f) * a.itau * (a.per_row ? 1.0f : a.beta[0]);
+  v.x *= g; v.y *= g; v.z *= g; v.w *= g;
+  o[c] = v;
 }
 
 // ------------------------------------------------------------------ host side
@@ -676,11 +752,11 @@ static bool loss_words(P... p) {
 }
 
 template <int MODE>
-static void head_go(HeadArgs &h, hipStream_t st) {
-  const bool wide = h.rows > 32, tail = h.cols % KC != 0;
-  h.ttiles = (h.rows + (wide ? 63 : 31)) / (wide ? 64 : 32);
+static void head_go(HeadArgs &h, uint32_t tokens, hipStream_t st) {
+  const bool wide = tokens > 32, tail = h.cols % KC != 0;
+  h.ttiles = (tokens + (wide ? 63 : 31)) / (wide ? 64 : 32);
   h.group = h.ttiles < 16 ? h.ttiles : 16;
-  const dim3 grid((uint32_t)((uint64_t)((h.ttiles + h.group - 1) / h.group) * h.group * ((h.vtiles + 7) / 8) * 8));
+  const dim3 grid((uint32_t)((uint64_t)((h.ttiles + h.group - 1) / h.group) * h.group * ((h.tiles + 7) / 8) * 8));
   if (wide && tail) hipLaunchKernelGGL((k_head<MODE, 2, true>), grid, dim3(256), 0, st, h);
   else if (wide) hipLaunchKernelGGL((k_head<MODE, 2, false>), grid, dim3(256), 0, st, h);
   else if (tail) hipLaunchKernelGGL((k_head<MODE, 1, true>), grid, dim3(256), 0, st, h);
@@ -720,9 +796,8 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
   h.xq = xq; h.gamma = gamma; h.w2 = w2; h.bias = bias; h.beta = beta; h.per_row = beta_per_row != 0;
   h.rows = rows; h.vocab = vocab; h.cols = cols; h.coef = NLG_LOG2E / tau;
   h.part = (float2 *)(ws + p.part); h.tiles = p.tiles; h.bmax = (float *)(ws + p.bmax);
-  h.lse = (float *)(ws + p.lse); h.sum = (float *)(ws + p.sum); h.prob = (uint4 *)(ws + p.prob); h.rows_pad = p.rows_pad;
-  h.vt0 = 0; h.vtiles = p.tiles;
-  head_go<LOGSUM>(h, st);
+  h.lse = (float *)(ws + p.lse); h.prob = (uint4 *)(ws + p.prob); h.chunk = p.chunk;
+  head_go<LOGSUM>(h, rows, st);
   NLG_LAUNCHED(what);
   LossArgs l{};
   l.xq = xq; l.gamma = gamma; l.w2 = w2; l.bias = bias; l.beta = beta; l.per_row = h.per_row;
@@ -733,29 +808,35 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
   hipLaunchKernelGGL(k_loss, dim3(rows), dim3(256), 0, st, l);
   NLG_LAUNCHED(what);
   if (!dx) return NLG_OK;
-  BackArgs b{};
-  b.prob = h.prob; b.w2 = w2; b.sum = l.sum; b.acc = (float *)(ws + p.acc); b.rows = rows; b.rows_pad = p.rows_pad;
-  b.cols = cols; b.wng = cols / 16; b.vocab = vocab; b.share = p.share; b.splits = p.splits;
-  for (uint32_t i = 0; i < p.pieces; i++) {
-    h.vt0 = i * (p.piece / LOSS_TILE);
-    h.vtiles = p.tiles - h.vt0 < p.piece / LOSS_TILE ? p.tiles - h.vt0 : p.piece / LOSS_TILE;
-    head_go<PROB>(h, st);
-    NLG_LAUNCHED(what);
-    b.v0 = h.vt0 * LOSS_TILE; b.count = h.vtiles * LOSS_TILE; b.more = i > 0;
-    const uint32_t ncol = (cols + LOSS_CUT - 1) / LOSS_CUT, pairs = p.rows_pad / p.bm * p.splits;
-    const dim3 grid((pairs + 7) / 8 * 8 * ncol);
-    if (p.bm == 256) hipLaunchKernelGGL((k_back<2, 4>), grid, dim3(256), 0, st, b);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_back<2, 2>), grid, dim3(256), 0, st, b);
-    else if (p.bm == 64) hipLaunchKernelGGL((k_back<1, 2>), grid, dim3(256), 0, st, b);
-    else hipLaunchKernelGGL((k_back<1, 1>), grid, dim3(256), 0, st, b);
+  // one tile of rows needs no order
+  int32_t *const order = rows > p.bm ? (int32_t *)(ws + p.order) : nullptr;
+  if (order) {
+    hipLaunchKernelGGL(k_order, dim3(1), dim3(1024), 0, st, l.sum, order, rows);
     NLG_LAUNCHED(what);
   }
+  h.order = order;
+  BackArgs b{};
+  b.prob = h.prob; b.w2 = w2; b.order = order; b.acc = (float *)(ws + p.acc); b.rows = rows; b.chunk = p.chunk;
+  b.cols = cols; b.wng = cols / 16; b.vocab = vocab; b.count = p.tiles * LOSS_TILE; b.share = p.share; b.splits = p.splits;
   DxArgs d{};
   d.acc = b.acc; d.w2 = w2; d.beta = beta; d.bmax = h.bmax; d.sum = l.sum; d.weight = l.weight; d.dloss = dloss;
-  d.index = index; d.dx = dx; d.rows = rows; d.cols = cols; d.wng = cols / 16; d.top = top; d.splits = p.splits;
-  d.vocab = vocab; d.itau = 1.0f / tau; d.per_row = h.per_row;
-  hipLaunchKernelGGL(k_dx, dim3(rows), dim3(256), 0, st, d);
-  NLG_LAUNCHED(what);
+  d.index = index; d.order = order; d.dx = dx; d.chunk = p.chunk; d.cols = cols; d.wng = cols / 16; d.top = top;
+  d.splits = p.splits; d.itau = 1.0f / tau; d.per_row = h.per_row;
+  for (uint32_t i = 0; i < p.chunks; i++) {
+    h.first = b.first = d.first = i * p.chunk;
+    const uint32_t n = rows - h.first < p.chunk ? rows - h.first : p.chunk;
+    head_go<PROB>(h, n, st);
+    NLG_LAUNCHED(what);
+    const uint32_t ncol = (cols + LOSS_CUT - 1) / LOSS_CUT, pairs = p.chunk / p.bm * p.splits;
+    const dim3 grid((pairs + 7) / 8 * 8 * ncol), blk(512);
+    if (p.bm == 256) hipLaunchKernelGGL((k_back<2, 4, 2>), grid, blk, 0, st, b);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_back<2, 2, 2>), grid, blk, 0, st, b);
+    else if (p.bm == 64) hipLaunchKernelGGL((k_back<2, 1, 2>), grid, blk, 0, st, b);
+    else hipLaunchKernelGGL((k_back<1, 1, 1>), grid, blk, 0, st, b);
+    NLG_LAUNCHED(what);
+    hipLaunchKernelGGL(k_dx, dim3(n, (cols + 1023) / 1024), dim3(256), 0, st, d);
+    NLG_LAUNCHED(what);
+  }
   return NLG_OK;
 }
 

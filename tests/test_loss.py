@@ -25,22 +25,20 @@ static int one(uint32_t rows, uint32_t vocab, uint32_t cols, uint32_t top, bool 
   const LossPlan p = loss_plan(rows, vocab, cols, top, grad);
   CHECK(p.ok && (uint64_t)p.tiles * LOSS_TILE >= vocab && (uint64_t)(p.tiles - 1) * LOSS_TILE < vocab);
   // regions in order, each as long as what it holds, 256-byte aligned
-  uint64_t at[10] = {p.xq, p.gamma, p.part, p.bmax, p.lse, p.sum, p.weight, p.bytes, 0, 0};
-  uint64_t len[10] = {(uint64_t)rows * cols, 4ull * rows, 8ull * rows * p.tiles, 4ull * p.tiles, 4ull * rows, 4ull * rows,
-                      4ull * rows * top, 0, 0, 0};
+  uint64_t at[11] = {p.xq, p.gamma, p.part, p.bmax, p.lse, p.sum, p.weight, p.bytes};
+  uint64_t len[11] = {(uint64_t)rows * cols, 4ull * rows, 8ull * rows * p.tiles, 4ull * p.tiles, 4ull * rows, 4ull * rows,
+                      4ull * rows * top};
   int n = 7;
   if (grad) {
-    CHECK(p.rows_pad >= rows && p.rows_pad % p.bm == 0 && p.rows_pad - rows < p.bm);
-    CHECK(p.piece % LOSS_TILE == 0 && p.piece >= LOSS_TILE);
-    CHECK((uint64_t)p.pieces * p.piece >= vocab && (uint64_t)(p.pieces - 1) * p.piece < vocab);
-    CHECK(p.share % LOSS_TILE == 0 && (uint64_t)p.share * p.splits >= p.piece && (uint64_t)p.share * (p.splits - 1) < p.piece);
-    // every part of the last piece has rows in it, or none at all
-    const uint64_t last = (vocab - (uint64_t)(p.pieces - 1) * p.piece + 255) / 256 * 256;
-    CHECK(last <= p.piece);
-    at[7] = p.prob; len[7] = 4ull * p.rows_pad * p.piece;
-    at[8] = p.acc; len[8] = 4ull * p.splits * rows * cols;
-    at[9] = p.bytes;
-    n = 9;
+    CHECK(p.chunk % p.bm == 0 && (uint64_t)p.chunks * p.chunk >= rows && (uint64_t)(p.chunks - 1) * p.chunk < rows);
+    const uint64_t all = (uint64_t)p.tiles * LOSS_TILE;
+    // every part has vocabulary rows
+    CHECK(p.share % LOSS_TILE == 0 && (uint64_t)p.share * p.splits >= all && (uint64_t)p.share * (p.splits - 1) < all);
+    at[7] = p.order; len[7] = 4ull * (rows + 1);
+    at[8] = p.prob; len[8] = 4ull * p.chunk * all;
+    at[9] = p.acc; len[9] = 4ull * p.splits * p.chunk * cols;
+    at[10] = p.bytes;
+    n = 10;
   }
   for (int i = 0; i < n; i++) CHECK(at[i] % 256 == 0 && at[i] + len[i] <= at[i + 1]);
   return 0;
