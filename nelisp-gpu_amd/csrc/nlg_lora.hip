@@ -108,7 +108,8 @@ struct DownArgs {
 // Sixteen rows a workgroup, all ranks (NT blocks of sixteen), the contraction
 // split over its eight waves.  Each adapter among the rows is one pass.
 // KMAJOR: weights [k][rmax] (B, in the backward pass), else [rmax][k] (A).
-// A step is sixteen k: lane group g holds k = 4 g .. 4 g + 3 of both operands.
+// A step is 32 k: lane group g holds k = 8 g .. 8 g + 7 of both operands, and
+// the next step's loads are out while one is multiplied.
 // Weights [k][rmax] are read as NT neighbouring ranks a lane, so block t of
 // the ranks is then NT i + t.
 template <bool BF, bool KMAJOR, int NT, bool VEC>
@@ -130,6 +131,8 @@ __global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
     else if (row0 + r < a.l.seq)
       for (uint32_t j = threadIdx.x; j < a.l.rmax; j += 512) a.u[(size_t)(row0 + r) * a.l.rmax + j] = 0.0f;
   }
+  constexpr int NW = KMAJOR ? 8 * ((NT + 1) / 2) : 4 * NT;  // words of weights a step
+  typedef uint32_t wvec __attribute__((ext_vector_type(NW)));
   while (todo) {
     const int32_t ad = __builtin_amdgcn_readfirstlane(s_ad[__builtin_ctz(todo)]);
     uint32_t mine = 0;
@@ -140,45 +143,70 @@ __global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
     v4f acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = (v4f){0, 0, 0, 0};
-    for (uint32_t k0 = w * 16; k0 < a.k; k0 += 128) {
-      const uint32_t k = k0 + 4 * g, n = k < a.k ? min(4u, a.k - k) : 0u;
-      const float4 xv = load4<VEC>(xr + k, n);
-      float wv[NT][4];
-      if (KMAJOR) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          // ranks NT i .. NT i + NT - 1 (rmax is a multiple of 8, so they are all there or none is; NT is 1, 2, 4 or 8)
-          union {
-            uint32_t u[(NT + 1) / 2];
-            uint16_t h[NT + NT % 2];
-          } v = {};
-          if ((uint32_t)e < n && (uint32_t)(NT * i) < rank) {
-            const uint16_t *p = wt + (size_t)(k + e) * a.l.rmax + NT * i;
-            if (NT == 1) v.h[0] = *p;
-            else if (NT == 2) v.u[0] = *(const uint32_t *)p;
-            else if (NT == 4) *(uint2 *)v.u = *(const uint2 *)p;
-            else *(uint4 *)v.u = *(const uint4 *)p;
-          }
-#pragma unroll
-          for (int t = 0; t < NT; t++) wv[t][e] = (uint32_t)(NT * i + t) < rank ? wide<BF>(v.h[t]) : 0.0f;
-        }
-      } else {
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          uint2 v = make_uint2(0, 0);
-          if (n && (uint32_t)(16 * t + i) < rank) v = *(const uint2 *)(wt + (size_t)(16 * t + i) * a.k + k);
-          wv[t][0] = wide<BF>(v.x & 0xffff);
-          wv[t][1] = wide<BF>(v.x >> 16);
-          wv[t][2] = wide<BF>(v.y & 0xffff);
-          wv[t][3] = wide<BF>(v.y >> 16);
-        }
+    // (macros: register sets handed to a lambda end up in scratch)
+#define LOAD(k0, X0, X1, W)                                                                              \
+    do {                                                                                                 \
+      const uint32_t k = (k0) + 8 * g, n = k < a.k ? min(8u, a.k - k) : 0u;                               \
+      X0 = load4<VEC>(xr + k, min(n, 4u));                                                               \
+      X1 = load4<VEC>(xr + k + 4, n > 4 ? n - 4 : 0u);                                                   \
+      if (KMAJOR) {                                                                                      \
+        _Pragma("unroll") for (int e = 0; e < 8; e++) {                                                  \
+          /* ranks NT i .. NT i + NT - 1: all of them lie in a row of rmax, or none */                   \
+          const bool in = (uint32_t)e < n && (uint32_t)(NT * i) < rank;                                  \
+          const uint16_t *p = wt + (in ? (size_t)(k + e) * a.l.rmax + NT * i : (size_t)0);                \
+          if (NT == 1) W[e] = *p;                                                                        \
+          else if (NT == 2) W[e] = *(const uint32_t *)p;                                                 \
+          else if (NT == 4) {                                                                            \
+            const uint2 v = *(const uint2 *)p;                                                           \
+            W[2 * e] = v.x; W[(2 * e + 1) % NW] = v.y;                                                   \
+          } else {                                                                                       \
+            const uint4 v = *(const uint4 *)p;                                                           \
+            W[(4 * e) % NW] = v.x; W[(4 * e + 1) % NW] = v.y;                                            \
+            W[(4 * e + 2) % NW] = v.z; W[(4 * e + 3) % NW] = v.w;                                        \
+          }                                                                                              \
+        }                                                                                                \
+      } else {                                                                                           \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                 \
+          const bool in = n && (uint32_t)(16 * t + i) < rank;                                            \
+          const uint4 v = *(const uint4 *)(wt + (in ? (size_t)(16 * t + i) * a.k + k : (size_t)0));       \
+          W[(4 * t) % NW] = v.x; W[(4 * t + 1) % NW] = v.y;                                              \
+          W[(4 * t + 2) % NW] = v.z; W[(4 * t + 3) % NW] = v.w;                                          \
+        }                                                                                                \
+      }                                                                                                  \
+    } while (0)
+#define MUL(k0, X0, X1, W)                                                                               \
+    do {                                                                                                 \
+      const uint32_t k = (k0) + 8 * g;                                                                   \
+      _Pragma("unroll") for (int e = 0; e < 8; e++) {                                                    \
+        const float xv = e < 4 ? at4(X0, e) : at4(X1, e - 4);                                            \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                 \
+          uint32_t h;                                                                                    \
+          bool in;                                                                                       \
+          if (KMAJOR) {                                                                                  \
+            h = NT == 1 ? W[e] : W[(e * (NT / 2) + t / 2) % NW] >> (16 * (t & 1));                       \
+            in = (uint32_t)(NT * i + t) < rank && k + e < a.k;                                           \
+          } else {                                                                                       \
+            h = W[(4 * t + e / 2) % NW] >> (16 * (e & 1));                                               \
+            in = (uint32_t)(16 * t + i) < rank && k < a.k;                                               \
+          }                                                                                              \
+          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv, in ? wide<BF>(h & 0xffff) : 0.0f, acc[t], 0, 0, 0); \
+        }                                                                                                \
+      }                                                                                                  \
+    } while (0)
+    float4 xa0, xa1, xb0, xb1;
+    wvec wa = {}, wb = {};
+    uint32_t k0 = w * 32;
+    LOAD(k0, xa0, xa1, wa);
+    for (; k0 < a.k; k0 += 512) {
+      if (k0 + 256 < a.k) LOAD(k0 + 256, xb0, xb1, wb);
+      MUL(k0, xa0, xa1, wa);
+      if (k0 + 256 < a.k) {
+        if (k0 + 512 < a.k) LOAD(k0 + 512, xa0, xa1, wa);
+        MUL(k0 + 256, xb0, xb1, wb);
       }
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(at4(xv, e), wv[t][e], acc[t], 0, 0, 0);
     }
+#undef MUL
+#undef LOAD
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -195,6 +223,52 @@ __global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
       }
     }
     __syncthreads();
+  }
+}
+
+// Few rows a request: a wave a row and four ranks, the contraction over its
+// lanes (eight neighbouring columns each, sixteen bytes of a rank's weights).
+#define TOK_RANKS 4
+template <bool BF>
+__device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, uint32_t rank, uint32_t row, uint32_t j0,
+                                         int lane, float (&u)[TOK_RANKS]) {
+  const float *const xr = a.x + (size_t)row * a.k;
+#pragma unroll
+  for (int t = 0; t < TOK_RANKS; t++) u[t] = 0.0f;
+#pragma unroll 2
+  for (uint32_t k = 8 * lane; k < a.k; k += 512) {
+    const float4 x0 = *(const float4 *)(xr + k), x1 = *(const float4 *)(xr + k + 4);
+    uint4 v[TOK_RANKS];
+#pragma unroll
+    for (int t = 0; t < TOK_RANKS; t++) v[t] = *(const uint4 *)(wt + (size_t)min(j0 + t, rank - 1) * a.k + k);
+#pragma unroll
+    for (int t = 0; t < TOK_RANKS; t++) {
+      u[t] = fmaf(x0.x, wide<BF>(v[t].x & 0xffff), u[t]);
+      u[t] = fmaf(x0.y, wide<BF>(v[t].x >> 16), u[t]);
+      u[t] = fmaf(x0.z, wide<BF>(v[t].y & 0xffff), u[t]);
+      u[t] = fmaf(x0.w, wide<BF>(v[t].y >> 16), u[t]);
+      u[t] = fmaf(x1.x, wide<BF>(v[t].z & 0xffff), u[t]);
+      u[t] = fmaf(x1.y, wide<BF>(v[t].z >> 16), u[t]);
+      u[t] = fmaf(x1.z, wide<BF>(v[t].w & 0xffff), u[t]);
+      u[t] = fmaf(x1.w, wide<BF>(v[t].w >> 16), u[t]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TOK_RANKS; t++) u[t] = nlg_wave_sum_f32(u[t]);
+}
+
+template <bool BF>
+__global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t row = blockIdx.x, j0 = (blockIdx.y * 4 + w) * TOK_RANKS;
+  if (j0 >= a.l.rmax) return;
+  const int32_t ad = __builtin_amdgcn_readfirstlane(lora_rows(a.l, row, 1, lane));
+  const uint32_t rank = ad < 0 ? 0u : lora_rank(a.l, ad);
+  float u[TOK_RANKS] = {};
+  if (j0 < rank) tok_down<BF>(a, a.l.a + (size_t)ad * a.l.rmax * a.k, rank, row, j0, lane, u);
+  if (lane < TOK_RANKS) {
+    const float v = lane == 0 ? u[0] : lane == 1 ? u[1] : lane == 2 ? u[2] : u[3];
+    a.u[(size_t)row * a.l.rmax + j0 + lane] = j0 + lane < rank ? v : 0.0f;
   }
 }
 
@@ -219,6 +293,15 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
   const uint32_t row0 = blockIdx.y * 32, col = blockIdx.x * 256 + w * 64 + 4 * i;
   const uint32_t nc = col < a.n ? min(4u, a.n - col) : 0u;
+  // what is added to: on the way from the start
+  float4 res[2][4];
+#pragma unroll
+  for (int m = 0; m < 2; m++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const uint32_t row = min(row0 + 16 * m + 4 * g + r, a.l.seq - 1);
+      res[m][r] = a.res ? load4<VEC>(a.res + (size_t)row * a.n + col, nc) : make_float4(0, 0, 0, 0);
+    }
   if (w == 0) {
     const int32_t ad = lora_rows(a.l, row0, 32, lane);
     if (lane < 32) s_ad[lane] = ad;
@@ -229,10 +312,12 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
     if (s_ad[r] >= 0) todo |= 1u << r;
   }
   if (a.y != a.res) {  // rows without an adapter
-    for (int r = g; r < 32; r += 4)
-      if (s_ad[r] < 0 && row0 + r < a.l.seq) {
-        const size_t o = (size_t)(row0 + r) * a.n + col;
-        store4<VEC>(a.y + o, nc, a.res ? load4<VEC>(a.res + o, nc) : make_float4(0, 0, 0, 0));
+#pragma unroll
+    for (int m = 0; m < 2; m++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t rr = 16 * m + 4 * g + r;
+        if (s_ad[rr] < 0 && row0 + rr < a.l.seq) store4<VEC>(a.y + (size_t)(row0 + rr) * a.n + col, nc, res[m][r]);
       }
   }
   while (todo) {
@@ -288,7 +373,7 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
         const uint32_t rr = 16 * m + 4 * g + r;
         if (!(mine >> rr & 1)) continue;
         const size_t o = (size_t)(row0 + rr) * a.n + col;
-        float4 v = a.res ? load4<VEC>(a.res + o, nc) : make_float4(0, 0, 0, 0);
+        float4 v = res[m][r];
         v.x = fmaf(sc, acc[m][0][r], v.x);
         v.y = fmaf(sc, acc[m][1][r], v.y);
         v.z = fmaf(sc, acc[m][2][r], v.z);
@@ -298,19 +383,72 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
   }
 }
 
+// Few rows a request: a wave a row and some columns, L lanes a column (eight
+// neighbouring ranks each: sixteen bytes), eight columns a lane on the way
+// together.
+template <bool BF, int L>
+__device__ __forceinline__ void tok_up(const UpArgs &a, const uint16_t *wt, uint32_t rank, float sc, uint32_t row,
+                                       const float (&u)[8], uint32_t c0, int lane) {
+  constexpr int PER = 64 / L, NC = 8;  // columns a step, steps
+  const uint32_t j = 8 * (lane % L), at = lane / L;
+  uint4 v[NC];
+#pragma unroll
+  for (int e = 0; e < NC; e++) {
+    const uint32_t c = c0 + e * PER + at;
+    v[e] = make_uint4(0, 0, 0, 0);
+    if (j < rank && c < a.n) v[e] = *(const uint4 *)(wt + (size_t)c * a.l.rmax + j);
+  }
+#pragma unroll
+  for (int e = 0; e < NC; e++) {
+    const uint32_t c = c0 + e * PER + at;
+    float y = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+      const uint32_t p = q < 2 ? v[e].x : q < 4 ? v[e].y : q < 6 ? v[e].z : v[e].w;
+      if (j + q < rank) y = fmaf(u[q], wide<BF>(p >> (16 * (q & 1)) & 0xffff), y);
+    }
+    if (L >= 2) y += __int_as_float(nlg_dpp<0xB1>(__float_as_int(y)));
+    if (L >= 4) y += __int_as_float(nlg_dpp<0x4E>(__float_as_int(y)));
+    if (L >= 8) y += __int_as_float(nlg_dpp<0x141>(__float_as_int(y)));  // half-row mirror
+    if (L >= 16) y += __int_as_float(nlg_dpp<0x140>(__float_as_int(y))); // row mirror
+    if (lane % L == 0 && c < a.n) {
+      const size_t o = (size_t)row * a.n + c;
+      a.y[o] = fmaf(sc, y, a.res ? a.res[o] : 0.0f);
+    }
+  }
+}
+
+template <bool BF, int L>
+__global__ __launch_bounds__(256) void k_lora_tok_up(UpArgs a) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t row = blockIdx.y, c0 = (blockIdx.x * 4 + w) * (64 / L * 8);
+  if (c0 >= a.n) return;
+  const int32_t ad = __builtin_amdgcn_readfirstlane(lora_rows(a.l, row, 1, lane));
+  if (ad < 0 && a.y == a.res) return;
+  const uint32_t rank = ad < 0 ? 0u : lora_rank(a.l, ad), j = 8 * (lane % L);
+  float u[8] = {};
+  if (j < a.l.rmax) {
+    const float4 u0 = *(const float4 *)(a.u + (size_t)row * a.l.rmax + j), u1 = *(const float4 *)(a.u + (size_t)row * a.l.rmax + j + 4);
+    u[0] = u0.x; u[1] = u0.y; u[2] = u0.z; u[3] = u0.w; u[4] = u1.x; u[5] = u1.y; u[6] = u1.z; u[7] = u1.w;
+  }
+  tok_up<BF, L>(a, a.l.b + (size_t)max(ad, 0) * a.l.rmax * a.n, rank, ad < 0 ? 0.0f : a.l.scale[ad], row, u, c0, lane);
+}
+
 // ------------------------------------------------------------------ the adapters' gradients
 
 struct OuterArgs {
   LoraArgs l;
   const float *p;    // [seq][rmax]
   const float *q;    // [seq][n]
-  float *out;        // [adapters][rmax][n], or [adapters][n][rmax]
+  float *out;        // [adapters][rmax][n], or [adapters][n][rmax]; of several parts, one after the other
   uint32_t n;
   bool scaled;
 };
 
 // sum over an adapter's rows of p[s, j] q[s, c], 64 columns and 16 NT ranks a
-// workgroup, its requests' rows over its eight waves.  TURN: stored [c][j].
+// workgroup, its requests' rows over the eight waves of gridDim.z workgroups,
+// four rows a wave at a time, four times of them on the way together.  TURN:
+// stored [c][j].
 template <int NT, bool TURN, bool VEC>
 __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
   __shared__ v4f s_acc[4][NT][4][64];
@@ -324,6 +462,7 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; e++) acc[t][e] = (v4f){0, 0, 0, 0};
   int64_t before = 0;  // rows that earlier requests have taken
+  const int64_t step = 32 * (int64_t)gridDim.z;
   for (uint32_t rq = 0; rq < a.l.requests; rq++) {
     int64_t s0 = a.l.start ? (int64_t)a.l.start[rq] : (int64_t)rq;
     int64_t s1 = a.l.start ? (int64_t)a.l.start[rq + 1] : (int64_t)rq + 1;
@@ -332,17 +471,27 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
     if (s1 <= s0) continue;
     before = s1;
     if (a.l.adapter[rq] != ad) continue;
-    for (int64_t s = s0 + 4 * w; s < s1; s += 32) {
-      const int64_t row = s + g;
-      const bool in = row < s1;
-      const float4 qv = load4<VEC>(a.q + (size_t)(in ? row : s) * a.n + col, in ? nc : 0);
+    for (int64_t s = s0 + 4 * (w + 8 * (int)blockIdx.z); s < s1; s += 4 * step) {
+      float4 qv[4];
+      float pv[4][NT];
 #pragma unroll
-      for (int t = 0; t < NT; t++) {
-        const uint32_t j = 16 * t + i;
-        const float pv = in && j < rank ? a.p[(size_t)row * a.l.rmax + j] : 0.0f;
+      for (int k = 0; k < 4; k++) {
+        const int64_t row = s + k * step + g;
+        const bool in = row < s1;
+        qv[k] = load4<VEC>(a.q + (size_t)(in ? row : s0) * a.n + col, in ? nc : 0);
 #pragma unroll
-        for (int e = 0; e < 4; e++) acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv, at4(qv, e), acc[t][e], 0, 0, 0);
+        for (int t = 0; t < NT; t++) {
+          const uint32_t j = 16 * t + i;
+          pv[k][t] = in && j < rank ? a.p[(size_t)row * a.l.rmax + j] : 0.0f;
+        }
       }
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[k][t], at4(qv[k], e), acc[t][e], 0, 0, 0);
     }
   }
   // the waves' sums, by halves
@@ -363,7 +512,7 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
   }
   if (w) return;
   const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
-  float *const o = a.out + (size_t)ad * a.l.rmax * a.n;
+  float *const o = a.out + ((size_t)blockIdx.z * a.l.adapters + ad) * a.l.rmax * a.n;
 #pragma unroll
   for (int t = 0; t < NT; t++) {
     if (TURN) {
@@ -383,6 +532,18 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
                       make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc));
       }
     }
+  }
+}
+
+// The parts of such sums, added in order.
+__global__ __launch_bounds__(256) void k_lora_sum(const float4 *part, float4 *out, uint64_t n4, uint32_t parts) {
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n4; i += gridDim.x * 256ull) {
+    float4 v = part[i];
+    for (uint32_t k = 1; k < parts; k++) {
+      const float4 f = part[k * n4 + i];
+      v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
+    }
+    out[i] = v;
   }
 }
 
@@ -463,9 +624,20 @@ static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipS
   return NLG_OK;
 }
 
-static int lora_outer(const char *what, const OuterArgs &d, bool turn, hipStream_t st) {
-  const dim3 grid((d.n + 63) / 64, d.l.adapters), blk(512);
-  const bool vec = d.n % 4 == 0 && (((uintptr_t)d.q | (turn ? 0 : (uintptr_t)d.out)) & 15) == 0;
+// How many parts an adapter's rows are summed in: until two workgroups a CU have some, each of 256 rows at least.
+static uint32_t lora_parts(uint32_t seq, uint32_t n, uint32_t adapters) {
+  const uint64_t wg = (uint64_t)((n + 63) / 64) * adapters, most = seq / 256;
+  uint64_t k = 512 / wg;
+  if (k > most) k = most;
+  return k < 1 ? 1 : k > 16 ? 16 : (uint32_t)k;
+}
+
+static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, hipStream_t st) {
+  const uint32_t np = lora_parts(d.l.seq, d.n, d.l.adapters);
+  float *const out = d.out;
+  if (np > 1) d.out = parts;
+  const dim3 grid((d.n + 63) / 64, d.l.adapters, np), blk(512);
+  const bool vec = d.n % 4 == 0 && ((uintptr_t)d.q & 15) == 0;
   const uint32_t nt = (d.l.rmax + 15) / 16;
 #define GO(N, T)                                                                           \
   do {                                                                                     \
@@ -482,6 +654,38 @@ static int lora_outer(const char *what, const OuterArgs &d, bool turn, hipStream
   if (turn) GO2(true);
   else GO2(false);
 #undef GO2
+#undef GO
+  NLG_LAUNCHED(what);
+  if (np > 1) {
+    const uint64_t n4 = (uint64_t)d.l.adapters * d.l.rmax * d.n / 4;
+    hipLaunchKernelGGL(k_lora_sum, dim3(nlg_blocks(n4, 256) < 2048 ? nlg_blocks(n4, 256) : 2048), dim3(256), 0, st,
+                       (const float4 *)parts, (float4 *)out, n4, np);
+    NLG_LAUNCHED(what);
+  }
+  return NLG_OK;
+}
+
+// Few rows a request, or few rows at all.
+static bool lora_by_token(const LoraArgs &l) { return l.seq <= 16 || (l.seq < 4ull * l.requests && l.seq < 65536); }
+
+static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool bf, hipStream_t st) {
+  const dim3 gd(d.l.seq, (d.l.rmax + 4 * TOK_RANKS - 1) / (4 * TOK_RANKS));
+  if (bf) hipLaunchKernelGGL((k_lora_tok_down<true>), gd, dim3(256), 0, st, d);
+  else hipLaunchKernelGGL((k_lora_tok_down<false>), gd, dim3(256), 0, st, d);
+  NLG_LAUNCHED(what);
+  const uint32_t lanes = d.l.rmax <= 8 ? 1 : d.l.rmax <= 16 ? 2 : d.l.rmax <= 32 ? 4 : d.l.rmax <= 64 ? 8 : 16;
+  const uint32_t per = 4 * (64 / lanes * 8);
+#define GO(L)                                                                                                       \
+  do {                                                                                                              \
+    const dim3 gu((p.n + per - 1) / per, d.l.seq);                                                                   \
+    if (bf) hipLaunchKernelGGL((k_lora_tok_up<true, L>), gu, dim3(256), 0, st, p);                                   \
+    else hipLaunchKernelGGL((k_lora_tok_up<false, L>), gu, dim3(256), 0, st, p);                                     \
+  } while (0)
+  if (lanes == 1) GO(1);
+  else if (lanes == 2) GO(2);
+  else if (lanes == 4) GO(4);
+  else if (lanes == 8) GO(8);
+  else GO(16);
 #undef GO
   NLG_LAUNCHED(what);
   return NLG_OK;
@@ -514,9 +718,10 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
-  if (lora_down(what, d, fmt == NLG_LORA_BF16, false, st)) return NLG_ERR;
   UpArgs p{};
   p.l = d.l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
+  if (lora_by_token(d.l)) return lora_tok(what, d, p, fmt == NLG_LORA_BF16, st);
+  if (lora_down(what, d, fmt == NLG_LORA_BF16, false, st)) return NLG_ERR;
   return lora_up(what, p, fmt == NLG_LORA_BF16, false, st);
 }
 
@@ -568,11 +773,18 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
                          u ? u : (float *)workspace, seq, out, cols, nullptr, 0, (void *)st);
 }
 
+// du and u, and the parts of one of the two gradients
 extern "C" size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters,
                                                  uint32_t rmax, uint32_t requests) {
-  (void)adapters;
   (void)requests;
-  return lora_sizes(seq, out, cols, rmax) ? 2 * lora_round((size_t)seq * rmax * 4) : 0;
+  if (!lora_sizes(seq, out, cols, rmax) || !adapters || adapters > 65535) return 0;
+  size_t most = 0;
+  for (const uint32_t n : {out, cols}) {
+    const uint32_t parts = lora_parts(seq, n, adapters);
+    const size_t bytes = parts > 1 ? (size_t)parts * adapters * rmax * n * 4 : 0;
+    most = bytes > most ? bytes : most;
+  }
+  return 2 * lora_round((size_t)seq * rmax * 4) + lora_round(most);
 }
 
 extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a,
@@ -618,9 +830,10 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   OuterArgs o{};
   o.l = d.l;
   o.p = u; o.q = dy; o.out = db; o.n = out; o.scaled = true;
-  if (lora_outer(what, o, true, st)) return NLG_ERR;
+  float *const parts = (float *)((uint8_t *)workspace + 2 * nu);
+  if (lora_outer(what, o, true, parts, st)) return NLG_ERR;
   o.p = du; o.q = x; o.out = da; o.n = cols; o.scaled = false;
-  if (lora_outer(what, o, false, st)) return NLG_ERR;
+  if (lora_outer(what, o, false, parts, st)) return NLG_ERR;
   if (!dx) return NLG_OK;
   UpArgs p{};
   p.l = d.l; p.u = du; p.res = dres; p.y = dx; p.n = cols; p.scaled = false;
