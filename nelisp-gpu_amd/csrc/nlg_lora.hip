@@ -14,7 +14,7 @@
 // r is C[4 g + r][i].
 #include <math.h>
 
-#include "nlg_quant.h"
+#include "nlg_act_q.h"
 #include "nlg_scope.h"
 
 int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *attn_mz, uint32_t attn_nc, uint32_t hd,
@@ -226,23 +226,22 @@ __global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
   }
 }
 
-// Few rows a request: a wave a row and four ranks, the contraction over its
+// Few rows a request: a wave a row and R ranks, the contraction over its
 // lanes (eight neighbouring columns each, sixteen bytes of a rank's weights).
-#define TOK_RANKS 4
-template <bool BF>
+template <bool BF, int R>
 __device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, uint32_t rank, uint32_t row, uint32_t j0,
-                                         int lane, float (&u)[TOK_RANKS]) {
+                                         int lane, float (&u)[R]) {
   const float *const xr = a.x + (size_t)row * a.k;
 #pragma unroll
-  for (int t = 0; t < TOK_RANKS; t++) u[t] = 0.0f;
+  for (int t = 0; t < R; t++) u[t] = 0.0f;
 #pragma unroll 2
   for (uint32_t k = 8 * lane; k < a.k; k += 512) {
     const float4 x0 = *(const float4 *)(xr + k), x1 = *(const float4 *)(xr + k + 4);
-    uint4 v[TOK_RANKS];
+    uint4 v[R];
 #pragma unroll
-    for (int t = 0; t < TOK_RANKS; t++) v[t] = *(const uint4 *)(wt + (size_t)min(j0 + t, rank - 1) * a.k + k);
+    for (int t = 0; t < R; t++) v[t] = *(const uint4 *)(wt + (size_t)min(j0 + t, rank - 1) * a.k + k);
 #pragma unroll
-    for (int t = 0; t < TOK_RANKS; t++) {
+    for (int t = 0; t < R; t++) {
       u[t] = fmaf(x0.x, wide<BF>(v[t].x & 0xffff), u[t]);
       u[t] = fmaf(x0.y, wide<BF>(v[t].x >> 16), u[t]);
       u[t] = fmaf(x0.z, wide<BF>(v[t].y & 0xffff), u[t]);
@@ -254,22 +253,34 @@ __device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, 
     }
   }
 #pragma unroll
-  for (int t = 0; t < TOK_RANKS; t++) u[t] = nlg_wave_sum_f32(u[t]);
+  for (int t = 0; t < R; t++) u[t] = nlg_wave_sum_f32(u[t]);
 }
 
+#define TOK_RANKS 4
+// a workgroup's 4 waves: sixteen ranks of a row
 template <bool BF>
-__global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {
+__device__ __forceinline__ void tok_down_group(const DownArgs &a, uint32_t row, uint32_t group) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t row = blockIdx.x, j0 = (blockIdx.y * 4 + w) * TOK_RANKS;
+  const uint32_t j0 = (group * 4 + w) * TOK_RANKS;
   if (j0 >= a.l.rmax) return;
   const int32_t ad = __builtin_amdgcn_readfirstlane(lora_rows(a.l, row, 1, lane));
   const uint32_t rank = ad < 0 ? 0u : lora_rank(a.l, ad);
   float u[TOK_RANKS] = {};
-  if (j0 < rank) tok_down<BF>(a, a.l.a + (size_t)ad * a.l.rmax * a.k, rank, row, j0, lane, u);
+  if (j0 < rank) tok_down<BF, TOK_RANKS>(a, a.l.a + (size_t)ad * a.l.rmax * a.k, rank, row, j0, lane, u);
   if (lane < TOK_RANKS) {
     const float v = lane == 0 ? u[0] : lane == 1 ? u[1] : lane == 2 ? u[2] : u[3];
     a.u[(size_t)row * a.l.rmax + j0 + lane] = j0 + lane < rank ? v : 0.0f;
   }
+}
+template <bool BF>
+__global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {
+  tok_down_group<BF>(a, blockIdx.x, blockIdx.y);
+}
+// That beside the rounding of the same rows to int8 for the shared projection, in one launch.
+template <bool BF, int G16>
+__global__ __launch_bounds__(256) void k_lora_tok_down_q(DownArgs a, ActQArgs q) {
+  if (blockIdx.y == 0) act_q_row<G16, NLG_PRO_NONE>(q, blockIdx.x);
+  else tok_down_group<BF>(a, blockIdx.x, blockIdx.y - 1);
 }
 
 // ------------------------------------------------------------------ up: from the ranks
@@ -383,55 +394,90 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
   }
 }
 
-// Few rows a request: a wave a row and some columns, L lanes a column (eight
-// neighbouring ranks each: sixteen bytes), eight columns a lane on the way
+// Few rows a request: a wave a row and NC steps of 64 / L columns, L lanes a
+// column (eight neighbouring ranks each: sixteen bytes), all on the way
 // together.
-template <bool BF, int L>
-__device__ __forceinline__ void tok_up(const UpArgs &a, const uint16_t *wt, uint32_t rank, float sc, uint32_t row,
-                                       const float (&u)[8], uint32_t c0, int lane) {
-  constexpr int PER = 64 / L, NC = 8;  // columns a step, steps
-  const uint32_t j = 8 * (lane % L), at = lane / L;
+template <int L, int NC>
+struct TokUp {
   uint4 v[NC];
+  float res[NC];
+  __device__ __forceinline__ void load(const UpArgs &a, const uint16_t *wt, uint32_t rank, uint32_t row, uint32_t c0,
+                                       int lane) {
 #pragma unroll
-  for (int e = 0; e < NC; e++) {
-    const uint32_t c = c0 + e * PER + at;
-    v[e] = make_uint4(0, 0, 0, 0);
-    if (j < rank && c < a.n) v[e] = *(const uint4 *)(wt + (size_t)c * a.l.rmax + j);
-  }
-#pragma unroll
-  for (int e = 0; e < NC; e++) {
-    const uint32_t c = c0 + e * PER + at;
-    float y = 0.0f;
-#pragma unroll
-    for (int q = 0; q < 8; q++) {
-      const uint32_t p = q < 2 ? v[e].x : q < 4 ? v[e].y : q < 6 ? v[e].z : v[e].w;
-      if (j + q < rank) y = fmaf(u[q], wide<BF>(p >> (16 * (q & 1)) & 0xffff), y);
-    }
-    if (L >= 2) y += __int_as_float(nlg_dpp<0xB1>(__float_as_int(y)));
-    if (L >= 4) y += __int_as_float(nlg_dpp<0x4E>(__float_as_int(y)));
-    if (L >= 8) y += __int_as_float(nlg_dpp<0x141>(__float_as_int(y)));  // half-row mirror
-    if (L >= 16) y += __int_as_float(nlg_dpp<0x140>(__float_as_int(y))); // row mirror
-    if (lane % L == 0 && c < a.n) {
-      const size_t o = (size_t)row * a.n + c;
-      a.y[o] = fmaf(sc, y, a.res ? a.res[o] : 0.0f);
+    for (int e = 0; e < NC; e++) {
+      const uint32_t c = c0 + e * (64 / L) + lane / L;
+      v[e] = make_uint4(0, 0, 0, 0);
+      if (8u * (lane % L) < rank && c < a.n) v[e] = *(const uint4 *)(wt + (size_t)c * a.l.rmax + 8 * (lane % L));
+      res[e] = lane % L == 0 && c < a.n && a.res ? a.res[(size_t)row * a.n + c] : 0.0f;
     }
   }
-}
+  template <bool BF>
+  __device__ __forceinline__ void store(const UpArgs &a, uint32_t rank, float sc, uint32_t row, const float (&u)[8],
+                                        uint32_t c0, int lane) {
+#pragma unroll
+    for (int e = 0; e < NC; e++) {
+      const uint32_t c = c0 + e * (64 / L) + lane / L;
+      float y = 0.0f;
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const uint32_t p = q < 2 ? v[e].x : q < 4 ? v[e].y : q < 6 ? v[e].z : v[e].w;
+        if (8u * (lane % L) + q < rank) y = fmaf(u[q], wide<BF>(p >> (16 * (q & 1)) & 0xffff), y);
+      }
+      if (L >= 2) y += __int_as_float(nlg_dpp<0xB1>(__float_as_int(y)));
+      if (L >= 4) y += __int_as_float(nlg_dpp<0x4E>(__float_as_int(y)));
+      if (L >= 8) y += __int_as_float(nlg_dpp<0x141>(__float_as_int(y)));   // half-row mirror
+      if (L >= 16) y += __int_as_float(nlg_dpp<0x140>(__float_as_int(y)));  // row mirror
+      if (lane % L == 0 && c < a.n) a.y[(size_t)row * a.n + c] = fmaf(sc, y, res[e]);
+    }
+  }
+};
 
-template <bool BF, int L>
+template <bool BF, int L, int NC>
 __global__ __launch_bounds__(256) void k_lora_tok_up(UpArgs a) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const uint32_t row = blockIdx.y, c0 = (blockIdx.x * 4 + w) * (64 / L * 8);
+  const uint32_t row = blockIdx.y, c0 = (blockIdx.x * 4 + w) * (64 / L * NC);
   if (c0 >= a.n) return;
   const int32_t ad = __builtin_amdgcn_readfirstlane(lora_rows(a.l, row, 1, lane));
   if (ad < 0 && a.y == a.res) return;
   const uint32_t rank = ad < 0 ? 0u : lora_rank(a.l, ad), j = 8 * (lane % L);
+  TokUp<L, NC> t;
+  t.load(a, a.l.b + (size_t)max(ad, 0) * a.l.rmax * a.n, rank, row, c0, lane);
   float u[8] = {};
   if (j < a.l.rmax) {
-    const float4 u0 = *(const float4 *)(a.u + (size_t)row * a.l.rmax + j), u1 = *(const float4 *)(a.u + (size_t)row * a.l.rmax + j + 4);
+    const float *p = a.u + (size_t)row * a.l.rmax + j;
+    const float4 u0 = *(const float4 *)p, u1 = *(const float4 *)(p + 4);
     u[0] = u0.x; u[1] = u0.y; u[2] = u0.z; u[3] = u0.w; u[4] = u1.x; u[5] = u1.y; u[6] = u1.z; u[7] = u1.w;
   }
-  tok_up<BF, L>(a, a.l.b + (size_t)max(ad, 0) * a.l.rmax * a.n, rank, ad < 0 ? 0.0f : a.l.scale[ad], row, u, c0, lane);
+  t.template store<BF>(a, rank, ad < 0 ? 0.0f : a.l.scale[ad], row, u, c0, lane);
+}
+
+// A few rows of small adapters in one launch: every workgroup finds its row's
+// u again (two ranks a wave at a time), while its columns' weights are on the
+// way.
+template <bool BF, int L>
+__global__ __launch_bounds__(512) void k_lora_tok(DownArgs d, UpArgs a) {
+  __shared__ float s_u[LORA_RANK];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint32_t row = blockIdx.y, c0 = (blockIdx.x * 8 + w) * (64 / L);
+  const int32_t ad = __builtin_amdgcn_readfirstlane(lora_rows(a.l, row, 1, lane));
+  const uint32_t rank = ad < 0 ? 0u : lora_rank(a.l, ad), j = 8 * (lane % L);
+  TokUp<L, 1> t;
+  t.load(a, a.l.b + (size_t)max(ad, 0) * a.l.rmax * a.n, rank, row, c0, lane);
+  const float sc = ad < 0 ? 0.0f : a.l.scale[ad];
+  for (uint32_t j0 = 2 * w; j0 < a.l.rmax; j0 += 16) {
+    float u[2] = {};
+    if (j0 < rank) tok_down<BF, 2>(d, d.l.a + (size_t)ad * d.l.rmax * d.k, rank, row, j0, lane, u);
+    if (lane < 2) s_u[j0 + lane] = j0 + lane < rank ? u[lane] : 0.0f;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x < a.l.rmax) d.u[(size_t)row * a.l.rmax + threadIdx.x] = s_u[threadIdx.x];
+  if (ad < 0 && a.y == a.res) return;
+  float u[8] = {};
+  if (j < a.l.rmax) {
+#pragma unroll
+    for (int q = 0; q < 8; q++) u[q] = s_u[j + q];
+  }
+  t.template store<BF>(a, rank, sc, row, u, c0, lane);
 }
 
 // ------------------------------------------------------------------ the adapters' gradients
@@ -668,25 +714,70 @@ static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, hi
 // Few rows a request, or few rows at all.
 static bool lora_by_token(const LoraArgs &l) { return l.seq <= 16 || (l.seq < 4ull * l.requests && l.seq < 65536); }
 
-static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool bf, hipStream_t st) {
-  const dim3 gd(d.l.seq, (d.l.rmax + 4 * TOK_RANKS - 1) / (4 * TOK_RANKS));
-  if (bf) hipLaunchKernelGGL((k_lora_tok_down<true>), gd, dim3(256), 0, st, d);
-  else hipLaunchKernelGGL((k_lora_tok_down<false>), gd, dim3(256), 0, st, d);
-  NLG_LAUNCHED(what);
-  const uint32_t lanes = d.l.rmax <= 8 ? 1 : d.l.rmax <= 16 ? 2 : d.l.rmax <= 32 ? 4 : d.l.rmax <= 64 ? 8 : 16;
-  const uint32_t per = 4 * (64 / lanes * 8);
-#define GO(L)                                                                                                       \
-  do {                                                                                                              \
-    const dim3 gu((p.n + per - 1) / per, d.l.seq);                                                                   \
-    if (bf) hipLaunchKernelGGL((k_lora_tok_up<true, L>), gu, dim3(256), 0, st, p);                                   \
-    else hipLaunchKernelGGL((k_lora_tok_up<false, L>), gu, dim3(256), 0, st, p);                                     \
+// Whether lora_tok alone does them: a few rows of small adapters.
+static bool lora_tok_whole(const DownArgs &d) { return d.l.seq <= 4 && (uint64_t)d.l.rmax * d.k <= 65536; }
+
+// q: the rows' rounding to int8, wanted beside (then without the way up)
+static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool bf, const ActQArgs *q, hipStream_t st) {
+  const uint32_t lanes = p.l.rmax <= 8 ? 1 : p.l.rmax <= 16 ? 2 : p.l.rmax <= 32 ? 4 : p.l.rmax <= 64 ? 8 : 16;
+  const uint32_t step = 64 / lanes, groups = (d.l.rmax + 4 * TOK_RANKS - 1) / (4 * TOK_RANKS);
+#define BY_LANES(GO)              \
+  do {                            \
+    if (lanes == 1) GO(1);        \
+    else if (lanes == 2) GO(2);   \
+    else if (lanes == 4) GO(4);   \
+    else if (lanes == 8) GO(8);   \
+    else GO(16);                  \
   } while (0)
-  if (lanes == 1) GO(1);
-  else if (lanes == 2) GO(2);
-  else if (lanes == 4) GO(4);
-  else if (lanes == 8) GO(8);
-  else GO(16);
+  if (!q && lora_tok_whole(d)) {
+    const dim3 grid((p.n + 8 * step - 1) / (8 * step), p.l.seq);
+#define GO(L)                                                                              \
+  do {                                                                                     \
+    if (bf) hipLaunchKernelGGL((k_lora_tok<true, L>), grid, dim3(512), 0, st, d, p);       \
+    else hipLaunchKernelGGL((k_lora_tok<false, L>), grid, dim3(512), 0, st, d, p);         \
+  } while (0)
+    BY_LANES(GO);
 #undef GO
+    NLG_LAUNCHED(what);
+    return NLG_OK;
+  }
+  const dim3 gd(d.l.seq, groups + (q ? 1 : 0));
+  if (q) {
+#define GO(G)                                                                                        \
+  do {                                                                                               \
+    if (bf) hipLaunchKernelGGL((k_lora_tok_down_q<true, G>), gd, dim3(256), 0, st, d, *q);           \
+    else hipLaunchKernelGGL((k_lora_tok_down_q<false, G>), gd, dim3(256), 0, st, d, *q);             \
+  } while (0)
+    if (q->cols <= 4096) GO(1);
+    else if (q->cols <= 8192) GO(2);
+    else GO(4);
+#undef GO
+  } else if (bf) {
+    hipLaunchKernelGGL((k_lora_tok_down<true>), gd, dim3(256), 0, st, d);
+  } else {
+    hipLaunchKernelGGL((k_lora_tok_down<false>), gd, dim3(256), 0, st, d);
+  }
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+static int lora_tok_up(const char *what, const UpArgs &p, bool bf, hipStream_t st) {
+  const uint32_t lanes = p.l.rmax <= 8 ? 1 : p.l.rmax <= 16 ? 2 : p.l.rmax <= 32 ? 4 : p.l.rmax <= 64 ? 8 : 16;
+  const uint32_t step = 64 / lanes;
+  // eight steps a wave where that leaves the card full
+  const bool many = (uint64_t)p.l.seq * p.n / (8 * step) >= 2048;
+  const uint32_t per = 4 * step * (many ? 8 : 2);
+  const dim3 grid((p.n + per - 1) / per, p.l.seq);
+#define GO(L)                                                                                          \
+  do {                                                                                                 \
+    if (bf && many) hipLaunchKernelGGL((k_lora_tok_up<true, L, 8>), grid, dim3(256), 0, st, p);        \
+    else if (bf) hipLaunchKernelGGL((k_lora_tok_up<true, L, 2>), grid, dim3(256), 0, st, p);           \
+    else if (many) hipLaunchKernelGGL((k_lora_tok_up<false, L, 8>), grid, dim3(256), 0, st, p);        \
+    else hipLaunchKernelGGL((k_lora_tok_up<false, L, 2>), grid, dim3(256), 0, st, p);                  \
+  } while (0)
+  BY_LANES(GO);
+#undef GO
+#undef BY_LANES
   NLG_LAUNCHED(what);
   return NLG_OK;
 }
@@ -720,7 +811,10 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
   d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
   UpArgs p{};
   p.l = d.l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
-  if (lora_by_token(d.l)) return lora_tok(what, d, p, fmt == NLG_LORA_BF16, st);
+  if (lora_by_token(d.l)) {
+    const bool bf = fmt == NLG_LORA_BF16;
+    return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
+  }
   if (lora_down(what, d, fmt == NLG_LORA_BF16, false, st)) return NLG_ERR;
   return lora_up(what, p, fmt == NLG_LORA_BF16, false, st);
 }
@@ -758,19 +852,31 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   uint8_t *const more = (uint8_t *)workspace + nu;
+  const bool bf = fmt == NLG_LORA_BF16;
+  float *const us = u ? u : (float *)workspace;
   if (nlg_batched(seq, cols)) {
     float *const gamma = (float *)(more + ((size_t)seq * cols + 255) / 256 * 256);
-    if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st)) return NLG_ERR;
     FusedArgs f{};
     f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;
     f.y = y; f.ystride = out;
-    if (nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st)) return NLG_ERR;
-  } else if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more,
-                                workspace_bytes - nu, (void *)st)) {
-    return NLG_ERR;
+    DownArgs d{};
+    d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = us;
+    UpArgs p{};
+    p.l = l; p.u = us; p.res = y; p.y = y; p.n = out; p.scaled = true;
+    if (lora_by_token(l)) {
+      const ActQArgs q{x, nullptr, 0.0f, nullptr, 0, 0, more, gamma, seq, cols, 0u};
+      return lora_tok(what, d, p, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) ||
+             lora_tok_up(what, p, bf, st);
+    }
+    if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st)) return NLG_ERR;
+    return nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) || lora_down(what, d, bf, false, st) ||
+           lora_up(what, p, bf, false, st);
   }
-  return nlg_lora_linear(x, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, y, y,
-                         u ? u : (float *)workspace, seq, out, cols, nullptr, 0, (void *)st);
+  if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more, workspace_bytes - nu,
+                         (void *)st))
+    return NLG_ERR;
+  return nlg_lora_linear(x, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, y, y, us, seq, out, cols,
+                         nullptr, 0, (void *)st);
 }
 
 // du and u, and the parts of one of the two gradients
