@@ -494,8 +494,7 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
 #define NLG_LORA_F16 0
 #define NLG_LORA_BF16 1
 /* y = res + the adapters' part (res NULL: that alone; res may be y).  u
- * [seq x rmax] (NULL: kept in the workspace, which is not read otherwise)
- * receives what the gradient needs. */
+ * [seq x rmax] (NULL: not wanted) receives what the gradient needs. */
 int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t *b, int fmt, const float *scale,
                     const int32_t *rank, const int32_t *start, const int32_t *adapter, uint32_t requests,
                     uint32_t adapters, uint32_t rmax, const float *res, float *y, float *u, uint32_t seq, uint32_t out,

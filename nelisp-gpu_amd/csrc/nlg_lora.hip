@@ -77,10 +77,12 @@ __device__ __forceinline__ float wide(uint32_t h) {  // a 16-bit value (low half
   return BF ? __uint_as_float(h << 16) : (float)__builtin_bit_cast(_Float16, (uint16_t)h);
 }
 
+// p[k] .. p[k + 3] of n values, or where those are not all there any others of
+// the n (VEC: n is a multiple of 4 and p aligned).
 template <bool VEC>
-__device__ __forceinline__ float4 load4(const float *p, uint32_t n) {  // n: how many of them there are
-  if (VEC) return n ? *(const float4 *)p : make_float4(0, 0, 0, 0);
-  return make_float4(n > 0 ? p[0] : 0, n > 1 ? p[1] : 0, n > 2 ? p[2] : 0, n > 3 ? p[3] : 0);
+__device__ __forceinline__ float4 inside4(const float *p, uint32_t k, uint32_t n) {
+  if (VEC) return *(const float4 *)(p + min(k, n - 4));
+  return make_float4(p[min(k, n - 1)], p[min(k + 1, n - 1)], p[min(k + 2, n - 1)], p[min(k + 3, n - 1)]);
 }
 template <bool VEC>
 __device__ __forceinline__ void store4(float *p, uint32_t n, float4 v) {
@@ -102,125 +104,235 @@ struct DownArgs {
   const float *x;   // [seq][k]
   uint32_t k;
   bool scaled;
-  float *u;         // [seq][rmax]
+  float *u;         // [seq][rmax]; of several parts, one after the other
 };
 
-// Sixteen rows a workgroup, all ranks (NT blocks of sixteen), the contraction
-// split over its eight waves.  Each adapter among the rows is one pass.
+// 32 rows a workgroup, all ranks (NT blocks of sixteen), the contraction over
+// its four waves and gridDim.y workgroups.  Each adapter among the rows is one
+// pass.
+// A step is 128 k, a wave 32 of them, on the bf16 matrix cores
+// (v_mfma_f32_16x16x32_bf16: lane 16 g + i holds k = 8 g .. 8 g + 7 of row or
+// column i): x as the three bf16 that make up its 24 bits, a bf16 weight as it
+// is, an f16 weight as two.  Of the products of parts only that of the last two
+// is left out, 2^-24 of the whole.
+// Both operands go from memory to LDS directly in runs of 256 bytes and more,
+// three stages, two on the way while one is multiplied.  (Read straight into
+// the products' layout, 128 bytes of each of 32 rows at a time, 4,731 rows of
+// 4,096 took 35 us, and 18.7 without the reads of x.)  An x row's 16-byte units
+// are swizzled by its number.
+// Every load is in bounds and none is masked: ranks behind the rank make sums
+// that are thrown away, and a k behind the row has its weights zeroed.
 // KMAJOR: weights [k][rmax] (B, in the backward pass), else [rmax][k] (A).
-// A step is 32 k: lane group g holds k = 8 g .. 8 g + 7 of both operands, and
-// the next step's loads are out while one is multiplied.
 // Weights [k][rmax] are read as NT neighbouring ranks a lane, so block t of
 // the ranks is then NT i + t.
+typedef __bf16 bf8v __attribute__((ext_vector_type(8)));
+union Bf8 {
+  uint32_t u[4];
+  uint4 q;
+  bf8v v;
+};
+// Two f32 as the pairs of bf16 that add up to them, largest first (what is
+// left after each is exact).
+__device__ __forceinline__ void split3(float a, float b, uint32_t &p0, uint32_t &p1, uint32_t &p2) {
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  p0 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+  const float ra = a - __uint_as_float(ua & 0xffff0000u), rb = b - __uint_as_float(ub & 0xffff0000u);
+  const uint32_t va = __float_as_uint(ra), vb = __float_as_uint(rb);
+  p1 = __builtin_amdgcn_perm(vb, va, 0x07060302u);
+  const float sa = ra - __uint_as_float(va & 0xffff0000u), sb = rb - __uint_as_float(vb & 0xffff0000u);
+  p2 = __builtin_amdgcn_perm(__float_as_uint(sb), __float_as_uint(sa), 0x07060302u);
+}
+// A pair of f16 as two pairs of bf16.
+__device__ __forceinline__ void split_f16(uint32_t h, uint32_t &p0, uint32_t &p1) {
+  const float a = wide<false>(h & 0xffff), b = wide<false>(h >> 16);
+  const uint32_t ua = __float_as_uint(a), ub = __float_as_uint(b);
+  p0 = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+  const float ra = a - __uint_as_float(ua & 0xffff0000u), rb = b - __uint_as_float(ub & 0xffff0000u);
+  p1 = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
+}
+
+// s_waitcnt vmcnt(n) lgkmcnt(0)
+#define WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (0x7 << 4) | (((n) >> 4) << 14))
+// no memory operation moves across it at compile time
+#define ORDER() asm volatile("" ::: "memory")
+
 template <bool BF, bool KMAJOR, int NT, bool VEC>
-__global__ __launch_bounds__(512) void k_lora_down(DownArgs a) {
-  __shared__ float s_u[8][16][NT * 16 + 4];
-  __shared__ int32_t s_ad[16];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const uint32_t row0 = blockIdx.x * 16;
+__global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
+  constexpr int MT = 2, ROWS = 16 * MT, NX = VEC ? 4 : 16, XB = ROWS * 512, STAGE = XB + NT * 4096;
+  __shared__ __align__(1024) uint8_t s_0[STAGE];
+  __shared__ __align__(1024) uint8_t s_1[STAGE];
+  __shared__ __align__(1024) uint8_t s_2[STAGE];
+  __shared__ int32_t s_ad[ROWS];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t row0 = blockIdx.x * ROWS;
+  float *const out = a.u + (size_t)blockIdx.y * a.l.seq * a.l.rmax;
   if (w == 0) {
-    const int32_t ad = lora_rows(a.l, row0, 16, lane);
-    if (lane < 16) s_ad[lane] = ad;
+    const int32_t ad = lora_rows(a.l, row0, ROWS, lane);
+    if (lane < ROWS) s_ad[lane] = ad;
   }
   __syncthreads();
-  const uint32_t row = min(row0 + i, a.l.seq - 1);
-  const float *const xr = a.x + (size_t)row * a.k;
-  uint32_t todo = 0;
-  for (int r = 0; r < 16; r++) {
-    if (s_ad[r] >= 0) todo |= 1u << r;
-    else if (row0 + r < a.l.seq)
-      for (uint32_t j = threadIdx.x; j < a.l.rmax; j += 512) a.u[(size_t)(row0 + r) * a.l.rmax + j] = 0.0f;
+  const int32_t own = lane < ROWS ? s_ad[lane] : -1;
+  uint64_t todo = __ballot(own >= 0);
+  // this workgroup's steps
+  const uint32_t all = (a.k + 127) / 128, s0 = (uint64_t)blockIdx.y * all / gridDim.y;
+  const uint32_t n = (uint32_t)((uint64_t)(blockIdx.y + 1) * all / gridDim.y) - s0;
+  const uint64_t none = ~todo;
+  for (uint32_t p = threadIdx.x; p < ROWS * a.l.rmax; p += 256) {
+    const uint32_t r = p / a.l.rmax;
+    if ((none >> r & 1) && row0 + r < a.l.seq) out[(size_t)row0 * a.l.rmax + p] = 0.0f;
   }
-  constexpr int NW = KMAJOR ? 8 * ((NT + 1) / 2) : 4 * NT;  // words of weights a step
-  typedef uint32_t wvec __attribute__((ext_vector_type(NW)));
   while (todo) {
-    const int32_t ad = __builtin_amdgcn_readfirstlane(s_ad[__builtin_ctz(todo)]);
-    uint32_t mine = 0;
-    for (int r = 0; r < 16; r++) mine |= s_ad[r] == ad ? 1u << r : 0u;
+    const int32_t ad = __builtin_amdgcn_readlane(own, __builtin_ctzll(todo));
+    const uint64_t mine = __ballot(own == ad);
     todo &= ~mine;
     const uint32_t rank = lora_rank(a.l, ad);
     const uint16_t *const wt = (KMAJOR ? a.l.b : a.l.a) + (size_t)ad * a.l.rmax * a.k;
-    v4f acc[NT];
+    v4f acc[MT][NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) acc[t] = (v4f){0, 0, 0, 0};
-    // (macros: register sets handed to a lambda end up in scratch)
-#define LOAD(k0, X0, X1, W)                                                                              \
-    do {                                                                                                 \
-      const uint32_t k = (k0) + 8 * g, n = k < a.k ? min(8u, a.k - k) : 0u;                               \
-      X0 = load4<VEC>(xr + k, min(n, 4u));                                                               \
-      X1 = load4<VEC>(xr + k + 4, n > 4 ? n - 4 : 0u);                                                   \
-      if (KMAJOR) {                                                                                      \
-        _Pragma("unroll") for (int e = 0; e < 8; e++) {                                                  \
-          /* ranks NT i .. NT i + NT - 1: all of them lie in a row of rmax, or none */                   \
-          const bool in = (uint32_t)e < n && (uint32_t)(NT * i) < rank;                                  \
-          const uint16_t *p = wt + (in ? (size_t)(k + e) * a.l.rmax + NT * i : (size_t)0);                \
-          if (NT == 1) W[e] = *p;                                                                        \
-          else if (NT == 2) W[e] = *(const uint32_t *)p;                                                 \
-          else if (NT == 4) {                                                                            \
-            const uint2 v = *(const uint2 *)p;                                                           \
-            W[2 * e] = v.x; W[(2 * e + 1) % NW] = v.y;                                                   \
-          } else {                                                                                       \
-            const uint4 v = *(const uint4 *)p;                                                           \
-            W[(4 * e) % NW] = v.x; W[(4 * e + 1) % NW] = v.y;                                            \
-            W[(4 * e + 2) % NW] = v.z; W[(4 * e + 3) % NW] = v.w;                                        \
-          }                                                                                              \
-        }                                                                                                \
-      } else {                                                                                           \
-        _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                 \
-          const bool in = n && (uint32_t)(16 * t + i) < rank;                                            \
-          const uint4 v = *(const uint4 *)(wt + (in ? (size_t)(16 * t + i) * a.k + k : (size_t)0));       \
-          W[(4 * t) % NW] = v.x; W[(4 * t + 1) % NW] = v.y;                                              \
-          W[(4 * t + 2) % NW] = v.z; W[(4 * t + 3) % NW] = v.w;                                          \
-        }                                                                                                \
-      }                                                                                                  \
-    } while (0)
-#define MUL(k0, X0, X1, W)                                                                               \
-    do {                                                                                                 \
-      const uint32_t k = (k0) + 8 * g;                                                                   \
-      _Pragma("unroll") for (int e = 0; e < 8; e++) {                                                    \
-        const float xv = e < 4 ? at4(X0, e) : at4(X1, e - 4);                                            \
-        _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                 \
-          uint32_t h;                                                                                    \
-          bool in;                                                                                       \
-          if (KMAJOR) {                                                                                  \
-            h = NT == 1 ? W[e] : W[(e * (NT / 2) + t / 2) % NW] >> (16 * (t & 1));                       \
-            in = (uint32_t)(NT * i + t) < rank && k + e < a.k;                                           \
-          } else {                                                                                       \
-            h = W[(4 * t + e / 2) % NW] >> (16 * (e & 1));                                               \
-            in = (uint32_t)(16 * t + i) < rank && k < a.k;                                               \
-          }                                                                                              \
-          acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv, in ? wide<BF>(h & 0xffff) : 0.0f, acc[t], 0, 0, 0); \
-        }                                                                                                \
-      }                                                                                                  \
-    } while (0)
-    float4 xa0, xa1, xb0, xb1;
-    wvec wa = {}, wb = {};
-    uint32_t k0 = w * 32;
-    LOAD(k0, xa0, xa1, wa);
-    for (; k0 < a.k; k0 += 512) {
-      if (k0 + 256 < a.k) LOAD(k0 + 256, xb0, xb1, wb);
-      MUL(k0, xa0, xa1, wa);
-      if (k0 + 256 < a.k) {
-        if (k0 + 512 < a.k) LOAD(k0 + 512, xa0, xa1, wa);
-        MUL(k0 + 256, xb0, xb1, wb);
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int t = 0; t < NT; t++) acc[m][t] = (v4f){0, 0, 0, 0};
+    const auto load = [&](uint32_t step, uint8_t *stage) {
+      const uint32_t k0 = (s0 + min(step, n - 1)) * 128;  // (past the end the last one repeats)
+#pragma unroll
+      for (int q = 0; q < NX; q++) {
+        // VEC: two rows of 32 units an instruction; else a quarter of a row in single values
+        const uint32_t at = (w * NX + q) * (VEC ? 1024 : 256), e = at + lane * (VEC ? 16 : 4);
+        const uint32_t r = e / 512, unit = e / 16 % 32 ^ (r & 15), k = k0 + 4 * unit + (VEC ? 0 : e / 4 % 4);
+        const float *p = a.x + (size_t)min(row0 + r, a.l.seq - 1) * a.k + min(k, a.k - (VEC ? 4 : 1));
+        if (VEC) __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 16, 0, 0);
+        else __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 4, 0, 0);
       }
+#pragma unroll
+      for (int q = 0; q < NT; q++) {
+        const uint32_t at = (w * NT + q) * 1024, e = at + lane * 16;
+        const uint16_t *p;
+        if (KMAJOR) {  // 128 rows of rmax as they lie
+          p = wt + min((size_t)k0 * a.l.rmax + e / 2, (size_t)a.k * a.l.rmax - 8);
+        } else {  // 256 bytes of each rank, units swizzled as x's
+          const uint32_t j = e / 256, unit = e / 16 % 16 ^ (j & 15);
+          p = wt + (size_t)min(j, a.l.rmax - 1) * a.k + min(k0 + 8 * unit, a.k - 8);
+        }
+        __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + XB + at), 16, 0, 0);
+      }
+    };
+    const auto mul = [&](uint32_t step, const uint8_t *stage) {
+      const uint32_t kk = 32 * w + 8 * g, k = (s0 + step) * 128 + kk;  // in the stage, and of the row
+      Bf8 p0[MT], p1[MT], p2[MT];
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const uint8_t *const xr = stage + (16 * m + i) * 512;
+        const float4 x0 = *(const float4 *)(xr + 16 * (kk / 4 ^ i)), x1 = *(const float4 *)(xr + 16 * ((kk / 4 + 1) ^ i));
+        split3(x0.x, x0.y, p0[m].u[0], p1[m].u[0], p2[m].u[0]);
+        split3(x0.z, x0.w, p0[m].u[1], p1[m].u[1], p2[m].u[1]);
+        split3(x1.x, x1.y, p0[m].u[2], p1[m].u[2], p2[m].u[2]);
+        split3(x1.z, x1.w, p0[m].u[3], p1[m].u[3], p2[m].u[3]);
+      }
+      // k's of the lane that are there
+      const uint32_t there = k < a.k ? a.k - k : 0u;
+      Bf8 h[NT];
+      if (KMAJOR) {
+        constexpr int NH = (NT + 1) / 2;
+        // (the lane's ranks NT i .. NT i + NT - 1 all lie in a row of rmax, or none does)
+        const uint32_t j = (uint32_t)(NT * i) < a.l.rmax ? NT * i : 0u;
+        uint32_t v[8][NH];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint16_t *const p = (const uint16_t *)(stage + XB) + (kk + e) * a.l.rmax + j;
+          if (NT == 1) v[e][0] = *p;
+          else if (NT == 2) v[e][0] = *(const uint32_t *)p;
+          else if (NT == 4) *(uint2 *)v[e] = *(const uint2 *)p;
+          else *(uint4 *)v[e] = *(const uint4 *)p;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            h[t].u[q] = __builtin_amdgcn_perm(v[2 * q + 1][t / 2], v[2 * q][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          h[t].q = *(const uint4 *)(stage + XB + (16 * t + i) * 256 + 16 * (kk / 8 ^ i));
+      }
+      if ((s0 + step + 1) * 128 > a.k) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int q = 0; q < 4; q++) {
+            if (2 * q >= (int)there) h[t].u[q] = 0;
+            else if (2 * q + 1 >= (int)there) h[t].u[q] &= 0xffffu;
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        Bf8 w0, w1;
+        if (BF) {
+          w0 = h[t];
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; q++) split_f16(h[t].u[q], w0.u[q], w1.u[q]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p0[m].v, w0.v, acc[m][t], 0, 0, 0);
+          acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p1[m].v, w0.v, acc[m][t], 0, 0, 0);
+          acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p2[m].v, w0.v, acc[m][t], 0, 0, 0);
+          if (!BF) {
+            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p0[m].v, w1.v, acc[m][t], 0, 0, 0);
+            acc[m][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p1[m].v, w1.v, acc[m][t], 0, 0, 0);
+          }
+        }
+      }
+    };
+    // step s: its stage has landed (the one behind it may be on the way), every wave is done with the one before it,
+    // whose room the loads of step s + 2 take
+#define STEP(s, CUR, FREE)            \
+    {                                 \
+      ORDER();                        \
+      WAIT_VM(NX + NT);               \
+      __builtin_amdgcn_s_barrier();   \
+      ORDER();                        \
+      load((s) + 2, FREE);            \
+      mul(s, CUR);                    \
     }
-#undef MUL
-#undef LOAD
+    load(0, s_0);
+    ORDER();
+    load(1, s_1);
+    for (uint32_t s = 0; s < n; s += 3) {
+      STEP(s, s_0, s_2)
+      if (s + 1 < n) STEP(s + 1, s_1, s_0)
+      if (s + 2 < n) STEP(s + 2, s_2, s_1)
+    }
+#undef STEP
+    ORDER();
+    WAIT_VM(0);
+    __syncthreads();
+    float *const su = (float *)s_0;  // [2][ROWS][16 NT + 4]
+    constexpr int PITCH = NT * 16 + 4;
+    // a wave's sums: the first two waves', then the others' on top
+    static_assert(2 * ROWS * PITCH * 4 <= STAGE, "two waves' sums in a stage");
+    if (w < 2)
 #pragma unroll
-    for (int t = 0; t < NT; t++)
+      for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) s_u[w][4 * g + r][KMAJOR ? NT * i + t : 16 * t + i] = acc[t][r];
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) su[(w * ROWS + 16 * m + 4 * g + r) * PITCH + (KMAJOR ? NT * i + t : 16 * t + i)] = acc[m][t][r];
+    __syncthreads();
+    if (w >= 2)
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) su[((w - 2) * ROWS + 16 * m + 4 * g + r) * PITCH + (KMAJOR ? NT * i + t : 16 * t + i)] += acc[m][t][r];
     __syncthreads();
     const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
-    for (uint32_t p = threadIdx.x; p < 16 * a.l.rmax; p += 512) {
+    for (uint32_t p = threadIdx.x; p < ROWS * a.l.rmax; p += 256) {
       const uint32_t r = p / a.l.rmax, j = p % a.l.rmax;
-      if (mine >> r & 1) {
-        float v = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 8; q++) v += s_u[q][r][j];
-        a.u[(size_t)(row0 + r) * a.l.rmax + j] = j < rank ? v * sc : 0.0f;
-      }
+      if (mine >> r & 1)
+        out[(size_t)row0 * a.l.rmax + p] = j < rank ? (su[r * PITCH + j] + su[(ROWS + r) * PITCH + j]) * sc : 0.0f;
     }
     __syncthreads();
   }
@@ -311,7 +423,7 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       const uint32_t row = min(row0 + 16 * m + 4 * g + r, a.l.seq - 1);
-      res[m][r] = a.res ? load4<VEC>(a.res + (size_t)row * a.n + col, nc) : make_float4(0, 0, 0, 0);
+      res[m][r] = a.res ? inside4<VEC>(a.res + (size_t)row * a.n, col, a.n) : make_float4(0, 0, 0, 0);
     }
   if (w == 0) {
     const int32_t ad = lora_rows(a.l, row0, 32, lane);
@@ -349,30 +461,46 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
 #pragma unroll
       for (int m = 0; m < 2; m++) {
         const uint32_t row = min(row0 + 16 * m + i, a.l.seq - 1);
-        uv[m] = j < a.l.rmax ? *(const float4 *)(a.u + (size_t)row * a.l.rmax + j) : make_float4(0, 0, 0, 0);
+        uv[m] = *(const float4 *)(a.u + (size_t)row * a.l.rmax + min(j, a.l.rmax - 4));
       }
       uint2 v[4];  // KMAJOR: rank j + q, columns col ..; else column col + q, ranks j ..
 #pragma unroll
       for (int q = 0; q < 4; q++) {
-        v[q] = make_uint2(0, 0);
-        if (KMAJOR) {
-          if (j + q < rank && nc) v[q] = *(const uint2 *)(wt + (size_t)(j + q) * a.n + col);
-        } else {
-          if (j < rank && (uint32_t)q < nc) v[q] = *(const uint2 *)(wt + (size_t)(col + q) * a.l.rmax + j);
+        if (KMAJOR) v[q] = *(const uint2 *)(wt + (size_t)min(j + q, a.l.rmax - 1) * a.n + min(col, a.n - 4));
+        else v[q] = *(const uint2 *)(wt + (size_t)min(col + q, a.n - 1) * a.l.rmax + min(j, a.l.rmax - 4));
+      }
+      if (j0 + 16 > rank) {  // ranks behind the rank: neither factor counts
+#pragma unroll
+        for (int m = 0; m < 2; m++) {
+          if (j >= rank) uv[m].x = 0.0f;
+          if (j + 1 >= rank) uv[m].y = 0.0f;
+          if (j + 2 >= rank) uv[m].z = 0.0f;
+          if (j + 3 >= rank) uv[m].w = 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint32_t c = KMAJOR ? j + q : j;
+          if (KMAJOR) {
+            if (c >= rank) v[q] = make_uint2(0, 0);
+          } else {
+            if (c >= rank) v[q].x &= 0xffff0000u;
+            if (c + 1 >= rank) v[q].x &= 0xffffu;
+            if (c + 2 >= rank) v[q].y &= 0xffff0000u;
+            if (c + 3 >= rank) v[q].y &= 0xffffu;
+          }
         }
       }
 #pragma unroll
       for (int s = 0; s < 4; s++) {  // rank j + s
-        const bool in = j + s < rank;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const uint2 p = v[KMAJOR ? s : e];
           const int f = KMAJOR ? e : s;
           const uint32_t h = (f & 2 ? p.y : p.x) >> (16 * (f & 1)) & 0xffff;
-          const float b = in ? wide<BF>(h) : 0.0f;
+          const float b = wide<BF>(h);
 #pragma unroll
           for (int m = 0; m < 2; m++)
-            acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(in ? at4(uv[m], s) : 0.0f, b, acc[m][e], 0, 0, 0);
+            acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(at4(uv[m], s), b, acc[m][e], 0, 0, 0);
         }
       }
     }
@@ -522,14 +650,19 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
       float pv[4][NT];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        const int64_t row = s + k * step + g;
-        const bool in = row < s1;
-        qv[k] = load4<VEC>(a.q + (size_t)(in ? row : s0) * a.n + col, in ? nc : 0);
+        const int64_t row = min(s + k * step + g, s1 - 1);
+        qv[k] = inside4<VEC>(a.q + (size_t)row * a.n, col, a.n);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-          const uint32_t j = 16 * t + i;
-          pv[k][t] = in && j < rank ? a.p[(size_t)row * a.l.rmax + j] : 0.0f;
-        }
+        for (int t = 0; t < NT; t++) pv[k][t] = a.p[(size_t)row * a.l.rmax + min(16u * t + i, a.l.rmax - 1)];
+      }
+      if (s + 3 * step + 4 > s1) {  // rows past the request's: neither factor counts
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (s + k * step + g >= s1) {
+            qv[k] = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < NT; t++) pv[k][t] = 0.0f;
+          }
       }
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -568,14 +701,16 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
       for (int e = 0; e < 4; e++)
         if ((uint32_t)e < nc)
           *(float4 *)(o + (size_t)(col + e) * a.l.rmax + j) =
-              make_float4(acc[t][e][0] * sc, acc[t][e][1] * sc, acc[t][e][2] * sc, acc[t][e][3] * sc);
+              make_float4(j < rank ? acc[t][e][0] * sc : 0.0f, j + 1 < rank ? acc[t][e][1] * sc : 0.0f,
+                          j + 2 < rank ? acc[t][e][2] * sc : 0.0f, j + 3 < rank ? acc[t][e][3] * sc : 0.0f);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const uint32_t j = 16 * t + 4 * g + r;
         if (j < a.l.rmax)
           store4<VEC>(o + (size_t)j * a.n + col, nc,
-                      make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc));
+                      j < rank ? make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc)
+                               : make_float4(0, 0, 0, 0));
       }
     }
   }
@@ -621,14 +756,39 @@ static bool lora_sizes(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax)
   return seq && out && cols && cols % 8 == 0 && rmax && rmax % 8 == 0 && rmax <= LORA_RANK && seq <= LORA_ROWS &&
          out <= 0x1000000u && cols <= 0x1000000u;
 }
-static size_t lora_round(size_t n) { return (n + 255) / 256 * 256; }
 static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
   return a && b && x < y + nb && y < x + na;
 }
 
-static int lora_down(const char *what, const DownArgs &d, bool bf, bool kmajor, hipStream_t st) {
-  const dim3 grid((d.l.seq + 15) / 16), blk(512);
+static int lora_sum(const char *what, const float *parts, float *out, uint64_t n4, uint32_t np, hipStream_t st) {
+  const uint32_t blocks = nlg_blocks(n4, 256);
+  hipLaunchKernelGGL(k_lora_sum, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, st, (const float4 *)parts,
+                     (float4 *)out, n4, np);
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+// How many parts a contraction over k columns is summed in: until two workgroups a CU have some, each of four steps at
+// least.
+static uint32_t lora_ksplit(uint32_t seq, uint32_t k) {
+  const uint64_t tiles = ((uint64_t)seq + 31) / 32, most = k / 512;
+  uint64_t n = 512 / tiles;
+  if (n > most) n = most;
+  return n < 1 ? 1 : n > 8 ? 8 : (uint32_t)n;
+}
+static size_t lora_round(size_t n) { return (n + 255) / 256 * 256; }
+static size_t lora_down_bytes(uint32_t seq, uint32_t k, uint32_t rmax) {
+  const uint32_t n = lora_ksplit(seq, k);
+  return n > 1 ? lora_round((size_t)n * seq * rmax * 4) : 0;
+}
+
+// parts: lora_down_bytes
+static int lora_down(const char *what, DownArgs d, bool bf, bool kmajor, float *parts, hipStream_t st) {
+  const uint32_t np = lora_ksplit(d.l.seq, d.k);
+  float *const u = d.u;
+  if (np > 1) d.u = parts;
+  const dim3 grid((d.l.seq + 31) / 32, np), blk(256);
   const bool vec = d.k % 4 == 0 && ((uintptr_t)d.x & 15) == 0;
   const uint32_t nt = (d.l.rmax + 15) / 16;
 #define GO(BF, KM, N)                                                                          \
@@ -650,7 +810,7 @@ static int lora_down(const char *what, const DownArgs &d, bool bf, bool kmajor, 
 #undef GO2
 #undef GO
   NLG_LAUNCHED(what);
-  return NLG_OK;
+  return np > 1 ? lora_sum(what, parts, u, (uint64_t)d.l.seq * d.l.rmax / 4, np, st) : NLG_OK;
 }
 
 static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipStream_t st) {
@@ -702,13 +862,7 @@ static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, hi
 #undef GO2
 #undef GO
   NLG_LAUNCHED(what);
-  if (np > 1) {
-    const uint64_t n4 = (uint64_t)d.l.adapters * d.l.rmax * d.n / 4;
-    hipLaunchKernelGGL(k_lora_sum, dim3(nlg_blocks(n4, 256) < 2048 ? nlg_blocks(n4, 256) : 2048), dim3(256), 0, st,
-                       (const float4 *)parts, (float4 *)out, n4, np);
-    NLG_LAUNCHED(what);
-  }
-  return NLG_OK;
+  return np > 1 ? lora_sum(what, parts, out, (uint64_t)d.l.adapters * d.l.rmax * d.n / 4, np, st) : NLG_OK;
 }
 
 // Few rows a request, or few rows at all.
@@ -784,7 +938,19 @@ static int lora_tok_up(const char *what, const UpArgs &p, bool bf, hipStream_t s
 
 extern "C" size_t nlg_lora_linear_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests) {
   (void)requests;
-  return lora_sizes(seq, out, cols, rmax) ? lora_round((size_t)seq * rmax * 4) : 0;
+  return lora_sizes(seq, out, cols, rmax) ? lora_round((size_t)seq * rmax * 4) + lora_down_bytes(seq, cols, rmax) : 0;
+}
+
+// ws: nlg_lora_linear_workspace
+static int lora_forward(const char *what, const LoraArgs &l, const float *x, bool bf, const float *res, float *y, float *u,
+                        uint32_t out, uint32_t cols, void *ws, hipStream_t st) {
+  DownArgs d{};
+  d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)ws;
+  UpArgs p{};
+  p.l = l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
+  if (lora_by_token(l)) return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
+  float *const parts = (float *)((uint8_t *)ws + lora_round((size_t)l.seq * l.rmax * 4));
+  return lora_down(what, d, bf, false, parts, st) || lora_up(what, p, bf, false, st);
 }
 
 extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t *b, int fmt, const float *scale,
@@ -793,30 +959,21 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
                                uint32_t out, uint32_t cols, void *workspace, size_t workspace_bytes, void *stream) {
   const char *what = "lora linear";
   if (!seq) return NLG_OK;
-  DownArgs d{};
-  if (lora_check(what, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, seq, out, cols, d.l)) return NLG_ERR;
+  LoraArgs l;
+  if (lora_check(what, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, seq, out, cols, l)) return NLG_ERR;
   if (!x || !y) return nlg_fail("%s: null pointer", what);
   if (((uintptr_t)x | (uintptr_t)u) & 15) return nlg_fail("%s: x and u must be 16-byte aligned", what);
   if (((uintptr_t)y | (uintptr_t)res) & 3) return nlg_fail("%s: y and res must be 4-byte aligned", what);
-  const size_t need = u ? 0 : nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
-  if (need && (!workspace || workspace_bytes < need))
+  const size_t need = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
+  if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
-  if (need && ((uintptr_t)workspace & 15)) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
+  if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
   const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nu = (uint64_t)seq * rmax * 4;
   if (overlap(y, ny, x, nx) || overlap(u, nu, x, nx) || overlap(u, nu, y, ny) || (res != y && overlap(y, ny, res, ny)) ||
       overlap(u, nu, res, ny))
     return nlg_fail("%s: outputs overlap each other or an input (y may be res itself)", what);
   NLG_SCOPE(what);
-  hipStream_t st = nlg_stream(stream);
-  d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
-  UpArgs p{};
-  p.l = d.l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
-  if (lora_by_token(d.l)) {
-    const bool bf = fmt == NLG_LORA_BF16;
-    return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
-  }
-  if (lora_down(what, d, fmt == NLG_LORA_BF16, false, st)) return NLG_ERR;
-  return lora_up(what, p, fmt == NLG_LORA_BF16, false, st);
+  return lora_forward(what, l, x, fmt == NLG_LORA_BF16, res, y, u, out, cols, workspace, nlg_stream(stream)) ? NLG_ERR : NLG_OK;
 }
 
 extern "C" size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax,
@@ -842,7 +999,8 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   if (((uintptr_t)y | (uintptr_t)bias | (uintptr_t)beta) & 3)
     return nlg_fail("%s: y, bias and beta must be 4-byte aligned", what);
   if (cols > 16384) return nlg_fail("%s: cols must be at most 16384 (got %u)", what, cols);
-  const size_t nu = lora_round((size_t)seq * rmax * 4), need = nlg_ternary_linear_lora_workspace(seq, out, cols, rmax, requests);
+  const size_t nu = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
+  const size_t need = nlg_ternary_linear_lora_workspace(seq, out, cols, rmax, requests);
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
@@ -853,30 +1011,30 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   hipStream_t st = nlg_stream(stream);
   uint8_t *const more = (uint8_t *)workspace + nu;
   const bool bf = fmt == NLG_LORA_BF16;
-  float *const us = u ? u : (float *)workspace;
   if (nlg_batched(seq, cols)) {
     float *const gamma = (float *)(more + ((size_t)seq * cols + 255) / 256 * 256);
     FusedArgs f{};
     f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;
     f.y = y; f.ystride = out;
-    DownArgs d{};
-    d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = us;
-    UpArgs p{};
-    p.l = l; p.u = us; p.res = y; p.y = y; p.n = out; p.scaled = true;
     if (lora_by_token(l)) {
+      DownArgs d{};
+      d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
+      UpArgs p{};
+      p.l = l; p.u = d.u; p.res = y; p.y = y; p.n = out; p.scaled = true;
       const ActQArgs q{x, nullptr, 0.0f, nullptr, 0, 0, more, gamma, seq, cols, 0u};
       return lora_tok(what, d, p, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) ||
-             lora_tok_up(what, p, bf, st);
+                     lora_tok_up(what, p, bf, st)
+                 ? NLG_ERR
+                 : NLG_OK;
     }
-    if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st)) return NLG_ERR;
-    return nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) || lora_down(what, d, bf, false, st) ||
-           lora_up(what, p, bf, false, st);
-  }
-  if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more, workspace_bytes - nu,
-                         (void *)st))
+    if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st) ||
+        nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st))
+      return NLG_ERR;
+  } else if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more,
+                                workspace_bytes - nu, (void *)st)) {
     return NLG_ERR;
-  return nlg_lora_linear(x, a, b, fmt, scale, rank, start, adapter, requests, adapters, rmax, y, y, us, seq, out, cols,
-                         nullptr, 0, (void *)st);
+  }
+  return lora_forward(what, l, x, bf, y, y, u, out, cols, workspace, st) ? NLG_ERR : NLG_OK;
 }
 
 // du and u, and the parts of one of the two gradients
@@ -888,6 +1046,10 @@ extern "C" size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uin
   for (const uint32_t n : {out, cols}) {
     const uint32_t parts = lora_parts(seq, n, adapters);
     const size_t bytes = parts > 1 ? (size_t)parts * adapters * rmax * n * 4 : 0;
+    most = bytes > most ? bytes : most;
+  }
+  for (const uint32_t k : {out, cols}) {  // (the same room: the contractions come first)
+    const size_t bytes = lora_down_bytes(seq, k, rmax);
     most = bytes > most ? bytes : most;
   }
   return 2 * lora_round((size_t)seq * rmax * 4) + lora_round(most);
@@ -925,18 +1087,17 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   const bool bf = fmt == NLG_LORA_BF16;
-  float *const du = (float *)workspace;
+  float *const du = (float *)workspace, *const parts = (float *)((uint8_t *)workspace + 2 * nu);
   if (!u) {
     d.x = x; d.k = cols; d.scaled = false; d.u = (float *)((uint8_t *)workspace + nu);
     u = d.u;
-    if (lora_down(what, d, bf, false, st)) return NLG_ERR;
+    if (lora_down(what, d, bf, false, parts, st)) return NLG_ERR;
   }
   d.x = dy; d.k = out; d.scaled = true; d.u = du;
-  if (lora_down(what, d, bf, true, st)) return NLG_ERR;
+  if (lora_down(what, d, bf, true, parts, st)) return NLG_ERR;
   OuterArgs o{};
   o.l = d.l;
   o.p = u; o.q = dy; o.out = db; o.n = out; o.scaled = true;
-  float *const parts = (float *)((uint8_t *)workspace + 2 * nu);
   if (lora_outer(what, o, true, parts, st)) return NLG_ERR;
   o.p = du; o.q = x; o.out = da; o.n = cols; o.scaled = false;
   if (lora_outer(what, o, false, parts, st)) return NLG_ERR;
