@@ -32,6 +32,7 @@
 #include <math.h>
 
 #include "nlg_act_q.h"
+#include "nlg_lora.h"
 
 typedef int v4i __attribute__((ext_vector_type(4)));
 
@@ -74,7 +75,14 @@ struct GemmArgs {
   int32_t *ksum;
   uint32_t *kctr;
   bool allow_split;  // the launcher may take split workspace from the library
+  // EPI_LORA_*: the rows' adapters and what they are on the way up from
+  LoraArgs lora;
+  const float *lu;     // [seq][rmax]
 };
+
+// kernel-internal: NLG_EPI_STORE with low-rank adapters of either format added
+enum { NLG_EPI_LORA_F16 = 100, NLG_EPI_LORA_BF16 = 101 };
+#define TG_LORA(epi) ((epi) == NLG_EPI_LORA_F16 || (epi) == NLG_EPI_LORA_BF16)
 
 // One output element of the batched linear (every lane calls it: the SwiGLU
 // and RoPE pairs are exchanged across lanes l, l^1, which hold rows 2j, 2j+1).
@@ -525,6 +533,84 @@ __device__ __forceinline__ bool tl_split_meet(const GemmArgs &a, v16i (&acc)[MB]
   return true;
 }
 
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// What the adapters add to the 32 tokens tok0 .. of rows rc[nt], added to val[nt] (register r:
+// token (r % 4) + 8 (r / 4) + 4 lg), with s_ad the tokens' adapters: u
+// in three bf16 parts times the adapter's rows (an f16 value in two), in 32
+// x 32 x 16 products, sixteen ranks at a time; of the products of parts that of
+// the last two is left out, 2^-24 of the whole.  Each adapter among the tokens is one
+// pass, whose sums count for its own tokens alone.
+template <int NB, bool BF>
+__device__ __forceinline__ void tl_lora(const GemmArgs &a, v16f (&val)[NB], const uint32_t (&rc)[NB], const int32_t *s_ad,
+                                        int lane, int lg, uint32_t tok0) {
+  const LoraArgs &l = a.lora;
+  const int li = lane & 31;
+  const int32_t own = s_ad[li];
+  uint64_t todo = __ballot(own >= 0) & 0xffffffffull;
+  const float *const ur = a.lu + (size_t)min(tok0 + li, a.seq - 1) * l.rmax;
+  while (todo) {
+    const int32_t ad = __builtin_amdgcn_readlane(own, __builtin_ctzll(todo));
+    const uint32_t mine = (uint32_t)(__ballot(own == ad) & 0xffffffffull);
+    todo &= ~(uint64_t)mine;
+    const uint32_t rank = lora_rank(l, ad);
+    const uint16_t *const wt = l.b + (size_t)ad * a.out * l.rmax;
+    v16f c[NB];
+#pragma unroll
+    for (int nt = 0; nt < NB; nt++) c[nt] = (v16f){};
+    for (uint32_t j0 = 0; j0 < rank; j0 += 16) {
+      const uint32_t j = j0 + 8 * lg, jc = min(j, l.rmax - 8);
+      const float4 u0 = *(const float4 *)(ur + jc), u1 = *(const float4 *)(ur + jc + 4);
+      Bf8 h[NB], p0, p1, p2;
+#pragma unroll
+      for (int nt = 0; nt < NB; nt++) h[nt].q = *(const uint4 *)(wt + (size_t)rc[nt] * l.rmax + jc);
+      split3(u0.x, u0.y, p0.u[0], p1.u[0], p2.u[0]);
+      split3(u0.z, u0.w, p0.u[1], p1.u[1], p2.u[1]);
+      split3(u1.x, u1.y, p0.u[2], p1.u[2], p2.u[2]);
+      split3(u1.z, u1.w, p0.u[3], p1.u[3], p2.u[3]);
+      if (j0 + 16 > rank) {  // ranks behind the rank: neither factor counts
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+          const uint32_t keep = j + 2 * q + 1 < rank ? 0xffffffffu : j + 2 * q < rank ? 0xffffu : 0u;
+          p0.u[q] &= keep;
+          p1.u[q] &= keep;
+          p2.u[q] &= keep;
+#pragma unroll
+          for (int nt = 0; nt < NB; nt++) h[nt].u[q] &= keep;
+        }
+      }
+      // the same accumulator comes every NB products
+      Bf8 w0[NB], w1[NB];
+#pragma unroll
+      for (int nt = 0; nt < NB; nt++) {
+        if (BF) {
+          w0[nt] = h[nt];
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; q++) split_f16(h[nt].u[q], w0[nt].u[q], w1[nt].u[q]);
+        }
+      }
+#define LORA_MUL(P, W) \
+  _Pragma("unroll") for (int nt = 0; nt < NB; nt++) c[nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(P.v, W[nt].v, c[nt], 0, 0, 0);
+      LORA_MUL(p0, w0)
+      LORA_MUL(p1, w0)
+      LORA_MUL(p2, w0)
+      if (!BF) {
+        LORA_MUL(p0, w1)
+        LORA_MUL(p1, w1)
+      }
+#undef LORA_MUL
+    }
+    const float sc = l.scale[ad];
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const bool in = mine >> ((r % 4) + 8 * (r / 4) + 4 * lg) & 1;
+#pragma unroll
+      for (int nt = 0; nt < NB; nt++) val[nt][r] = in ? __fadd_rn(val[nt][r], __fmul_rn(sc, c[nt][r])) : val[nt][r];
+    }
+  }
+}
+
 // The epilogue of k_tgemm_w: acc[mt][nt] of lane (li, lg) of the wave (MB
 // token blocks from token tok0 + 64 wm; the kernel passes wm = 0), rows
 // rw[nt] (clamped rc[nt]), with bias bo and beta be per row block and the
@@ -539,6 +625,30 @@ __device__ __forceinline__ void tl_epilogue(const GemmArgs &a, const v16i (&acc)
                                             const uint32_t (&rc)[NB], const float (&bo)[NB], const float (&be)[NB],
                                             const float *s_gm, int lane, int wm, int lg, uint32_t tok0,
                                             const int32_t *s_tp, const uint64_t *s_tb) {
+  if (TG_LORA(EPI)) {
+#pragma unroll
+    for (int mt = 0; mt < MB; mt++) {
+      // the projection's values, then the adapters' on top
+      v16f val[NB];
+#pragma unroll
+      for (int nt = 0; nt < NB; nt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const float g = s_gm[32 * mt + (r % 4) + 8 * (r / 4) + 4 * lg];
+          val[nt][r] = __fadd_rn(bo[nt], __fmul_rn(__fmul_rn(be[nt], g), (float)(acc[mt][nt][r] >> 6)));
+        }
+      tl_lora<NB, EPI == NLG_EPI_LORA_BF16>(a, val, rc, s_tp + 32 * mt, lane, lg, tok0 + 32 * mt);
+#pragma unroll
+      for (int nt = 0; nt < NB; nt++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const uint32_t tk = tok0 + 32 * mt + (r % 4) + 8 * (r / 4) + 4 * lg;
+          if (rw[nt] < a.out && tk < a.seq) a.y[(size_t)tk * a.ystride + rw[nt]] = val[nt][r];
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
   // acc[mt][nt] register r is token tok0 + 64 wm + 32 mt + (r%4) + 8 (r/4) + 4 lg,
   // row rw[nt].  gamma comes from LDS; the residual and RoPE
   // operands of a (token block, row block) are all fetched before its first
@@ -730,7 +840,7 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
   __shared__ __align__(1024) uint8_t s_a0[STAGE];
   __shared__ __align__(1024) uint8_t s_a1[STAGE];
   __shared__ float s_gm[128];
-  __shared__ int32_t s_tp[EPI == NLG_EPI_QKV ? 128 : 1];
+  __shared__ int32_t s_tp[EPI == NLG_EPI_QKV || TG_LORA(EPI) ? 128 : 1];  // LORA: the tokens' adapters
   __shared__ uint64_t s_tb[EPI == NLG_EPI_QKV ? 128 : 1];
   asm volatile("" ::"s"(a.xq), "s"(a.gamma), "s"(a.w2), "s"(a.bias), "s"(a.beta), "s"(a.y), "s"(a.seq),
                "s"(a.out), "s"(a.cols), "s"(a.wng), "s"(a.ystride), "s"(a.beta_per_row));
@@ -917,6 +1027,13 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
     __shared__ uint32_t s_last;
     if (!tl_split_meet<MB, NB>(a, acc, &s_last)) return;
   }
+  if (TG_LORA(EPI)) {
+    if (wn == 0) {
+      const int32_t ad = lora_rows(a.lora, tok0, MT, lane);
+      if (lane < MT) s_tp[lane] = ad;
+    }
+    __syncthreads();
+  }
   tl_epilogue<MB, NB, EPI>(a, acc, rw, rc, bo, be, s_gm, lane, 0, lg, tok0, s_tp, s_tb);
 }
 #undef TW_ORDER
@@ -946,6 +1063,8 @@ int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *
   return NLG_OK;
 }
 
+// (of an EPI_LORA_* launch: another form than k_tgemm_w would run, so none did)
+#define NLG_TGEMM_OTHER 2
 int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
   GemmArgs a = a0;
   if (!a.seq || !a.out) return NLG_OK;
@@ -971,6 +1090,7 @@ int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
   // 8.7 against 9.6; at 432 tiles k_tgemm kept the lead (gate|up at 64
   // tokens 10.9 against 11.7, 6,912 x 2560 at 112 10.6 against 12.0).
   const bool wide = a.seq >= 128 || (a.seq > 64 && t64x32 > 512);
+  if (TG_LORA(epi) && (!wide || one_phase)) return NLG_TGEMM_OTHER;
   if (wide && epi != NLG_EPI_ARGMAX && !one_phase) {
     // 256-row tiles of the wide-wave kernel (k_tgemm_w), 64-token tiles
     // once there are 400 of them, else 32-token ones; a few tiles of long
@@ -1050,6 +1170,8 @@ int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
       case NLG_EPI_RESID: TWG(NLG_EPI_RESID); break;
       case NLG_EPI_SWIGLU: TWG(NLG_EPI_SWIGLU); break;
       case NLG_EPI_QKV: TWG(NLG_EPI_QKV); break;
+      case NLG_EPI_LORA_F16: TWG(NLG_EPI_LORA_F16); break;
+      case NLG_EPI_LORA_BF16: TWG(NLG_EPI_LORA_BF16); break;
       default: return nlg_fail("ternary GEMM: unknown epilogue %d", epi);
     }
 #undef TWG
@@ -1206,7 +1328,7 @@ int nlg_batched_launch(const FusedArgs &f, int pro, int epi, hipStream_t st) {
   return nlg_batched_gemm(f, xq, gamma, epi, st);
 }
 
-int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st) {
+static GemmArgs gemm_args(const FusedArgs &f, const uint8_t *xq, const float *gamma) {
   GemmArgs g{};
   g.xq = xq; g.gamma = gamma; g.w2 = f.w2; g.bias = f.bias; g.beta = f.beta; g.beta_per_row = f.beta_per_row;
   g.seq = f.seq; g.out = f.out; g.cols = f.cols; g.y = f.y; g.ystride = f.ystride; g.res = f.res;
@@ -1214,5 +1336,19 @@ int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, 
   g.co = f.co; g.si = f.si; g.pos = f.pos; g.kc = f.kc; g.vc = f.vc; g.qper = f.qper;
   g.pval = f.pval; g.pidx = f.pidx;
   g.allow_split = !f.act_scratch;  // caller-provided scratch: no library allocation
-  return nlg_tgemm_launch(g, epi, st);
+  return g;
+}
+
+int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st) {
+  return nlg_tgemm_launch(gemm_args(f, xq, gamma), epi, st);
+}
+
+int nlg_batched_gemm_lora(const FusedArgs &f, const uint8_t *xq, const float *gamma, const LoraArgs &l, const float *u,
+                          bool bf, bool *done, hipStream_t st) {
+  GemmArgs g = gemm_args(f, xq, gamma);
+  g.lora = l;
+  g.lu = u;
+  const int rc = nlg_tgemm_launch(g, bf ? NLG_EPI_LORA_BF16 : NLG_EPI_LORA_F16, st);
+  *done = rc != NLG_TGEMM_OTHER;
+  return *done ? rc : nlg_tgemm_launch(g, NLG_EPI_STORE, st);
 }

@@ -122,3 +122,49 @@ def test_backward(i, bf):
     for g, w, n in zip(c.backward(dres=False), c.want_grad(u, dres=False), ("dx", "da", "db")):
         close(g, w, n)
     assert c.backward(u=given, dx=False)[0] is None
+
+
+# ------------------------------------------------------------------ beside the ternary linear
+
+def ternary(c, per_row, bias, keep=True, stream=None):
+    """The whole call on a Case (with weights made here); y, u, and the base alone as nlg_ternary_linear gives it."""
+    rng = np.random.default_rng(c.seq + c.out)
+    w = nlgpu.pack_ternary(nlgpu.trits(c.out, (c.out, c.cols)))
+    beta = rng.uniform(0.01, 0.05, c.out if per_row else 1).astype(F32)
+    bo = rng.standard_normal(c.out).astype(F32) if bias else None
+    d = {k: up(v) for k, v in dict(x=c.x, w=w, beta=beta, bias=bo).items()}
+    base, y = up(np.full((c.seq, c.out), np.nan, F32)), up(np.full((c.seq, c.out), np.nan, F32))
+    ws = nlgpu.DeviceArray(max(16, nlgpu.ternary_linear_workspace(c.seq, c.cols)))
+    nlgpu.ternary_linear(d["x"], d["w"], d["bias"], d["beta"], base, c.seq, c.out, c.cols, beta_per_row=per_row, workspace=ws)
+    nlgpu.sync()
+    u = up(np.full((c.seq, c.rmax), np.nan, F32)) if keep else None
+    ws = nlgpu.DeviceArray(nlgpu.ternary_linear_lora_workspace(c.seq, c.out, c.cols, c.rmax, len(c.adapter)))
+    nlgpu.ternary_linear_lora(d["x"], d["w"], d["bias"], d["beta"], up(c.a16), up(c.b16), up(c.scale), up(c.adapter), y,
+                              c.seq, c.out, c.cols, c.n, c.rmax, len(c.adapter), ws, start=up(c.start), rank=up(c.rank),
+                              u=u, fmt=c.fmt, beta_per_row=per_row, stream=stream)
+    nlgpu.sync(stream)
+    return y.download(F32), u.download(F32) if keep else None, base.download(F32).reshape(c.seq, c.out)
+
+
+# one row; a few; rows of a step; column tiles cut; prompts on the wide kernel (64-token tiles, split columns, one phase)
+BESIDE = [dict(lengths=[1], adapter=[0], adapters=1, rmax=16, out=100, cols=256),
+          dict(lengths=[1, 1, 1], adapter=[1, -1, 0], adapters=2, rmax=8, out=64, cols=72),
+          dict(lengths=[1] * 33, adapter=[i % 5 - 1 for i in range(33)], adapters=4, rmax=40, out=320, cols=512, mixed=True),
+          dict(lengths=[1] * 6, adapter=[0, 1] * 3, adapters=2, rmax=16, out=70, cols=192),
+          dict(lengths=[40, 60], adapter=[0, 1], adapters=2, rmax=24, out=200, cols=768, mixed=True),
+          dict(lengths=[70, 1, 0, 200], adapter=[2, 1, 0, 0], adapters=3, rmax=32, out=520, cols=1024, mixed=True, behind=3),
+          dict(lengths=[100, 200, 33], adapter=[0, -1, 1], adapters=2, rmax=128, out=300, cols=4352, mixed=True),
+          dict(lengths=[513, 700], adapter=[1, 0], adapters=2, rmax=16, out=6700, cols=256, first=5)]
+
+
+@pytest.mark.parametrize("bf", [False, True])
+@pytest.mark.parametrize("i", range(len(BESIDE)))
+def test_beside_ternary(i, bf):
+    c = Case(bf=bf, **BESIDE[i])
+    y, u, base = ternary(c, per_row=i % 2 == 0, bias=i % 3 == 0)
+    want, wu = ref.forward(c.x.astype(float), c.a, c.b, c.scale.astype(float), c.rank, c.of, ref.Sums(base.astype(float)))
+    close(u, wu, "u")
+    close(y, want, "y")
+    none = c.of < 0
+    assert np.array_equal(y.reshape(c.seq, c.out)[none], base[none])  # the linear's own bits
+    assert np.array_equal(ternary(c, i % 2 == 0, i % 3 == 0, keep=False)[0], y)
