@@ -88,6 +88,25 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t row0 = blockIdx.x * ROWS;
   float *const out = a.u + (size_t)blockIdx.y * a.l.seq * a.l.rmax;
+  // this workgroup's steps
+  const uint32_t all = (a.k + 127) / 128, s0 = (uint64_t)blockIdx.y * all / gridDim.y;
+  const uint32_t n = (uint32_t)((uint64_t)(blockIdx.y + 1) * all / gridDim.y) - s0;
+  const auto loadx = [&](uint32_t step, uint8_t *stage) {
+    const uint32_t k0 = (s0 + min(step, n - 1)) * 128;  // (past the end the last one repeats)
+#pragma unroll
+    for (int q = 0; q < NX; q++) {
+      // VEC: two rows of 32 units an instruction; else a quarter of a row in single values
+      const uint32_t at = (w * NX + q) * (VEC ? 1024 : 256), e = at + lane * (VEC ? 16 : 4);
+      const uint32_t r = e / 512, unit = e / 16 % 32 ^ (r & 15), k = k0 + 4 * unit + (VEC ? 0 : e / 4 % 4);
+      const float *p = a.x + (size_t)min(row0 + r, a.l.seq - 1) * a.k + min(k, a.k - (VEC ? 4 : 1));
+      if (VEC) __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 16, 0, 0);
+      else __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 4, 0, 0);
+    }
+  };
+  // (the first rows are on the way while their adapters are found)
+  loadx(0, s_0);
+  loadx(1, s_1);
+  ORDER();
   if (w == 0) {
     const int32_t ad = lora_rows(a.l, row0, ROWS, lane);
     if (lane < ROWS) s_ad[lane] = ad;
@@ -95,10 +114,8 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
   __syncthreads();
   const int32_t own = lane < ROWS ? s_ad[lane] : -1;
   uint64_t todo = __ballot(own >= 0);
-  // this workgroup's steps
-  const uint32_t all = (a.k + 127) / 128, s0 = (uint64_t)blockIdx.y * all / gridDim.y;
-  const uint32_t n = (uint32_t)((uint64_t)(blockIdx.y + 1) * all / gridDim.y) - s0;
   const uint64_t none = ~todo;
+  bool first = true;
   for (uint32_t p = threadIdx.x; p < ROWS * a.l.rmax; p += 256) {
     const uint32_t r = p / a.l.rmax;
     if ((none >> r & 1) && row0 + r < a.l.seq) out[(size_t)row0 * a.l.rmax + p] = 0.0f;
@@ -114,17 +131,8 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
     for (int m = 0; m < MT; m++)
 #pragma unroll
       for (int t = 0; t < NT; t++) acc[m][t] = (v4f){0, 0, 0, 0};
-    const auto load = [&](uint32_t step, uint8_t *stage) {
-      const uint32_t k0 = (s0 + min(step, n - 1)) * 128;  // (past the end the last one repeats)
-#pragma unroll
-      for (int q = 0; q < NX; q++) {
-        // VEC: two rows of 32 units an instruction; else a quarter of a row in single values
-        const uint32_t at = (w * NX + q) * (VEC ? 1024 : 256), e = at + lane * (VEC ? 16 : 4);
-        const uint32_t r = e / 512, unit = e / 16 % 32 ^ (r & 15), k = k0 + 4 * unit + (VEC ? 0 : e / 4 % 4);
-        const float *p = a.x + (size_t)min(row0 + r, a.l.seq - 1) * a.k + min(k, a.k - (VEC ? 4 : 1));
-        if (VEC) __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 16, 0, 0);
-        else __builtin_amdgcn_global_load_lds((const void *)p, (__attribute__((address_space(3))) void *)(stage + at), 4, 0, 0);
-      }
+    const auto loadw = [&](uint32_t step, uint8_t *stage) {
+      const uint32_t k0 = (s0 + min(step, n - 1)) * 128;
 #pragma unroll
       for (int q = 0; q < NT; q++) {
         const uint32_t at = (w * NT + q) * 1024, e = at + lane * 16;
@@ -206,20 +214,27 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
         }
       }
     };
-    // step s: its stage has landed (the one behind it may be on the way), every wave is done with the one before it,
-    // whose room the loads of step s + 2 take
-#define STEP(s, CUR, FREE)            \
-    {                                 \
-      ORDER();                        \
-      WAIT_VM(NX + NT);               \
-      __builtin_amdgcn_s_barrier();   \
-      ORDER();                        \
-      load((s) + 2, FREE);            \
-      mul(s, CUR);                    \
+    // step s: its stage has landed (the one behind it may be on the way: of the first two stages, whose rows come ahead
+    // of their weights, only the second's weights), every wave is done with the one before it, whose room the loads of step
+    // s + 2 take
+#define STEP(s, CUR, FREE)              \
+    {                                   \
+      ORDER();                          \
+      if ((s) == 0) WAIT_VM(NT);        \
+      else WAIT_VM(NX + NT);            \
+      __builtin_amdgcn_s_barrier();     \
+      ORDER();                          \
+      loadx((s) + 2, FREE);             \
+      loadw((s) + 2, FREE);             \
+      mul(s, CUR);                      \
     }
-    load(0, s_0);
-    ORDER();
-    load(1, s_1);
+    if (!first) {
+      loadx(0, s_0);
+      loadx(1, s_1);
+    }
+    first = false;
+    loadw(0, s_0);
+    loadw(1, s_1);
     for (uint32_t s = 0; s < n; s += 3) {
       STEP(s, s_0, s_2)
       if (s + 1 < n) STEP(s + 1, s_1, s_0)
@@ -257,6 +272,7 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
     }
     __syncthreads();
   }
+  WAIT_VM(0);  // (where no row has an adapter: the LDS is not given back before its loads have landed)
 }
 
 // Few rows a request: a wave a row and R ranks, the contraction over its
