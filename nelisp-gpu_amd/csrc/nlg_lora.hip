@@ -653,15 +653,373 @@ __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
   }
 }
 
-// The parts of such sums, added in order.
-__global__ __launch_bounds__(256) void k_lora_sum(const float4 *part, float4 *out, uint64_t n4, uint32_t parts) {
-  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n4; i += gridDim.x * 256ull) {
-    float4 v = part[i];
-    for (uint32_t k = 1; k < parts; k++) {
-      const float4 f = part[k * n4 + i];
+// Blocks of sixteen rows of an adapter, in its requests' order, every parts-th
+// from part on; a wave looks at 64 requests at a time.
+struct LoraBlocks {
+  uint32_t r0 = 0, skip;   // the next 64 requests; how many blocks lie before the next of this part
+  uint64_t mine = 0;       // those of the last 64 that are the adapter's and not yet begun
+  int32_t s = 0, e = 0;    // the lane's request of the last 64
+  uint32_t at = 0, end = 0;
+  __device__ __forceinline__ explicit LoraBlocks(uint32_t part) : skip(part) {}
+  // the next block's first row, and the end of its request's rows (the same in every lane); false: there is none
+  __device__ __forceinline__ bool next(const LoraArgs &l, int32_t ad, uint32_t parts, uint32_t &row, uint32_t &stop) {
+    while (at >= end) {
+      while (!mine) {
+        if (r0 >= l.requests) return false;
+        const uint32_t i = r0 + (threadIdx.x & 63);
+        const bool in = i < l.requests;
+        s = !in ? 0 : l.start ? max(l.start[i], 0) : (int32_t)i;
+        e = !in ? 0 : l.start ? min(l.start[i + 1], (int32_t)l.seq) : (int32_t)min(i + 1, l.seq);
+        mine = __ballot(in && s < e && l.adapter[i] == ad);
+        r0 += 64;
+      }
+      const int k = __builtin_ctzll(mine);
+      mine &= mine - 1;
+      at = __builtin_amdgcn_readlane(s, k);
+      end = __builtin_amdgcn_readlane(e, k);
+      const uint32_t n = (end - at + 15) / 16;
+      at += 16 * (skip < n ? skip : n);  // (seq is under 2^21, parts at most 16)
+      skip = skip < n ? (parts - (n - skip) % parts) % parts : skip - n;
+    }
+    row = at;
+    stop = end;
+    at += 16 * parts;
+    return true;
+  }
+};
+// What lies `off` bytes behind a place that is the same in every lane: the load takes both as they are, without an
+// address of its own to be made in each lane.
+template <class T>
+__device__ __forceinline__ T behind(const void *p, uint32_t off) {
+  return *(const T *)((const uint8_t *)p + off);
+}
+
+// One pass over dy [seq][n]: the adapters' dB, and du = scale B^T dy.  A
+// workgroup has 256 columns (16 E a wave) of an adapter's rows, every
+// gridDim.z-th block of sixteen.  dB is summed in 16 x 16 x 4 f32 products (a
+// lane has E neighbouring columns, so block e of the columns is E i + e); for du the
+// rows turn in LDS and meet B, which stays in registers, on the bf16 cores
+// as in k_lora_down; the waves' sums for the block meet in LDS and are left in
+// one of gridDim.x parts.  It waits for memory: 4,616 rows of 2560, rank up to
+// 32, three adapters 28 us (1.7 TB/s of dy; a pass for each, 24 and 21); 241 rows
+// 5.4 us.
+// E neighbouring columns of a lane
+template <int E>
+struct Cols {
+  typedef float vec __attribute__((ext_vector_type(E)));
+};
+struct GyArgs {
+  LoraArgs l;
+  const float *dy, *u;  // [seq][n], [seq][rmax]
+  float *du;            // [gridDim.x][seq][rmax]
+  float *db;            // [gridDim.z][adapters][n][rmax]
+  uint32_t n;
+};
+template <bool BF, int NT, int E, bool VEC>
+__global__ __launch_bounds__(1024 / E, NT <= 2 ? 4 : 2) void k_lora_gy(GyArgs a) {
+  typedef typename Cols<E>::vec vec;
+  constexpr int NW = 16 / E, H = E / 2, P = 16 * E + 4, Q = 16 * NT + 1;
+  __shared__ float s_t[NW][16][P];
+  __shared__ float s_du[2][NW][16][Q];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t ad = blockIdx.y;
+  const uint32_t rank = lora_rank(a.l, ad), rmax = a.l.rmax;
+  const uint32_t col0 = blockIdx.x * 256 + w * (16 * E), col = col0 + E * i;
+  const float sc = a.l.scale[ad];
+  // B of the wave's columns: lane (i, g) rank 16 t + i of columns 32 h + 8 g .. + 7
+  const uint16_t *const wt = a.l.b + (size_t)ad * a.n * rmax;
+  Bf8 w0[H][NT], w1[BF ? 1 : H][NT];
+#pragma unroll
+  for (int h = 0; h < H; h++)
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int q = 0; q < 4; q++) {
+        uint32_t v[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const uint32_t c = col0 + 32 * h + 8 * g + 2 * q + e;
+          v[e] = wt[(size_t)min(c, a.n - 1) * rmax + min(16u * t + i, rmax - 1)];
+          if (c >= a.n) v[e] = 0;
+        }
+        const uint32_t pair = v[0] | v[1] << 16;
+        if (BF) w0[h][t].u[q] = pair;
+        else split_f16(pair, w0[h][t].u[q], w1[h][t].u[q]);
+      }
+  v4f acc[NT][E];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[t][e] = (v4f){0, 0, 0, 0};
+  float *const out = a.du + (size_t)blockIdx.x * a.l.seq * rmax;
+  // (macros: register sets handed to a lambda end up in scratch)
+#define LOAD(r0, stop, D, U)                                                                                     \
+  do {                                                                                                           \
+    const uint32_t last = stop - 1 - r0; /* of the block's rows; those behind it read that one */                \
+    const float *const bd = a.dy + (size_t)r0 * a.n, *const bu = a.u + (size_t)r0 * rmax;                         \
+    if (VEC && last >= 15) {                                                                                     \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) {                                                            \
+        D[q] = behind<vec>(bd + (size_t)(4 * q) * a.n, vd);                                                      \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) U[q][t] = behind<float>(bu + (4 * q) * rmax, vp[t]);       \
+      }                                                                                                          \
+    } else {                                                                                                     \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) {                                                            \
+        const uint32_t row = min(4u * q + g, last);                                                              \
+        if (VEC) D[q] = behind<vec>(bd, 4 * (row * a.n + min(col, a.n - E)));                                    \
+        else _Pragma("unroll") for (int e = 0; e < E; e++) D[q][e] = behind<float>(bd, 4 * (row * a.n + min(col + e, a.n - 1))); \
+        _Pragma("unroll") for (int t = 0; t < NT; t++)                                                           \
+          U[q][t] = behind<float>(bu, 4 * (row * rmax + min(16u * t + i, rmax - 1)));                            \
+      }                                                                                                          \
+    }                                                                                                            \
+  } while (0)
+  // a block, its sums left in half b of s_du (free again after the next block's barrier)
+#define MUL(r0, stop, D, U, b)                                                                                   \
+  do {                                                                                                           \
+    if (r0 + 16 > stop || col0 + 16 * E > a.n) { /* rows past the request's, columns past the matrix: neither factor counts */ \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) {                                                            \
+        const bool in = r0 + 4 * q + g < stop;                                                                   \
+        _Pragma("unroll") for (int e = 0; e < E; e++) if (!in || col + e >= a.n) D[q][e] = 0.0f;                 \
+        if (!in) _Pragma("unroll") for (int t = 0; t < NT; t++) U[q][t] = 0.0f;                                  \
+      }                                                                                                          \
+    }                                                                                                            \
+    _Pragma("unroll") for (int q = 0; q < 4; q++) *(vec *)&s_t[w][4 * q + g][E * i] = D[q];                      \
+    ORDER(); /* the wave's own rows: LDS takes a wave's accesses in order */                                     \
+    _Pragma("unroll") for (int q = 0; q < 4; q++)                                                                \
+      _Pragma("unroll") for (int t = 0; t < NT; t++)                                                             \
+        _Pragma("unroll") for (int e = 0; e < E; e++)                                                            \
+          acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(U[q][t], D[q][e], acc[t][e], 0, 0, 0);                \
+    v4f du[NT];                                                                                                  \
+    _Pragma("unroll") for (int t = 0; t < NT; t++) du[t] = (v4f){0, 0, 0, 0};                                    \
+    _Pragma("unroll") for (int h = 0; h < H; h++) {                                                              \
+      const float *const p = &s_t[w][i][32 * h + 8 * g];                                                         \
+      const float4 x0 = *(const float4 *)p, x1 = *(const float4 *)(p + 4);                                       \
+      Bf8 p0, p1, p2;                                                                                            \
+      split3(x0.x, x0.y, p0.u[0], p1.u[0], p2.u[0]);                                                             \
+      split3(x0.z, x0.w, p0.u[1], p1.u[1], p2.u[1]);                                                             \
+      split3(x1.x, x1.y, p0.u[2], p1.u[2], p2.u[2]);                                                             \
+      split3(x1.z, x1.w, p0.u[3], p1.u[3], p2.u[3]);                                                             \
+      _Pragma("unroll") for (int t = 0; t < NT; t++) {                                                           \
+        du[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p0.v, w0[h][t].v, du[t], 0, 0, 0);                       \
+        du[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p1.v, w0[h][t].v, du[t], 0, 0, 0);                       \
+        du[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p2.v, w0[h][t].v, du[t], 0, 0, 0);                       \
+        if (!BF) {                                                                                               \
+          du[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p0.v, w1[BF ? 0 : h][t].v, du[t], 0, 0, 0);            \
+          du[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p1.v, w1[BF ? 0 : h][t].v, du[t], 0, 0, 0);            \
+        }                                                                                                        \
+      }                                                                                                          \
+    }                                                                                                            \
+    _Pragma("unroll") for (int t = 0; t < NT; t++)                                                               \
+      _Pragma("unroll") for (int r = 0; r < 4; r++) s_du[b][w][4 * g + r][16 * t + i] = du[t][r];                \
+    __syncthreads();                                                                                             \
+    for (uint32_t k = threadIdx.x; k < 16 * rmax; k += 1024 / E) {                                               \
+      const uint32_t r = k / rmax, j = k % rmax;                                                                 \
+      if (r0 + r < stop) {                                                                                       \
+        float v = 0.0f;                                                                                          \
+        _Pragma("unroll") for (int q = 0; q < NW; q++) v += s_du[b][q][r][j];                                    \
+        out[(size_t)r0 * rmax + k] = j < rank ? v * sc : 0.0f;                                                   \
+      }                                                                                                          \
+    }                                                                                                            \
+  } while (0)
+  // bytes from a block's q-th four rows to what the lane reads there
+  const uint32_t vd = 4 * (g * a.n + min(col, a.n - min(a.n, (uint32_t)E)));
+  uint32_t vp[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) vp[t] = 4 * (g * rmax + min(16u * t + i, rmax - 1));
+  LoraBlocks blocks(blockIdx.z);
+  vec dv[4];
+  float uv[4][NT];
+  uint32_t r0, s0;
+  for (uint32_t b = 0; blocks.next(a.l, ad, gridDim.z, r0, s0); b ^= 1) {
+    LOAD(r0, s0, dv, uv);
+    MUL(r0, s0, dv, uv, b);
+  }
+#undef MUL
+#undef LOAD
+  // acc[t][e] register r: rank 16 t + 4 g + r, column col + e
+  float *const o = a.db + ((size_t)blockIdx.z * a.l.adapters + ad) * rmax * a.n;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    const uint32_t j = 16 * t + 4 * g;
+    if (j >= rmax) continue;
+#pragma unroll
+    for (int e = 0; e < E; e++)
+      if (col + e < a.n)
+        *(float4 *)(o + (size_t)(col + e) * rmax + j) =
+            make_float4(j < rank ? acc[t][e][0] * sc : 0.0f, j + 1 < rank ? acc[t][e][1] * sc : 0.0f,
+                        j + 2 < rank ? acc[t][e][2] * sc : 0.0f, j + 3 < rank ? acc[t][e][3] * sc : 0.0f);
+  }
+}
+
+// One pass over x [seq][n]: the adapters' dA, and dx = dres + A^T du.  A
+// workgroup has 256 columns of an adapter's rows (those of none: blockIdx.y ==
+// adapters), every gridDim.z-th block of sixteen, its waves 16 E columns each, E
+// neighbouring ones a lane, in 16 x 16 x 4 f32 products.  x, dres and dx move
+// once, a row 1 KB at a time.  It waits for memory (the matrix cores are busy 21 %
+// of the time): 241 rows of 2560 5.9 us; 4,616 of 6912 112 to 125 us, the same with
+// the next block's loads in flight, which is why larger calls take two passes.
+struct GxArgs {
+  LoraArgs l;
+  const float *x, *du, *dres;  // [seq][n], [seq][rmax], [seq][n] or null
+  float *dx;                   // [seq][n] or null
+  float *da;                   // [gridDim.z][adapters][rmax][n]
+  uint32_t n;
+};
+template <bool BF, int NT, int E>
+__global__ __launch_bounds__(1024 / E, NT <= 2 ? 4 : 2) void k_lora_gx(GxArgs a) {
+  typedef typename Cols<E>::vec vec;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t rmax = a.l.rmax, col = blockIdx.x * 256 + w * (16 * E) + E * i, cc = min(col, a.n - E);
+  const bool here = col < a.n;
+  if (blockIdx.y == a.l.adapters) {
+    for (uint32_t r0 = 64 * blockIdx.z; r0 < a.l.seq; r0 += 64 * gridDim.z) {
+      const int32_t ad = lora_rows(a.l, r0, 64, lane);
+      uint64_t none = __ballot(ad < 0);
+      for (int r = g; r < 64; r += 4)
+        if ((none >> r & 1) && r0 + r < a.l.seq && here) {
+          const size_t o = (size_t)(r0 + r) * a.n + col;
+          *(vec *)(a.dx + o) = a.dres ? *(const vec *)(a.dres + o) : (vec)0.0f;
+        }
+    }
+    return;
+  }
+  const int32_t ad = blockIdx.y;
+  const uint32_t rank = lora_rank(a.l, ad);
+  // A of the columns: ranks 16 t + 4 g + s
+  const uint16_t *const wt = a.l.a + (size_t)ad * rmax * a.n;
+  uint32_t wv[NT][4][E / 2];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const uint32_t j = 16 * t + 4 * g + s;
+#pragma unroll
+      for (int e = 0; e < E / 2; e++) {
+        wv[t][s][e] = *(const uint32_t *)(wt + (size_t)min(j, rmax - 1) * a.n + cc + 2 * e);
+        if (j >= rank) wv[t][s][e] = 0;  // (du is 0 there)
+      }
+    }
+  v4f acc[NT][E];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[t][e] = (v4f){0, 0, 0, 0};
+  // (macros: register sets handed to a lambda end up in scratch)
+#define LOAD(r0, stop, X, R, U, P)                                                                                  \
+  do {                                                                                                              \
+    const uint32_t last = stop - 1 - r0; /* of the block's rows; those behind it read that one */                   \
+    const float *const bx = a.x + (size_t)r0 * a.n, *const bu = a.du + (size_t)r0 * rmax;                            \
+    const float *const br = a.dres + (size_t)r0 * a.n;                                                              \
+    if (last >= 15) {                                                                                               \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) {                                                               \
+        X[q] = behind<vec>(bx + (size_t)(4 * q) * a.n, vx);                                                         \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) P[q][t] = behind<float>(bu + (4 * q) * rmax, vp[t]);          \
+      }                                                                                                             \
+      if (a.dx) {                                                                                                   \
+        _Pragma("unroll") for (int r = 0; r < 4; r++)                                                               \
+          R[r] = a.dres ? behind<vec>(br + (size_t)r * a.n, vr) : (vec)0.0f;                                        \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) U[t] = behind<float4>(bu, vu[t]);                            \
+      }                                                                                                             \
+    } else {                                                                                                        \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) {                                                               \
+        const uint32_t row = min(4u * q + g, last);                                                                 \
+        X[q] = behind<vec>(bx, 4 * (row * a.n + cc));                                                               \
+        _Pragma("unroll") for (int t = 0; t < NT; t++)                                                              \
+          P[q][t] = behind<float>(bu, 4 * (row * rmax + min(16u * t + i, rmax - 1)));                               \
+      }                                                                                                             \
+      if (a.dx) {                                                                                                   \
+        _Pragma("unroll") for (int r = 0; r < 4; r++)                                                               \
+          R[r] = a.dres ? behind<vec>(br, 4 * (min(4u * g + r, last) * a.n + cc)) : (vec)0.0f;                      \
+        _Pragma("unroll") for (int t = 0; t < NT; t++)                                                              \
+          U[t] = behind<float4>(bu, 4 * (min((uint32_t)i, last) * rmax + min(16u * t + 4 * g, rmax - 4)));          \
+      }                                                                                                             \
+    }                                                                                                               \
+  } while (0)
+  // rows past the request's: neither factor counts.  (Of the way up: a rank that rmax has no room for reads another's
+  // du, with weights of 0.)
+#define MUL(r0, stop, X, R, U, P)                                                                                   \
+  do {                                                                                                              \
+    if (r0 + 16 > stop) {                                                                                           \
+      _Pragma("unroll") for (int q = 0; q < 4; q++) if (r0 + 4 * q + g >= stop) {                                   \
+        X[q] = (vec)0.0f;                                                                                           \
+        _Pragma("unroll") for (int t = 0; t < NT; t++) P[q][t] = 0.0f;                                              \
+      }                                                                                                             \
+    }                                                                                                               \
+    _Pragma("unroll") for (int q = 0; q < 4; q++)                                                                   \
+      _Pragma("unroll") for (int t = 0; t < NT; t++)                                                                \
+        _Pragma("unroll") for (int e = 0; e < E; e++)                                                               \
+          acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(P[q][t], X[q][e], acc[t][e], 0, 0, 0);                   \
+    if (a.dx) {                                                                                                     \
+      v4f up[E];                                                                                                    \
+      _Pragma("unroll") for (int e = 0; e < E; e++) up[e] = (v4f){0, 0, 0, 0};                                      \
+      _Pragma("unroll") for (int t = 0; t < NT; t++)                                                                \
+        _Pragma("unroll") for (int s = 0; s < 4; s++)                                                               \
+          _Pragma("unroll") for (int e = 0; e < E; e++) {                                                           \
+            const uint32_t h = wv[t][s][e / 2] >> (16 * (e & 1)) & 0xffff;                                          \
+            up[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(at4(U[t], s), wide<BF>(h), up[e], 0, 0, 0);                \
+          }                                                                                                         \
+      float *const bd = a.dx + (size_t)r0 * a.n;                                                                    \
+      _Pragma("unroll") for (int r = 0; r < 4; r++) {                                                               \
+        vec v = R[r];                                                                                               \
+        _Pragma("unroll") for (int e = 0; e < E; e++) v[e] += up[e][r];                                             \
+        if (here && r0 + 4 * g + r < stop) *(vec *)((uint8_t *)(bd + (size_t)r * a.n) + vr) = v;                    \
+      }                                                                                                             \
+    }                                                                                                               \
+  } while (0)
+  // bytes from a block's first row (or the q-th four of its rows, or its r-th row) to what the lane reads there
+  const uint32_t vx = 4 * (g * a.n + cc), vr = 4 * (4 * g * a.n + cc);
+  uint32_t vp[NT], vu[NT];
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    vp[t] = 4 * (g * rmax + min(16u * t + i, rmax - 1));
+    vu[t] = 4 * (i * rmax + min(16u * t + 4 * g, rmax - 4));
+  }
+  LoraBlocks blocks(blockIdx.z);
+  vec xv[4], res[4];
+  float4 uv[NT];
+  float pv[4][NT];
+  uint32_t r0, s0;
+  while (blocks.next(a.l, ad, gridDim.z, r0, s0)) {
+    LOAD(r0, s0, xv, res, uv, pv);
+    MUL(r0, s0, xv, res, uv, pv);
+  }
+#undef MUL
+#undef LOAD
+  if (!here) return;
+  float *const o = a.da + ((size_t)blockIdx.z * a.l.adapters + ad) * rmax * a.n;
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const uint32_t j = 16 * t + 4 * g + r;
+      if (j < rmax) {
+        vec v;
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = j < rank ? acc[t][e][r] : 0.0f;
+        *(vec *)(o + (size_t)j * a.n + col) = v;
+      }
+    }
+}
+
+struct LoraSum {
+  const float4 *part;  // [parts][n4]
+  float4 *out;
+  uint64_t n4;
+  uint32_t parts;
+};
+// The parts of such sums, added in order; of two of them in one launch.
+__global__ __launch_bounds__(256) void k_lora_sum(LoraSum a, LoraSum b) {
+  for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < a.n4 + b.n4; i += gridDim.x * 256ull) {
+    const bool second = i >= a.n4;
+    const LoraSum &s = second ? b : a;
+    const uint64_t k = second ? i - a.n4 : i;
+    float4 v = s.part[k];
+    for (uint32_t q = 1; q < s.parts; q++) {
+      const float4 f = s.part[q * s.n4 + k];
       v.x += f.x; v.y += f.y; v.z += f.z; v.w += f.w;
     }
-    out[i] = v;
+    s.out[k] = v;
   }
 }
 
@@ -677,7 +1035,7 @@ static int lora_check(const char *what, const void *a, const void *b, int fmt, c
     return nlg_fail("%s: rmax must be a multiple of 8 up to %d (got %u)", what, LORA_RANK, rmax);
   if (!cols || cols % 8) return nlg_fail("%s: cols must be a multiple of 8 (got %u)", what, cols);
   if (!out) return nlg_fail("%s: out must be nonzero", what);
-  if (seq > LORA_ROWS || out > 0x1000000u || cols > 0x1000000u || adapters > 65535 || requests > 0x1000000u)
+  if (seq > LORA_ROWS || out > 0x1000000u || cols > 0x1000000u || adapters > 65534 || requests > 0x1000000u)
     return nlg_fail("%s: too many rows, columns, requests or adapters", what);
   if (((uintptr_t)a & 15) || ((uintptr_t)b & 15)) return nlg_fail("%s: adapters must be 16-byte aligned", what);
   if (((uintptr_t)scale | (uintptr_t)rank | (uintptr_t)start | (uintptr_t)adapter) & 3)
@@ -698,10 +1056,13 @@ static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
   return a && b && x < y + nb && y < x + na;
 }
 
-static int lora_sum(const char *what, const float *parts, float *out, uint64_t n4, uint32_t np, hipStream_t st) {
-  const uint32_t blocks = nlg_blocks(n4, 256);
-  hipLaunchKernelGGL(k_lora_sum, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, st, (const float4 *)parts,
-                     (float4 *)out, n4, np);
+static LoraSum lora_parts_of(const float *part, float *out, uint64_t n, uint32_t parts) {
+  return {(const float4 *)part, (float4 *)out, parts > 1 ? n / 4 : 0, parts};
+}
+static int lora_sum(const char *what, const LoraSum &a, const LoraSum &b, hipStream_t st) {
+  if (!a.n4 && !b.n4) return NLG_OK;
+  const uint32_t blocks = nlg_blocks(a.n4 + b.n4, 256);
+  hipLaunchKernelGGL(k_lora_sum, dim3(blocks < 2048 ? blocks : 2048), dim3(256), 0, st, a, b);
   NLG_LAUNCHED(what);
   return NLG_OK;
 }
@@ -740,14 +1101,15 @@ static int lora_down(const char *what, DownArgs d, bool bf, bool kmajor, float *
     else if (nt <= 4) GO(BF, KM, 4); \
     else GO(BF, KM, 8);              \
   } while (0)
-  if (bf && kmajor) GO2(true, true);
+  // (the gradient's way down of up to 64 ranks is k_lora_gy)
+  if (bf && kmajor) GO(true, true, 8);
   else if (bf) GO2(true, false);
-  else if (kmajor) GO2(false, true);
+  else if (kmajor) GO(false, true, 8);
   else GO2(false, false);
 #undef GO2
 #undef GO
   NLG_LAUNCHED(what);
-  return np > 1 ? lora_sum(what, parts, u, (uint64_t)d.l.seq * d.l.rmax / 4, np, st) : NLG_OK;
+  return lora_sum(what, lora_parts_of(parts, u, (uint64_t)d.l.seq * d.l.rmax, np), {}, st);
 }
 
 static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipStream_t st) {
@@ -775,31 +1137,21 @@ static uint32_t lora_parts(uint32_t seq, uint32_t n, uint32_t adapters) {
   return k < 1 ? 1 : k > 16 ? 16 : (uint32_t)k;
 }
 
-static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, hipStream_t st) {
-  const uint32_t np = lora_parts(d.l.seq, d.n, d.l.adapters);
-  float *const out = d.out;
+// The launch alone: of np parts, to `parts` where that is more than one.
+static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, uint32_t np, hipStream_t st) {
   if (np > 1) d.out = parts;
   const dim3 grid((d.n + 63) / 64, d.l.adapters, np), blk(512);
   const bool vec = d.n % 4 == 0 && ((uintptr_t)d.q & 15) == 0;
   const uint32_t nt = (d.l.rmax + 15) / 16;
-#define GO(N, T)                                                                           \
-  do {                                                                                     \
-    if (vec) hipLaunchKernelGGL((k_lora_outer<N, T, true>), grid, blk, 0, st, d);          \
-    else hipLaunchKernelGGL((k_lora_outer<N, T, false>), grid, blk, 0, st, d);             \
-  } while (0)
-#define GO2(T)                  \
-  do {                          \
-    if (nt <= 1) GO(1, T);      \
-    else if (nt <= 2) GO(2, T); \
-    else if (nt <= 4) GO(4, T); \
-    else GO(8, T);              \
-  } while (0)
-  if (turn) GO2(true);
-  else GO2(false);
-#undef GO2
-#undef GO
+  // (dB of up to 64 ranks is k_lora_gy's; x has whole float4s)
+  if (turn && vec) hipLaunchKernelGGL((k_lora_outer<8, true, true>), grid, blk, 0, st, d);
+  else if (turn) hipLaunchKernelGGL((k_lora_outer<8, true, false>), grid, blk, 0, st, d);
+  else if (nt <= 1) hipLaunchKernelGGL((k_lora_outer<1, false, true>), grid, blk, 0, st, d);
+  else if (nt <= 2) hipLaunchKernelGGL((k_lora_outer<2, false, true>), grid, blk, 0, st, d);
+  else if (nt <= 4) hipLaunchKernelGGL((k_lora_outer<4, false, true>), grid, blk, 0, st, d);
+  else hipLaunchKernelGGL((k_lora_outer<8, false, true>), grid, blk, 0, st, d);
   NLG_LAUNCHED(what);
-  return np > 1 ? lora_sum(what, parts, out, (uint64_t)d.l.adapters * d.l.rmax * d.n / 4, np, st) : NLG_OK;
+  return NLG_OK;
 }
 
 // Few rows a request, or few rows at all.
@@ -982,22 +1334,104 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   return lora_forward(what, l, x, bf, y, y, u, out, cols, workspace, st) ? NLG_ERR : NLG_OK;
 }
 
-// du and u, and the parts of one of the two gradients
+// What a gradient call keeps: du and u, and the parts of their sums and the gradients'.  Up to 64 ranks it makes one pass over dy
+// (parts: of 256 columns of dy each, and every zy-th block of rows) and, while x, dres and dx are 128 MiB or less, one over x.
+// Whole calls with that pass and with one for dA and one for dx, at rank 16, two adapters, out = cols = 2560: 250 rows 24.8 and
+// 30.3 us, 1,000 rows 30.8 and 35.8, 4,000 rows (117 MiB) 54.6 and 61.0; at rank 32, three adapters, 6912 -> 2560: 1,200 rows
+// (95 MiB) 58.6 and 67.2, 2,400 rows (190 MiB) 91.7 and 86.9, 4,616 rows 156 and 144.  More ranks take a pass for each sum.
+struct LoraGradPlan {
+  bool gx;                       // one pass over x
+  uint32_t gy, wx, zy, zx;       // workgroups along the columns, parts of the rows
+  size_t u, du_parts, db_parts, da_parts, bytes;
+};
+#define LORA_GRAD_RANK 64
+static LoraGradPlan lora_grad_plan(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters, uint32_t rmax) {
+  LoraGradPlan p = {};
+  if (!lora_sizes(seq, out, cols, rmax) || !adapters || adapters > 65534) return p;
+  const size_t row = lora_round((size_t)seq * rmax * 4), down = lora_down_bytes(seq, cols, rmax);
+  const uint64_t na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out, blocks = ((uint64_t)seq + 15) / 16;
+  p.u = row;
+  p.du_parts = 2 * row;
+  if (rmax > LORA_GRAD_RANK) {
+    p.zy = lora_parts(seq, out, adapters);
+    p.zx = lora_parts(seq, cols, adapters);
+    const size_t more = lora_down_bytes(seq, out, rmax);
+    p.db_parts = p.du_parts + (down > more ? down : more);
+  } else {
+    // three workgroups a CU, of a block of rows at least
+    const auto parts = [&](uint64_t wg) {
+      uint64_t z = (768 + wg - 1) / wg;
+      if (z > blocks) z = blocks;
+      return (uint32_t)(z < 1 ? 1 : z > 16 ? 16 : z);
+    };
+    p.gy = (out + 255) / 256;
+    p.zy = parts((uint64_t)p.gy * adapters);
+    p.gx = 12ull * seq * cols <= (128u << 20);
+    p.wx = (cols + 255) / 256;
+    p.zx = p.gx ? parts((uint64_t)p.wx * adapters) : lora_parts(seq, cols, adapters);
+    const size_t du = p.gy > 1 ? p.gy * ((size_t)seq * rmax * 4) : 0;
+    p.db_parts = p.du_parts + lora_round(du > down ? du : down);
+  }
+  p.da_parts = p.db_parts + (p.zy > 1 ? lora_round(p.zy * nb * 4) : 0);
+  p.bytes = p.da_parts + (p.zx > 1 ? lora_round(p.zx * na * 4) : 0);
+  return p;
+}
+
 extern "C" size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters,
                                                  uint32_t rmax, uint32_t requests) {
   (void)requests;
-  if (!lora_sizes(seq, out, cols, rmax) || !adapters || adapters > 65535) return 0;
-  size_t most = 0;
-  for (const uint32_t n : {out, cols}) {
-    const uint32_t parts = lora_parts(seq, n, adapters);
-    const size_t bytes = parts > 1 ? (size_t)parts * adapters * rmax * n * 4 : 0;
-    most = bytes > most ? bytes : most;
-  }
-  for (const uint32_t k : {out, cols}) {  // (the same room: the contractions come first)
-    const size_t bytes = lora_down_bytes(seq, k, rmax);
-    most = bytes > most ? bytes : most;
-  }
-  return 2 * lora_round((size_t)seq * rmax * 4) + lora_round(most);
+  return lora_grad_plan(seq, out, cols, adapters, rmax).bytes;
+}
+
+// du and dB of up to 64 ranks
+static int lora_gy(const char *what, const LoraArgs &l, const LoraGradPlan &p, const float *u, const float *dy, float *du,
+                   float *db, uint32_t out, bool bf, uint8_t *ws, hipStream_t st) {
+  GyArgs y{};
+  y.l = l; y.dy = dy; y.u = u; y.n = out;
+  y.du = p.gy > 1 ? (float *)(ws + p.du_parts) : du;
+  y.db = p.zy > 1 ? (float *)(ws + p.db_parts) : db;
+  const uint32_t nt = (l.rmax + 15) / 16;
+  const bool vec = out % 4 == 0 && ((uintptr_t)dy & 15) == 0;
+  const dim3 grid(p.gy, l.adapters, p.zy);
+#define BY_RANK(GO)           \
+  do {                        \
+    if (nt <= 1) GO(1);       \
+    else if (nt <= 2) GO(2);  \
+    else GO(4);               \
+  } while (0)
+#define GO(N)                                                                              \
+  do {                                                                                     \
+    constexpr int E = N == 1 ? 4 : 2;                                                      \
+    const dim3 blk(1024 / E);                                                              \
+    if (bf && vec) hipLaunchKernelGGL((k_lora_gy<true, N, E, true>), grid, blk, 0, st, y);  \
+    else if (bf) hipLaunchKernelGGL((k_lora_gy<true, N, E, false>), grid, blk, 0, st, y);   \
+    else if (vec) hipLaunchKernelGGL((k_lora_gy<false, N, E, true>), grid, blk, 0, st, y);  \
+    else hipLaunchKernelGGL((k_lora_gy<false, N, E, false>), grid, blk, 0, st, y);          \
+  } while (0)
+  BY_RANK(GO);
+#undef GO
+  NLG_LAUNCHED(what);
+  return lora_sum(what, lora_parts_of(y.du, du, (uint64_t)l.seq * l.rmax, p.gy), {}, st);
+}
+
+// dA and dx of up to 64 ranks in one pass; da: where its parts go
+static int lora_gx(const char *what, const LoraArgs &l, const LoraGradPlan &p, const float *x, const float *du,
+                   const float *dres, float *dx, float *da, uint32_t cols, bool bf, hipStream_t st) {
+  GxArgs g{};
+  g.l = l; g.x = x; g.du = du; g.dres = dres; g.dx = dx; g.n = cols; g.da = da;
+  const uint32_t nt = (l.rmax + 15) / 16;
+  const dim3 grid(p.wx, l.adapters + (dx && dx != dres ? 1 : 0), p.zx);
+#define GO(N)                                                                                   \
+  do {                                                                                          \
+    constexpr int E = N == 1 ? 4 : 2;                                                           \
+    if (bf) hipLaunchKernelGGL((k_lora_gx<true, N, E>), grid, dim3(1024 / E), 0, st, g);        \
+    else hipLaunchKernelGGL((k_lora_gx<false, N, E>), grid, dim3(1024 / E), 0, st, g);          \
+  } while (0)
+  BY_RANK(GO);
+#undef GO
+#undef BY_RANK
+  NLG_LAUNCHED(what);
+  return NLG_OK;
 }
 
 extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a,
@@ -1014,8 +1448,8 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   if (((uintptr_t)x | (uintptr_t)u | (uintptr_t)da | (uintptr_t)db | (uintptr_t)dx | (uintptr_t)dres) & 15)
     return nlg_fail("%s: x, u, dres, dx, da and db must be 16-byte aligned", what);
   if ((uintptr_t)dy & 3) return nlg_fail("%s: dy must be 4-byte aligned", what);
-  const size_t nu = lora_round((size_t)seq * rmax * 4);
-  const size_t need = nlg_lora_linear_grad_workspace(seq, out, cols, adapters, rmax, requests);
+  const LoraGradPlan plan = lora_grad_plan(seq, out, cols, adapters, rmax);
+  const size_t need = plan.bytes;
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
@@ -1032,22 +1466,34 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   const bool bf = fmt == NLG_LORA_BF16;
-  float *const du = (float *)workspace, *const parts = (float *)((uint8_t *)workspace + 2 * nu);
+  uint8_t *const ws = (uint8_t *)workspace;
+  float *const du = (float *)ws, *const parts = (float *)(ws + plan.du_parts);
   if (!u) {
-    d.x = x; d.k = cols; d.scaled = false; d.u = (float *)((uint8_t *)workspace + nu);
+    d.x = x; d.k = cols; d.scaled = false; d.u = (float *)(ws + plan.u);
     u = d.u;
     if (lora_down(what, d, bf, false, parts, st)) return NLG_ERR;
   }
-  d.x = dy; d.k = out; d.scaled = true; d.u = du;
-  if (lora_down(what, d, bf, true, parts, st)) return NLG_ERR;
-  OuterArgs o{};
-  o.l = d.l;
-  o.p = u; o.q = dy; o.out = db; o.n = out; o.scaled = true;
-  if (lora_outer(what, o, true, parts, st)) return NLG_ERR;
-  o.p = du; o.q = x; o.out = da; o.n = cols; o.scaled = false;
-  if (lora_outer(what, o, false, parts, st)) return NLG_ERR;
-  if (!dx) return NLG_OK;
-  UpArgs p{};
-  p.l = d.l; p.u = du; p.res = dres; p.y = dx; p.n = cols; p.scaled = false;
-  return lora_up(what, p, bf, true, st);
+  float *const dbp = plan.zy > 1 ? (float *)(ws + plan.db_parts) : db, *const dap = plan.zx > 1 ? (float *)(ws + plan.da_parts) : da;
+  if (rmax <= LORA_GRAD_RANK) {
+    if (lora_gy(what, d.l, plan, u, dy, du, db, out, bf, ws, st)) return NLG_ERR;
+  } else {
+    d.x = dy; d.k = out; d.scaled = true; d.u = du;
+    OuterArgs o{};
+    o.l = d.l; o.p = u; o.q = dy; o.out = db; o.n = out; o.scaled = true;
+    if (lora_down(what, d, bf, true, parts, st) || lora_outer(what, o, true, dbp, plan.zy, st)) return NLG_ERR;
+  }
+  if (plan.gx) {
+    if (lora_gx(what, d.l, plan, x, du, dres, dx, dap, cols, bf, st)) return NLG_ERR;
+  } else {
+    OuterArgs o{};
+    o.l = d.l; o.p = du; o.q = x; o.out = da; o.n = cols; o.scaled = false;
+    if (lora_outer(what, o, false, dap, plan.zx, st)) return NLG_ERR;
+    if (dx) {
+      UpArgs p{};
+      p.l = d.l; p.u = du; p.res = dres; p.y = dx; p.n = cols; p.scaled = false;
+      if (lora_up(what, p, bf, true, st)) return NLG_ERR;
+    }
+  }
+  const uint64_t nb4 = (uint64_t)adapters * rmax * out, na4 = (uint64_t)adapters * rmax * cols;
+  return lora_sum(what, lora_parts_of(dbp, db, nb4, plan.zy), lora_parts_of(dap, da, na4, plan.zx), st);
 }

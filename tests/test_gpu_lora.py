@@ -124,6 +124,21 @@ def test_backward(i, bf):
     assert c.backward(u=given, dx=False)[0] is None
 
 
+@pytest.mark.parametrize("rmax", [8, 24, 64])
+def test_backward_of_long_prompts(rmax):
+    """x, dres and dx of more than 128 MiB together: dA and dx in passes of their own."""
+    c = Case([300, 0, 411, 2], [1, 0, 0, 1], 2, rmax, out=40, cols=16388 - 4 * 5, mixed=True, first=1, behind=2)
+    assert 12 * c.seq * c.cols > 128 << 20
+    u = ref.Sums(c.want()[1].value.astype(F32).astype(float))
+    got = c.backward(u=u.value.astype(F32))
+    for g, w, n in zip(got, c.want_grad(u), ("dx", "da", "db")):
+        close(g, w, n)
+    again = c.backward(u=u.value.astype(F32), inplace=True)
+    assert all(np.array_equal(x, y) for x, y in zip(again, got))
+    none = c.of < 0
+    assert np.array_equal(got[0].reshape(c.dres.shape)[none], c.dres[none])
+
+
 # ------------------------------------------------------------------ beside the ternary linear
 
 def ternary(c, per_row, bias, keep=True, stream=None):

@@ -30,7 +30,7 @@ BAD = [(dict(a=NULL), "null"), (dict(b=NULL), "null"), (dict(scale=NULL), "null"
        (dict(x=NULL), "null"), (dict(fmt=2), "format"), (dict(fmt=-1), "format"), (dict(adapters=0), "adapters"),
        (dict(rmax=0), "rmax"), (dict(rmax=12), "rmax"), (dict(rmax=136), "rmax"), (dict(cols=0), "cols"),
        (dict(cols=60), "cols"), (dict(out=0), "out"), (dict(seq=1 << 22), "many"), (dict(out=1 << 25), "many"),
-       (dict(adapters=65536), "many"), (dict(requests=1 << 25), "many"), (dict(a=Ptr(1 << 30 | 8)), "aligned"),
+       (dict(adapters=65535), "many"), (dict(requests=1 << 25), "many"), (dict(a=Ptr(1 << 30 | 8)), "aligned"),
        (dict(b=Ptr(1 << 30 | 8)), "aligned"), (dict(x=Ptr(1 << 30 | 4)), "aligned"), (dict(scale=Ptr(6)), "aligned"),
        (dict(start=Ptr(2)), "aligned"), (dict(rank=Ptr(1)), "aligned"), (dict(adapter=Ptr(3)), "aligned"),
        (dict(workspace=NULL), "workspace"), (dict(workspace=Ptr(1 << 40, 100)), "workspace"),
