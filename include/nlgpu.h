@@ -489,7 +489,10 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
  * 16-byte aligned; calls that share a workspace run in stream order.  Nothing
  * here allocates, so every call may be captured into a graph (but for the
  * column split of nlg_ternary_linear_lora's base, which goes without its
- * scratch if a capture is the first call that wants it).
+ * scratch if a capture is the first call that wants it).  Rows have no part in
+ * each other; an infinity in x (dy) makes NaN of its row's u, and values below
+ * 2^-100 may lose the last bits of their products there.  seq is at most
+ * 2,097,120, out and cols 2^24, adapters 65534.
  * ---------------------------------------------------------------------- */
 #define NLG_LORA_F16 0
 #define NLG_LORA_BF16 1
@@ -544,7 +547,10 @@ size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols,
  * sizes that the calls do not take; grad: whether dx is wanted) holds the
  * probabilities of a piece of the vocabulary; calls that share one run in
  * stream order.  Nothing here allocates, so every call may be captured into a
- * graph.  dx may not overlap x.
+ * graph.  No output may overlap another or an input.  Rows have no part in each
+ * other: an infinity in x makes NaN of its own row's outputs (a NaN is rounded
+ * as nlg_ternary_linear rounds it).  Where no logit is above -inf, lse is -inf,
+ * the loss of a row with targets NaN, and its gradient the targets' part alone.
  * ---------------------------------------------------------------------- */
 
 /* Softmax cross entropy: loss[s] = lse[s] - z[s, label[s]].  Rows whose label

@@ -1051,10 +1051,6 @@ static bool lora_sizes(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax)
   return seq && out && cols && cols % 8 == 0 && rmax && rmax % 8 == 0 && rmax <= LORA_RANK && seq <= LORA_ROWS &&
          out <= 0x1000000u && cols <= 0x1000000u;
 }
-static bool overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
-  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return a && b && x < y + nb && y < x + na;
-}
 
 static LoraSum lora_parts_of(const float *part, float *out, uint64_t n, uint32_t parts) {
   return {(const float4 *)part, (float4 *)out, parts > 1 ? n / 4 : 0, parts};
@@ -1258,8 +1254,8 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
   const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nu = (uint64_t)seq * rmax * 4;
-  if (overlap(y, ny, x, nx) || overlap(u, nu, x, nx) || overlap(u, nu, y, ny) || (res != y && overlap(y, ny, res, ny)) ||
-      overlap(u, nu, res, ny))
+  if (nlg_overlap(y, ny, x, nx) || nlg_overlap(u, nu, x, nx) || nlg_overlap(u, nu, y, ny) || (res != y && nlg_overlap(y, ny, res, ny)) ||
+      nlg_overlap(u, nu, res, ny))
     return nlg_fail("%s: outputs overlap each other or an input (y may be res itself)", what);
   NLG_SCOPE(what);
   return lora_forward(what, l, x, fmt == NLG_LORA_BF16, res, y, u, out, cols, workspace, nlg_stream(stream)) ? NLG_ERR : NLG_OK;
@@ -1294,7 +1290,7 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
   const uint64_t bx = (uint64_t)seq * cols * 4, by = (uint64_t)seq * out * 4, bu = (uint64_t)seq * rmax * 4;
-  if (overlap(y, by, x, bx) || overlap(u, bu, x, bx) || overlap(u, bu, y, by))
+  if (nlg_overlap(y, by, x, bx) || nlg_overlap(u, bu, x, bx) || nlg_overlap(u, bu, y, by))
     return nlg_fail("%s: outputs overlap each other or x", what);
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
@@ -1461,7 +1457,7 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   for (int o = 6; o < 9; o++)
     for (int i = 0; i < 9; i++)
       if (i < 6 || i > o)
-        if (overlap(in[o].p, in[o].n, in[i].p, in[i].n))
+        if (nlg_overlap(in[o].p, in[o].n, in[i].p, in[i].n))
           return nlg_fail("%s: outputs overlap each other or an input (dx may be dres itself)", what);
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);

@@ -1,7 +1,14 @@
-// nlg_scope.h -- the library's device for the length of a call.
+// nlg_scope.h -- what an entry point begins with: its arguments against each other, and the library's device for the
+// length of the call.
 #pragma once
 
 #include "nlg_internal.h"
+
+// Whether two arrays of na and nb bytes share any (a null one shares none).
+static inline bool nlg_overlap(const void *a, uint64_t na, const void *b, uint64_t nb) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return a && b && x < y + nb && y < x + na;
+}
 
 // The device the library runs on made the calling thread's for one call.
 struct NlgDeviceScope {

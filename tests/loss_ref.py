@@ -71,7 +71,7 @@ def tolerances(x, w, bias, beta, index, teacher, teacher_lse, t, tau, p):
     lse = H * (8 * z + 2 + 56 + 3 * (z + np.log(w.shape[0])))
     y = np.zeros_like(z)
     if teacher is not None:  # the same of the teacher's
-        y = np.where((index >= 0) & (index < w.shape[0]), np.abs(teacher), 0).max(axis=1) / tau
+        y = np.where((index >= 0) & (index < w.shape[0]) & np.isfinite(teacher), np.abs(teacher), 0).max(axis=1) / tau
         if teacher_lse is not None:
             y = y + np.abs(teacher_lse)
     lt = 0 if teacher is None else H * (8 * y + 64 + 3 * np.log(index.shape[1] + 1.0))

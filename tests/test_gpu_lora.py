@@ -183,3 +183,204 @@ def test_beside_ternary(i, bf):
     none = c.of < 0
     assert np.array_equal(y.reshape(c.seq, c.out)[none], base[none])  # the linear's own bits
     assert np.array_equal(ternary(c, i % 2 == 0, i % 3 == 0, keep=False)[0], y)
+
+
+# ------------------------------------------------------------------ what the documentation allows besides
+
+def same(a, b):
+    return np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+# the few-row forms, the tiles of 32 rows, both backward forms
+SHAPES = [dict(lengths=[1] * 12, adapter=[0, 1, 2] * 4, adapters=3, rmax=16, out=70, cols=136),
+          dict(lengths=[1] * 150, adapter=[i % 4 for i in range(150)], adapters=4, rmax=8, out=130, cols=256),
+          dict(lengths=[20, 3, 40, 50], adapter=[0, 1, 2, 1], adapters=3, rmax=32, out=96, cols=264),
+          dict(lengths=[33, 20, 60], adapter=[1, 0, 2], adapters=3, rmax=104, out=100, cols=328)]
+
+
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+def test_a_row_of_nan(i):
+    """Reaches its own row's outputs and its adapter's gradients, and nothing else."""
+    c = Case(**SHAPES[i])
+    y, u = c.forward()
+    g = c.backward(u=u)
+    row = c.seq // 2
+    rest = np.arange(c.seq) != row
+    ad = c.of[row]
+    c.x[row, 3], c.dy[row, 1] = np.nan, np.inf
+    by, bu = c.forward()
+    by, bu, y, u = (v.reshape(c.seq, -1) for v in (by, bu, y, u))
+    assert np.isnan(by[row]).all() and same(by[rest], y[rest]) and same(bu[rest], u[rest])
+    bg = c.backward(u=np.where(rest[:, None], u, np.nan).astype(F32))
+    a, b = (v[0].reshape(c.seq, -1) for v in (bg, g))
+    assert not np.isfinite(a[row]).any() and same(a[rest], b[rest])
+    others = np.arange(c.n) != ad
+    for k, shape in ((1, c.a.shape), (2, c.b.shape)):
+        assert same(bg[k].reshape(shape)[others], g[k].reshape(shape)[others])
+    assert np.isnan(bg[1].reshape(c.a.shape)[ad, :, 3]).all() and np.isnan(bg[2].reshape(c.b.shape)[ad]).all()
+
+
+@pytest.mark.parametrize("rmax", [8, 32, 72])
+def test_many_requests(rmax):
+    """More requests than a wave looks at together, most of them empty."""
+    rng = np.random.default_rng(rmax)
+    lengths = np.where(rng.random(700) < 0.8, 0, rng.integers(1, 9, 700))
+    c = Case(list(lengths), rng.integers(-1, 6, 700), 5, rmax, out=84, cols=72, mixed=True, first=2, behind=5)
+    y, u = c.forward()
+    want, wu = c.want()
+    close(u, wu, "u")
+    close(y, want, "y")
+    for g, w, n in zip(c.backward(u=u), c.want_grad(ref.Sums(u.reshape(c.seq, rmax).astype(float))), ("dx", "da", "db")):
+        close(g, w, n)
+
+
+@pytest.mark.parametrize("rmax", [16, 128])
+def test_rows_that_are_not_there(rmax):
+    """Requests that begin before the first row or end behind the last have the rows between; no request at all has none."""
+    c = Case([40], [0], 2, rmax, out=50, cols=64, mixed=False)
+    c.start, c.adapter = np.array([-7, 5, 33, 2 ** 31 - 1], np.int32), np.array([1, 0, 1], np.int32)
+    c.of = ref.owners(c.seq, c.start, c.adapter, c.n)
+    assert (c.of >= 0).all()
+    for _ in range(2):
+        y, u = c.forward()
+        close(y, c.want()[0], "y")
+        for g, w, n in zip(c.backward(u=u), c.want_grad(ref.Sums(u.reshape(c.seq, rmax).astype(float))), ("dx", "da", "db")):
+            close(g, w, n)
+        c.start = np.array([2 ** 31 - 3, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31 - 1], np.int32)
+        c.of = ref.owners(c.seq, c.start, c.adapter, c.n)
+        assert (c.of < 0).all()
+
+
+class Part:
+    """An array `off` bytes into a larger one, with bytes on both sides that nothing may write."""
+
+    def __init__(self, nbytes, off=0, a=None):
+        self.off, self.nbytes, self.all = off, nbytes, nlgpu.DeviceArray(nbytes + off + 4096)
+        whole = np.full(nbytes + off + 4096, 0xA5, np.uint8)
+        if a is not None:
+            whole[off:off + nbytes] = a.reshape(-1).view(np.uint8)
+        self.all.upload(whole)
+        self.ptr = self.all.ptr + off
+
+    def get(self):
+        v = self.all.download(np.uint8)
+        assert (v[:self.off] == 0xA5).all() and (v[self.off + self.nbytes:] == 0xA5).all()
+        return v[self.off:self.off + self.nbytes].view(F32)
+
+
+@pytest.mark.parametrize("i", range(len(SHAPES)))
+@pytest.mark.parametrize("seq_out", [0, 2])
+def test_alignment_and_ends(i, seq_out):
+    """y, res and dy a word off their vectors' alignment, every array and workspace exactly as long as it must be."""
+    c = Case(**{**SHAPES[i], "out": SHAPES[i]["out"] // 4 * 4 + seq_out})
+    n = len(c.adapter)
+    d = {k: up(getattr(c, k)) for k in ("x", "a16", "b16", "scale", "adapter", "start", "rank", "dres")}
+    res, dy = Part(c.res.nbytes, 4, c.res), Part(c.dy.nbytes, 4, c.dy)
+    y, u = Part(c.res.nbytes, 4), Part(4 * c.seq * c.rmax)
+    ws = Part(nlgpu.lora_linear_workspace(c.seq, c.out, c.cols, c.rmax, n))
+    nlgpu.lora_linear(d["x"], d["a16"], d["b16"], d["scale"], d["adapter"], res, y, c.seq, c.out, c.cols, c.n, c.rmax, n, ws,
+                      start=d["start"], rank=d["rank"], u=u, fmt=c.fmt)
+    nlgpu.sync()
+    want, wu = c.want()
+    close(y.get(), want, "y")
+    close(u.get(), wu, "u")
+    ws.get()
+    da, db, dx = Part(4 * c.a.size), Part(4 * c.b.size), Part(c.x.nbytes)
+    ws = Part(nlgpu.lora_linear_grad_workspace(c.seq, c.out, c.cols, c.n, c.rmax, n))
+    nlgpu.lora_linear_grad(d["x"], None, dy, d["a16"], d["b16"], d["scale"], d["adapter"], da, db, c.seq, c.out, c.cols, c.n,
+                           c.rmax, n, ws, dres=d["dres"], dx=dx, start=d["start"], rank=d["rank"], fmt=c.fmt)
+    nlgpu.sync()
+    for g, w, name in zip((dx, da, db), c.want_grad(wu), ("dx", "da", "db")):
+        close(g.get(), w, name)
+    ws.get()
+
+
+def test_row_is_its_request():
+    """No `start`: request i is row i, and rows behind the last request have no adapter."""
+    c = Case([1] * 30, [i % 3 for i in range(30)], 3, 16, out=40, cols=64, behind=6)
+    y, u = c.forward(start=False)
+    want, wu = c.want()
+    close(u, wu, "u")
+    close(y, want, "y")
+
+
+@pytest.mark.parametrize("i", [0, 2])
+def test_captured(i):
+    """Two captured calls that share a workspace (a projection with its adapters, their gradients), replayed in turn and
+    between eager calls while rows, adapters and requests change: the eager bits each time."""
+    c = Case(**SHAPES[i])
+    n = len(c.adapter)
+    st = nlgpu.lib().nlg_stream_create()
+    w = up(nlgpu.pack_ternary(nlgpu.trits(c.out, (c.out, c.cols))))
+    d = {k: up(getattr(c, k)) for k in ("x", "a16", "b16", "scale", "adapter", "start", "rank", "dres", "dy")}
+    beta = up(np.array([0.03], F32))
+    need = max(nlgpu.ternary_linear_lora_workspace(c.seq, c.out, c.cols, c.rmax, n),
+               nlgpu.lora_linear_grad_workspace(c.seq, c.out, c.cols, c.n, c.rmax, n))
+    ws = nlgpu.DeviceArray(need)
+    o = [nlgpu.DeviceArray(4 * k) for k in (c.seq * c.out, c.seq * c.rmax, c.x.size, c.a.size, c.b.size)]
+
+    def forward():
+        nlgpu.ternary_linear_lora(d["x"], w, None, beta, d["a16"], d["b16"], d["scale"], d["adapter"], o[0], c.seq, c.out,
+                                  c.cols, c.n, c.rmax, n, ws, start=d["start"], rank=d["rank"], u=o[1], stream=st)
+
+    def backward():
+        nlgpu.lora_linear_grad(d["x"], o[1], d["dy"], d["a16"], d["b16"], d["scale"], d["adapter"], o[3], o[4], c.seq, c.out,
+                               c.cols, c.n, c.rmax, n, ws, dres=d["dres"], dx=o[2], start=d["start"], rank=d["rank"],
+                               stream=st)
+
+    def run(*go):
+        for a in o:
+            a.zero(st)
+        for g in go:
+            g()
+        nlgpu.sync(st)
+        return [a.download(F32) for a in o]
+
+    run(forward, backward)  # (before a capture: the base's column split wants its scratch from an eager call)
+    graphs = []
+    for f in (forward, backward):
+        nlgpu.graph_begin(st)
+        f()
+        graphs.append(nlgpu.graph_end(st))
+    rng = np.random.default_rng(1)
+    seen = None
+    for k in range(4):
+        if k:
+            d["x"].upload(c.x * F32(k + 1))
+            d["a16"].upload(rng.permutation(c.a16.reshape(c.n, -1)))
+            d["adapter"].upload(rng.permutation(c.adapter))
+        eager = run(forward, backward)
+        for _ in range(2):
+            got = run(*[lambda g=g: nlgpu.graph_launch(g, st) for g in graphs])
+            assert all(same(a, b) for a, b in zip(got, eager))
+        assert seen is None or not same(seen, eager[0])
+        seen = eager[0]
+    for g in graphs:
+        nlgpu.graph_destroy(g)
+    nlgpu.lib().nlg_stream_destroy(st)
+
+
+def test_two_streams():
+    """Calls that overlap on two streams, each with its own workspace, give the bits of calls alone."""
+    cs = [Case(**{**SHAPES[2], "seed": k}) for k in range(2)]
+    want = [(c.forward(), c.backward(u=c.forward()[1])) for c in cs]
+    st = [nlgpu.lib().nlg_stream_create() for _ in cs]
+    got = [(c.forward(stream=s), c.backward(u=w[0][1], stream=s)) for c, s, w in zip(cs, st, want)]
+    for g, w in zip(got, want):
+        assert all(same(a, b) for x, y in zip(g, w) for a, b in zip(x, y))
+    n = len(cs[0].adapter)
+    runs = []
+    for c, s in zip(cs, st):
+        d = {k: up(getattr(c, k)) for k in ("x", "a16", "b16", "scale", "adapter", "start", "rank", "res")}
+        d["y"], d["ws"] = nlgpu.DeviceArray(c.res.nbytes), nlgpu.DeviceArray(
+            nlgpu.lora_linear_workspace(c.seq, c.out, c.cols, c.rmax, n))
+        runs.append((c, s, d))
+    nlgpu.sync()
+    for _ in range(5):
+        for c, s, d in runs:
+            nlgpu.lora_linear(d["x"], d["a16"], d["b16"], d["scale"], d["adapter"], d["res"], d["y"], c.seq, c.out, c.cols,
+                              c.n, c.rmax, n, d["ws"], start=d["start"], rank=d["rank"], fmt=c.fmt, stream=s)
+    for (c, s, d), w in zip(runs, want):
+        nlgpu.sync(s)
+        assert same(d["y"].download(F32), w[0][0].ravel())
+        nlgpu.lib().nlg_stream_destroy(s)

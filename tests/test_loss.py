@@ -109,6 +109,25 @@ def test_distill_refusals(change, word):
         nlgpu.ternary_distill(**{**a, **change})
 
 
+@pytest.mark.parametrize("change", [
+    dict(dx="x"), dict(loss="x"), dict(lse="loss"), dict(dx="loss"), dict(dx="lse"), dict(lse="index"), dict(loss="dloss"),
+    dict(dx="w2"), dict(lse="beta"), dict(loss="bias"), dict(dx="teacher"), dict(lse="teacher_lse")])
+def test_overlaps(change):
+    a = {n: Ptr((i + 1) << 36) for i, n in enumerate(("x", "w2", "bias", "beta", "index", "teacher", "teacher_lse", "dloss",
+                                                       "loss", "lse", "dx", "workspace"))}
+    for out, other in change.items():
+        a[out] = Ptr(a[other].ptr)
+    a.update(rows=3, vocab=1000, cols=256, top=4, temperature=1.0)
+    with pytest.raises(nlgpu.NlgError, match="overlap"):
+        nlgpu.ternary_distill(**a)
+    if "teacher" not in str(change):
+        for k in ("teacher", "teacher_lse", "top", "temperature"):
+            del a[k]
+        a["label"] = a.pop("index")
+        with pytest.raises(nlgpu.NlgError, match="overlap"):
+            nlgpu.ternary_xent(**a)
+
+
 def test_no_rows_is_no_call():
     nlgpu.ternary_xent(**{**GOOD, "rows": 0})
 
