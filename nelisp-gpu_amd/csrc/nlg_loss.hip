@@ -365,9 +365,11 @@ struct LossArgs {
 
 // A workgroup a row: the tiles' maxima and sums joined, the targets' logits
 // (each wave one target at a time: the row's int8 values stay in the lanes),
-// the teacher's probabilities, the loss.
-__global__ __launch_bounds__(256) void k_loss(LossArgs a) {
-  __shared__ float s_z[LOSS_TOP], s_r[4], s_r2[4];
+// the teacher's probabilities, the loss.  It waits for the targets' rows of
+// weights: W waves, so that up to 4 W of them are on the way together.
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_loss(LossArgs a) {
+  __shared__ float s_z[LOSS_TOP], s_r[W], s_r2[W];
   const uint32_t s = blockIdx.x;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   // targets' logits, in base 2
@@ -375,7 +377,7 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
   const uint4 *xr = (const uint4 *)(a.xq + (size_t)s * a.cols);
   const float gm = a.gamma[s];
   // four targets at a time a wave: their weights are on the way together
-  for (uint32_t k0 = 4 * w; k0 < a.top; k0 += 16) {
+  for (uint32_t k0 = 4 * w; k0 < a.top; k0 += 4 * W) {
     int32_t at[4];
     const uint32_t *wr[4];
     int q[4];
@@ -404,13 +406,13 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
   }
   // the tiles' parts
   float m = -INFINITY, l = 0.0f;
-  for (uint32_t i = threadIdx.x; i < a.tiles; i += 256) {
+  for (uint32_t i = threadIdx.x; i < a.tiles; i += 64 * W) {
     const float2 p = a.part[(size_t)s * a.tiles + i];
     join(m, l, p.x, p.y);
   }
-  const float top = nlg_block_max_f32<4>(m, s_r);
+  const float top = nlg_block_max_f32<W>(m, s_r);
   const float at = top == -INFINITY ? 0.0f : top;
-  const float total = nlg_block_sum_f32<4>(l * nlg_exp2(m - at), s_r2);
+  const float total = nlg_block_sum_f32<W>(l * nlg_exp2(m - at), s_r2);
   const float tail = __builtin_amdgcn_logf(total);  // base 2
   const float ln2 = 0.69314718055994531f;
   // the targets' weights
@@ -423,16 +425,16 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
     tm = a.teacher_lse[s];
   } else if (tl) {
     float mx = -INFINITY, sm = 0.0f;
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256)
+    for (uint32_t k = threadIdx.x; k < a.top; k += 64 * W)
       if (ix[k] >= 0 && (uint32_t)ix[k] < a.vocab) mx = max_nn(mx, tl[k]);
-    tm = nlg_block_max_f32<4>(mx, s_r);
-    for (uint32_t k = threadIdx.x; k < a.top; k += 256)
+    tm = nlg_block_max_f32<W>(mx, s_r);
+    for (uint32_t k = threadIdx.x; k < a.top; k += 64 * W)
       if (ix[k] >= 0 && (uint32_t)ix[k] < a.vocab) sm += nlg_exp2((tl[k] - tm) * c2);
-    base = __builtin_amdgcn_logf(nlg_block_sum_f32<4>(sm, s_r2));
+    base = __builtin_amdgcn_logf(nlg_block_sum_f32<W>(sm, s_r2));
   }
   float loss = 0.0f, sum = 0.0f;
   __syncthreads();
-  for (uint32_t k = threadIdx.x; k < a.top; k += 256) {
+  for (uint32_t k = threadIdx.x; k < a.top; k += 64 * W) {
     float t = 0.0f;
     if (ix[k] >= 0 && (uint32_t)ix[k] < a.vocab) {
       // log2 of the target's weight and of the row's probability of it
@@ -444,12 +446,12 @@ __global__ __launch_bounds__(256) void k_loss(LossArgs a) {
     }
     a.weight[(size_t)s * a.top + k] = t;
   }
-  loss = nlg_block_sum_f32<4>(loss, s_r);
-  sum = nlg_block_sum_f32<4>(sum, s_r2);
+  loss = nlg_block_sum_f32<W>(loss, s_r);
+  sum = nlg_block_sum_f32<W>(sum, s_r2);
   float bm = 0.0f;
   if (a.per_row && s == 0) {
-    for (uint32_t i = threadIdx.x; i < a.tiles; i += 256) bm = max_nn(bm, a.bmax[i]);
-    bm = nlg_block_max_f32<4>(bm, s_r);
+    for (uint32_t i = threadIdx.x; i < a.tiles; i += 64 * W) bm = max_nn(bm, a.bmax[i]);
+    bm = nlg_block_max_f32<W>(bm, s_r);
   }
   if (threadIdx.x == 0) {
     a.loss[s] = loss * ln2;
@@ -814,7 +816,8 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
   l.part = h.part; l.bmax = h.bmax; l.index = index; l.teacher = teacher; l.teacher_lse = teacher_lse;
   l.loss = loss; l.lse = lse; l.lse2 = (float *)(ws + p.lse); l.sum = (float *)(ws + p.sum);
   l.weight = (float *)(ws + p.weight);
-  hipLaunchKernelGGL(k_loss, dim3(rows), dim3(256), 0, st, l);
+  if (top > 16) hipLaunchKernelGGL((k_loss<16>), dim3(rows), dim3(1024), 0, st, l);
+  else hipLaunchKernelGGL((k_loss<4>), dim3(rows), dim3(256), 0, st, l);
   NLG_LAUNCHED(what);
   if (!dx) return NLG_OK;
   // one tile of rows needs no order
