@@ -543,17 +543,20 @@ __device__ __forceinline__ void turn16(uint32_t (&w)[16]) {
 // vocabulary rows at a time (waves 0..3 the even ones, 4..7 the odd ones); a
 // lane makes f16 of its eight fields with one byte permutation a pair (the
 // high byte of 0, +1, -2, -1).  Probabilities go from memory to LDS directly,
-// 32 vocabulary rows at a time, two stages, the second loaded while the first
-// is multiplied.
-template <int WM, int TM, int TN>
+// 32 vocabulary rows at a time, NS - 1 steps ahead: one is enough for 256 rows,
+// fewer are multiplied sooner than memory answers.
+template <int WM, int TM, int TN, int NS>
 __global__ __launch_bounds__(512) void k_back(BackArgs a) {
   constexpr int WN = 8 / WM, BM = 32 * TM * WM;
   static_assert(WN * TN == 8, "256 columns");
   constexpr int STAGE = 4 * 2 * BM;                        // 16-byte units of 32 vocabulary rows
   constexpr int NL = STAGE / 64, PI = NL < 8 ? 1 : NL / 8; // loads a stage, a wave's
+  // (apart: a read of one stage waits for no load of another)
   __shared__ __align__(1024) uint4 s_p0[STAGE];
   __shared__ __align__(1024) uint4 s_p1[STAGE];
-  __shared__ uint32_t s_w[2][16][256];
+  __shared__ __align__(1024) uint4 s_p2[NS > 2 ? STAGE : 1];
+  __shared__ __align__(1024) uint4 s_p3[NS > 2 ? STAGE : 1];
+  __shared__ __align__(16) uint32_t s_w[2 * 16 * 256];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 31, lg = lane >> 5;
@@ -581,7 +584,7 @@ __global__ __launch_bounds__(512) void k_back(BackArgs a) {
     turn16(wv);
 #pragma unroll
     for (int q = 0; q < 4; q++)
-      *(uint4 *)&s_w[odd][wr][16 * wi + 4 * q] = make_uint4(wv[4 * q], wv[4 * q + 1], wv[4 * q + 2], wv[4 * q + 3]);
+      *(uint4 *)&s_w[odd * 4096 + wr * 256 + 16 * wi + 4 * q] = make_uint4(wv[4 * q], wv[4 * q + 1], wv[4 * q + 2], wv[4 * q + 3]);
   };
   const uint4 *const p0 = a.prob + (size_t)(k0 / 8) * 2 * a.chunk + row0;
   const auto loadp = [&](uint32_t step, uint4 *stage) {
@@ -599,17 +602,25 @@ __global__ __launch_bounds__(512) void k_back(BackArgs a) {
 #pragma unroll
     for (int n = 0; n < TN; n++) acc[m][n] = (v16f){};
   const auto mma = [&](uint32_t step, const uint4 *stage) {
-    const uint32_t buf = step / 8 % 2, g = step % 8 * 2;
+    const uint32_t wa = step / 8 % 2 * 4096 + wn * TN * 32 + li, g = step % 8 * 2;
+    uint32_t pa = 2 * lg * BM + wm * TM * 32 + li;
+    asm volatile("" : "+v"(pa));
     half8v p[2][TM][2];
     uint32_t t[2][TN];
     const auto read = [&](int h) {
 #pragma unroll
-      for (int n = 0; n < TN; n++) t[h][n] = s_w[buf][g + h][(wn * TN + n) * 32 + li];
+      for (int n = 0; n < TN; n++) {
+        // (an index of its own, as of a stage in each step: of addresses derived from one another the compiler no longer
+        // knows which array they are in, and waits for every load that is on its way to LDS)
+        uint32_t at = wa + (g + h) * 256 + n * 32;
+        asm volatile("" : "+v"(at));
+        t[h][n] = s_w[at];
+      }
 #pragma unroll
       for (int m = 0; m < TM; m++)
 #pragma unroll
         for (int q = 0; q < 2; q++)
-          p[h][m][q] = __builtin_bit_cast(half8v, stage[((2 * h + lg) * 2 + q) * BM + (wm * TM + m) * 32 + li]);
+          p[h][m][q] = __builtin_bit_cast(half8v, stage[pa + (4 * h + q) * BM + m * 32]);
     };
     read(0);
 #pragma unroll
@@ -634,32 +645,45 @@ __global__ __launch_bounds__(512) void k_back(BackArgs a) {
     }
   };
   // the first two blocks' weights, each by its half of the waves
-  if (odd < chunks) {
-    loadw(odd);
-    loadp(0, s_p0);
-    storew();
+  if (odd < chunks) loadw(odd);
+  loadp(0, s_p0);
+  if (NS > 2) {
+    loadp(1, s_p1);
+    loadp(2, s_p2);
+  }
+  if (odd < chunks) storew();
+  // A step: its stage has landed (newer: those of the next NS - 2 steps, and a block's weights where they were asked
+  // for after it), every wave is done with the stage before, which is loaded anew (the last one again at the end).
+  // While one block is multiplied, the half whose block is done loads its next one.
+#define STEP(j, SCUR, SLOAD)                                                     \
+  {                                                                              \
+    const uint32_t s = s0 + (j), next = s / 8 + 1;                               \
+    const bool turn = s >= 8 && next < chunks && next % 2 == odd;                \
+    if (NS > 2 && turn && s % 8 >= 1 && s % 8 < NS) WAIT_VM((NS - 2) * PI + 16); \
+    else WAIT_VM((NS - 2) * PI);                                                 \
+    __builtin_amdgcn_s_barrier();                                                \
+    ORDER();                                                                     \
+    loadp(s + NS - 1 < steps ? s + NS - 1 : steps - 1, SLOAD);                   \
+    if (turn && s % 8 == 0) loadw(next);                                         \
+    if (turn && s % 8 == 7) storew();                                            \
+    mma(s, SCUR);                                                                \
+    ORDER();                                                                     \
+  }
+  if (NS == 2) {
+    for (uint32_t s0 = 0; s0 < steps; s0 += 2) {
+      STEP(0, s_p0, s_p1)
+      STEP(1, s_p1, s_p0)
+    }
   } else {
-    loadp(0, s_p0);
+    for (uint32_t s0 = 0; s0 < steps; s0 += 4) {
+      STEP(0, s_p0, s_p3)
+      STEP(1, s_p1, s_p0)
+      STEP(2, s_p2, s_p1)
+      STEP(3, s_p3, s_p2)
+    }
   }
-  for (uint32_t s = 0; s < steps; s += 2) {
-    WAIT_VM(0);
-    __builtin_amdgcn_s_barrier();
-    ORDER();
-    loadp(s + 1, s_p1);
-    // while one block is multiplied, the half whose block is done loads its next one
-    const uint32_t block = s / 8, next = block + 1;
-    const bool turn = block > 0 && next < chunks && next % 2 == odd;
-    if (turn && s % 8 == 0) loadw(next);
-    mma(s, s_p0);
-    ORDER();
-    WAIT_VM(0);
-    __builtin_amdgcn_s_barrier();
-    ORDER();
-    if (s + 2 < steps) loadp(s + 2, s_p0);
-    if (turn && s % 8 == 6) storew();
-    mma(s + 1, s_p1);
-    ORDER();
-  }
+#undef STEP
+  WAIT_VM(0);  // the last (repeated) stages land before the LDS is given back
   // register r: row (r % 4) + 8 (r / 4) + 4 lg of the block, column li
 #pragma unroll
   for (int m = 0; m < TM; m++)
@@ -841,10 +865,10 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
     NLG_LAUNCHED(what);
     const uint32_t ncol = (cols + LOSS_CUT - 1) / LOSS_CUT, pairs = p.chunk / p.bm * p.splits;
     const dim3 grid((pairs + 7) / 8 * 8 * ncol), blk(512);
-    if (p.bm == 256) hipLaunchKernelGGL((k_back<2, 4, 2>), grid, blk, 0, st, b);
-    else if (p.bm == 128) hipLaunchKernelGGL((k_back<2, 2, 2>), grid, blk, 0, st, b);
-    else if (p.bm == 64) hipLaunchKernelGGL((k_back<2, 1, 2>), grid, blk, 0, st, b);
-    else hipLaunchKernelGGL((k_back<1, 1, 1>), grid, blk, 0, st, b);
+    if (p.bm == 256) hipLaunchKernelGGL((k_back<2, 4, 2, 2>), grid, blk, 0, st, b);
+    else if (p.bm == 128) hipLaunchKernelGGL((k_back<2, 2, 2, 4>), grid, blk, 0, st, b);
+    else if (p.bm == 64) hipLaunchKernelGGL((k_back<2, 1, 2, 4>), grid, blk, 0, st, b);
+    else hipLaunchKernelGGL((k_back<1, 1, 1, 4>), grid, blk, 0, st, b);
     NLG_LAUNCHED(what);
     hipLaunchKernelGGL(k_dx, dim3(n, (cols + 1023) / 1024), dim3(256), 0, st, d);
     NLG_LAUNCHED(what);
