@@ -25,14 +25,14 @@ struct LossPlan {
 static inline uint64_t loss_round(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // How many parts the gradient's product takes its `tiles` tiles of vocabulary in: those of the shortest time by a
-// measured 1 us for 32 vocabulary rows of a 256 x 256 tile (as many such tiles as CUs side by side, smaller ones in
+// measured 13 us for 256 vocabulary rows of a 256 x 256 tile (as many such tiles as CUs side by side, smaller ones in
 // proportion), 6 us to begin and end one, and 4 TB/s for what the parts leave and is read again.
 static inline uint32_t loss_splits(uint32_t tiles, uint32_t bm, uint64_t workgroups, uint64_t values) {
   uint32_t best = 1;
   double least = 0;
   for (uint32_t n = 1; n <= 64 && n <= tiles; n++) {
     const double rounds = (double)((workgroups * n + 255) / 256), share = (double)((tiles + n - 1) / n);
-    const double t = rounds * (share * 8 * bm / 256 + 6) + (double)n * (double)values * 8 / 4e6;
+    const double t = rounds * (share * 13 * bm / 256 + 6) + (double)n * (double)values * 8 / 4e6;
     if (n == 1 || t < least) {
       least = t;
       best = n;

@@ -652,15 +652,14 @@ __global__ __launch_bounds__(512) void k_back(BackArgs a) {
     loadp(2, s_p2);
   }
   if (odd < chunks) storew();
-  // A step: its stage has landed (newer: those of the next NS - 2 steps, and a block's weights where they were asked
-  // for after it), every wave is done with the stage before, which is loaded anew (the last one again at the end).
-  // While one block is multiplied, the half whose block is done loads its next one.
+  // A step: its stage has landed (at least those of the next NS - 2 steps are newer), every wave is done with the stage
+  // before, which is loaded anew (the last one again at the end).  While one block is multiplied, the half whose block is
+  // done loads its next one.
 #define STEP(j, SCUR, SLOAD)                                                     \
   {                                                                              \
     const uint32_t s = s0 + (j), next = s / 8 + 1;                               \
     const bool turn = s >= 8 && next < chunks && next % 2 == odd;                \
-    if (NS > 2 && turn && s % 8 >= 1 && s % 8 < NS) WAIT_VM((NS - 2) * PI + 16); \
-    else WAIT_VM((NS - 2) * PI);                                                 \
+    WAIT_VM((NS - 2) * PI);                                                      \
     __builtin_amdgcn_s_barrier();                                                \
     ORDER();                                                                     \
     loadp(s + NS - 1 < steps ? s + NS - 1 : steps - 1, SLOAD);                   \
