@@ -94,6 +94,10 @@ enum { LOGSUM, PROB };
 // times its value (the sums are 64 times the exact ones).
 // TAIL: cols is no multiple of 256, and the last step's words past the row
 // are zeroed.
+// Vocabulary tiles of one token group follow each other on an XCD, so weights
+// come from HBM once and activations from L2.  From 64 rows on the matrix cores
+// bound it: 4,096 rows of 128,256 x 2,560 1.14 ms (2.35 POP/s), 512 rows 150 us;
+// one row reads the weights, 82 MB in 19.9 us (4.1 TB/s).  PROB: 1,024 rows 336 us.
 template <int MODE, int MB, bool TAIL>
 __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
   constexpr int NB = 2, MT = 32 * MB, STAGE = MT * KC;
@@ -150,12 +154,22 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
   // (macros: register sets handed to a lambda end up in scratch)
 #define LOADW(c, dst)                                                                              \
   do {                                                                                             \
+    if (TAIL && 16 * (c) + 16 > wng) LOADW_END(c, dst);                                            \
+    else _Pragma("unroll") for (int nt = 0; nt < NB; nt++) {                                       \
+      const uint4 u0 = wp[nt][4 * (c)], u1 = wp[nt][4 * (c) + 1];                                  \
+      dst[8 * nt + 0] = u0.x; dst[8 * nt + 1] = u0.y; dst[8 * nt + 2] = u0.z;                      \
+      dst[8 * nt + 3] = u0.w; dst[8 * nt + 4] = u1.x; dst[8 * nt + 5] = u1.y;                      \
+      dst[8 * nt + 6] = u1.z; dst[8 * nt + 7] = u1.w;                                              \
+    }                                                                                              \
+  } while (0)
+  // (a unit past the row reads the row's first; in the last step alone, as the masks wait for the loads)
+#define LOADW_END(c, dst)                                                                          \
+  do {                                                                                             \
+    /* 16-byte units: cols is a multiple of 64 */                                                  \
+    const bool in0 = 16 * (c) + 8 * lg < wng, in1 = 16 * (c) + 8 * lg + 4 < wng;                   \
+    const uint32_t k0 = in0 ? 0xffffffffu : 0u, k1 = in1 ? 0xffffffffu : 0u;                       \
     _Pragma("unroll") for (int nt = 0; nt < NB; nt++) {                                            \
-      /* 16-byte units: cols is a multiple of 64 */                                                \
-      const uint32_t at = 4 * (c);                                                                 \
-      const bool in0 = !TAIL || 4 * at + 8 * lg < wng, in1 = !TAIL || 4 * at + 8 * lg + 4 < wng;   \
-      const uint4 u0 = wp[nt][in0 ? at : 0], u1 = wp[nt][in1 ? at + 1 : 0];                        \
-      const uint32_t k0 = in0 ? 0xffffffffu : 0u, k1 = in1 ? 0xffffffffu : 0u;                     \
+      const uint4 u0 = wp[nt][in0 ? (int)(4 * (c)) : -2 * lg], u1 = wp[nt][in1 ? (int)(4 * (c) + 1) : -2 * lg]; \
       dst[8 * nt + 0] = u0.x & k0; dst[8 * nt + 1] = u0.y & k0; dst[8 * nt + 2] = u0.z & k0;       \
       dst[8 * nt + 3] = u0.w & k0; dst[8 * nt + 4] = u1.x & k1; dst[8 * nt + 5] = u1.y & k1;       \
       dst[8 * nt + 6] = u1.z & k1; dst[8 * nt + 7] = u1.w & k1;                                    \
@@ -266,6 +280,7 @@ __global__ __launch_bounds__(256, 2) void k_head(HeadArgs a) {
 #undef RDA
 #undef LOADA
 #undef LOADW
+#undef LOADW_END
   WAIT_VM(0);  // the last (repeated) stage loads land before the LDS is given back
   // acc[nt][mt] register r of lane (li, lg): vocabulary row 32 nt + (r % 4) +
   // 8 (r / 4) + 4 lg of the wave's 64, token 32 mt + li
@@ -366,7 +381,8 @@ struct LossArgs {
 // A workgroup a row: the tiles' maxima and sums joined, the targets' logits
 // (each wave one target at a time: the row's int8 values stay in the lanes),
 // the teacher's probabilities, the loss.  It waits for the targets' rows of
-// weights: W waves, so that up to 4 W of them are on the way together.
+// weights: W waves, so that up to 4 W of them are on the way together (333 rows
+// of 100 targets: 26.4 us with four waves, 14.3 with sixteen; of one target 5 us).
 template <int W>
 __global__ __launch_bounds__(64 * W) void k_loss(LossArgs a) {
   __shared__ float s_z[LOSS_TOP], s_r[W], s_r2[W];
@@ -466,7 +482,8 @@ __global__ __launch_bounds__(64 * W) void k_loss(LossArgs a) {
   }
 }
 
-// The rows with targets in order, then those without; order[rows]: how many have.
+// The rows with targets in order, then those without; order[rows]: how many have.  (One workgroup, two passes: 5.8 us for
+// 4,096 rows, where it saves a third of 4 ms.)
 __global__ __launch_bounds__(1024) void k_order(const float *sum, int32_t *order, uint32_t rows) {
   __shared__ uint32_t s_n[16];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -544,7 +561,11 @@ __device__ __forceinline__ void turn16(uint32_t (&w)[16]) {
 // lane makes f16 of its eight fields with one byte permutation a pair (the
 // high byte of 0, +1, -2, -1).  Probabilities go from memory to LDS directly,
 // 32 vocabulary rows at a time, NS - 1 steps ahead: one is enough for 256 rows,
-// fewer are multiplied sooner than memory answers.
+// fewer are multiplied sooner than memory answers (100 rows of 32,003 x 2,048
+// with one step 43.8 us, with three 37.5; 37 rows 30.9 and 27.9; 256 rows a tile
+// the same either way).
+// The matrix cores bound it: 1,024 rows of 128,256 x 2,560 1.10 ms, 1.22 PFLOP/s
+// of both halves.
 template <int WM, int TM, int TN, int NS>
 __global__ __launch_bounds__(512) void k_back(BackArgs a) {
   constexpr int WN = 8 / WM, BM = 32 * TM * WM;
@@ -710,7 +731,8 @@ struct DxArgs {
 };
 
 // dx of 1,024 columns of a row: four a thread (a byte of the targets' words),
-// eight targets' loads and eight parts' at a time.
+// eight targets' loads and eight parts' at a time.  100 rows of 2,048 in 32 parts
+// 5.8 us, 1,024 of 2,560 in 6 parts 14, with 64 targets each 30.
 __global__ __launch_bounds__(256) void k_dx(DxArgs a) {
   __shared__ float s_f[LOSS_TOP];
   __shared__ uint32_t s_at[LOSS_TOP];
