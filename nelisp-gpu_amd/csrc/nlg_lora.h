@@ -85,6 +85,9 @@ __device__ __forceinline__ void split_f16(uint32_t h, uint32_t &p0, uint32_t &p1
   p1 = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
 }
 
+// Whether the call below (and nlg_batched_gemm with NLG_EPI_STORE) takes rows of so many columns: also multiples of 64
+// that nlg_batched leaves to the kernels of few tokens.
+bool nlg_batched_lora(uint32_t seq, uint32_t cols);
 // The shared projection on the matrix cores with the adapters added to it
 // (nlg_batched_gemm otherwise); *done: whether the form that this size takes
 // adds them, or only the projection was run.  u [seq][rmax].

@@ -67,6 +67,8 @@ struct DownArgs {
 // the products' layout, 128 bytes of each of 32 rows at a time, 4,731 rows of
 // 4,096 took 35 us, and 18.7 without the reads of x.)  An x row's 16-byte units
 // are swizzled by its number.
+// Waits for memory: 4,731 rows of 4,096 down to 32 ranks 31 us (2.5 TB/s of x, in
+// three parts), 241 rows of 2,560 to 8 6.8 us.
 // Every load is in bounds and none is masked: ranks behind the rank make sums
 // that are thrown away, and a k behind the row has its weights zeroed.
 // KMAJOR: weights [k][rmax] (B, in the backward pass), else [rmax][k] (A).
@@ -306,7 +308,9 @@ __device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, 
 }
 
 #define TOK_RANKS 4
-// a workgroup's 4 waves: sixteen ranks of a row
+// a workgroup's 4 waves: sixteen ranks of a row, four a wave (each read of x feeds four dots, and a row of 64 ranks has
+// sixteen waves), in plain f32: an adapter's rows are too few for a tile.  Waits for memory; 64 rows of 2,560 with 48
+// adapters of up to 64 ranks 6.6 us with their rounding to int8 (tiles of 32 rows, a pass for each adapter among them: 324).
 template <bool BF>
 __device__ __forceinline__ void tok_down_group(const DownArgs &a, uint32_t row, uint32_t group) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -345,7 +349,9 @@ struct UpArgs {
 
 // 32 rows x 256 columns a workgroup, a wave 64 columns: four neighbouring
 // columns a lane, in four blocks (block e of the columns is 4 i + e), so that
-// results are stored sixteen bytes a lane.
+// results are stored sixteen bytes a lane.  f32 matrix cores (16 x 16 x 4: no
+// operand is rounded further); bound by what moves, 4,616 rows of 6,912 with
+// rank up to 32 58 us (4.4 TB/s of res and y).
 // KMAJOR: weights [rmax][n] (A, in the backward pass), else [n][rmax] (B).
 template <bool BF, bool KMAJOR, bool VEC>
 __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
@@ -461,7 +467,8 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
 
 // Few rows a request: a wave a row and NC steps of 64 / L columns, L lanes a
 // column (eight neighbouring ranks each: sixteen bytes), all on the way
-// together.
+// together.  Bound by the adapters' bytes: 64 rows of 48 adapters, up to 64
+// ranks to 6,912 columns, 9.9 us (tiles of 32 rows: 120).
 template <int L, int NC>
 struct TokUp {
   uint4 v[NC];
@@ -518,7 +525,9 @@ __global__ __launch_bounds__(256) void k_lora_tok_up(UpArgs a) {
 
 // A few rows of small adapters in one launch: every workgroup finds its row's
 // u again (two ranks a wave at a time), while its columns' weights are on the
-// way.
+// way.  One token, 2,560 -> 2,560 at rank 16: 4.4 us, a launch and two round trips
+// to memory (the call with its projection 8.2 us; with the ways down and up
+// apart, of tiles, 13).
 template <bool BF, int L>
 __global__ __launch_bounds__(512) void k_lora_tok(DownArgs d, UpArgs a) {
   __shared__ float s_u[LORA_RANK];
@@ -558,8 +567,10 @@ struct OuterArgs {
 
 // sum over an adapter's rows of p[s, j] q[s, c], 64 columns and 16 NT ranks a
 // workgroup, its requests' rows over the eight waves of gridDim.z workgroups,
-// four rows a wave at a time, four times of them on the way together.  TURN:
-// stored [c][j].
+// four rows a wave at a time, four times of them on the way together, in 16 x
+// 16 x 4 f32 products.  Waits for memory: 4,616 rows of 6,912, rank up to 32,
+// three adapters 46 us (2.7 TB/s); in 2, 3, 4 and 8 parts 52, 49, 51 and 59.
+// TURN: stored [c][j].
 template <int NT, bool TURN, bool VEC>
 __global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
   __shared__ v4f s_acc[4][NT][4][64];
@@ -1008,7 +1019,8 @@ struct LoraSum {
   uint64_t n4;
   uint32_t parts;
 };
-// The parts of such sums, added in order; of two of them in one launch.
+// The parts of such sums, added in order (so the bits are the same each time); of two of them in one launch, which is
+// what it costs at small sizes: 4 to 7 us.
 __global__ __launch_bounds__(256) void k_lora_sum(LoraSum a, LoraSum b) {
   for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < a.n4 + b.n4; i += gridDim.x * 256ull) {
     const bool second = i >= a.n4;
@@ -1296,7 +1308,7 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   hipStream_t st = nlg_stream(stream);
   uint8_t *const more = (uint8_t *)workspace + nu;
   const bool bf = fmt == NLG_LORA_BF16;
-  if (nlg_batched(seq, cols)) {
+  if (nlg_batched_lora(seq, cols)) {
     float *const gamma = (float *)(more + ((size_t)seq * cols + 255) / 256 * 256);
     FusedArgs f{};
     f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;

@@ -830,8 +830,11 @@ __device__ __forceinline__ void tl_epilogue(const GemmArgs &a, const v16i (&acc)
 // a compiler-level fence: no memory operation moves across it
 #define TW_ORDER() asm volatile("" ::: "memory")
 
-template <int EPI, bool TILED = false, int MB = 4, bool SPLIT = false>
+// TAIL: cols is a multiple of 64 only, in row layout and unsplit; the last
+// chunk's words past the row are zeroed (and meet the row's first activations).
+template <int EPI, bool TILED = false, int MB = 4, bool SPLIT = false, bool TAIL = false>
 __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
+  static_assert(!TAIL || (!TILED && !SPLIT), "");
   constexpr int WR = 4, NB = 2, MT = 32 * MB;  // MT tokens per workgroup
   constexpr int STAGE = MT * TG_KC;
   constexpr int PI = STAGE / 1024 / WR;  // 1 KiB stage loads per wave and chunk
@@ -850,7 +853,7 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
   const uint32_t rbase = blockIdx.x * (64 * WR) + wn * 64;
   const uint32_t tok0 = blockIdx.y * MT;
   // SPLIT: slice blockIdx.z of gridDim.z takes chunks cfirst .. + nchunks - 1
-  const uint32_t ntot = a.cols / TG_KC, ks = SPLIT ? gridDim.z : 1;
+  const uint32_t ntot = TAIL ? (a.cols + TG_KC - 1) / TG_KC : a.cols / TG_KC, ks = SPLIT ? gridDim.z : 1;
   const uint32_t cfirst = SPLIT ? blockIdx.z * ntot / ks : 0;
   const uint32_t nchunks = SPLIT ? (blockIdx.z + 1) * ntot / ks - cfirst : ntot;
   // weight rows of this lane: lane group lg holds words 8 lg .. 8 lg + 7 of
@@ -873,16 +876,18 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
   // real token), slot j % 16, i.e. unit (j % 16) ^ (k % 16) of its chunk row,
   // at byte offset xo[i] from column 0 of the workgroup's first token row
   // (under MT x 16384 bytes: the loads take a scalar base + 32-bit offset)
-  uint32_t xo[PI];
+  uint32_t xo[PI], xu[PI];
 #pragma unroll
   for (int i = 0; i < PI; i++) {
     const uint32_t k = 4 * (wn * PI + i) + lane / 16, tk = tok0 + k < a.seq ? tok0 + k : a.seq - 1;
-    xo[i] = (tk - tok0) * a.cols + 16 * ((lane % 16) ^ (k % 16));
+    xu[i] = 16 * ((lane % 16) ^ (k % 16));
+    xo[i] = (tk - tok0) * a.cols + xu[i];
   }
   const uint8_t *const xrow0 = a.xq + (size_t)tok0 * a.cols + (size_t)cfirst * TG_KC;
 #define TW_LOADW(c, dst)                                                                   \
   do {                                                                                     \
-    _Pragma("unroll") for (int nt = 0; nt < NB; nt++) {                                    \
+    if (TAIL && 16 * (c) + 16 > a.wng) TW_LOADW_END(c, dst);                               \
+    else _Pragma("unroll") for (int nt = 0; nt < NB; nt++) {                               \
       const uint4 u0 = TILED ? wp[nt][128 * (c)] : wp[nt][4 * (c)];                         \
       const uint4 u1 = TILED ? wp[nt][128 * (c) + 64] : wp[nt][4 * (c) + 1];                \
       dst[8 * nt + 0] = u0.x; dst[8 * nt + 1] = u0.y; dst[8 * nt + 2] = u0.z;               \
@@ -890,12 +895,25 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
       dst[8 * nt + 6] = u1.z; dst[8 * nt + 7] = u1.w;                                       \
     }                                                                                      \
   } while (0)
+  // (a unit past the row reads the row's first; in the last chunk alone, as the masks wait for the loads)
+#define TW_LOADW_END(c, dst)                                                               \
+  do {                                                                                     \
+    const bool in0 = 16 * (c) + 8 * lg < a.wng, in1 = 16 * (c) + 8 * lg + 4 < a.wng;       \
+    const uint32_t k0 = in0 ? 0xffffffffu : 0u, k1 = in1 ? 0xffffffffu : 0u;               \
+    _Pragma("unroll") for (int nt = 0; nt < NB; nt++) {                                    \
+      const uint4 u0 = wp[nt][in0 ? (int)(4 * (c)) : -2 * lg];                              \
+      const uint4 u1 = wp[nt][in1 ? (int)(4 * (c) + 1) : -2 * lg];                          \
+      dst[8 * nt + 0] = u0.x & k0; dst[8 * nt + 1] = u0.y & k0; dst[8 * nt + 2] = u0.z & k0; \
+      dst[8 * nt + 3] = u0.w & k0; dst[8 * nt + 4] = u1.x & k1; dst[8 * nt + 5] = u1.y & k1; \
+      dst[8 * nt + 6] = u1.z & k1; dst[8 * nt + 7] = u1.w & k1;                            \
+    }                                                                                      \
+  } while (0)
 #define TW_LOADA(c, stage)                                                                 \
   do {                                                                                     \
     const uint8_t *xc = xrow0 + (size_t)(c) * TG_KC;                                       \
     _Pragma("unroll") for (int i = 0; i < PI; i++)                                         \
       __builtin_amdgcn_global_load_lds(                                                    \
-          (const void *)(xc + xo[i]),                                                      \
+          (const void *)(TAIL && (c) * TG_KC + xu[i] >= a.cols ? xrow0 + (xo[i] - xu[i]) : xc + xo[i]), \
           (__attribute__((address_space(3))) void *)((stage) + 1024 * (wn * PI + i)), 16, 0, 0); \
   } while (0)
   // the epilogue operands first (their loads precede every stage load, so
@@ -1019,6 +1037,7 @@ __global__ __launch_bounds__(256, 2) void k_tgemm_w(GemmArgs a) {
 #undef TW_MMA
 #undef TW_RDA
 #undef TW_LOADW
+#undef TW_LOADW_END
 #undef TW_LOADA
   // the last (repeated) stage loads must land before the workgroup's LDS is
   // released
@@ -1068,9 +1087,28 @@ int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *
 int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
   GemmArgs a = a0;
   if (!a.seq || !a.out) return NLG_OK;
-  if (a.cols % TG_KC || !a.cols) return nlg_fail("ternary GEMM: cols must be a multiple of %d", TG_KC);
+  const bool tail = TG_LORA(epi) || epi == NLG_EPI_STORE ? a.cols % TG_KC && a.cols % 64 == 0 : false;
+  if ((a.cols % TG_KC && !tail) || !a.cols) return nlg_fail("ternary GEMM: cols must be a multiple of %d", TG_KC);
   if (((uintptr_t)a.w2 & 15) || ((uintptr_t)a.xq & 15)) return nlg_fail("ternary GEMM: 16-byte alignment");
   a.wng = a.cols / 16;
+  if (tail) {
+    // the wide-wave kernel alone, in 64-token tiles from 400 of them as below
+    const uint32_t rt = nlg_blocks(a.out, 256);
+    const bool t64 = (uint64_t)rt * ((a.seq + 63) / 64) >= 400;
+    const dim3 gt(rt, t64 ? (a.seq + 63) / 64 : (a.seq + 31) / 32);
+    if (gt.y > 65535) return nlg_fail("ternary GEMM: seq too large");
+#define TWT(E)                                                                                             \
+  do {                                                                                                     \
+    if (t64) hipLaunchKernelGGL((k_tgemm_w<E, false, 2, false, true>), gt, dim3(256), 0, st, a);           \
+    else hipLaunchKernelGGL((k_tgemm_w<E, false, 1, false, true>), gt, dim3(256), 0, st, a);               \
+  } while (0)
+    if (epi == NLG_EPI_STORE) TWT(NLG_EPI_STORE);
+    else if (epi == NLG_EPI_LORA_F16) TWT(NLG_EPI_LORA_F16);
+    else TWT(NLG_EPI_LORA_BF16);
+#undef TWT
+    NLG_LAUNCHED("ternary GEMM (int8 MFMA, wide waves, rows of 64s)");
+    return NLG_OK;
+  }
   // a registered tiled copy of the weights (nlg_ternary_tiled_register)
   // replaces the row layout: the same words, in load order
   const uint32_t *wt = nlg_tiled_find(a.w2, a.out, a.cols);
@@ -1297,6 +1335,7 @@ int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
 }
 
 bool nlg_batched(uint32_t seq, uint32_t cols) { return seq >= NLG_BATCHED_MIN && cols % TG_KC == 0; }
+bool nlg_batched_lora(uint32_t seq, uint32_t cols) { return seq >= NLG_BATCHED_MIN && cols % 64 == 0; }
 
 size_t nlg_batched_scratch_bytes(uint32_t seq, uint32_t cols) {
   return ((size_t)seq * cols + 255) / 256 * 256 + (size_t)seq * 4;

@@ -169,7 +169,13 @@ BESIDE = [dict(lengths=[1], adapter=[0], adapters=1, rmax=16, out=100, cols=256)
           dict(lengths=[40, 60], adapter=[0, 1], adapters=2, rmax=24, out=200, cols=768, mixed=True),
           dict(lengths=[70, 1, 0, 200], adapter=[2, 1, 0, 0], adapters=3, rmax=32, out=520, cols=1024, mixed=True, behind=3),
           dict(lengths=[100, 200, 33], adapter=[0, -1, 1], adapters=2, rmax=128, out=300, cols=4352, mixed=True),
-          dict(lengths=[513, 700], adapter=[1, 0], adapters=2, rmax=16, out=6700, cols=256, first=5)]
+          dict(lengths=[513, 700], adapter=[1, 0], adapters=2, rmax=16, out=6700, cols=256, first=5),
+          # rows of 64s: one unit, half a chunk, chunks and a rest; tiles of 32 and of 64 tokens
+          dict(lengths=[30, 41], adapter=[0, 1], adapters=2, rmax=16, out=300, cols=64),
+          dict(lengths=[200, 0, 90], adapter=[1, 1, 0], adapters=2, rmax=24, out=257, cols=128, behind=4),
+          dict(lengths=[1] * 40, adapter=[i % 3 for i in range(40)], adapters=3, rmax=16, out=130, cols=320),
+          dict(lengths=[600, 500, 700], adapter=[0, -1, 1], adapters=2, rmax=16, out=4000, cols=704),
+          dict(lengths=[1000, 777], adapter=[0, 1], adapters=2, rmax=8, out=4000, cols=1088)]
 
 
 @pytest.mark.parametrize("bf", [False, True])
