@@ -1162,10 +1162,19 @@ static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, ui
   return NLG_OK;
 }
 
-// Few rows a request, or few rows at all.
-static bool lora_by_token(const LoraArgs &l) { return l.seq <= 16 || (l.seq < 4ull * l.requests && l.seq < 65536); }
+// A wave a row, which reads its adapter anew, or tiles of 32 rows, a pass for each adapter among them: the former while what
+// is read so stays small (`most` ranks times columns), or requests have fewer than four rows.  Measured, us a call, by row
+// and by tile, 2560 -> 2560 at rank 16 unless told.  Alone (most 2^27): 256 rows of a request 8.5 and 14.8, 1,024 16.7 and
+// 18.3, 64 requests of 8 rows with 64 adapters 20.0 and 31.1, of 16 23.5 and 24.8, of 32 (1.25 times `most`) 30.2 and 24.4;
+// 512 rows at rank 64 22.6 and 22.2; 64 requests of 2 rows 8.4 and 84.  With the ternary linear (3 2^24: tiles save reading
+// and writing y again): 256 rows 19.9 and 23.2, 512 24.6 and 26.1, 1,024 37.2 and 36.3; 1,000 rows of 704 29.6 and 23.5.
+static bool lora_by_token(const LoraArgs &l, uint32_t cols, uint32_t out, uint64_t most) {
+  return l.seq <= 16 ||
+         (l.seq < 65536 && ((uint64_t)l.seq * l.rmax * ((uint64_t)cols + out) <= most || l.seq < 4ull * l.requests));
+}
 
-// Whether lora_tok alone does them: a few rows of small adapters.
+// Whether one launch does them, each workgroup finding u again: a few rows of small adapters (four rows of 2,560 at rank 16
+// 4.2 us for 6.4 in two, at rank 64 8.4 for 6.5).
 static bool lora_tok_whole(const DownArgs &d) { return d.l.seq <= 4 && (uint64_t)d.l.rmax * d.k <= 65536; }
 
 // q: the rows' rounding to int8, wanted beside (then without the way up)
@@ -1245,7 +1254,7 @@ static int lora_forward(const char *what, const LoraArgs &l, const float *x, boo
   d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)ws;
   UpArgs p{};
   p.l = l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
-  if (lora_by_token(l)) return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
+  if (lora_by_token(l, cols, out, 1u << 27)) return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
   float *const parts = (float *)((uint8_t *)ws + lora_round((size_t)l.seq * l.rmax * 4));
   return lora_down(what, d, bf, false, parts, st) || lora_up(what, p, bf, false, st);
 }
@@ -1313,7 +1322,7 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
     FusedArgs f{};
     f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;
     f.y = y; f.ystride = out;
-    if (lora_by_token(l)) {
+    if (lora_by_token(l, cols, out, 3u << 24)) {
       DownArgs d{};
       d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
       UpArgs p{};

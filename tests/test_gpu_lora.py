@@ -88,7 +88,13 @@ CASES = [dict(lengths=[1], adapter=[0], adapters=1, rmax=8, out=1, cols=8),
          dict(lengths=[17, 0, 40, 3, 1], adapter=[1, 0, 0, -5, 1], adapters=2, rmax=24, out=130, cols=200, first=3, behind=9),
          dict(lengths=[100, 33], adapter=[0, 0], adapters=1, rmax=32, out=256, cols=512),
          dict(lengths=[64, 64, 70], adapter=[3, 1, 3], adapters=5, rmax=128, out=72, cols=1000, mixed=True),
-         dict(lengths=[5, 6, 7], adapter=[0, 1, 2], adapters=3, rmax=40, out=333, cols=96, behind=40)]
+         dict(lengths=[5, 6, 7], adapter=[0, 1, 2], adapters=3, rmax=40, out=333, cols=96, behind=40),
+         # long enough for tiles of 32 rows, at each width of the ranks
+         dict(lengths=[400, 0, 5, 700, 90], adapter=[1, 0, 2, 0, -1], adapters=3, rmax=8, out=514, cols=14000, mixed=True),
+         dict(lengths=[9] * 150, adapter=[i % 7 for i in range(150)], adapters=7, rmax=16, out=1003, cols=5304, first=2, behind=30),
+         dict(lengths=[333, 500, 250], adapter=[1, -1, 0], adapters=2, rmax=24, out=260, cols=5000, mixed=True),
+         dict(lengths=[4] * 190, adapter=[i % 11 for i in range(190)], adapters=11, rmax=64, out=801, cols=2048, mixed=True),
+         dict(lengths=[100, 33, 170], adapter=[0, 2, 1], adapters=3, rmax=128, out=640, cols=2904, behind=3)]
 
 
 @pytest.mark.parametrize("bf", [False, True])
@@ -175,7 +181,20 @@ BESIDE = [dict(lengths=[1], adapter=[0], adapters=1, rmax=16, out=100, cols=256)
           dict(lengths=[200, 0, 90], adapter=[1, 1, 0], adapters=2, rmax=24, out=257, cols=128, behind=4),
           dict(lengths=[1] * 40, adapter=[i % 3 for i in range(40)], adapters=3, rmax=16, out=130, cols=320),
           dict(lengths=[600, 500, 700], adapter=[0, -1, 1], adapters=2, rmax=16, out=4000, cols=704),
-          dict(lengths=[1000, 777], adapter=[0, 1], adapters=2, rmax=8, out=4000, cols=1088)]
+          dict(lengths=[1000, 777], adapter=[0, 1], adapters=2, rmax=8, out=4000, cols=1088),
+          dict(lengths=[150, 100, 60], adapter=[2, 0, 1], adapters=3, rmax=128, out=1000, cols=576, mixed=True),
+          # the other forms of the projection beside tiles of adapters: 32-token tiles, one phase, few tokens
+          dict(lengths=[300, 200], adapter=[1, 0], adapters=2, rmax=64, out=701, cols=1024),
+          dict(lengths=[60, 68], adapter=[1, 0], adapters=2, rmax=128, out=2560, cols=2560),
+          dict(lengths=[60, 40], adapter=[1, 0], adapters=2, rmax=128, out=2001, cols=2048)]
+
+
+def test_forms_of_the_cases():
+    """That the cases are on both sides of what decides between a wave a row and tiles of 32."""
+    size = [sum(c["lengths"]) * c["rmax"] * (c["cols"] + c["out"]) for c in CASES]
+    assert sum(s > 1 << 27 for s in size) >= 5 and sum(s <= 1 << 27 for s in size) >= 7
+    size = [sum(c["lengths"]) * c["rmax"] * (c["cols"] + c["out"]) for c in BESIDE]
+    assert sum(s > 3 << 24 for s in size) >= 8 and sum(s <= 3 << 24 for s in size) >= 8
 
 
 @pytest.mark.parametrize("bf", [False, True])
@@ -201,7 +220,8 @@ def same(a, b):
 SHAPES = [dict(lengths=[1] * 12, adapter=[0, 1, 2] * 4, adapters=3, rmax=16, out=70, cols=136),
           dict(lengths=[1] * 150, adapter=[i % 4 for i in range(150)], adapters=4, rmax=8, out=130, cols=256),
           dict(lengths=[20, 3, 40, 50], adapter=[0, 1, 2, 1], adapters=3, rmax=32, out=96, cols=264),
-          dict(lengths=[33, 20, 60], adapter=[1, 0, 2], adapters=3, rmax=104, out=100, cols=328)]
+          dict(lengths=[33, 20, 60], adapter=[1, 0, 2], adapters=3, rmax=104, out=100, cols=328),
+          dict(lengths=[200, 33, 160], adapter=[1, 0, 2], adapters=3, rmax=104, out=340, cols=3000 - 56)]
 
 
 @pytest.mark.parametrize("i", range(len(SHAPES)))
@@ -310,7 +330,7 @@ def test_row_is_its_request():
     close(y, want, "y")
 
 
-@pytest.mark.parametrize("i", [0, 2])
+@pytest.mark.parametrize("i", [0, 2, 4])
 def test_captured(i):
     """Two captured calls that share a workspace (a projection with its adapters, their gradients), replayed in turn and
     between eager calls while rows, adapters and requests change: the eager bits each time."""
