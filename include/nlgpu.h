@@ -505,7 +505,8 @@ int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t *b, int fm
 size_t nlg_lora_linear_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests);
 /* nlg_ternary_linear with the adapters of its rows' requests: the shared
  * projection on the rounded rows, the adapters on the rows as they are.
- * cols is at most 16384; w2 is 16-byte aligned. */
+ * cols is at most 16384 (multiples of 64 run on the matrix cores from four
+ * rows on); w2 is 16-byte aligned. */
 int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const float *bias, const float *beta, int beta_per_row,
                             const uint16_t *a, const uint16_t *b, int fmt, const float *scale, const int32_t *rank,
                             const int32_t *start, const int32_t *adapter, uint32_t requests, uint32_t adapters,

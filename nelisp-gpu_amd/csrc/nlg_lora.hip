@@ -164,17 +164,14 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
       const uint32_t there = k < a.k ? a.k - k : 0u;
       Bf8 h[NT];
       if (KMAJOR) {
-        constexpr int NH = (NT + 1) / 2;
-        // (the lane's ranks NT i .. NT i + NT - 1 all lie in a row of rmax, or none does)
-        const uint32_t j = (uint32_t)(NT * i) < a.l.rmax ? NT * i : 0u;
-        uint32_t v[8][NH];
+        // (the lane's ranks 8 i .. 8 i + 7 all lie in a row of rmax, or none does)
+        static_assert(!KMAJOR || NT == 8, "eight ranks a lane");
+        const uint32_t j = 8u * i < a.l.rmax ? 8 * i : 0u;
+        uint32_t v[8][4];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
           const uint16_t *const p = (const uint16_t *)(stage + XB) + (kk + e) * a.l.rmax + j;
-          if (NT == 1) v[e][0] = *p;
-          else if (NT == 2) v[e][0] = *(const uint32_t *)p;
-          else if (NT == 4) *(uint2 *)v[e] = *(const uint2 *)p;
-          else *(uint4 *)v[e] = *(const uint4 *)p;
+          *(uint4 *)v[e] = *(const uint4 *)p;
         }
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -1097,23 +1094,25 @@ static int lora_down(const char *what, DownArgs d, bool bf, bool kmajor, float *
   const dim3 grid((d.l.seq + 31) / 32, np), blk(256);
   const bool vec = d.k % 4 == 0 && ((uintptr_t)d.x & 15) == 0;
   const uint32_t nt = (d.l.rmax + 15) / 16;
-#define GO(BF, KM, N)                                                                          \
-  do {                                                                                         \
-    if (vec) hipLaunchKernelGGL((k_lora_down<BF, KM, N, true>), grid, blk, 0, st, d);          \
-    else hipLaunchKernelGGL((k_lora_down<BF, KM, N, false>), grid, blk, 0, st, d);             \
+#define GO(BF, KM, N, V) hipLaunchKernelGGL((k_lora_down<BF, KM, N, V>), grid, blk, 0, st, d)
+#define GO2(BF)                               \
+  do {                                        \
+    if (nt <= 1) GO(BF, false, 1, true);      \
+    else if (nt <= 2) GO(BF, false, 2, true); \
+    else if (nt <= 4) GO(BF, false, 4, true); \
+    else GO(BF, false, 8, true);              \
   } while (0)
-#define GO2(BF, KM)                  \
-  do {                               \
-    if (nt <= 1) GO(BF, KM, 1);      \
-    else if (nt <= 2) GO(BF, KM, 2); \
-    else if (nt <= 4) GO(BF, KM, 4); \
-    else GO(BF, KM, 8);              \
-  } while (0)
-  // (the gradient's way down of up to 64 ranks is k_lora_gy)
-  if (bf && kmajor) GO(true, true, 8);
-  else if (bf) GO2(true, false);
-  else if (kmajor) GO(false, true, 8);
-  else GO2(false, false);
+  // (the gradient's way down of up to 64 ranks is k_lora_gy; x has whole float4s)
+  if (kmajor) {
+    if (bf && vec) GO(true, true, 8, true);
+    else if (bf) GO(true, true, 8, false);
+    else if (vec) GO(false, true, 8, true);
+    else GO(false, true, 8, false);
+  } else if (bf) {
+    GO2(true);
+  } else {
+    GO2(false);
+  }
 #undef GO2
 #undef GO
   NLG_LAUNCHED(what);
@@ -1123,15 +1122,14 @@ static int lora_down(const char *what, DownArgs d, bool bf, bool kmajor, float *
 static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipStream_t st) {
   const dim3 grid((d.n + 255) / 256, (d.l.seq + 31) / 32), blk(256);
   const bool vec = d.n % 4 == 0 && (((uintptr_t)d.y | (uintptr_t)d.res) & 15) == 0;
-#define GO(BF, KM)                                                                       \
-  do {                                                                                   \
-    if (vec) hipLaunchKernelGGL((k_lora_up<BF, KM, true>), grid, blk, 0, st, d);         \
-    else hipLaunchKernelGGL((k_lora_up<BF, KM, false>), grid, blk, 0, st, d);            \
-  } while (0)
-  if (bf && kmajor) GO(true, true);
-  else if (bf) GO(true, false);
-  else if (kmajor) GO(false, true);
-  else GO(false, false);
+#define GO(BF, KM, V) hipLaunchKernelGGL((k_lora_up<BF, KM, V>), grid, blk, 0, st, d)
+  // (dx has whole float4s)
+  if (bf && kmajor) GO(true, true, true);
+  else if (kmajor) GO(false, true, true);
+  else if (bf && vec) GO(true, false, true);
+  else if (bf) GO(true, false, false);
+  else if (vec) GO(false, false, true);
+  else GO(false, false, false);
 #undef GO
   NLG_LAUNCHED(what);
   return NLG_OK;
