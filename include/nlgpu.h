@@ -542,7 +542,8 @@ size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols,
  * the rounded rows gamma*q, which passes straight through the rounding; it is
  * overwritten.  lse [rows] (may be NULL) receives log(sum(exp(z/temperature))).
  * Logits of -inf (a bias that forbids a token) have no part in a row.  The
- * probabilities carry 22 bits of those from 2^-15 on and steps of 2^-39
+ * probabilities (times |beta[b]| over the power of two above the largest, where
+ * it differs by row) carry 22 bits of those from 2^-15 on and steps of 2^-39
  * below.  cols is a multiple of 64, at most 16384; x, w2 and dx are 16-byte
  * aligned.  The workspace (16-byte aligned, nlg_*_workspace bytes, 0 for
  * sizes that the calls do not take; grad: whether dx is wanted) holds the

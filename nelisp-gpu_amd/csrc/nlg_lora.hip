@@ -1175,30 +1175,9 @@ static bool lora_by_token(const LoraArgs &l, uint32_t cols, uint32_t out, uint64
 // 4.2 us for 6.4 in two, at rank 64 8.4 for 6.5).
 static bool lora_tok_whole(const DownArgs &d) { return d.l.seq <= 4 && (uint64_t)d.l.rmax * d.k <= 65536; }
 
-// q: the rows' rounding to int8, wanted beside (then without the way up)
-static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool bf, const ActQArgs *q, hipStream_t st) {
-  const uint32_t lanes = p.l.rmax <= 8 ? 1 : p.l.rmax <= 16 ? 2 : p.l.rmax <= 32 ? 4 : p.l.rmax <= 64 ? 8 : 16;
-  const uint32_t step = 64 / lanes, groups = (d.l.rmax + 4 * TOK_RANKS - 1) / (4 * TOK_RANKS);
-#define BY_LANES(GO)              \
-  do {                            \
-    if (lanes == 1) GO(1);        \
-    else if (lanes == 2) GO(2);   \
-    else if (lanes == 4) GO(4);   \
-    else if (lanes == 8) GO(8);   \
-    else GO(16);                  \
-  } while (0)
-  if (!q && lora_tok_whole(d)) {
-    const dim3 grid((p.n + 8 * step - 1) / (8 * step), p.l.seq);
-#define GO(L)                                                                              \
-  do {                                                                                     \
-    if (bf) hipLaunchKernelGGL((k_lora_tok<true, L>), grid, dim3(512), 0, st, d, p);       \
-    else hipLaunchKernelGGL((k_lora_tok<false, L>), grid, dim3(512), 0, st, d, p);         \
-  } while (0)
-    BY_LANES(GO);
-#undef GO
-    NLG_LAUNCHED(what);
-    return NLG_OK;
-  }
+// q: the rows' rounding to int8, wanted beside
+static int lora_tok_down(const char *what, const DownArgs &d, bool bf, const ActQArgs *q, hipStream_t st) {
+  const uint32_t groups = (d.l.rmax + 4 * TOK_RANKS - 1) / (4 * TOK_RANKS);
   const dim3 gd(d.l.seq, groups + (q ? 1 : 0));
   if (q) {
 #define GO(G)                                                                                        \
@@ -1215,6 +1194,30 @@ static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool b
   } else {
     hipLaunchKernelGGL((k_lora_tok_down<false>), gd, dim3(256), 0, st, d);
   }
+  NLG_LAUNCHED(what);
+  return NLG_OK;
+}
+
+// down and up
+static int lora_tok(const char *what, const DownArgs &d, const UpArgs &p, bool bf, hipStream_t st) {
+  const uint32_t lanes = p.l.rmax <= 8 ? 1 : p.l.rmax <= 16 ? 2 : p.l.rmax <= 32 ? 4 : p.l.rmax <= 64 ? 8 : 16;
+  const uint32_t step = 64 / lanes;
+#define BY_LANES(GO)              \
+  do {                            \
+    if (lanes == 1) GO(1);        \
+    else if (lanes == 2) GO(2);   \
+    else if (lanes == 4) GO(4);   \
+    else if (lanes == 8) GO(8);   \
+    else GO(16);                  \
+  } while (0)
+  const dim3 grid((p.n + 8 * step - 1) / (8 * step), p.l.seq);
+#define GO(L)                                                                              \
+  do {                                                                                     \
+    if (bf) hipLaunchKernelGGL((k_lora_tok<true, L>), grid, dim3(512), 0, st, d, p);       \
+    else hipLaunchKernelGGL((k_lora_tok<false, L>), grid, dim3(512), 0, st, d, p);         \
+  } while (0)
+  BY_LANES(GO);
+#undef GO
   NLG_LAUNCHED(what);
   return NLG_OK;
 }
@@ -1252,7 +1255,9 @@ static int lora_forward(const char *what, const LoraArgs &l, const float *x, boo
   d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)ws;
   UpArgs p{};
   p.l = l; p.u = d.u; p.res = res; p.y = y; p.n = out; p.scaled = true;
-  if (lora_by_token(l, cols, out, 1u << 27)) return lora_tok(what, d, p, bf, nullptr, st) || (!lora_tok_whole(d) && lora_tok_up(what, p, bf, st));
+  if (lora_by_token(l, cols, out, 1u << 27))
+    return lora_tok_whole(d) ? lora_tok(what, d, p, bf, st)
+                             : lora_tok_down(what, d, bf, nullptr, st) || lora_tok_up(what, p, bf, st);
   float *const parts = (float *)((uint8_t *)ws + lora_round((size_t)l.seq * l.rmax * 4));
   return lora_down(what, d, bf, false, parts, st) || lora_up(what, p, bf, false, st);
 }
@@ -1326,7 +1331,7 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
       UpArgs p{};
       p.l = l; p.u = d.u; p.res = y; p.y = y; p.n = out; p.scaled = true;
       const ActQArgs q{x, nullptr, 0.0f, nullptr, 0, 0, more, gamma, seq, cols, 0u};
-      return lora_tok(what, d, p, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) ||
+      return lora_tok_down(what, d, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) ||
                      lora_tok_up(what, p, bf, st)
                  ? NLG_ERR
                  : NLG_OK;
@@ -1486,7 +1491,8 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   if (!u) {
     d.x = x; d.k = cols; d.scaled = false; d.u = (float *)(ws + plan.u);
     u = d.u;
-    if (lora_down(what, d, bf, false, parts, st)) return NLG_ERR;
+    if (lora_by_token(d.l, cols, 0, 1u << 27) ? lora_tok_down(what, d, bf, nullptr, st) : lora_down(what, d, bf, false, parts, st))
+      return NLG_ERR;
   }
   float *const dbp = plan.zy > 1 ? (float *)(ws + plan.db_parts) : db, *const dap = plan.zx > 1 ? (float *)(ws + plan.da_parts) : da;
   if (rmax <= LORA_GRAD_RANK) {
