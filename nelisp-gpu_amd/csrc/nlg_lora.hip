@@ -562,105 +562,6 @@ struct OuterArgs {
   bool scaled;
 };
 
-// sum over an adapter's rows of p[s, j] q[s, c], 64 columns and 16 NT ranks a
-// workgroup, its requests' rows over the eight waves of gridDim.z workgroups,
-// four rows a wave at a time, four times of them on the way together, in 16 x
-// 16 x 4 f32 products.  Waits for memory: 4,616 rows of 6,912, rank up to 32,
-// three adapters 46 us (2.7 TB/s); in 2, 3, 4 and 8 parts 52, 49, 51 and 59.
-// TURN: stored [c][j].
-template <int NT, bool TURN, bool VEC>
-__global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
-  __shared__ v4f s_acc[4][NT][4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
-  const int32_t ad = blockIdx.y;
-  const uint32_t rank = lora_rank(a.l, ad);
-  const uint32_t col = blockIdx.x * 64 + 4 * i, nc = col < a.n ? min(4u, a.n - col) : 0u;
-  v4f acc[NT][4];
-#pragma unroll
-  for (int t = 0; t < NT; t++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc[t][e] = (v4f){0, 0, 0, 0};
-  int64_t before = 0;  // rows that earlier requests have taken
-  const int64_t step = 32 * (int64_t)gridDim.z;
-  for (uint32_t rq = 0; rq < a.l.requests; rq++) {
-    int64_t s0 = a.l.start ? (int64_t)a.l.start[rq] : (int64_t)rq;
-    int64_t s1 = a.l.start ? (int64_t)a.l.start[rq + 1] : (int64_t)rq + 1;
-    if (s0 < before) s0 = before;
-    if (s1 > (int64_t)a.l.seq) s1 = a.l.seq;
-    if (s1 <= s0) continue;
-    before = s1;
-    if (a.l.adapter[rq] != ad) continue;
-    for (int64_t s = s0 + 4 * (w + 8 * (int)blockIdx.z); s < s1; s += 4 * step) {
-      float4 qv[4];
-      float pv[4][NT];
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int64_t row = min(s + k * step + g, s1 - 1);
-        qv[k] = inside4<VEC>(a.q + (size_t)row * a.n, col, a.n);
-#pragma unroll
-        for (int t = 0; t < NT; t++) pv[k][t] = a.p[(size_t)row * a.l.rmax + min(16u * t + i, a.l.rmax - 1)];
-      }
-      if (s + 3 * step + 4 > s1) {  // rows past the request's: neither factor counts
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-          if (s + k * step + g >= s1) {
-            qv[k] = make_float4(0, 0, 0, 0);
-#pragma unroll
-            for (int t = 0; t < NT; t++) pv[k][t] = 0.0f;
-          }
-      }
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-#pragma unroll
-        for (int t = 0; t < NT; t++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[k][t], at4(qv[k], e), acc[t][e], 0, 0, 0);
-    }
-  }
-  // the waves' sums, by halves
-#pragma unroll
-  for (int half = 4; half; half /= 2) {
-    if (w >= half && w < 2 * half)
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) s_acc[w - half][t][e][lane] = acc[t][e];
-    __syncthreads();
-    if (w < half)
-#pragma unroll
-      for (int t = 0; t < NT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[t][e] += s_acc[w][t][e][lane];
-    __syncthreads();
-  }
-  if (w) return;
-  const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
-  float *const o = a.out + ((size_t)blockIdx.z * a.l.adapters + ad) * a.l.rmax * a.n;
-#pragma unroll
-  for (int t = 0; t < NT; t++) {
-    if (TURN) {
-      const uint32_t j = 16 * t + 4 * g;
-      if (j >= a.l.rmax) continue;
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if ((uint32_t)e < nc)
-          *(float4 *)(o + (size_t)(col + e) * a.l.rmax + j) =
-              make_float4(j < rank ? acc[t][e][0] * sc : 0.0f, j + 1 < rank ? acc[t][e][1] * sc : 0.0f,
-                          j + 2 < rank ? acc[t][e][2] * sc : 0.0f, j + 3 < rank ? acc[t][e][3] * sc : 0.0f);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const uint32_t j = 16 * t + 4 * g + r;
-        if (j < a.l.rmax)
-          store4<VEC>(o + (size_t)j * a.n + col, nc,
-                      j < rank ? make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc)
-                               : make_float4(0, 0, 0, 0));
-      }
-    }
-  }
-}
-
 // Blocks of sixteen rows of an adapter, in its requests' order, every parts-th
 // from part on; a wave looks at 64 requests at a time.
 struct LoraBlocks {
@@ -686,7 +587,7 @@ struct LoraBlocks {
       at = __builtin_amdgcn_readlane(s, k);
       end = __builtin_amdgcn_readlane(e, k);
       const uint32_t n = (end - at + 15) / 16;
-      at += 16 * (skip < n ? skip : n);  // (seq is under 2^21, parts at most 16)
+      at += 16 * (skip < n ? skip : n);  // (seq is under 2^21, parts at most 128)
       skip = skip < n ? (parts - (n - skip) % parts) % parts : skip - n;
     }
     row = at;
@@ -695,6 +596,98 @@ struct LoraBlocks {
     return true;
   }
 };
+
+// sum over an adapter's rows of p[s, j] q[s, c], 64 columns and 16 NT ranks (of
+// more than 64 the workgroups behind have the others: 128 at once spill) a workgroup, blocks of sixteen rows over the eight waves of gridDim.z
+// workgroups, in 16 x 16 x 4 f32 products.  Waits for memory: 4,616 rows of 6,912, rank up to 32,
+// three adapters 46 us (2.7 TB/s); in 2, 3, 4 and 8 parts 52, 49, 51 and 59.
+// TURN: stored [c][j].
+template <int NT, bool TURN, bool VEC>
+__global__ __launch_bounds__(512) void k_lora_outer(OuterArgs a) {
+  __shared__ v4f s_acc[4][NT][4][64];
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int32_t ad = blockIdx.y;
+  const uint32_t rank = lora_rank(a.l, ad);
+  const uint32_t ncol = (a.n + 63) / 64, j0 = blockIdx.x / ncol * 64;  // the first rank
+  const uint32_t col = blockIdx.x % ncol * 64 + 4 * i, nc = col < a.n ? min(4u, a.n - col) : 0u;
+  v4f acc[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; t++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc[t][e] = (v4f){0, 0, 0, 0};
+  LoraBlocks blocks(w + 8 * blockIdx.z);
+  uint32_t s0, s1;
+  while (blocks.next(a.l, ad, 8 * gridDim.z, s0, s1)) {
+    float4 qv[4];
+    float pv[4][NT];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const uint32_t row = min(s0 + 4 * k + g, s1 - 1);
+      qv[k] = inside4<VEC>(a.q + (size_t)row * a.n, col, a.n);
+#pragma unroll
+      for (int t = 0; t < NT; t++) pv[k][t] = a.p[(size_t)row * a.l.rmax + min(j0 + 16u * t + i, a.l.rmax - 1)];
+    }
+    if (s0 + 16 > s1) {  // rows past the request's: neither factor counts
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        if (s0 + 4 * k + g >= s1) {
+          qv[k] = make_float4(0, 0, 0, 0);
+#pragma unroll
+          for (int t = 0; t < NT; t++) pv[k][t] = 0.0f;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          acc[t][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(pv[k][t], at4(qv[k], e), acc[t][e], 0, 0, 0);
+  }
+  // the waves' sums, by halves
+#pragma unroll
+  for (int half = 4; half; half /= 2) {
+    if (w >= half && w < 2 * half)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s_acc[w - half][t][e][lane] = acc[t][e];
+    __syncthreads();
+    if (w < half)
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[t][e] += s_acc[w][t][e][lane];
+    __syncthreads();
+  }
+  if (w) return;
+  const float sc = a.scaled ? a.l.scale[ad] : 1.0f;
+  float *const o = a.out + ((size_t)blockIdx.z * a.l.adapters + ad) * a.l.rmax * a.n;
+#pragma unroll
+  for (int t = 0; t < NT; t++) {
+    if (TURN) {
+      const uint32_t j = j0 + 16 * t + 4 * g;
+      if (j >= a.l.rmax) continue;
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if ((uint32_t)e < nc)
+          *(float4 *)(o + (size_t)(col + e) * a.l.rmax + j) =
+              make_float4(j < rank ? acc[t][e][0] * sc : 0.0f, j + 1 < rank ? acc[t][e][1] * sc : 0.0f,
+                          j + 2 < rank ? acc[t][e][2] * sc : 0.0f, j + 3 < rank ? acc[t][e][3] * sc : 0.0f);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const uint32_t j = j0 + 16 * t + 4 * g + r;
+        if (j < a.l.rmax)
+          store4<VEC>(o + (size_t)j * a.n + col, nc,
+                      j < rank ? make_float4(acc[t][0][r] * sc, acc[t][1][r] * sc, acc[t][2][r] * sc, acc[t][3][r] * sc)
+                               : make_float4(0, 0, 0, 0));
+      }
+    }
+  }
+}
+
 // What lies `off` bytes behind a place that is the same in every lane: the load takes both as they are, without an
 // address of its own to be made in each lane.
 template <class T>
@@ -1146,16 +1139,15 @@ static uint32_t lora_parts(uint32_t seq, uint32_t n, uint32_t adapters) {
 // The launch alone: of np parts, to `parts` where that is more than one.
 static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, uint32_t np, hipStream_t st) {
   if (np > 1) d.out = parts;
-  const dim3 grid((d.n + 63) / 64, d.l.adapters, np), blk(512);
+  const dim3 grid((d.n + 63) / 64 * ((d.l.rmax + 63) / 64), d.l.adapters, np), blk(512);
   const bool vec = d.n % 4 == 0 && ((uintptr_t)d.q & 15) == 0;
   const uint32_t nt = (d.l.rmax + 15) / 16;
   // (dB of up to 64 ranks is k_lora_gy's; x has whole float4s)
-  if (turn && vec) hipLaunchKernelGGL((k_lora_outer<8, true, true>), grid, blk, 0, st, d);
-  else if (turn) hipLaunchKernelGGL((k_lora_outer<8, true, false>), grid, blk, 0, st, d);
+  if (turn && vec) hipLaunchKernelGGL((k_lora_outer<4, true, true>), grid, blk, 0, st, d);
+  else if (turn) hipLaunchKernelGGL((k_lora_outer<4, true, false>), grid, blk, 0, st, d);
   else if (nt <= 1) hipLaunchKernelGGL((k_lora_outer<1, false, true>), grid, blk, 0, st, d);
   else if (nt <= 2) hipLaunchKernelGGL((k_lora_outer<2, false, true>), grid, blk, 0, st, d);
-  else if (nt <= 4) hipLaunchKernelGGL((k_lora_outer<4, false, true>), grid, blk, 0, st, d);
-  else hipLaunchKernelGGL((k_lora_outer<8, false, true>), grid, blk, 0, st, d);
+  else hipLaunchKernelGGL((k_lora_outer<4, false, true>), grid, blk, 0, st, d);
   NLG_LAUNCHED(what);
   return NLG_OK;
 }
