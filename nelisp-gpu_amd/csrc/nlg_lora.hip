@@ -1128,9 +1128,9 @@ static int lora_up(const char *what, const UpArgs &d, bool bf, bool kmajor, hipS
   return NLG_OK;
 }
 
-// How many parts an adapter's rows are summed in: until two workgroups a CU have some, each of 256 rows at least.
+// How many parts an adapter's rows are summed in: until two workgroups a CU have some, each of 64 rows at least.
 static uint32_t lora_parts(uint32_t seq, uint32_t n, uint32_t adapters) {
-  const uint64_t wg = (uint64_t)((n + 63) / 64) * adapters, most = seq / 256;
+  const uint64_t wg = (uint64_t)((n + 63) / 64) * adapters, most = seq / 64;
   uint64_t k = 512 / wg;
   if (k > most) k = most;
   return k < 1 ? 1 : k > 16 ? 16 : (uint32_t)k;
