@@ -487,10 +487,10 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
  * in 32 bits.  x [seq x cols] f32; cols is a multiple of 8.  a, b, x, u and
  * the workspace (nlg_*_workspace bytes; 0: sizes that are not taken) are
  * 16-byte aligned; calls that share a workspace run in stream order.  Nothing
- * here allocates, so every call may be captured into a graph (but for the
- * column split of nlg_ternary_linear_lora's base, which goes without its
- * scratch if a capture is the first call that wants it).  Rows have no part in
- * each other; an infinity in x (dy) makes NaN of its row's u, and values below
+ * here allocates or uses a scratch of the library's, so every call may be
+ * captured into a graph, and graphs with workspaces of their own may be
+ * replayed on any streams beside each other and beside other calls.  Rows have
+ * no part in each other; an infinity in x (dy) makes NaN of its row's u, and values below
  * 2^-100 may lose the last bits of their products there.  seq is at most
  * 2,097,120, out and cols 2^24, adapters 65534.
  * ---------------------------------------------------------------------- */

@@ -334,8 +334,15 @@ int nlg_fused_launch(const FusedArgs &a, int pro, int epi, int rows_per_wave, hi
 bool nlg_batched(uint32_t seq, uint32_t cols);
 int nlg_batched_launch(const FusedArgs &a, int pro, int epi, hipStream_t st);
 // Its GEMM alone, over activations already quantised into xq / gamma (as
-// k_act_q leaves them); f's x, gain and prologue fields are not used.
-int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st);
+// k_act_q leaves them); f's x, gain and prologue fields are not used.  split:
+// the caller's nlg_batched_split_bytes, 16-byte aligned, for the sums and
+// counters of a launch that splits its columns, the first
+// TG_SPLIT_COUNTERS words zero by then (and after it); null: the library's
+// scratch for the stream.
+#define TG_SPLIT_COUNTERS 256
+int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st,
+                     uint32_t *split = nullptr);
+size_t nlg_batched_split_bytes(uint32_t seq, uint32_t out, uint32_t cols);  // 0: such a launch does not split
 // (max, index) partials per token an ARGMAX launch of `out` rows writes.
 uint32_t nlg_argmax_parts(uint32_t seq, uint32_t cols, uint32_t out);
 // Grow-only device scratch owned by the library, one per stream (NULL on

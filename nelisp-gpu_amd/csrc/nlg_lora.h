@@ -89,7 +89,7 @@ __device__ __forceinline__ void split_f16(uint32_t h, uint32_t &p0, uint32_t &p1
 // that nlg_batched leaves to the kernels of few tokens.
 bool nlg_batched_lora(uint32_t seq, uint32_t cols);
 // The shared projection on the matrix cores with the adapters added to it
-// (nlg_batched_gemm otherwise); *done: whether the form that this size takes
-// adds them, or only the projection was run.  u [seq][rmax].
+// (nlg_batched_gemm otherwise, split as there); *done: whether the form that
+// this size takes adds them, or only the projection was run.  u [seq][rmax].
 int nlg_batched_gemm_lora(const FusedArgs &f, const uint8_t *xq, const float *gamma, const LoraArgs &l, const float *u,
-                          bool bf, bool *done, hipStream_t st);
+                          bool bf, uint32_t *split, bool *done, hipStream_t st);

@@ -52,7 +52,13 @@ struct DownArgs {
   uint32_t k;
   bool scaled;
   float *u;         // [seq][rmax]; of several parts, one after the other
+  uint32_t *zero;   // TG_SPLIT_COUNTERS words to be zeroed for the projection behind this launch, or null
 };
+// (256 threads)
+__device__ __forceinline__ void zero_counters(const DownArgs &a) {
+  static_assert(TG_SPLIT_COUNTERS == 256, "one a thread");
+  if (a.zero && blockIdx.x == 0 && blockIdx.y == 0) a.zero[threadIdx.x] = 0;
+}
 
 // 32 rows a workgroup, all ranks (NT blocks of sixteen), the contraction over
 // its four waves and gridDim.y workgroups.  Each adapter among the rows is one
@@ -89,6 +95,7 @@ __global__ __launch_bounds__(256) void k_lora_down(DownArgs a) {
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t row0 = blockIdx.x * ROWS;
+  zero_counters(a);
   float *const out = a.u + (size_t)blockIdx.y * a.l.seq * a.l.rmax;
   // this workgroup's steps
   const uint32_t all = (a.k + 127) / 128, s0 = (uint64_t)blockIdx.y * all / gridDim.y;
@@ -323,12 +330,13 @@ __device__ __forceinline__ void tok_down_group(const DownArgs &a, uint32_t row, 
   }
 }
 template <bool BF>
-__global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {
+__global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {  // (never ahead of a projection: no zero)
   tok_down_group<BF>(a, blockIdx.x, blockIdx.y);
 }
 // That beside the rounding of the same rows to int8 for the shared projection, in one launch.
 template <bool BF, int G16>
 __global__ __launch_bounds__(256) void k_lora_tok_down_q(DownArgs a, ActQArgs q) {
+  zero_counters(a);
   if (blockIdx.y == 0) act_q_row<G16, NLG_PRO_NONE>(q, blockIdx.x);
   else tok_down_group<BF>(a, blockIdx.x, blockIdx.y - 1);
 }
@@ -1277,12 +1285,17 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
   return lora_forward(what, l, x, fmt == NLG_LORA_BF16, res, y, u, out, cols, workspace, nlg_stream(stream)) ? NLG_ERR : NLG_OK;
 }
 
+// What the projection keeps apart from its column split: rows as int8 and their scales, in either form's layout.
+static size_t ternary_bytes(uint32_t seq, uint32_t cols) {
+  const size_t rows = nlg_ternary_linear_workspace(seq, cols), batched = nlg_batched_scratch_bytes(seq, cols);
+  return lora_round(rows > batched ? rows : batched);
+}
+
 extern "C" size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax,
                                                     uint32_t requests) {
   const size_t u = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
   if (!u) return 0;
-  const size_t rows = nlg_ternary_linear_workspace(seq, cols), batched = nlg_batched_scratch_bytes(seq, cols);
-  return u + lora_round(rows > batched ? rows : batched);
+  return u + ternary_bytes(seq, cols) + nlg_batched_split_bytes(seq, out, cols);
 }
 
 extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const float *bias, const float *beta,
@@ -1317,23 +1330,25 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
     FusedArgs f{};
     f.w2 = w2; f.bias = bias; f.beta = beta; f.beta_per_row = beta_per_row; f.seq = seq; f.out = out; f.cols = cols;
     f.y = y; f.ystride = out;
+    // the projection's column split, in this call's own workspace: its counters are zeroed by the launch ahead of it
+    uint32_t *const split = nlg_batched_split_bytes(seq, out, cols) ? (uint32_t *)(more + ternary_bytes(seq, cols)) : nullptr;
     if (lora_by_token(l, cols, out, 3u << 24)) {
       DownArgs d{};
-      d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
+      d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace; d.zero = split;
       UpArgs p{};
       p.l = l; p.u = d.u; p.res = y; p.y = y; p.n = out; p.scaled = true;
       const ActQArgs q{x, nullptr, 0.0f, nullptr, 0, 0, more, gamma, seq, cols, 0u};
-      return lora_tok_down(what, d, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st) ||
+      return lora_tok_down(what, d, bf, &q, st) || nlg_batched_gemm(f, more, gamma, NLG_EPI_STORE, st, split) ||
                      lora_tok_up(what, p, bf, st)
                  ? NLG_ERR
                  : NLG_OK;
     }
     DownArgs d{};
-    d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace;
+    d.l = l; d.x = x; d.k = cols; d.scaled = false; d.u = u ? u : (float *)workspace; d.zero = split;
     float *const parts = (float *)((uint8_t *)workspace + lora_round((size_t)seq * rmax * 4));
     bool done = false;
     if (nlg_act_q_launch(x, nullptr, 0.0f, nullptr, 0, 0, NLG_PRO_NONE, more, gamma, seq, cols, st) ||
-        lora_down(what, d, bf, false, parts, st) || nlg_batched_gemm_lora(f, more, gamma, l, d.u, bf, &done, st))
+        lora_down(what, d, bf, false, parts, st) || nlg_batched_gemm_lora(f, more, gamma, l, d.u, bf, split, &done, st))
       return NLG_ERR;
     if (done) return NLG_OK;
     UpArgs p{};

@@ -74,7 +74,9 @@ struct GemmArgs {
   // runs the epilogue
   int32_t *ksum;
   uint32_t *kctr;
-  bool allow_split;  // the launcher may take split workspace from the library
+  // (the launcher sets ksum; kctr null: it takes both from the library's
+  // scratch if allow_split, else it does not split)
+  bool allow_split;
   // EPI_LORA_*: the rows' adapters and what they are on the way up from
   LoraArgs lora;
   const float *lu;     // [seq][rmax]
@@ -1082,6 +1084,60 @@ int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *
   return NLG_OK;
 }
 
+// Which kernel the sizes take, but for ARGMAX: the wide-wave one, and how many
+// slices of the columns share each of its 256-row x 32-token tiles then.
+struct TgForm {
+  bool wide;
+  uint32_t slices;
+  uint64_t tiles;
+};
+static TgForm tg_form(uint32_t seq, uint32_t out, uint32_t cols) {
+  // Rows of 9..10 chunks over 128..256 64-row x 32-token tiles take
+  // k_tgemm's single 10-chunk phase below at any token count: at 128..192
+  // tokens (QKV 3,840 rows at 128, O 2,560 rows up to 192) it beat the
+  // wide-wave kernel's 32-token tiles 6.2..6.4 against 10.2..10.4 us, while
+  // its two-phase forms (more tiles) lost or tied.
+  const uint32_t nch = cols / TG_KC;
+  const uint64_t t64x32 = (uint64_t)nlg_blocks(out, 64) * ((seq + 31) / 32);
+  const bool one_phase = nch > TG_PH && nch <= 10 && t64x32 >= 128 && t64x32 <= 256;
+  // From 65 tokens, more than 512 such tiles (k_tgemm holds two 64-row
+  // workgroups per CU, so a second round) go to the wide-wave kernel too:
+  // gate|up (13,824 x 2560) at 72 / 96 / 112 / 127 tokens 12.8 / 12.4 /
+  // 12.5 / 13.9 against 15.8 / 16.2 / 19.6 / 19.9 us, 13,824 x 1280 at 72
+  // 8.7 against 9.6; at 432 tiles k_tgemm kept the lead (gate|up at 64
+  // tokens 10.9 against 11.7, 6,912 x 2560 at 112 10.6 against 12.0).
+  const bool wide = seq >= 128 || (seq > 64 && t64x32 > 512);
+  TgForm f = {wide && !one_phase, 1, (uint64_t)nlg_blocks(out, 256) * ((seq + 31) / 32)};
+  // The column split of 32-token tiles, 2 / 3 / 4 slices against none,
+  // tiled weights (row layout within 1 us of these): down projection
+  // (2560 x 6912, 27 chunks) at 128 tokens (40 tiles) 15.0 / 14.3 /
+  // 14.4 against 19.4, 256 (80) 15.9 / 15.1 / 17.7 against 19.6, 384
+  // (120) 17.2 / 19.2 / 18.2 against 20.0, 512 (160) 22.6 / 20.0 / 22.7
+  // against 21.0, 640 (200) 23.2 / 24.9 / 26.1 against 21.5; 1024 x 6912
+  // at 128 (16) 15.0 / 14.3 / 13.3 against 18.5; 2560 x 4096 at 128 (40)
+  // 12.8 / 12.1 / 12.5 against 14.2; but rows of 10 chunks never gain
+  // (O 2560 x 2560 at 128 / 256 / 512 tokens 10.3 / 10.5 / 11.9 unsplit,
+  // 10.9 / 11.8 / 15.3 in 2 slices; QKV 3840 x 2560 likewise).  The
+  // split form the kernel replaced (64-row tiles of token-half waves)
+  // took 16.2 / 20.0 / 20.5 us for the down projection at 128 / 256 /
+  // 384 tokens.  Every slice leaves a 32 KB block of partial sums and
+  // the last to arrive reads the others (tl_split_meet), so a slice
+  // must carry enough chunks: rows of 16+ chunks only, and about one
+  // workgroup per CU in all (two at 160 tiles).
+  if (f.wide && nch >= 16) {
+    if (f.tiles <= 128) f.slices = 256 / (uint32_t)f.tiles < 4 ? 256 / (uint32_t)f.tiles : 4;  // >= 2
+    else if (f.tiles <= 170) f.slices = 3;
+  }
+  return f;
+}
+
+// What a split launch shares between its slices: the tiles' counters, the same region for every launch (a split grid has
+// at most 170 tiles), so that partial sums never land on a counter, and the sums, one 32-register block per (slice, tile,
+// thread).
+static size_t tg_split_bytes(const TgForm &f) {
+  return f.slices > 1 ? TG_SPLIT_COUNTERS * 4 + (size_t)f.slices * f.tiles * 256 * 32 * 4 : 0;
+}
+
 // (of an EPI_LORA_* launch: another form than k_tgemm_w would run, so none did)
 #define NLG_TGEMM_OTHER 2
 int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
@@ -1113,26 +1169,12 @@ int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
   // replaces the row layout: the same words, in load order
   const uint32_t *wt = nlg_tiled_find(a.w2, a.out, a.cols);
   if (wt) a.w2 = wt;
-  // Rows of 9..10 chunks over 128..256 64-row x 32-token tiles take
-  // k_tgemm's single 10-chunk phase below at any token count: at 128..192
-  // tokens (QKV 3,840 rows at 128, O 2,560 rows up to 192) it beat the
-  // wide-wave kernel's 32-token tiles 6.2..6.4 against 10.2..10.4 us, while
-  // its two-phase forms (more tiles) lost or tied.
-  const uint32_t nch_all = a.cols / TG_KC;
-  const uint64_t t64x32 = (uint64_t)nlg_blocks(a.out, 64) * ((a.seq + 31) / 32);
-  const bool one_phase = nch_all > TG_PH && nch_all <= 10 && t64x32 >= 128 && t64x32 <= 256;
-  // From 65 tokens, more than 512 such tiles (k_tgemm holds two 64-row
-  // workgroups per CU, so a second round) go to the wide-wave kernel too:
-  // gate|up (13,824 x 2560) at 72 / 96 / 112 / 127 tokens 12.8 / 12.4 /
-  // 12.5 / 13.9 against 15.8 / 16.2 / 19.6 / 19.9 us, 13,824 x 1280 at 72
-  // 8.7 against 9.6; at 432 tiles k_tgemm kept the lead (gate|up at 64
-  // tokens 10.9 against 11.7, 6,912 x 2560 at 112 10.6 against 12.0).
-  const bool wide = a.seq >= 128 || (a.seq > 64 && t64x32 > 512);
-  if (TG_LORA(epi) && (!wide || one_phase)) return NLG_TGEMM_OTHER;
-  if (wide && epi != NLG_EPI_ARGMAX && !one_phase) {
+  const TgForm form = tg_form(a.seq, a.out, a.cols);
+  if (TG_LORA(epi) && !form.wide) return NLG_TGEMM_OTHER;
+  if (form.wide && epi != NLG_EPI_ARGMAX) {
     // 256-row tiles of the wide-wave kernel (k_tgemm_w), 64-token tiles
     // once there are 400 of them, else 32-token ones; a few tiles of long
-    // rows split their columns over gridDim.z slices.  From sweeps of the
+    // rows split their columns over gridDim.z slices (tg_form).  From sweeps of the
     // config-5 linears and config 4 at 128..16384 tokens, kernel trace,
     // median of 6..20 interleaved launches of each form:
     //  * 32-token tiles against the token-half 64-row-tile form this kernel
@@ -1152,39 +1194,14 @@ int nlg_tgemm_launch(const GemmArgs &a0, int epi, hipStream_t st) {
     //    at 1024 / 2048 / 4096 / 16384 tokens 40.3 / 75.6 / 156.5 / 550.4
     //    against 40.2 / 68.9 / 150.2 / 550.0, down (STORE) 49.8 / 54.7 /
     //    102.1 / 265.3 against 29.8 / 44.8 / 81.9 / 251.5: not kept.
-    //  * the column split of 32-token tiles, 2 / 3 / 4 slices against none,
-    //    tiled weights (row layout within 1 us of these): down projection
-    //    (2560 x 6912, 27 chunks) at 128 tokens (40 tiles) 15.0 / 14.3 /
-    //    14.4 against 19.4, 256 (80) 15.9 / 15.1 / 17.7 against 19.6, 384
-    //    (120) 17.2 / 19.2 / 18.2 against 20.0, 512 (160) 22.6 / 20.0 / 22.7
-    //    against 21.0, 640 (200) 23.2 / 24.9 / 26.1 against 21.5; 1024 x 6912
-    //    at 128 (16) 15.0 / 14.3 / 13.3 against 18.5; 2560 x 4096 at 128 (40)
-    //    12.8 / 12.1 / 12.5 against 14.2; but rows of 10 chunks never gain
-    //    (O 2560 x 2560 at 128 / 256 / 512 tokens 10.3 / 10.5 / 11.9 unsplit,
-    //    10.9 / 11.8 / 15.3 in 2 slices; QKV 3840 x 2560 likewise).  The
-    //    split form the kernel replaced (64-row tiles of token-half waves)
-    //    took 16.2 / 20.0 / 20.5 us for the down projection at 128 / 256 /
-    //    384 tokens.  Every slice leaves a 32 KB block of partial sums and
-    //    the last to arrive reads the others (tl_split_meet), so a slice
-    //    must carry enough chunks: rows of 16+ chunks only, and about one
-    //    workgroup per CU in all (two at 160 tiles).
     const uint32_t rt = nlg_blocks(a.out, 256);
-    const uint64_t n32 = (a.seq + 31) / 32, t1 = (uint64_t)rt * n32, t2 = (uint64_t)rt * ((a.seq + 63) / 64);
-    const uint32_t nch = a.cols / TG_KC;
-    uint32_t ks = 1;
-    if (a.allow_split && nch >= 16) {
-      if (t1 <= 128) ks = 256 / (uint32_t)t1 < 4 ? 256 / (uint32_t)t1 : 4;  // >= 2
-      else if (t1 <= 170) ks = 3;
-    }
+    const uint64_t n32 = (a.seq + 31) / 32, t2 = (uint64_t)rt * ((a.seq + 63) / 64);
+    uint32_t ks = a.allow_split || a.kctr ? form.slices : 1;
     if (ks > 1) {
-      // partial sums: one 32-register block per (slice, tile, thread); the
-      // counters' region is the same for every launch (a split grid has at
-      // most 170 tiles), so partial sums never land on a counter
-      const size_t ctr_bytes = 256 * 4;
-      uint8_t *w = (uint8_t *)nlg_scratch_try(ctr_bytes + (size_t)ks * t1 * 256 * 32 * 4, st, 1);
+      uint8_t *w = a.kctr ? (uint8_t *)a.kctr : (uint8_t *)nlg_scratch_try(tg_split_bytes(form), st, 1);
       if (w) {
         a.kctr = (uint32_t *)w;
-        a.ksum = (int32_t *)(w + ctr_bytes);
+        a.ksum = (int32_t *)(w + TG_SPLIT_COUNTERS * 4);
       } else {
         ks = 1;
       }
@@ -1378,13 +1395,20 @@ static GemmArgs gemm_args(const FusedArgs &f, const uint8_t *xq, const float *ga
   return g;
 }
 
-int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st) {
-  return nlg_tgemm_launch(gemm_args(f, xq, gamma), epi, st);
+int nlg_batched_gemm(const FusedArgs &f, const uint8_t *xq, const float *gamma, int epi, hipStream_t st, uint32_t *split) {
+  GemmArgs g = gemm_args(f, xq, gamma);
+  g.kctr = split;
+  return nlg_tgemm_launch(g, epi, st);
+}
+
+size_t nlg_batched_split_bytes(uint32_t seq, uint32_t out, uint32_t cols) {
+  return nlg_batched(seq, cols) ? tg_split_bytes(tg_form(seq, out, cols)) : 0;
 }
 
 int nlg_batched_gemm_lora(const FusedArgs &f, const uint8_t *xq, const float *gamma, const LoraArgs &l, const float *u,
-                          bool bf, bool *done, hipStream_t st) {
+                          bool bf, uint32_t *split, bool *done, hipStream_t st) {
   GemmArgs g = gemm_args(f, xq, gamma);
+  g.kctr = split;
   g.lora = l;
   g.lu = u;
   const int rc = nlg_tgemm_launch(g, bf ? NLG_EPI_LORA_BF16 : NLG_EPI_LORA_F16, st);
