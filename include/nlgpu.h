@@ -486,13 +486,15 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
  *   y[s,o] = res[s,o] + scale * sum_j b[o,j] u[s,j]
  * in 32 bits.  x [seq x cols] f32; cols is a multiple of 8.  a, b, x, u and
  * the workspace (nlg_*_workspace bytes; 0: sizes that are not taken) are
- * 16-byte aligned; calls that share a workspace run in stream order.  Nothing
- * here allocates or uses a scratch of the library's, so every call may be
- * captured into a graph, and graphs with workspaces of their own may be
- * replayed on any streams beside each other and beside other calls.  Rows have
- * no part in each other; an infinity in x (dy) makes NaN of its row's u, and values below
- * 2^-100 may lose the last bits of their products there.  seq is at most
- * 2,097,120, out and cols 2^24, adapters 65534.
+ * 16-byte aligned; calls that share a workspace run in stream order.  Neither an
+ * output nor the workspace may overlap another array of the call, but y may be
+ * res and dx may be dres.  Nothing here allocates or uses a scratch of the
+ * library's, so every call may be captured into a graph, and graphs with
+ * workspaces of their own may be replayed on any streams beside each other and
+ * beside other calls.  Rows have no part in each other; an infinity in x (dy)
+ * makes NaN of its row's u, and values below 2^-100 may lose the last bits of
+ * their products there.  seq is at most 2,097,120, out and cols 2^24, adapters
+ * 65534.
  * ---------------------------------------------------------------------- */
 #define NLG_LORA_F16 0
 #define NLG_LORA_BF16 1
@@ -518,8 +520,7 @@ size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t co
  * for adapters without rows), and dx = dres + the adapters' part (dx NULL: not
  * wanted; dres NULL: that part alone; dres may be dx: the base's input gradient,
  * as ternary-rows-t leaves it, goes there).  u: what the forward call left
- * (NULL: computed again).  seq is nonzero.  No output may overlap another
- * or an input.  Sums over rows run in an order of the sizes alone, so the same
+ * (NULL: computed again).  seq is nonzero.  Sums over rows run in an order of the sizes alone, so the same
  * call gives the same bits. */
 int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a, const uint16_t *b, int fmt,
                          const float *scale, const int32_t *rank, const int32_t *start, const int32_t *adapter,
@@ -549,8 +550,8 @@ size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols,
  * sizes that the calls do not take; grad: whether dx is wanted) holds the
  * probabilities of a piece of the vocabulary; calls that share one run in
  * stream order.  Nothing here allocates, so every call may be captured into a
- * graph.  No output may overlap another or an input.  Rows have no part in each
- * other: an infinity in x makes NaN of its own row's outputs (a NaN is rounded
+ * graph.  Neither an output nor the workspace may overlap another array
+ * of the call.  Rows have no part in each other: an infinity in x makes NaN of its own row's outputs (a NaN is rounded
  * as nlg_ternary_linear rounds it).  Where no logit is above -inf, lse is -inf,
  * the loss of a row with targets NaN, and its gradient the targets' part alone.
  * ---------------------------------------------------------------------- */

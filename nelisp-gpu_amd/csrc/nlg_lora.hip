@@ -1277,10 +1277,12 @@ extern "C" int nlg_lora_linear(const float *x, const uint16_t *a, const uint16_t
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
-  const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nu = (uint64_t)seq * rmax * 4;
-  if (nlg_overlap(y, ny, x, nx) || nlg_overlap(u, nu, x, nx) || nlg_overlap(u, nu, y, ny) || (res != y && nlg_overlap(y, ny, res, ny)) ||
-      nlg_overlap(u, nu, res, ny))
-    return nlg_fail("%s: outputs overlap each other or an input (y may be res itself)", what);
+  const uint64_t r4 = (uint64_t)seq * 4, na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out;
+  const NlgSpan at[] = {{x, r4 * cols}, {a, 2 * na}, {b, 2 * nb}, {scale, 4ull * adapters}, {rank, 4ull * adapters},
+                        {start, 4ull * requests + 4}, {adapter, 4ull * requests}, {res == y ? nullptr : res, r4 * out},
+                        {y, r4 * out}, {u, r4 * rmax}, {workspace, need}};
+  if (nlg_outputs_overlap(at, 11, 3))
+    return nlg_fail("%s: outputs or the workspace overlap each other or an input (y may be res itself)", what);
   NLG_SCOPE(what);
   return lora_forward(what, l, x, fmt == NLG_LORA_BF16, res, y, u, out, cols, workspace, nlg_stream(stream)) ? NLG_ERR : NLG_OK;
 }
@@ -1318,9 +1320,13 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
-  const uint64_t bx = (uint64_t)seq * cols * 4, by = (uint64_t)seq * out * 4, bu = (uint64_t)seq * rmax * 4;
-  if (nlg_overlap(y, by, x, bx) || nlg_overlap(u, bu, x, bx) || nlg_overlap(u, bu, y, by))
-    return nlg_fail("%s: outputs overlap each other or x", what);
+  const uint64_t r4 = (uint64_t)seq * 4, na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out;
+  const NlgSpan at[] = {{x, r4 * cols}, {w2, (uint64_t)out * ((cols + 15) / 16) * 4}, {bias, 4ull * out},
+                        {beta, beta_per_row ? 4ull * out : 4}, {a, 2 * na}, {b, 2 * nb}, {scale, 4ull * adapters},
+                        {rank, 4ull * adapters}, {start, 4ull * requests + 4}, {adapter, 4ull * requests},
+                        {y, r4 * out}, {u, r4 * rmax}, {workspace, need}};
+  if (nlg_outputs_overlap(at, 13, 3))
+    return nlg_fail("%s: outputs or the workspace overlap each other or an input", what);
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   uint8_t *const more = (uint8_t *)workspace + nu;
@@ -1480,16 +1486,13 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
-  // each output against the inputs and the outputs behind it
-  const uint64_t nx = (uint64_t)seq * cols * 4, ny = (uint64_t)seq * out * 4, nr = (uint64_t)seq * rmax * 4;
-  const uint64_t na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out;
-  const struct { const void *p; uint64_t n; } in[] = {{x, nx}, {u, nr}, {dy, ny}, {a, 2 * na}, {b, 2 * nb},
-                                                      {dres == dx ? nullptr : dres, nx}, {dx, nx}, {da, 4 * na}, {db, 4 * nb}};
-  for (int o = 6; o < 9; o++)
-    for (int i = 0; i < 9; i++)
-      if (i < 6 || i > o)
-        if (nlg_overlap(in[o].p, in[o].n, in[i].p, in[i].n))
-          return nlg_fail("%s: outputs overlap each other or an input (dx may be dres itself)", what);
+  const uint64_t r4 = (uint64_t)seq * 4, na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out;
+  const NlgSpan at[] = {{x, r4 * cols}, {u, r4 * rmax}, {dy, r4 * out}, {a, 2 * na}, {b, 2 * nb}, {scale, 4ull * adapters},
+                        {rank, 4ull * adapters}, {start, 4ull * requests + 4}, {adapter, 4ull * requests},
+                        {dres == dx ? nullptr : dres, r4 * cols}, {dx, r4 * cols}, {da, 4 * na}, {db, 4 * nb},
+                        {workspace, need}};
+  if (nlg_outputs_overlap(at, 14, 4))
+    return nlg_fail("%s: outputs or the workspace overlap each other or an input (dx may be dres itself)", what);
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   const bool bf = fmt == NLG_LORA_BF16;

@@ -831,15 +831,11 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
     return nlg_fail("%s: workspace holds %zu bytes, needs %llu", what, workspace ? workspace_bytes : 0,
                     (unsigned long long)p.bytes);
   if ((uintptr_t)workspace & 15) return nlg_fail("%s: the workspace must be 16-byte aligned", what);
-  // each output against the inputs and the outputs behind it
   const uint64_t nr = (uint64_t)rows * 4, nv = beta_per_row ? (uint64_t)vocab * 4 : 4;
-  const struct { const void *p; uint64_t n; } at[] = {
+  const NlgSpan at[] = {
       {x, nr * cols}, {w2, (uint64_t)vocab * (cols / 4)}, {bias, (uint64_t)vocab * 4}, {beta, nv}, {index, nr * top},
-      {teacher, nr * top}, {teacher_lse, nr}, {dloss, nr}, {loss, nr}, {lse, nr}, {dx, nr * cols}};
-  for (int o = 8; o < 11; o++)
-    for (int i = 0; i < 11; i++)
-      if ((i < 8 || i > o) && nlg_overlap(at[o].p, at[o].n, at[i].p, at[i].n))
-        return nlg_fail("%s: outputs overlap each other or an input", what);
+      {teacher, nr * top}, {teacher_lse, nr}, {dloss, nr}, {loss, nr}, {lse, nr}, {dx, nr * cols}, {workspace, p.bytes}};
+  if (nlg_outputs_overlap(at, 12, 4)) return nlg_fail("%s: outputs or the workspace overlap each other or an input", what);
   const uint64_t ht = ((uint64_t)rows + 31) / 32 + 16, hb = ht * (p.tiles + 8);
   if (!nlg_fits(hb, 256)) return nlg_fail("%s: %u rows of %u logits are too many for one launch", what, rows, vocab);
   NLG_SCOPE(what);

@@ -10,6 +10,18 @@ static inline bool nlg_overlap(const void *a, uint64_t na, const void *b, uint64
   return a && b && x < y + nb && y < x + na;
 }
 
+// Arrays of a call, the inputs first: whether any of the last `outs` (outputs, the workspace) shares bytes with another.
+struct NlgSpan {
+  const void *p;
+  uint64_t n;
+};
+static inline bool nlg_outputs_overlap(const NlgSpan *a, int n, int outs) {
+  for (int o = n - outs; o < n; o++)
+    for (int i = 0; i < n; i++)
+      if ((i < n - outs || i > o) && nlg_overlap(a[o].p, a[o].n, a[i].p, a[i].n)) return true;
+  return false;
+}
+
 // The device the library runs on made the calling thread's for one call.
 struct NlgDeviceScope {
   int was = -1;
