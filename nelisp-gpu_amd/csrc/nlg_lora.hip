@@ -1360,10 +1360,12 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
     UpArgs p{};
     p.l = l; p.u = d.u; p.res = y; p.y = y; p.n = out; p.scaled = true;
     return lora_up(what, p, bf, false, st) ? NLG_ERR : NLG_OK;
-  } else if (nlg_ternary_linear(x, w2, bias, beta, beta_per_row, y, nullptr, seq, out, cols, more,
-                                workspace_bytes - nu, (void *)st)) {
-    return NLG_ERR;
   }
+  // (a row is a grid's y there)
+  for (uint32_t r = 0; r < seq; r += 65535)
+    if (nlg_ternary_linear(x + (size_t)r * cols, w2, bias, beta, beta_per_row, y + (size_t)r * out, nullptr,
+                           seq - r < 65535 ? seq - r : 65535, out, cols, more, workspace_bytes - nu, (void *)st))
+      return NLG_ERR;
   return lora_forward(what, l, x, bf, y, y, u, out, cols, workspace, st) ? NLG_ERR : NLG_OK;
 }
 
