@@ -492,8 +492,8 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
  * library's, so every call may be captured into a graph, and graphs with
  * workspaces of their own may be replayed on any streams beside each other and
  * beside other calls.  Rows have no part in each other; an infinity in x (dy)
- * makes NaN of its row's u, and values below 2^-100 may lose the last bits of
- * their products there.  seq is at most 2,097,120, out and cols 2^24, adapters
+ * makes NaN of its row's u (a sum past f32's range may), and values below
+ * 2^-100 may lose the last bits of their products there.  seq is at most 2,097,120, out and cols 2^24, adapters
  * 65534.
  * ---------------------------------------------------------------------- */
 #define NLG_LORA_F16 0

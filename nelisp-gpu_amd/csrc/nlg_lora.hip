@@ -307,8 +307,12 @@ __device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, 
       u[t] = fmaf(x1.w, wide<BF>(v[t].w >> 16), u[t]);
     }
   }
+  // (an infinity becomes NaN, which is what three parts of x make of it: a row's u does not depend on the form)
 #pragma unroll
-  for (int t = 0; t < R; t++) u[t] = nlg_wave_sum_f32(u[t]);
+  for (int t = 0; t < R; t++) {
+    const float v = nlg_wave_sum_f32(u[t]);
+    u[t] = fmaf(v, 0.0f, v);
+  }
 }
 
 #define TOK_RANKS 4
