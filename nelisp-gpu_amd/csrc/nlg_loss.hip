@@ -857,7 +857,7 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
   l.part = h.part; l.bmax = h.bmax; l.index = index; l.teacher = teacher; l.teacher_lse = teacher_lse;
   l.loss = loss; l.lse = lse; l.lse2 = (float *)(ws + p.lse); l.sum = (float *)(ws + p.sum);
   l.weight = (float *)(ws + p.weight);
-  if (top > 16) hipLaunchKernelGGL((k_loss<16>), dim3(rows), dim3(1024), 0, st, l);
+  if (top > 16 && nlg_fits(rows, 1024)) hipLaunchKernelGGL((k_loss<16>), dim3(rows), dim3(1024), 0, st, l);
   else hipLaunchKernelGGL((k_loss<4>), dim3(rows), dim3(256), 0, st, l);
   NLG_LAUNCHED(what);
   if (!dx) return NLG_OK;
