@@ -23,6 +23,8 @@ int nlg_act_q_launch(const float *x, const float *gain, float eps, const float *
 
 #define LORA_RANK 128            // most ranks of an adapter
 #define LORA_ROWS (65535u * 32)  // most rows (a grid's y dimension)
+#define LORA_REQUESTS 0x1000000u
+#define LORA_TERNARY_COLS 16384  // most columns beside a ternary linear (its quantiser's)
 
 // p[k] .. p[k + 3] of n values, or where those are not all there any others of
 // the n (VEC: n is a multiple of 4 and p aligned).
@@ -1049,7 +1051,7 @@ static int lora_check(const char *what, const void *a, const void *b, int fmt, c
     return nlg_fail("%s: rmax must be a multiple of 8 up to %d (got %u)", what, LORA_RANK, rmax);
   if (!cols || cols % 8) return nlg_fail("%s: cols must be a multiple of 8 (got %u)", what, cols);
   if (!out) return nlg_fail("%s: out must be nonzero", what);
-  if (seq > LORA_ROWS || out > 0x1000000u || cols > 0x1000000u || adapters > 65534 || requests > 0x1000000u)
+  if (seq > LORA_ROWS || out > 0x1000000u || cols > 0x1000000u || adapters > 65534 || requests > LORA_REQUESTS)
     return nlg_fail("%s: too many rows, columns, requests or adapters", what);
   if (((uintptr_t)a & 15) || ((uintptr_t)b & 15)) return nlg_fail("%s: adapters must be 16-byte aligned", what);
   if (((uintptr_t)scale | (uintptr_t)rank | (uintptr_t)start | (uintptr_t)adapter) & 3)
@@ -1061,9 +1063,9 @@ static int lora_check(const char *what, const void *a, const void *b, int fmt, c
 }
 
 // sizes alone (the workspace functions have no pointers)
-static bool lora_sizes(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax) {
+static bool lora_sizes(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests) {
   return seq && out && cols && cols % 8 == 0 && rmax && rmax % 8 == 0 && rmax <= LORA_RANK && seq <= LORA_ROWS &&
-         out <= 0x1000000u && cols <= 0x1000000u;
+         out <= 0x1000000u && cols <= 0x1000000u && requests <= LORA_REQUESTS;
 }
 
 static LoraSum lora_parts_of(const float *part, float *out, uint64_t n, uint32_t parts) {
@@ -1248,8 +1250,7 @@ static int lora_tok_up(const char *what, const UpArgs &p, bool bf, hipStream_t s
 }
 
 extern "C" size_t nlg_lora_linear_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax, uint32_t requests) {
-  (void)requests;
-  return lora_sizes(seq, out, cols, rmax) ? lora_round((size_t)seq * rmax * 4) + lora_down_bytes(seq, cols, rmax) : 0;
+  return lora_sizes(seq, out, cols, rmax, requests) ? lora_round((size_t)seq * rmax * 4) + lora_down_bytes(seq, cols, rmax) : 0;
 }
 
 // ws: nlg_lora_linear_workspace
@@ -1300,7 +1301,7 @@ static size_t ternary_bytes(uint32_t seq, uint32_t cols) {
 extern "C" size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t rmax,
                                                     uint32_t requests) {
   const size_t u = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
-  if (!u) return 0;
+  if (!u || cols > LORA_TERNARY_COLS) return 0;
   return u + ternary_bytes(seq, cols) + nlg_batched_split_bytes(seq, out, cols);
 }
 
@@ -1318,7 +1319,7 @@ extern "C" int nlg_ternary_linear_lora(const float *x, const uint32_t *w2, const
   if (((uintptr_t)x | (uintptr_t)w2 | (uintptr_t)u) & 15) return nlg_fail("%s: x, w2 and u must be 16-byte aligned", what);
   if (((uintptr_t)y | (uintptr_t)bias | (uintptr_t)beta) & 3)
     return nlg_fail("%s: y, bias and beta must be 4-byte aligned", what);
-  if (cols > 16384) return nlg_fail("%s: cols must be at most 16384 (got %u)", what, cols);
+  if (cols > LORA_TERNARY_COLS) return nlg_fail("%s: cols must be at most %d (got %u)", what, LORA_TERNARY_COLS, cols);
   const size_t nu = nlg_lora_linear_workspace(seq, out, cols, rmax, requests);
   const size_t need = nlg_ternary_linear_lora_workspace(seq, out, cols, rmax, requests);
   if (!workspace || workspace_bytes < need)
@@ -1384,9 +1385,10 @@ struct LoraGradPlan {
   size_t u, du_parts, db_parts, da_parts, bytes;
 };
 #define LORA_GRAD_RANK 64
-static LoraGradPlan lora_grad_plan(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters, uint32_t rmax) {
+static LoraGradPlan lora_grad_plan(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters, uint32_t rmax,
+                                   uint32_t requests) {
   LoraGradPlan p = {};
-  if (!lora_sizes(seq, out, cols, rmax) || !adapters || adapters > 65534) return p;
+  if (!lora_sizes(seq, out, cols, rmax, requests) || !adapters || adapters > 65534) return p;
   const size_t row = lora_round((size_t)seq * rmax * 4), down = lora_down_bytes(seq, cols, rmax);
   const uint64_t na = (uint64_t)adapters * rmax * cols, nb = (uint64_t)adapters * rmax * out, blocks = ((uint64_t)seq + 15) / 16;
   p.u = row;
@@ -1418,8 +1420,7 @@ static LoraGradPlan lora_grad_plan(uint32_t seq, uint32_t out, uint32_t cols, ui
 
 extern "C" size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols, uint32_t adapters,
                                                  uint32_t rmax, uint32_t requests) {
-  (void)requests;
-  return lora_grad_plan(seq, out, cols, adapters, rmax).bytes;
+  return lora_grad_plan(seq, out, cols, adapters, rmax, requests).bytes;
 }
 
 // du and dB of up to 64 ranks
@@ -1487,7 +1488,7 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   if (((uintptr_t)x | (uintptr_t)u | (uintptr_t)da | (uintptr_t)db | (uintptr_t)dx | (uintptr_t)dres) & 15)
     return nlg_fail("%s: x, u, dres, dx, da and db must be 16-byte aligned", what);
   if ((uintptr_t)dy & 3) return nlg_fail("%s: dy must be 4-byte aligned", what);
-  const LoraGradPlan plan = lora_grad_plan(seq, out, cols, adapters, rmax);
+  const LoraGradPlan plan = lora_grad_plan(seq, out, cols, adapters, rmax, requests);
   const size_t need = plan.bytes;
   if (!workspace || workspace_bytes < need)
     return nlg_fail("%s: workspace holds %zu bytes, needs %zu", what, workspace ? workspace_bytes : 0, need);

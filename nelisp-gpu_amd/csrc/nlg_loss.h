@@ -48,6 +48,8 @@ static inline LossPlan loss_plan(uint32_t rows, uint32_t vocab, uint32_t cols, u
       vocab > 0x1000000u)
     return p;
   p.tiles = (uint32_t)((vocab + (uint64_t)LOSS_TILE - 1) / LOSS_TILE);
+  // one launch of the logits' product: 256 threads a tile of 32 rows, tiles rounded up to the XCDs and their groups
+  if ((((uint64_t)rows + 31) / 32 + 16) * (p.tiles + 8) * 256 >= 1ull << 32) return p;
   uint64_t at = 0;
   const auto take = [&](uint64_t bytes) {
     const uint64_t a = at;

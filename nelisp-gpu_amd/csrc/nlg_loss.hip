@@ -836,8 +836,6 @@ static int loss_run(const char *what, const float *x, const uint32_t *w2, const 
       {x, nr * cols}, {w2, (uint64_t)vocab * (cols / 4)}, {bias, (uint64_t)vocab * 4}, {beta, nv}, {index, nr * top},
       {teacher, nr * top}, {teacher_lse, nr}, {dloss, nr}, {loss, nr}, {lse, nr}, {dx, nr * cols}, {workspace, p.bytes}};
   if (nlg_outputs_overlap(at, 12, 4)) return nlg_fail("%s: outputs or the workspace overlap each other or an input", what);
-  const uint64_t ht = ((uint64_t)rows + 31) / 32 + 16, hb = ht * (p.tiles + 8);
-  if (!nlg_fits(hb, 256)) return nlg_fail("%s: %u rows of %u logits are too many for one launch", what, rows, vocab);
   NLG_SCOPE(what);
   hipStream_t st = nlg_stream(stream);
   uint8_t *const ws = (uint8_t *)workspace;
