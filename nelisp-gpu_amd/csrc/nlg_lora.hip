@@ -8,7 +8,9 @@
 //   dA[a][j][c] = sum_{s of a} du[s, j] x[s, c],  dB[a][o][j] = scale[a] sum_{s of a} dy[s, o] u[s, j]
 //
 // with a the adapter of row s's request.  Rows and adapters' values meet in
-// 32 bits (16 x 16 x 4 f32 products; the 16-bit values are exact there).
+// 32 bits: on the bf16 matrix cores in parts (the way down in tiles, du, the way
+// up in the ternary linear's epilogue), a wave a row in plain f32, else in 16 x
+// 16 x 4 f32 products, where the 16-bit values are exact.
 //
 // v_mfma_f32_16x16x4_f32: lane 16 g + i gives A[i][g] and B[g][i]; its result
 // r is C[4 g + r][i].
@@ -69,7 +71,7 @@ __device__ __forceinline__ void zero_counters(const DownArgs &a) {
 // (v_mfma_f32_16x16x32_bf16: lane 16 g + i holds k = 8 g .. 8 g + 7 of row or
 // column i): x as the three bf16 that make up its 24 bits, a bf16 weight as it
 // is, an f16 weight as two.  Of the products of parts only that of the last two
-// is left out, 2^-24 of the whole.
+// is left out: under 2^-22 of a product, 2^-25 on average.
 // Both operands go from memory to LDS directly in runs of 256 bytes and more,
 // three stages, two on the way while one is multiplied.  (Read straight into
 // the products' layout, 128 bytes of each of 32 rows at a time, 4,731 rows of

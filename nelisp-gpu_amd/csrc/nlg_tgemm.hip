@@ -541,8 +541,8 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 // token (r % 4) + 8 (r / 4) + 4 lg), with s_ad the tokens' adapters: u
 // in three bf16 parts times the adapter's rows (an f16 value in two), in 32
 // x 32 x 16 products, sixteen ranks at a time; of the products of parts that of
-// the last two is left out, 2^-24 of the whole.  Each adapter among the tokens is one
-// pass, whose sums count for its own tokens alone.
+// the last two is left out, under 2^-22 of a product and 2^-25 on average.  Each
+// adapter among the tokens is one pass, whose sums count for its own tokens alone.
 template <int NB, bool BF>
 __device__ __forceinline__ void tl_lora(const GemmArgs &a, v16f (&val)[NB], const uint32_t (&rc)[NB], const int32_t *s_ad,
                                         int lane, int lg, uint32_t tok0) {
