@@ -344,9 +344,9 @@ __global__ __launch_bounds__(256) void k_lora_tok_down(DownArgs a) {  // (never 
 // That beside the rounding of the same rows to int8 for the shared projection, in one launch.
 template <bool BF, int G16>
 __global__ __launch_bounds__(256) void k_lora_tok_down_q(DownArgs a, ActQArgs q) {
-  zero_counters(a);
   if (blockIdx.y == 0) act_q_row<G16, NLG_PRO_NONE>(q, blockIdx.x);
   else tok_down_group<BF>(a, blockIdx.x, blockIdx.y - 1);
+  zero_counters(a);
 }
 
 // ------------------------------------------------------------------ up: from the ranks
