@@ -481,7 +481,9 @@ int nlg_cache_read_paged_q8(const uint8_t *kpool, const uint8_t *vpool, int fmt,
  * factor scale[i].  Request i's rows are start[i] .. start[i+1]-1 (start
  * [requests + 1], not falling; NULL: request i is row i) and its adapter is
  * adapter[i]; any number outside [0, adapters) means none, and so do rows of
- * no request.  start, adapter, rank and scale are device arrays.
+ * no request.  start, adapter, rank and scale are device arrays.  Requests
+ * without rows are taken, but the calls choose their form by how many requests
+ * there are: many empty ones beside a long one make it slower.
  *   u[s,j] = sum_c a[j,c] x[s,c]    (0 behind the rank)
  *   y[s,o] = res[s,o] + scale * sum_j b[o,j] u[s,j]
  * in 32 bits.  x [seq x cols] f32; cols is a multiple of 8.  a, b, x, u and
@@ -520,8 +522,9 @@ size_t nlg_ternary_linear_lora_workspace(uint32_t seq, uint32_t out, uint32_t co
  * for adapters without rows), and dx = dres + the adapters' part (dx NULL: not
  * wanted; dres NULL: that part alone; dres may be dx: the base's input gradient,
  * as ternary-rows-t leaves it, goes there).  u: what the forward call left
- * (NULL: computed again).  seq is nonzero.  Sums over rows run in an order of the sizes alone, so the same
- * call gives the same bits. */
+ * (NULL: computed again, the last bits perhaps others).  seq is nonzero.  Sums
+ * over rows run in an order of the sizes alone, so the same call gives the same
+ * bits. */
 int nlg_lora_linear_grad(const float *x, const float *u, const float *dy, const uint16_t *a, const uint16_t *b, int fmt,
                          const float *scale, const int32_t *rank, const int32_t *start, const int32_t *adapter,
                          uint32_t requests, uint32_t adapters, uint32_t rmax, const float *dres, float *dx, float *da,
@@ -547,13 +550,15 @@ size_t nlg_lora_linear_grad_workspace(uint32_t seq, uint32_t out, uint32_t cols,
  * it differs by row) carry 22 bits of those from 2^-15 on and steps of 2^-39
  * below.  cols is a multiple of 64, at most 16384; x, w2 and dx are 16-byte
  * aligned.  The workspace (16-byte aligned, nlg_*_workspace bytes, 0 for
- * sizes that the calls do not take; grad: whether dx is wanted) holds the
- * probabilities of a piece of the vocabulary; calls that share one run in
- * stream order.  Nothing here allocates, so every call may be captured into a
- * graph.  Neither an output nor the workspace may overlap another array
- * of the call.  Rows have no part in each other: an infinity in x makes NaN of its own row's outputs (a NaN is rounded
- * as nlg_ternary_linear rounds it).  Where no logit is above -inf, lse is -inf,
- * the loss of a row with targets NaN, and its gradient the targets' part alone.
+ * sizes that the calls do not take; grad: whether dx is wanted) holds, with a
+ * gradient, the probabilities of as many rows as take 512 MB (of 256 rows, or
+ * all, where those take more); calls that share one run in stream order.
+ * Nothing here allocates, so every call may be captured into a graph.  Neither
+ * an output nor the workspace may overlap another array of the call.  Rows
+ * have no part in each other: an infinity in x makes NaN of its own row's
+ * outputs (a NaN is rounded as nlg_ternary_linear rounds it).  Where no logit
+ * is above -inf, lse is -inf, the loss of a row with targets NaN, and its
+ * gradient the targets' part alone.
  * ---------------------------------------------------------------------- */
 
 /* Softmax cross entropy: loss[s] = lse[s] - z[s, label[s]].  Rows whose label

@@ -322,7 +322,7 @@ __device__ __forceinline__ void tok_down(const DownArgs &a, const uint16_t *wt, 
 #define TOK_RANKS 4
 // a workgroup's 4 waves: sixteen ranks of a row, four a wave (each read of x feeds four dots, and a row of 64 ranks has
 // sixteen waves), in plain f32: an adapter's rows are too few for a tile.  Waits for memory; 64 rows of 2,560 with 48
-// adapters of up to 64 ranks 6.6 us with their rounding to int8 (tiles of 32 rows, a pass for each adapter among them: 324).
+// adapters of up to 64 ranks 7.3 us with their rounding to int8 (tiles of 32 rows, a pass for each adapter among them: 324).
 template <bool BF>
 __device__ __forceinline__ void tok_down_group(const DownArgs &a, uint32_t row, uint32_t group) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256) void k_lora_up(UpArgs a) {
 // Few rows a request: a wave a row and NC steps of 64 / L columns, L lanes a
 // column (eight neighbouring ranks each: sixteen bytes), all on the way
 // together.  Bound by the adapters' bytes: 64 rows of 48 adapters, up to 64
-// ranks to 6,912 columns, 9.9 us (tiles of 32 rows: 120).
+// ranks to 6,912 columns, 11.9 us (tiles of 32 rows: 120).
 template <int L, int NC>
 struct TokUp {
   uint4 v[NC];
@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256) void k_lora_tok_up(UpArgs a) {
 
 // A few rows of small adapters in one launch: every workgroup finds its row's
 // u again (two ranks a wave at a time), while its columns' weights are on the
-// way.  One token, 2,560 -> 2,560 at rank 16: 4.4 us, a launch and two round trips
+// way.  One token, 2,560 -> 2,560 at rank 16: 4.6 us, a launch and two round trips
 // to memory (the call with its projection 8.2 us; with the ways down and up
 // apart, of tiles, 13).
 template <bool BF, int L>
@@ -872,9 +872,9 @@ __global__ __launch_bounds__(1024 / E, NT <= 2 ? 4 : 2) void k_lora_gy(GyArgs a)
 // workgroup has 256 columns of an adapter's rows (those of none: blockIdx.y ==
 // adapters), every gridDim.z-th block of sixteen, its waves 16 E columns each, E
 // neighbouring ones a lane, in 16 x 16 x 4 f32 products.  x, dres and dx move
-// once, a row 1 KB at a time.  It waits for memory (the matrix cores are busy 21 %
-// of the time): 241 rows of 2560 5.9 us; 4,616 of 6912 112 to 125 us, the same with
-// the next block's loads in flight, which is why larger calls take two passes.
+// once, a row 1 KB at a time.  It waits for memory: 241 rows of 2560 6.0 us; 4,616
+// of 6912 112 to 125 us, the same with the next block's loads in flight, which is
+// why larger calls take two passes.
 struct GxArgs {
   LoraArgs l;
   const float *x, *du, *dres;  // [seq][n], [seq][rmax], [seq][n] or null
@@ -1174,6 +1174,8 @@ static int lora_outer(const char *what, OuterArgs d, bool turn, float *parts, ui
 // 18.3, 64 requests of 8 rows with 64 adapters 20.0 and 31.1, of 16 23.5 and 24.8, of 32 (1.25 times `most`) 30.2 and 24.4;
 // 512 rows at rank 64 22.6 and 22.2; 64 requests of 2 rows 8.4 and 84.  With the ternary linear (3 2^24: tiles save reading
 // and writing y again): 256 rows 19.9 and 23.2, 512 24.6 and 26.1, 1,024 37.2 and 36.3; 1,000 rows of 704 29.6 and 23.5.
+// The sizes know no lengths, so requests without rows count as short ones: 4,000 rows of one request at rank 128, 4096 ->
+// 4096, 104 us, among 1,023 empty ones 418.
 static bool lora_by_token(const LoraArgs &l, uint32_t cols, uint32_t out, uint64_t most) {
   return l.seq <= 16 ||
          (l.seq < 65536 && ((uint64_t)l.seq * l.rmax * ((uint64_t)cols + out) <= most || l.seq < 4ull * l.requests));
@@ -1507,7 +1509,7 @@ extern "C" int nlg_lora_linear_grad(const float *x, const float *u, const float 
   const bool bf = fmt == NLG_LORA_BF16;
   uint8_t *const ws = (uint8_t *)workspace;
   float *const du = (float *)ws, *const parts = (float *)(ws + plan.du_parts);
-  if (!u) {
+  if (!u) {  // (in the form that this call's own size takes: the last bits may differ from the forward call's)
     d.x = x; d.k = cols; d.scaled = false; d.u = (float *)(ws + plan.u);
     u = d.u;
     if (lora_by_token(d.l, cols, 0, 1u << 27) ? lora_tok_down(what, d, bf, nullptr, st) : lora_down(what, d, bf, false, parts, st))

@@ -25,8 +25,11 @@ struct LossPlan {
 static inline uint64_t loss_round(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // How many parts the gradient's product takes its `tiles` tiles of vocabulary in: those of the shortest time by a
-// measured 13 us for 256 vocabulary rows of a 256 x 256 tile (as many such tiles as CUs side by side, smaller ones in
-// proportion), 6 us to begin and end one, and 4 TB/s for what the parts leave and is read again.
+// measured 13 us for 256 vocabulary rows of a 256 x 256 tile (as many such tiles as CUs side by side), 6 us to begin and
+// end one, and 4 TB/s for what the parts leave and is read again.  Tiles of fewer rows are taken in proportion, 6.5 us for
+// 128 and 3.25 for 64, which is less than they were traced at (8 and 5.7, in 38 and 29 us of four such steps): the parts
+// are then fewer than those times alone would ask for, as their sum costs more than it gains there (37 rows in 64 parts for
+// 32: the product 28 -> 25.6 us, the sum 5 -> 8.4).
 static inline uint32_t loss_splits(uint32_t tiles, uint32_t bm, uint64_t workgroups, uint64_t values) {
   uint32_t best = 1;
   double least = 0;
@@ -66,7 +69,8 @@ static inline LossPlan loss_plan(uint32_t rows, uint32_t vocab, uint32_t cols, u
   if (grad) {
     p.order = take(((uint64_t)rows + 1) * 4);
     p.bm = rows > 128 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : 32;
-    // chunks of rows whose probabilities (two f16 each) are at most 512 MB, of 256 rows at least
+    // chunks of rows whose probabilities (two f16 each) are at most 512 MB, or of bm rows where those have more (256 rows
+    // past 524,288 tokens, 16 GB of 2^24)
     const uint64_t row = 4ull * p.tiles * LOSS_TILE;
     uint64_t most = (512ull << 20) / row / p.bm * p.bm;
     if (most < p.bm) most = p.bm;
